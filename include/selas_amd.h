@@ -46,6 +46,9 @@ extern "C" {
 #define SELAS_F32 0
 #define SELAS_F16 1
 #define SELAS_BF16 2
+/* Integer types of selas_rope's positions. */
+#define SELAS_I32 3
+#define SELAS_I64 4
 
 /* Weight codecs (the `codec` argument of selas_linear_workspace_bytes). */
 #define SELAS_CODEC_NF4 0
@@ -426,6 +429,95 @@ int selas_attention_workspace_bytes(int64_t B, int64_t H, int64_t L, int64_t *by
  * the value layout selas_attention reads. No counterpart in the reference.
  */
 int selas_transpose_heads(const void *v, int64_t BH, int64_t L, int64_t Dh, void *vt, int dtype, void *stream);
+
+/* ------------------------------------------------------------ rotary positions */
+
+/* At most this many tensors per selas_rope call, and position axes. */
+#define SELAS_ROPE_MAX_PARTS 3
+#define SELAS_ROPE_MAX_AXES 4
+
+/* One tensor of a selas_rope call (host-memory array element): x and y are
+ * [B, heads, L, Dh] with unit channel stride and any batch, head and row strides
+ * (elements). scale: the RMS norm's scale [Dh] fp32, NULL for no norm. rotate 0
+ * leaves the angles out (the values, which are laid out along with q and k). */
+typedef struct selas_rope_part {
+  const void *x;
+  int64_t x_sb, x_sh, x_sl;
+  void *y;
+  int64_t y_sb, y_sh, y_sl;
+  const float *scale;
+  int64_t heads;
+  int64_t rotate;
+} selas_rope_part;
+
+/*
+ * Rotary positions with several axes, taken from the positions themselves:
+ *   z = x, or x / sqrt(mean(x^2) + 1e-6) * scale over a head's Dh channels;
+ *   pair j of axis a turns by pos[b, l, a] * theta^(-2j / axis_dim[a]):
+ *   (z0, z1) -> (z0 cos - z1 sin, z0 sin + z1 cos), by the negative angle when
+ *   inverse != 0 (the rotation's gradient; no part may then have a scale).
+ * The pairs of the axes follow each other; with R = sum(axis_dim) pair i is
+ * channels (2i, 2i + 1), or (i, i + R/2) when halves != 0, and channels from R on
+ * are not rotated. ids is [B, L, axes] (fp32, SELAS_I32 or SELAS_I64, unit last
+ * stride; ids_sb 0 where the images share their positions). Each axis_dim is
+ * even, R <= Dh. Angles are formed and reduced in fp64, the rest is fp32 and
+ * rounded once. dtype is the tensors' type. y may be x (same address and strides);
+ * otherwise no y may overlap an x or another y. Dh <= 256 where the tensors can be read
+ * in vectors (4 elements or 8 bytes: addresses, strides, Dh, R and, with halves, R/2),
+ * Dh <= 128 otherwise (SELAS_EUNSUPPORTED).
+ * Next to selas_qkv_single and selas_qkv_double, which take cos/sin tables that a
+ * batch shares. Restates qk_rms, apply_rope and rope_tables (flux.py:106-126).
+ */
+int selas_rope(const selas_rope_part *parts, int64_t count, int64_t B, int64_t L, int64_t Dh, const void *ids,
+               int ids_dtype, int64_t ids_sb, int64_t ids_sl, int64_t axes, const int64_t *axis_dim, double theta,
+               int halves, int inverse, int dtype, void *stream);
+
+/* ------------------------------------------------------------ raw linear */
+
+/* Activations of selas_raw_linear. */
+#define SELAS_ACT_NONE 0
+#define SELAS_ACT_GELU 1 /* tanh approximation */
+#define SELAS_ACT_SILU 2
+
+/* One linear of a selas_raw_linear call (host-memory array element):
+ *   y[b, l, n] = residual[b, l, n] + gate[b, n] * act(sum_k x[b, l, k] w[n, k] + bias[n])
+ * with unit column strides, batch strides *_sb and row strides *_sl in elements,
+ * and the rows of w ldw elements apart. bias, gate and residual may be NULL. The
+ * dtypes of bias, gate, residual and y are each SELAS_F32 or the call's dtype.
+ * y may be the residual (same address, strides and dtype) and overlap nothing else. */
+typedef struct selas_raw_linear_problem {
+  const void *x;
+  int64_t x_sb, x_sl;
+  const void *w;
+  int64_t ldw;
+  const void *bias;
+  const void *gate;
+  int64_t gate_sb;
+  const void *residual;
+  int64_t r_sb, r_sl;
+  void *y;
+  int64_t y_sb, y_sl;
+  int64_t B, L, N, K;
+  int bias_dtype, gate_dtype, residual_dtype, y_dtype, act, reserved;
+} selas_raw_linear_problem;
+
+/*
+ * Up to SELAS_MAX_BATCHED_LINEARS independent linears with unquantized weights,
+ * x and w in dtype (bf16 or fp16, otherwise SELAS_EUNSUPPORTED), fp32 accumulation
+ * and epilogue, one rounding at the end. K may be 0 (act(bias) remains).
+ * workspace: device memory of at least selas_raw_linear_workspace_bytes for
+ * these problems, 16-byte aligned, not used by anything else until the call has
+ * run; NULL and 0 where that size is 0, otherwise SELAS_EINVAL. The kernels, tiles
+ * and K ranges depend on the problems' shapes, strides, alignment and the CU count
+ * only, so equal calls give equal bits.
+ * Next to selas_nf4_linear_batched, for the raw codec's weights: UnitView.linear
+ * (selas/store.py:289-293) with the activation (flux.py:150-151, 194-195) and the
+ * gated residual add (flux.py:169-171) that follow it.
+ */
+int selas_raw_linear(const selas_raw_linear_problem *problems, int64_t count, int dtype, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+int selas_raw_linear_workspace_bytes(const selas_raw_linear_problem *problems, int64_t count, int dtype,
+                                     int64_t *bytes);
 
 #ifdef __cplusplus
 }

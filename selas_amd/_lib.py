@@ -14,10 +14,11 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libselas_amd.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 OK, EINVAL, EUNSUPPORTED, EHIP = 0, 1, 2, 3
 F32, F16, BF16 = 0, 1, 2
+I32, I64 = 3, 4  # position types of selas_rope
 CODEC_NF4, CODEC_INT8_ROW = 0, 1
 
 DTYPE_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
@@ -55,6 +56,9 @@ SIGNATURES: dict[str, list] = {
     "selas_attention_split": [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _INT, _P, _I64, _P],
     "selas_attention_workspace_bytes": [_I64, _I64, _I64, ctypes.POINTER(ctypes.c_int64)],
     "selas_transpose_heads": [_P, _I64, _I64, _I64, _P, _INT, _P],
+    "selas_rope": [_P, _I64, _I64, _I64, _I64, _P, _INT, _I64, _I64, _I64, _P, ctypes.c_double, _INT, _INT, _INT, _P],
+    "selas_raw_linear": [_P, _I64, _INT, _P, _I64, _P],
+    "selas_raw_linear_workspace_bytes": [_P, _I64, _INT, ctypes.POINTER(ctypes.c_int64)],
 }
 
 
@@ -74,6 +78,23 @@ class GemvDesc(ctypes.Structure):
     _fields_ = [("packed", _P), ("absmax", _P), ("bias", _P), ("y", _P), ("n", _I64), ("ldy", _I64)]
 
 
+class RopePart(ctypes.Structure):
+    """selas_rope_part (include/selas_amd.h): one tensor of a rotation."""
+
+    _fields_ = [("x", _P), ("x_sb", _I64), ("x_sh", _I64), ("x_sl", _I64), ("y", _P), ("y_sb", _I64), ("y_sh", _I64),
+                ("y_sl", _I64), ("scale", _P), ("heads", _I64), ("rotate", _I64)]
+
+
+class RawLinearProblem(ctypes.Structure):
+    """selas_raw_linear_problem (include/selas_amd.h)."""
+
+    _fields_ = [("x", _P), ("x_sb", _I64), ("x_sl", _I64), ("w", _P), ("ldw", _I64), ("bias", _P), ("gate", _P),
+                ("gate_sb", _I64), ("residual", _P), ("r_sb", _I64), ("r_sl", _I64), ("y", _P), ("y_sb", _I64),
+                ("y_sl", _I64), ("B", _I64), ("L", _I64), ("N", _I64), ("K", _I64), ("bias_dtype", _INT),
+                ("gate_dtype", _INT), ("residual_dtype", _INT), ("y_dtype", _INT), ("act", _INT), ("reserved", _INT)]
+
+
+ROPE_MAX_PARTS, ROPE_MAX_AXES = 3, 4
 STATIC_MAX_WEIGHTS = 1023
 STATIC_MAX_STREAMS = 8
 

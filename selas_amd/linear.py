@@ -12,11 +12,13 @@ GPU, by the bit-exact decode kernel) and a library GEMM runs.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
 
 from . import _lib
+from ._layout import distinct, may_meet, same_elements
 from .codecs import EncodedTensor, decode, int8_row_dequant, nf4_dequant
 
 
@@ -308,6 +310,151 @@ def _gelu_chunk(codec: str, problems):
         return [_gelu_composed(codec, *p[:8], o) for p, (_, o) in zip(problems, outs)]
     del keep
     return outs
+
+
+class RawLinear(NamedTuple):
+    """One linear with an unquantized weight and its epilogue (the arguments of ``raw_linear``)."""
+
+    x: torch.Tensor
+    weight: torch.Tensor
+    bias: torch.Tensor | None = None
+    act: str | None = None
+    gate: torch.Tensor | None = None
+    residual: torch.Tensor | None = None
+    out: torch.Tensor | None = None
+    out_dtype: torch.dtype | None = None
+
+
+ACTS = {None: 0, "gelu": 1, "silu": 2}  # SELAS_ACT_*
+
+
+def raw_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, act: str | None = None,
+               gate: torch.Tensor | None = None, residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
+               out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``residual + gate * act(x @ weight.T + bias)`` with an unquantized weight, in one kernel.
+
+    x [..., K] and weight [N, K] (bf16 or fp16, unit column stride or copied); ``act``: None, "gelu" (tanh
+    approximation, flux.py:194-195) or "silu" (flux.py:150-151); ``gate``: one row per image, [B, 1, N], or one
+    for all ([N], [1, N], [1, 1, N]), where x is [B, L, K]; ``residual``: [..., N]. Bias, gate, residual and the
+    result are each fp32 or x's dtype; the result has ``out``'s dtype, or ``out_dtype``, or the residual's, or x's.
+    The sum, the activation, the gate and the residual are fp32, rounded once.
+
+    ``out``: optional [..., N] destination with unit column stride (returned); it may be the residual itself
+    (the residual stream updated in place), any other overlap is refused. Other dtypes raise ``Unsupported``."""
+    return raw_linear_batched([RawLinear(x, weight, bias, act, gate, residual, out, out_dtype)])[0]
+
+
+def raw_linear_batched(problems) -> list[torch.Tensor]:
+    """``[raw_linear(...) for each]`` of independent ``RawLinear`` problems of one dtype, up to four per launch (e.g.
+    the image and text streams of a double block, selas/models/flux.py:300-324). No problem's ``out`` may overlap
+    another problem's tensors."""
+    problems = [RawLinear(*p) for p in problems]
+    outs: list[torch.Tensor] = []
+    for i in range(0, len(problems), _lib.MAX_BATCHED_LINEARS):
+        outs += _raw_chunk(problems[i:i + _lib.MAX_BATCHED_LINEARS])
+    return outs
+
+
+def _raw_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """(t, batch stride, row stride) of a [..., L, C] tensor seen as [B, L, C] with unit column stride."""
+    if t.dim() > 3:
+        t = t.reshape(-1, *t.shape[-2:])
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.dim() == 3 else 0), (t.stride(-2) if t.dim() > 1 else 0)
+
+
+def _raw_vector(v: torch.Tensor, b: int, n: int) -> tuple[torch.Tensor, int]:
+    """A gate ([B|1, 1, N], [B|1, N] or [N]) and its batch stride."""
+    lead = v.shape[:-1]
+    if v.dim() == 3 and lead[1] == 1:
+        lead = lead[:1]
+    if v.shape[-1] != n or len(lead) > 1 or (lead and lead[0] not in (1, b)):
+        raise ValueError(f"raw_linear: gate {tuple(v.shape)} is not one row per image (batch {b}, width {n})")
+    if n > 1 and v.stride(-1) != 1:
+        v = v.contiguous()
+    return v, (v.stride(0) if lead and lead[0] > 1 else 0)
+
+
+def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
+    if not problems:
+        return []
+    dt = problems[0].x.dtype
+    arr = (_lib.RawLinearProblem * len(problems))()
+    outs, keep, given = [], [], []
+    dev = _lib.require_gpu(*(t for p in problems for t in p if isinstance(t, torch.Tensor)))
+    if dt not in (torch.bfloat16, torch.float16):
+        raise _lib.Unsupported(f"raw_linear: takes bf16 or fp16, got {dt}")
+    for i, (x, w, bias, act, gate, residual, out, out_dtype) in enumerate(problems):
+        if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+            raise ValueError(f"raw_linear: x {tuple(x.shape)} does not go with weight {tuple(w.shape)}")
+        if x.dtype != dt or w.dtype != dt:
+            raise ValueError(f"raw_linear: x {x.dtype} and weight {w.dtype} must be {dt}")
+        if act not in ACTS:
+            raise ValueError(f"raw_linear: act must be None, 'gelu' or 'silu', got {act!r}")
+        n, k = w.shape
+        shape = (*x.shape[:-1], n)
+        _check_bias(bias, n)
+        if residual is not None and residual.shape != shape:
+            raise ValueError(f"raw_linear: residual {tuple(residual.shape)} is not {shape}")
+        ydt = out.dtype if out is not None else out_dtype or (dt if residual is None else residual.dtype)
+        for name, d in (("out", ydt), *((m, t.dtype) for m, t in (("bias", bias), ("gate", gate), ("residual", residual))
+                                        if t is not None)):
+            if d != dt and d != torch.float32:
+                raise ValueError(f"raw_linear: {name} is {d}, takes {dt} or float32")
+        if out is not None and out_dtype not in (None, out.dtype):
+            raise ValueError(f"raw_linear: out is {out.dtype}, out_dtype {out_dtype}")
+        x3, x_sb, x_sl = _raw_rows(x)
+        if w.shape[1] > 1 and w.stride(1) != 1:
+            w = w.contiguous()
+        b, l = (x3.shape[0], x3.shape[1]) if x3.dim() == 3 else (1, x3.shape[0] if x3.dim() == 2 else 1)
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+        g, g_sb = (None, 0) if gate is None else _raw_vector(gate, b, n)
+        r, r_sb, r_sl = (None, 0, 0) if residual is None else _raw_rows(residual)
+        if out is None:
+            out = torch.empty(shape, dtype=ydt, device=dev)
+            y, y_sb, y_sl = out, l * n, n
+        else:
+            y = _check_raw_out(out, shape, (x, w, bias, gate), residual)
+            y_sb, y_sl = (y.stride(0) if y.dim() == 3 else 0), (y.stride(-2) if y.dim() > 1 else 0)
+            given.append(i)
+        outs.append(out)
+        keep += (x3, w, bias, g, r)
+        code = _lib.DTYPE_CODES
+        arr[i] = _lib.RawLinearProblem(
+            x3.data_ptr(), x_sb, x_sl, w.data_ptr(), w.stride(0), _lib.ptr(bias), _lib.ptr(g), g_sb, _lib.ptr(r), r_sb,
+            r_sl, y.data_ptr(), y_sb, y_sl, b, l, n, k, code[bias.dtype] if bias is not None else 0,
+            code[g.dtype] if g is not None else 0, code[r.dtype] if r is not None else 0, code[ydt], ACTS[act], 0)
+    for i in given if len(problems) > 1 else ():
+        for j, p in enumerate(problems):
+            if j != i and any(t is not None and may_meet(outs[i], t) for t in (*p[:3], *p[4:6], outs[j])):
+                raise ValueError(f"raw_linear: out of problem {i} overlaps a tensor of problem {j}")
+    size = ctypes.c_int64()
+    with torch.cuda.device(dev):
+        _lib.call("selas_raw_linear_workspace_bytes", ctypes.addressof(arr), len(problems), _lib.DTYPE_CODES[dt],
+                  ctypes.byref(size))
+        ws = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
+        _lib.call("selas_raw_linear", ctypes.addressof(arr), len(problems), _lib.DTYPE_CODES[dt], _lib.ptr(ws), size.value,
+                  _lib.stream(dev))
+    del keep  # the launch is queued on the stream that later reuses this memory
+    return outs
+
+
+def _check_raw_out(out: torch.Tensor, shape, inputs, residual) -> torch.Tensor:
+    """``out`` as [B, L, N], or an error: wrong shape or layout, or an overlap with a tensor that the launch reads."""
+    if out.shape != shape or (shape[-1] > 1 and out.stride(-1) != 1) or not distinct(out):
+        raise ValueError(f"raw_linear: out must be {shape} with unit column stride and every element at its own address, "
+                         f"got {tuple(out.shape)} strides {out.stride()}")
+    if any(t is not None and may_meet(out, t) for t in inputs) or (
+            residual is not None and not same_elements(out, residual) and may_meet(out, residual)):
+        raise ValueError("raw_linear: out overlaps a tensor that the call reads")
+    if out.dim() <= 3:
+        return out
+    try:
+        return out.view(-1, *out.shape[-2:])
+    except RuntimeError:
+        raise ValueError(f"raw_linear: out's leading dims do not fold into one, strides {out.stride()}") from None
 
 
 class GroupedPlan:
