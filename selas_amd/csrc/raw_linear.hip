@@ -19,6 +19,7 @@ struct RawProblem {
   FastDiv by_l;
   int act;
   bool bias_f32, gate_f32, residual_f32, y_f32;
+  bool vec;  // N is a multiple of 8 and bias, gate, residual and y take 16-byte accesses at every 8th column
 };
 
 // v_mfma_f32_16x16x32 of two 16-bit fragments: D(16x16) += A(16x32) B(32x16). Lane l supplies A[l % 16][8 (l / 16) ..
@@ -33,6 +34,24 @@ __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
                                                   0);
 }
 
+// The same, accumulated in place in accumulation registers. The builtin leaves the compiler free to give the sum
+// other registers than the addend; with 256 accumulators it then moves and spills them inside the K loop. The hazards of
+// an instruction that the compiler does not know: a is not read by anything but later calls until settle_mfma(), and the
+// same a comes again 16 calls (4 in the 128 x 128 tile) later at the earliest.
+template <int DT>
+__device__ __forceinline__ void mfma16_inplace(uint4 a, uint4 b, f32x4 &c) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 av = {a.x, a.y, a.z, a.w}, bv = {b.x, b.y, b.z, b.w};
+  if constexpr (DT == SELAS_BF16) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(av), "v"(bv));
+  else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(av), "v"(bv));
+}
+// The products in flight reach their registers.
+__device__ __forceinline__ void settle_mfma() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // x / (1 + e^-x) by the hardware base-2 exponential and reciprocal, like gelu_tanh_fast.
 __device__ __forceinline__ float silu_fast(float x) {
   return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
@@ -45,6 +64,18 @@ __device__ __forceinline__ float activate(float v, int act) {
 template <int DT>
 __device__ __forceinline__ float load_either(const void *p, int64_t i, bool f32) {
   return f32 ? static_cast<const float *>(p)[i] : load_f<DT>(p, i);
+}
+
+// One output from its sum: the epilogue and the store.
+template <int DT>
+__device__ __forceinline__ void finish_one(const RawProblem &P, int b, int l, int n, float v) {
+  if (P.bias) v += load_either<DT>(P.bias, n, P.bias_f32);
+  v = activate(v, P.act);
+  if (P.gate) v *= load_either<DT>(P.gate, b * P.gate_sb + n, P.gate_f32);
+  if (P.residual) v = load_either<DT>(P.residual, b * P.r_sb + l * P.r_sl + n, P.residual_f32) + v;
+  const int64_t o = b * P.y_sb + l * P.y_sl + n;
+  if (P.y_f32) static_cast<float *>(P.y)[o] = v;
+  else store_f<DT>(P.y, o, v);
 }
 
 // Eight elements of a row from k on, zeros from K on. The address need not be aligned: global loads may start at any
@@ -129,15 +160,377 @@ __global__ __launch_bounds__(256) void raw_any_kernel(RawProblem P) {
       for (int r = 0; r < 4; ++r) {
         const int n = n0 + wn + 16 * i + 4 * (lane >> 4) + r;
         if (n >= P.N) continue;
-        float v = acc[i][j][r];
-        if (P.bias) v += load_either<DT>(P.bias, n, P.bias_f32);
-        v = activate(v, P.act);
-        if (P.gate) v *= load_either<DT>(P.gate, b * P.gate_sb + n, P.gate_f32);
-        if (P.residual) v += load_either<DT>(P.residual, b * P.r_sb + l * P.r_sl + n, P.residual_f32);
-        const int64_t o = b * P.y_sb + l * P.y_sl + n;
-        if (P.y_f32) static_cast<float *>(P.y)[o] = v;
-        else store_f<DT>(P.y, o, v);
+        finish_one<DT>(P, b, l, n, acc[i][j][r]);
       }
+  }
+}
+
+// ------------------------------------------------------------------ tiled
+
+constexpr int kMaxProblems = SELAS_MAX_BATCHED_LINEARS;
+
+// The problems of one launch. Problem i's tiles are [tile0[i], tile0[i + 1]) of the whole ones followed by its split ones'
+// K ranges: see plan_tiles.
+struct RawBatch {
+  RawProblem p[kMaxProblems];
+  int tiles_m[kMaxProblems], tiles_n[kMaxProblems], tile0[kMaxProblems];
+  int count, tiles, per_xcd;
+};
+
+__device__ __forceinline__ void wait_lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>): a loop over register arrays that cannot stay rolled.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void for_each_index(F &&f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    for_each_index<N, I + 1>(f);
+  }
+}
+
+// W consecutive columns of a row as fp32, from 16-byte aligned addresses (8-byte for four 16-bit ones).
+template <int DT, int W>
+__device__ __forceinline__ void load_cols(const void *p, int64_t i, bool f32, float (&v)[W]) {
+  if (f32) {
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const float4 u = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + j);
+      v[j] = u.x; v[j + 1] = u.y; v[j + 2] = u.z; v[j + 3] = u.w;
+    }
+  } else {
+    uint32_t w[W / 2];
+    const uint16_t *q = static_cast<const uint16_t *>(p) + i;
+    if constexpr (W == 8) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(q);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2 *>(q);
+      w[0] = u.x; w[1] = u.y;
+    }
+#pragma unroll
+    for (int t = 0; t < W / 2; ++t) {
+      if constexpr (DT == SELAS_BF16) {
+        v[2 * t] = __uint_as_float(w[t] << 16);
+        v[2 * t + 1] = __uint_as_float(w[t] & 0xffff0000u);
+      } else {
+        v[2 * t] = f16_bits_to_f32(w[t] & 0xffffu);
+        v[2 * t + 1] = f16_bits_to_f32(w[t] >> 16);
+      }
+    }
+  }
+}
+
+// W == 4: fp32 outputs; W == 8: 16-bit ones.
+template <int DT, int W>
+__device__ __forceinline__ void store_cols(void *y, int64_t i, const float (&v)[W]) {
+  if constexpr (W == 4) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(y) + i) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == SELAS_BF16) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+      else w[j] = f16_bits_rne(v[2 * j]) | (static_cast<uint32_t>(f16_bits_rne(v[2 * j + 1])) << 16);
+    }
+    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(y) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// 4 waves (WM x WN), each with MB x NB blocks of 16 x 16 outputs: tiles of TM rows of x by TN rows of w, K in steps of 64.
+//
+// LDS holds two steps, each operand in halves: half h of x is the first or second half of every wave's rows. A step runs
+// as four phases, one quarter of each wave's outputs each, (x0, w0), (x0, w1), (x1, w1), (x1, w0), in odd steps with w0
+// and w1 exchanged, so that every phase needs one operand half in registers that the phase before did not, and one
+// half's registers are free for it. Phase p:
+//   waits until the fragments read in phase p - 1 are in registers and the half that it reads now has landed, barrier;
+//   reads the fragments of phase p + 1 from LDS, issues the DMA of the half that phase p - 1 read (which no wave needs
+//   any more), and multiplies.
+// A half is read 7 phases after its DMA was issued, so 6 newer halves' loads may be pending at each wait. Past the end
+// of K the loads are out of range: they bring zeros and no traffic, and the counts stay the same.
+template <int DT, int WM, int WN, int MB, int NB, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch batch) {
+  constexpr int TM = WM * MB * 16, TN = WN * NB * 16, HM = MB / 2, HN = NB / 2, NW = WM * WN;
+  constexpr int XB = TM / 2 * 128, WB = TN / 2 * 128;      // bytes of one half of x and of w
+  constexpr int DX = XB / (1024 * NW), DW = WB / (1024 * NW);  // DMAs of a wave per half
+  constexpr int ER = 32;                                   // rows that the epilogue stages at once
+  constexpr int EB = ER * NB * 16 * 4;                     // bytes of them
+  static_assert(DX >= 1 && DW >= 1 && NW <= 8 && XB <= 16384 && WB <= 16384, "tile");
+  constexpr bool kStageX = XB >= EB;
+  static_assert((kStageX ? XB : WB) >= EB && (NW <= 4 || XB == WB), "epilogue");
+  __shared__ __attribute__((aligned(1024))) uint8_t x00[XB], x01[XB], x10[XB], x11[XB], w00[WB], w01[WB], w10[WB], w11[WB];
+
+  const int t = (blockIdx.x & 7) * batch.per_xcd + (blockIdx.x >> 3);
+  if (t >= batch.tiles) return;
+  // The tile's problem (uniform: scalar selects over the kernel arguments).
+  RawProblem P = batch.p[0];
+  int tile0 = 0, tn = batch.tiles_n[0], tm = batch.tiles_m[0];
+#pragma unroll
+  for (int i = 1; i < kMaxProblems; ++i)
+    if (i < batch.count && t >= batch.tile0[i]) {
+      P = batch.p[i];
+      tile0 = batch.tile0[i];
+      tn = batch.tiles_n[i];
+      tm = batch.tiles_m[i];
+    }
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  int m0, n0;
+  {
+    // Groups of 4 row slabs, the row fastest: the tiles that an XCD runs at once share both operands in its L2.
+    const int lt = t - tile0;
+    const int group = lt / (4 * tn), gm = min(4, tm - 4 * group), in = lt - group * 4 * tn;
+    m0 = (4 * group + in % gm) * TM;
+    n0 = (in / gm) * TN;
+  }
+  const int M = P.M, N = P.N, K = P.K;
+
+  // Operand bases: the tile's lowest row, so that the rows' offsets fit the buffer's 31 bits (checked on the host).
+  const int b0 = static_cast<int>(div31(static_cast<uint32_t>(m0), P.by_l)), l0 = m0 - b0 * P.L;
+  int64_t x_base = b0 * P.x_sb + l0 * P.x_sl;
+  if (l0 + min(TM, M - m0) > P.L) x_base = min(x_base, (b0 + 1) * P.x_sb);
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(static_cast<const uint16_t *>(P.x) + x_base, 0x7fffffffu);
+  const __amdgpu_buffer_rsrc_t wr =
+      make_rsrc(static_cast<const uint16_t *>(P.w) + static_cast<int64_t>(n0) * P.ldw, 0x7fffffffu);
+  constexpr uint32_t kOut = 0x80000000u;  // past every range
+
+  // DMA j of a half writes its LDS rows 8 j .. 8 j + 7: lane i row 8 j + i / 8, physical chunk i % 8, which holds logical
+  // chunk (i % 8) ^ (row / 2) % 8, (row / 2) % 8 = 4 (j % 2) + i / 16.
+  uint32_t xo[2][DX], wo[2][DW];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int j = 0; j < DX; ++j) {
+      const int lr = 8 * (wave * DX + j) + (lane >> 3);
+      const int m = m0 + (lr / (8 * MB)) * (16 * MB) + h * (8 * MB) + lr % (8 * MB);
+      const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l)), l = m - b * P.L;
+      const uint32_t c = (lane & 7) ^ (4 * ((wave * DX + j) & 1) + (lane >> 4));
+      xo[h][j] = m < M ? static_cast<uint32_t>((b * P.x_sb + l * P.x_sl - x_base) * 2) + 16 * c : kOut;
+    }
+#pragma unroll
+    for (int j = 0; j < DW; ++j) {
+      const int lr = 8 * (wave * DW + j) + (lane >> 3);
+      const int r = (lr / (8 * NB)) * (16 * NB) + h * (8 * NB) + lr % (8 * NB);
+      const uint32_t c = (lane & 7) ^ (4 * ((wave * DW + j) & 1) + (lane >> 4));
+      wo[h][j] = n0 + r < N ? static_cast<uint32_t>(r * P.ldw * 2) + 16 * c : kOut;
+    }
+  }
+  // The columns of K that this lane's chunks of even and odd DMAs start at.
+  const int kc[2] = {8 * static_cast<int>((lane & 7) ^ (lane >> 4)), 8 * static_cast<int>((lane & 7) ^ (4 + (lane >> 4)))};
+  auto dma_x = [&](uint8_t *dst, int h, int step, int j) __attribute__((always_inline)) {
+    load_lds16(xr, dst + (wave * DX + j) * 1024, kc[(wave * DX + j) & 1] + 64 * step < K ? xo[h][j] : kOut, 128u * step);
+  };
+  auto dma_w = [&](uint8_t *dst, int h, int step, int j) __attribute__((always_inline)) {
+    load_lds16(wr, dst + (wave * DW + j) * 1024, kc[(wave * DW + j) & 1] + 64 * step < K ? wo[h][j] : kOut, 128u * step);
+  };
+
+  // Fragment i (16 rows) of k half s: row 16 i + lane % 16 of the wave's rows, chunk 4 s + lane / 16.
+  uint32_t rd[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) rd[s] = (lane & 15) * 128 + (((4 * s + (lane >> 4)) ^ ((lane & 15) >> 1)) << 4);
+  const uint32_t xrow = wm * HM * 2048, wrow = wn * HN * 2048;
+  uint4 x0[HM][2], x1[HM][2], w0[HN][2], w1[HN][2];
+  f32x4 acc[MB][NB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{};
+  // One phase: products of quarter (HX, HW) from (xf, wf); between them, in this order, the reads of the next fragments
+  // (`read` i of R) and the DMAs (`dma` j of D), one after each product. Reads come first: they have the rest of the
+  // phase to arrive.
+  auto phase = [&](auto hx, auto hw, const uint4 (&xf)[HM][2], const uint4 (&wf)[HN][2], auto reads, auto &&read, auto dmas,
+                   auto &&dma) __attribute__((always_inline)) {
+    constexpr int HX = decltype(hx)::value, HW = decltype(hw)::value, R = decltype(reads)::value, D = decltype(dmas)::value;
+    constexpr int F = HM * HN * 2, PER = (R + D + F - 1) / F;
+    for_each_index<F>([&](auto index) __attribute__((always_inline)) {
+      constexpr int q = decltype(index)::value, s = q / (HM * HN), i = q / HN % HM, j = q % HN;
+      mfma16_inplace<DT>(wf[j][s], xf[i][s], acc[HX * HM + i][HW * HN + j]);
+      for_each_index<PER>([&](auto slot) __attribute__((always_inline)) {
+        constexpr int u = q * PER + decltype(slot)::value;
+        if constexpr (u < R) read(std::integral_constant<int, u>{});
+        else if constexpr (u < R + D) dma(u - R);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  auto read_x = [&](uint4 (&f)[HM][2], const uint8_t *src, int u) {
+    f[u % HM][u / HM] = *reinterpret_cast<const uint4 *>(src + xrow + (u % HM) * 2048 + rd[u / HM]);
+  };
+  auto read_w = [&](uint4 (&f)[HN][2], const uint8_t *src, int u) {
+    f[u % HN][u / HN] = *reinterpret_cast<const uint4 *>(src + wrow + (u % HN) * 2048 + rd[u / HN]);
+  };
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using RX = std::integral_constant<int, 2 * HM>;
+  using RW = std::integral_constant<int, 2 * HN>;
+  using CX = std::integral_constant<int, DX>;
+  using CW = std::integral_constant<int, DW>;
+
+  const int steps = ((K + 63) / 64 + 1) & ~1;
+  auto all_x = [&](uint8_t *dst, int h, int step) {
+#pragma unroll
+    for (int j = 0; j < DX; ++j) dma_x(dst, h, step, j);
+  };
+  auto all_w = [&](uint8_t *dst, int h, int step) {
+#pragma unroll
+    for (int j = 0; j < DW; ++j) dma_w(dst, h, step, j);
+  };
+  all_x(x00, 0, 0); all_w(w00, 0, 0); all_w(w01, 1, 0); all_x(x01, 1, 0);
+  all_x(x10, 0, 1); all_w(w11, 1, 1); all_w(w10, 0, 1); all_x(x11, 1, 1);
+  __builtin_amdgcn_sched_barrier(0);
+  wait_vmcnt<4 * DW + 3 * DX>();
+  wait_lds_barrier();
+#pragma unroll
+  for (int u = 0; u < 2 * HM; ++u) read_x(x0, x00, u);
+  wait_vmcnt<3 * DW + 3 * DX>();
+  wait_lds_barrier();
+#pragma unroll
+  for (int u = 0; u < 2 * HN; ++u) read_w(w0, w00, u);
+  all_x(x00, 0, 2);
+  __builtin_amdgcn_sched_barrier(0);
+  for (int k = 0; k < steps; k += 2) {
+    // Arrays: operand, step % 2, half.
+    wait_vmcnt<2 * DW + 4 * DX>();
+    wait_lds_barrier();
+    phase(I0{}, I0{}, x0, w0, RW{}, [&](auto u) { read_w(w1, w01, decltype(u)::value); },
+          CW{}, [&](int j) { dma_w(w00, 0, k + 2, j); });
+    wait_vmcnt<3 * DW + 3 * DX>();
+    wait_lds_barrier();
+    phase(I0{}, I1{}, x0, w1, RX{}, [&](auto u) { read_x(x1, x01, decltype(u)::value); },
+          CW{}, [&](int j) { dma_w(w01, 1, k + 2, j); });
+    wait_vmcnt<4 * DW + 2 * DX>();
+    wait_lds_barrier();
+    phase(I1{}, I1{}, x1, w1, RX{}, [&](auto u) { read_x(x0, x10, decltype(u)::value); },
+          CX{}, [&](int j) { dma_x(x01, 1, k + 2, j); });
+    wait_vmcnt<3 * DW + 3 * DX>();
+    wait_lds_barrier();
+    phase(I1{}, I0{}, x1, w0, RW{}, [&](auto u) { read_w(w1, w11, decltype(u)::value); },
+          CX{}, [&](int j) { dma_x(x10, 0, k + 3, j); });
+    wait_vmcnt<2 * DW + 4 * DX>();
+    wait_lds_barrier();
+    phase(I0{}, I1{}, x0, w1, RW{}, [&](auto u) { read_w(w0, w10, decltype(u)::value); },
+          CW{}, [&](int j) { dma_w(w11, 1, k + 3, j); });
+    wait_vmcnt<3 * DW + 3 * DX>();
+    wait_lds_barrier();
+    phase(I0{}, I0{}, x0, w0, RX{}, [&](auto u) { read_x(x1, x11, decltype(u)::value); },
+          CW{}, [&](int j) { dma_w(w10, 0, k + 3, j); });
+    wait_vmcnt<4 * DW + 2 * DX>();
+    wait_lds_barrier();
+    phase(I1{}, I0{}, x1, w0, RX{}, [&](auto u) { read_x(x0, x00, decltype(u)::value); },
+          CX{}, [&](int j) { dma_x(x11, 1, k + 3, j); });
+    wait_vmcnt<3 * DW + 3 * DX>();
+    wait_lds_barrier();
+    phase(I1{}, I1{}, x1, w1, RW{}, [&](auto u) { read_w(w0, w00, decltype(u)::value); },
+          CX{}, [&](int j) { dma_x(x00, 0, k + 4, j); });
+  }
+  settle_mfma();
+  // No DMA may land in LDS that the epilogue (or a later workgroup) uses.
+  wait_vmcnt<0>();
+  wait_lds_barrier();
+
+  // Epilogue: each wave passes its outputs, 32 rows at a time, through its own part of LDS, so that a lane owns W
+  // adjacent columns and a row leaves in whole lines.
+  uint8_t *st;
+  {
+    uint8_t *const a0 = kStageX ? x00 : w00, *const a1 = kStageX ? x01 : w01, *const a2 = kStageX ? x10 : w10,
+                   *const a3 = kStageX ? x11 : w11;
+    st = wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? a2 : wave == 3 ? a3 : wave == 4 ? w00 : wave == 5 ? w01
+         : wave == 6 ? w10 : w11;
+  }
+  const int nw = n0 + wn * NB * 16;  // first column of this wave
+  auto stage = [&](int e) __attribute__((always_inline)) {
+    for_each_index<MB / 2>([&](auto part) __attribute__((always_inline)) {
+      constexpr int E = decltype(part)::value;
+      if (e != E) return;
+      // Each case keeps its code: merged into one, the accumulators would be indexed at run time, in scratch memory.
+      asm volatile("; rows %0" ::"i"(E) : "memory");
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int r = 16 * i + (lane & 15), c = 4 * j + (lane >> 4);  // row, 16-byte chunk of it
+          f32x4 q = acc[2 * E + i][j];
+          asm volatile("" : "+a"(q));
+          *reinterpret_cast<f32x4 *>(st + r * (NB * 64) + ((c ^ (r & 15)) << 4)) = q;
+        }
+      asm volatile("; rows %0 done" ::"i"(E) : "memory");
+    });
+  };
+  // Rows [32 e, 32 e + 32) of the wave in LDS -> memory, W columns per lane. One wave reads what it wrote: no barrier.
+  auto finish = [&](auto width, int e) __attribute__((always_inline)) {
+    constexpr int W = decltype(width)::value;
+    constexpr int LPR = NB * 16 / W, RPI = 64 / LPR;  // lanes per row, rows per instruction
+    constexpr int U = ER / RPI < 4 ? ER / RPI : 4;    // row groups whose residuals are loaded together
+    const int n = nw + (lane % LPR) * W;
+    float bias[W] = {};
+    if (P.bias && n < N) load_cols<DT, W>(P.bias, n, P.bias_f32, bias);
+#pragma unroll 1
+    for (int it = 0; it < ER / RPI; it += U) {
+      float v[U][W], res[U][W] = {};
+      int bs[U], ls[U];
+      bool on[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int m = m0 + wm * MB * 16 + e * ER + (it + u) * RPI + lane / LPR;
+        on[u] = m < M && n < N;
+        bs[u] = static_cast<int>(div31(static_cast<uint32_t>(min(m, M - 1)), P.by_l));
+        ls[u] = m - bs[u] * P.L;
+        if (P.residual && on[u])
+          load_cols<DT, W>(P.residual, bs[u] * P.r_sb + ls[u] * P.r_sl + n, P.residual_f32, res[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int q = 0; q < W / 4; ++q) {
+          const int r = (it + u) * RPI + lane / LPR, c = (lane % LPR) * (W / 4) + q;
+          const f32x4 f = *reinterpret_cast<const f32x4 *>(st + r * (NB * 64) + ((c ^ (r & 15)) << 4));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[u][4 * q + j] = f[j] + bias[4 * q + j];
+        }
+      if (P.act == SELAS_ACT_GELU) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[u][j] = gelu_tanh_fast(v[u][j]);
+      } else if (P.act == SELAS_ACT_SILU) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[u][j] = silu_fast(v[u][j]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!on[u]) continue;
+        if (P.gate) {
+          float g[W];
+          load_cols<DT, W>(P.gate, bs[u] * P.gate_sb + n, P.gate_f32, g);
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[u][j] *= g[j];
+        }
+        if (P.residual) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[u][j] = res[u][j] + v[u][j];
+        }
+        store_cols<DT, W>(P.y, bs[u] * P.y_sb + ls[u] * P.y_sl + n, v[u]);
+      }
+    }
+  };
+  auto finish_columns = [&](int e) __attribute__((always_inline)) {  // no vectors: a lane per column
+#pragma unroll 1
+    for (int r = 0; r < ER; ++r) {
+      const int m = m0 + wm * MB * 16 + e * ER + r;
+      if (m >= M) return;
+      const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l)), l = m - b * P.L;
+#pragma unroll 1
+      for (int i = lane; i < NB * 16 && nw + i < N; i += 64)
+        finish_one<DT>(P, b, l, nw + i, *reinterpret_cast<const float *>(st + r * (NB * 64) + (((i >> 2) ^ (r & 15)) << 4) + (i & 3) * 4));
+    }
+  };
+#pragma unroll 1
+  for (int e = 0; e < MB / 2; ++e) {
+    stage(e);
+    if (!P.vec) finish_columns(e);
+    else if (P.y_f32) finish(std::integral_constant<int, 4>{}, e);
+    else finish(std::integral_constant<int, 8>{}, e);
   }
 }
 
@@ -163,6 +556,26 @@ int check_problem(const selas_raw_linear_problem &p, int64_t i, int dtype) {
   return SELAS_OK;
 }
 
+template <int DT>
+int launch_any(const RawProblem &P, hipStream_t s) {
+  const int64_t tn = cdiv(P.N, kAnyT), tm = cdiv(P.M, kAnyT);
+  if (tm > 65535) return set_error(SELAS_EUNSUPPORTED, "raw_linear: too many rows (%d)", P.M);
+  raw_any_kernel<DT><<<dim3(static_cast<uint32_t>(tn), static_cast<uint32_t>(tm)), dim3(256), 0, s>>>(P);
+  return check_launch("raw_linear");
+}
+
+// Whether rows of p (stride s, batch stride sb, in elements of `size` bytes) take 16-byte accesses at every 8th element.
+bool rows_ok(const void *p, int64_t sb, int64_t s, int size) {
+  return aligned(p, 16) && sb * size % 16 == 0 && s * size % 16 == 0;
+}
+
+bool epilogue_vec(const selas_raw_linear_problem &p) {
+  auto size = [](int dt) { return dt == SELAS_F32 ? 4 : 2; };
+  return p.N % 8 == 0 && rows_ok(p.y, p.y_sb, p.y_sl, size(p.y_dtype)) && (!p.bias || aligned(p.bias, 16)) &&
+         (!p.gate || rows_ok(p.gate, p.gate_sb, 0, size(p.gate_dtype))) &&
+         (!p.residual || rows_ok(p.residual, p.r_sb, p.r_sl, size(p.residual_dtype)));
+}
+
 RawProblem make_problem(const selas_raw_linear_problem &p) {
   RawProblem r{};
   r.x = p.x; r.w = p.w; r.bias = p.bias; r.gate = p.gate; r.residual = p.residual; r.y = p.y;
@@ -174,15 +587,54 @@ RawProblem make_problem(const selas_raw_linear_problem &p) {
   r.act = p.act;
   r.bias_f32 = p.bias_dtype == SELAS_F32; r.gate_f32 = p.gate_dtype == SELAS_F32;
   r.residual_f32 = p.residual_dtype == SELAS_F32; r.y_f32 = p.y_dtype == SELAS_F32;
+  r.vec = epilogue_vec(p);
   return r;
 }
 
+// Whether the tiled kernel's DMA can read the operands: whole 16-byte chunks, and a tile's rows within 31 bits of bytes.
+bool tiled_ok(const selas_raw_linear_problem &p) {
+  if (p.K % 8 || p.K == 0 || !rows_ok(p.x, p.x_sb, p.x_sl, 2) || !rows_ok(p.w, 0, p.ldw, 2)) return false;
+  const int64_t rows = 256, gap = p.x_sb - (p.L - 1) * p.x_sl, crossings = p.B > 1 ? rows / p.L + 1 : 0;
+  if (p.x_sl >= (1ll << 40) || p.x_sb >= (1ll << 40) || p.ldw >= (1ll << 40)) return false;
+  const int64_t span = gap >= 0 || p.B == 1 ? rows * p.x_sl + crossings * gap : p.L * p.x_sl + crossings * p.x_sb;
+  return (span + p.K) * 2 < (1ll << 31) - 4096 && (rows * p.ldw + p.K) * 2 < (1ll << 31) - 4096;
+}
+
+int cu_count() {
+  int dev = 0, n = 0;
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    return 256;
+  return n;
+}
+
+struct TileShape {
+  int tm, tn;
+};
+
 template <int DT>
-int launch_any(const RawProblem &P, hipStream_t s) {
-  const int64_t tn = cdiv(P.N, kAnyT), tm = cdiv(P.M, kAnyT);
-  if (tm > 65535) return set_error(SELAS_EUNSUPPORTED, "raw_linear: too many rows (%d)", P.M);
-  raw_any_kernel<DT><<<dim3(static_cast<uint32_t>(tn), static_cast<uint32_t>(tm)), dim3(256), 0, s>>>(P);
+int launch_tiled(RawBatch &batch, TileShape shape, hipStream_t s) {
+  batch.tiles = 0;
+  for (int i = 0; i < batch.count; ++i) {
+    const RawProblem &P = batch.p[i];
+    batch.tiles_m[i] = static_cast<int>(cdiv(P.M, shape.tm));
+    batch.tiles_n[i] = static_cast<int>(cdiv(P.N, shape.tn));
+    batch.tile0[i] = batch.tiles;
+    if (static_cast<int64_t>(batch.tiles_m[i]) * batch.tiles_n[i] >= (1ll << 30) - batch.tiles)
+      return set_error(SELAS_EUNSUPPORTED, "raw_linear: too many tiles");
+    batch.tiles += batch.tiles_m[i] * batch.tiles_n[i];
+  }
+  batch.per_xcd = static_cast<int>(cdiv(batch.tiles, 8));
+  const dim3 grid(static_cast<uint32_t>(batch.per_xcd * 8)), blk(256);
+  if (shape.tm == 256 && shape.tn == 256) raw_tile_kernel<DT, 2, 2, 8, 8, 1><<<grid, blk, 0, s>>>(batch);
+  else if (shape.tm == 256) raw_tile_kernel<DT, 2, 2, 8, 4, 1><<<grid, blk, 0, s>>>(batch);
+  else raw_tile_kernel<DT, 2, 2, 4, 4, 2><<<grid, blk, 0, s>>>(batch);
   return check_launch("raw_linear");
+}
+
+TileShape pick_tile(const RawBatch &batch) {
+  int64_t wide = 0;
+  for (int i = 0; i < batch.count; ++i) wide += cdiv(batch.p[i].M, 256) * cdiv(batch.p[i].N, 256);
+  return wide >= cu_count() / 2 ? TileShape{256, 256} : TileShape{128, 128};
 }
 
 int check_call(const selas_raw_linear_problem *problems, int64_t count, int dtype) {
@@ -219,11 +671,18 @@ extern "C" int selas_raw_linear(const selas_raw_linear_problem *problems, int64_
   }
   (void)workspace, (void)workspace_bytes;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  RawBatch batch{};
   for (int64_t i = 0; i < count; ++i) {
     const selas_raw_linear_problem &p = problems[i];
     if (p.B * p.L == 0 || p.N == 0) continue;
     const RawProblem P = make_problem(p);
+    if (P.M > 64 && tiled_ok(p)) {
+      batch.p[batch.count++] = P;
+      continue;
+    }
     if (int e = dtype == SELAS_BF16 ? launch_any<SELAS_BF16>(P, s) : launch_any<SELAS_F16>(P, s)) return e;
   }
-  return ok();
+  if (batch.count == 0) return ok();
+  const TileShape shape = pick_tile(batch);
+  return dtype == SELAS_BF16 ? launch_tiled<SELAS_BF16>(batch, shape, s) : launch_tiled<SELAS_F16>(batch, shape, s);
 }
