@@ -19,7 +19,10 @@ struct RawProblem {
   FastDiv by_l;
   int act;
   bool bias_f32, gate_f32, residual_f32, y_f32;
-  bool vec;  // N is a multiple of 8 and bias, gate, residual and y take 16-byte accesses at every 8th column
+  // N is a multiple of 8, bias, gate, residual and y take 16-byte accesses at every 8th column, and the rows of y and
+  // of the residual are equally spaced over the batches, a tile of them within 31 bits of bytes.
+  bool vec;
+  bool one_gate;  // one gate row for all batches
 };
 
 // v_mfma_f32_16x16x32 of two 16-bit fragments: D(16x16) += A(16x32) B(32x16). Lane l supplies A[l % 16][8 (l / 16) ..
@@ -220,22 +223,6 @@ __device__ __forceinline__ void load_cols(const void *p, int64_t i, bool f32, fl
   }
 }
 
-// W == 4: fp32 outputs; W == 8: 16-bit ones.
-template <int DT, int W>
-__device__ __forceinline__ void store_cols(void *y, int64_t i, const float (&v)[W]) {
-  if constexpr (W == 4) {
-    *reinterpret_cast<float4 *>(static_cast<float *>(y) + i) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (DT == SELAS_BF16) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-      else w[j] = f16_bits_rne(v[2 * j]) | (static_cast<uint32_t>(f16_bits_rne(v[2 * j + 1])) << 16);
-    }
-    *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(y) + i) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
 // 4 waves (WM x WN), each with MB x NB blocks of 16 x 16 outputs: tiles of TM rows of x by TN rows of w, K in steps of 64.
 //
 // LDS holds two steps, each operand in halves: half h of x is the first or second half of every wave's rows. A step runs
@@ -247,7 +234,7 @@ __device__ __forceinline__ void store_cols(void *y, int64_t i, const float (&v)[
 //   any more), and multiplies.
 // A half is read 7 phases after its DMA was issued, so 6 newer halves' loads may be pending at each wait. Past the end
 // of K the loads are out of range: they bring zeros and no traffic, and the counts stay the same.
-template <int DT, int WM, int WN, int MB, int NB, int OCC>
+template <int DT, int WM, int WN, int MB, int NB, int OCC, bool TAIL>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch batch) {
   constexpr int TM = WM * MB * 16, TN = WN * NB * 16, HM = MB / 2, HN = NB / 2, NW = WM * WN;
   constexpr int XB = TM / 2 * 128, WB = TN / 2 * 128;      // bytes of one half of x and of w
@@ -288,9 +275,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
   const int b0 = static_cast<int>(div31(static_cast<uint32_t>(m0), P.by_l)), l0 = m0 - b0 * P.L;
   int64_t x_base = b0 * P.x_sb + l0 * P.x_sl;
   if (l0 + min(TM, M - m0) > P.L) x_base = min(x_base, (b0 + 1) * P.x_sb);
-  const __amdgpu_buffer_rsrc_t xr = make_rsrc(static_cast<const uint16_t *>(P.x) + x_base, 0x7fffffffu);
-  const __amdgpu_buffer_rsrc_t wr =
-      make_rsrc(static_cast<const uint16_t *>(P.w) + static_cast<int64_t>(n0) * P.ldw, 0x7fffffffu);
+  const uint16_t *const xb = static_cast<const uint16_t *>(P.x) + x_base;
+  const uint16_t *const wb = static_cast<const uint16_t *>(P.w) + static_cast<int64_t>(n0) * P.ldw;
   constexpr uint32_t kOut = 0x80000000u;  // past every range
 
   // DMA j of a half writes its LDS rows 8 j .. 8 j + 7: lane i row 8 j + i / 8, physical chunk i % 8, which holds logical
@@ -314,13 +300,20 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
       wo[h][j] = n0 + r < N ? static_cast<uint32_t>(r * P.ldw * 2) + 16 * c : kOut;
     }
   }
-  // The columns of K that this lane's chunks of even and odd DMAs start at.
+  // Steps past the end of K load through an empty range. A last step of fewer than 64 columns (TAIL) compares, per lane,
+  // the column that its chunks of even and odd DMAs start at.
   const int kc[2] = {8 * static_cast<int>((lane & 7) ^ (lane >> 4)), 8 * static_cast<int>((lane & 7) ^ (4 + (lane >> 4)))};
+  auto load_step = [&](__amdgpu_buffer_rsrc_t r, uint8_t *dst, uint32_t off, int par, int step) __attribute__((always_inline)) {
+    if constexpr (TAIL) off = kc[par] + 64 * step < K ? off : kOut;
+    load_lds16(r, dst, off, 128u * step);
+  };
   auto dma_x = [&](uint8_t *dst, int h, int step, int j) __attribute__((always_inline)) {
-    load_lds16(xr, dst + (wave * DX + j) * 1024, kc[(wave * DX + j) & 1] + 64 * step < K ? xo[h][j] : kOut, 128u * step);
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(xb, TAIL || 64 * step < K ? 0x7fffffffu : 0u);
+    load_step(r, dst + (wave * DX + j) * 1024, xo[h][j], (wave * DX + j) & 1, step);
   };
   auto dma_w = [&](uint8_t *dst, int h, int step, int j) __attribute__((always_inline)) {
-    load_lds16(wr, dst + (wave * DW + j) * 1024, kc[(wave * DW + j) & 1] + 64 * step < K ? wo[h][j] : kOut, 128u * step);
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(wb, TAIL || 64 * step < K ? 0x7fffffffu : 0u);
+    load_step(r, dst + (wave * DW + j) * 1024, wo[h][j], (wave * DW + j) & 1, step);
   };
 
   // Fragment i (16 rows) of k half s: row 16 i + lane % 16 of the wave's rows, chunk 4 s + lane / 16.
@@ -340,14 +333,16 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
   auto phase = [&](auto hx, auto hw, const uint4 (&xf)[HM][2], const uint4 (&wf)[HN][2], auto reads, auto &&read, auto dmas,
                    auto &&dma) __attribute__((always_inline)) {
     constexpr int HX = decltype(hx)::value, HW = decltype(hw)::value, R = decltype(reads)::value, D = decltype(dmas)::value;
-    constexpr int F = HM * HN * 2, PER = (R + D + F - 1) / F;
+    constexpr int F = HM * HN * 2, SPAN = F * 7 / 8;
     for_each_index<F>([&](auto index) __attribute__((always_inline)) {
       constexpr int q = decltype(index)::value, s = q / (HM * HN), i = q / HN % HM, j = q % HN;
       mfma16_inplace<DT>(wf[j][s], xf[i][s], acc[HX * HM + i][HW * HN + j]);
-      for_each_index<PER>([&](auto slot) __attribute__((always_inline)) {
-        constexpr int u = q * PER + decltype(slot)::value;
-        if constexpr (u < R) read(std::integral_constant<int, u>{});
-        else if constexpr (u < R + D) dma(u - R);
+      for_each_index<R>([&](auto slot) __attribute__((always_inline)) {
+        if constexpr (decltype(slot)::value * SPAN / R == q) read(slot);
+      });
+      for_each_index<D>([&](auto slot) __attribute__((always_inline)) {
+        constexpr int u = decltype(slot)::value;
+        if constexpr (((2 * u + 1) * F / (2 * D)) == q) dma(u);
       });
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -377,50 +372,39 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
   all_x(x00, 0, 0); all_w(w00, 0, 0); all_w(w01, 1, 0); all_x(x01, 1, 0);
   all_x(x10, 0, 1); all_w(w11, 1, 1); all_w(w10, 0, 1); all_x(x11, 1, 1);
   __builtin_amdgcn_sched_barrier(0);
-  wait_vmcnt<4 * DW + 3 * DX>();
-  wait_lds_barrier();
-#pragma unroll
-  for (int u = 0; u < 2 * HM; ++u) read_x(x0, x00, u);
   wait_vmcnt<3 * DW + 3 * DX>();
   wait_lds_barrier();
 #pragma unroll
+  for (int u = 0; u < 2 * HM; ++u) read_x(x0, x00, u);
+#pragma unroll
   for (int u = 0; u < 2 * HN; ++u) read_w(w0, w00, u);
-  all_x(x00, 0, 2);
   __builtin_amdgcn_sched_barrier(0);
   for (int k = 0; k < steps; k += 2) {
     // Arrays: operand, step % 2, half.
-    wait_vmcnt<2 * DW + 4 * DX>();
+    wait_vmcnt<2 * DW + 2 * DX>();
     wait_lds_barrier();
     phase(I0{}, I0{}, x0, w0, RW{}, [&](auto u) { read_w(w1, w01, decltype(u)::value); },
-          CW{}, [&](int j) { dma_w(w00, 0, k + 2, j); });
-    wait_vmcnt<3 * DW + 3 * DX>();
-    wait_lds_barrier();
+          CX{}, [&](int j) { dma_x(x00, 0, k + 2, j); });
     phase(I0{}, I1{}, x0, w1, RX{}, [&](auto u) { read_x(x1, x01, decltype(u)::value); },
-          CW{}, [&](int j) { dma_w(w01, 1, k + 2, j); });
-    wait_vmcnt<4 * DW + 2 * DX>();
+          CW{}, [&](int j) { dma_w(w00, 0, k + 2, j); });
+    wait_vmcnt<2 * DW + 2 * DX>();
     wait_lds_barrier();
     phase(I1{}, I1{}, x1, w1, RX{}, [&](auto u) { read_x(x0, x10, decltype(u)::value); },
-          CX{}, [&](int j) { dma_x(x01, 1, k + 2, j); });
-    wait_vmcnt<3 * DW + 3 * DX>();
-    wait_lds_barrier();
+          CW{}, [&](int j) { dma_w(w01, 1, k + 2, j); });
     phase(I1{}, I0{}, x1, w0, RW{}, [&](auto u) { read_w(w1, w11, decltype(u)::value); },
-          CX{}, [&](int j) { dma_x(x10, 0, k + 3, j); });
-    wait_vmcnt<2 * DW + 4 * DX>();
+          CX{}, [&](int j) { dma_x(x01, 1, k + 2, j); });
+    wait_vmcnt<2 * DW + 2 * DX>();
     wait_lds_barrier();
     phase(I0{}, I1{}, x0, w1, RW{}, [&](auto u) { read_w(w0, w10, decltype(u)::value); },
-          CW{}, [&](int j) { dma_w(w11, 1, k + 3, j); });
-    wait_vmcnt<3 * DW + 3 * DX>();
-    wait_lds_barrier();
+          CX{}, [&](int j) { dma_x(x10, 0, k + 3, j); });
     phase(I0{}, I0{}, x0, w0, RX{}, [&](auto u) { read_x(x1, x11, decltype(u)::value); },
-          CW{}, [&](int j) { dma_w(w10, 0, k + 3, j); });
-    wait_vmcnt<4 * DW + 2 * DX>();
+          CW{}, [&](int j) { dma_w(w11, 1, k + 3, j); });
+    wait_vmcnt<2 * DW + 2 * DX>();
     wait_lds_barrier();
     phase(I1{}, I0{}, x1, w0, RX{}, [&](auto u) { read_x(x0, x00, decltype(u)::value); },
-          CX{}, [&](int j) { dma_x(x11, 1, k + 3, j); });
-    wait_vmcnt<3 * DW + 3 * DX>();
-    wait_lds_barrier();
+          CW{}, [&](int j) { dma_w(w10, 0, k + 3, j); });
     phase(I1{}, I1{}, x1, w1, RW{}, [&](auto u) { read_w(w0, w00, decltype(u)::value); },
-          CX{}, [&](int j) { dma_x(x00, 0, k + 4, j); });
+          CX{}, [&](int j) { dma_x(x11, 1, k + 3, j); });
   }
   settle_mfma();
   // No DMA may land in LDS that the epilogue (or a later workgroup) uses.
@@ -455,62 +439,116 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
       asm volatile("; rows %0 done" ::"i"(E) : "memory");
     });
   };
-  // Rows [32 e, 32 e + 32) of the wave in LDS -> memory, W columns per lane. One wave reads what it wrote: no barrier.
-  auto finish = [&](auto width, int e) __attribute__((always_inline)) {
+  // The wave's outputs by way of LDS, 32 rows (a part) at a time, W columns per lane. One wave reads what it wrote: no
+  // barrier. Addresses are a lane's offset plus a scalar for the rows, out of range for rows past M and columns past N.
+  // The residual of a part is loaded while the part before is stored.
+  auto finish = [&](auto width) __attribute__((always_inline)) {
     constexpr int W = decltype(width)::value;
-    constexpr int LPR = NB * 16 / W, RPI = 64 / LPR;  // lanes per row, rows per instruction
-    constexpr int U = ER / RPI < 4 ? ER / RPI : 4;    // row groups whose residuals are loaded together
-    const int n = nw + (lane % LPR) * W;
-    float bias[W] = {};
+    constexpr int LPR = NB * 16 / W, RPI = 64 / LPR, G = ER / RPI;  // lanes per row, rows per instruction, groups of them
+    const int n = nw + (lane % LPR) * W, row = lane / LPR;
+    const int mw = m0 + wm * MB * 16, rows = M - mw;  // first row of the wave, rows there are
+    const int ye = P.y_f32 ? 4 : 2, re = P.residual_f32 ? 4 : 2;
+    const __amdgpu_buffer_rsrc_t yr =
+        make_rsrc(static_cast<uint8_t *>(P.y) + (mw * P.y_sl + nw) * ye, 0x7fffffffu);
+    const __amdgpu_buffer_rsrc_t rr =
+        make_rsrc(static_cast<const uint8_t *>(P.residual) + (mw * P.r_sl + nw) * re, 0x7fffffffu);
+    const uint32_t ys = static_cast<uint32_t>(P.y_sl) * ye, rs = static_cast<uint32_t>(P.r_sl) * re;
+    const uint32_t yv = row * ys + (n - nw) * ye, rv = row * rs + (n - nw) * re;
+    float bias[W] = {}, gate[W];
     if (P.bias && n < N) load_cols<DT, W>(P.bias, n, P.bias_f32, bias);
-#pragma unroll 1
-    for (int it = 0; it < ER / RPI; it += U) {
-      float v[U][W], res[U][W] = {};
-      int bs[U], ls[U];
-      bool on[U];
+    if (P.gate && P.one_gate && n < N) load_cols<DT, W>(P.gate, n, P.gate_f32, gate);
+    uint4 res[G][W / 4] = {};
+    auto load_res = [&](int e) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int m = m0 + wm * MB * 16 + e * ER + (it + u) * RPI + lane / LPR;
-        on[u] = m < M && n < N;
-        bs[u] = static_cast<int>(div31(static_cast<uint32_t>(min(m, M - 1)), P.by_l));
-        ls[u] = m - bs[u] * P.L;
-        if (P.residual && on[u])
-          load_cols<DT, W>(P.residual, bs[u] * P.r_sb + ls[u] * P.r_sl + n, P.residual_f32, res[u]);
+      for (int g = 0; g < G; ++g) {
+        const uint32_t at = e * ER + g * RPI + row < rows && n < N ? rv : kOut, so = (e * ER + g * RPI) * rs;
+        if (P.residual_f32) {
+#pragma unroll
+          for (int q = 0; q < W / 4; ++q) res[g][q] = load_b128(rr, at + 16 * q, so);
+        } else if constexpr (W == 8) {
+          res[g][0] = load_b128(rr, at, so);
+        } else {
+          const auto u = __builtin_amdgcn_raw_buffer_load_b64(rr, at, so, 0);
+          res[g][0].x = u[0], res[g][0].y = u[1];
+        }
       }
+    };
+    if (P.residual) load_res(0);
+#pragma unroll 1
+    for (int e = 0; e < MB / 2; ++e) {
+      stage(e);
+      float v[G][W];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int q = 0; q < W / 4; ++q) {
-          const int r = (it + u) * RPI + lane / LPR, c = (lane % LPR) * (W / 4) + q;
+          const int r = g * RPI + row, c = (lane % LPR) * (W / 4) + q;
           const f32x4 f = *reinterpret_cast<const f32x4 *>(st + r * (NB * 64) + ((c ^ (r & 15)) << 4));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[u][4 * q + j] = f[j] + bias[4 * q + j];
+          for (int j = 0; j < 4; ++j) v[g][4 * q + j] = f[j] + bias[4 * q + j];
         }
       if (P.act == SELAS_ACT_GELU) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int j = 0; j < W; ++j) v[u][j] = gelu_tanh_fast(v[u][j]);
+          for (int j = 0; j < W; ++j) v[g][j] = gelu_tanh_fast(v[g][j]);
       } else if (P.act == SELAS_ACT_SILU) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int j = 0; j < W; ++j) v[u][j] = silu_fast(v[u][j]);
+          for (int j = 0; j < W; ++j) v[g][j] = silu_fast(v[g][j]);
+      }
+      if (P.gate) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          if (!P.one_gate) {
+            const int m = min(mw + e * ER + g * RPI + row, M - 1);
+            const int64_t at = static_cast<int64_t>(div31(static_cast<uint32_t>(m), P.by_l)) * P.gate_sb + n;
+            if (n < N) load_cols<DT, W>(P.gate, at, P.gate_f32, gate);
+          }
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[g][j] *= gate[j];
+        }
+      }
+      if (P.residual) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          if (P.residual_f32) {
+#pragma unroll
+            for (int q = 0; q < W / 4; ++q) {
+              const uint4 u = res[g][q];
+              v[g][4 * q] = __uint_as_float(u.x) + v[g][4 * q];
+              v[g][4 * q + 1] = __uint_as_float(u.y) + v[g][4 * q + 1];
+              v[g][4 * q + 2] = __uint_as_float(u.z) + v[g][4 * q + 2];
+              v[g][4 * q + 3] = __uint_as_float(u.w) + v[g][4 * q + 3];
+            }
+          } else {
+            const uint32_t w[4] = {res[g][0].x, res[g][0].y, res[g][0].z, res[g][0].w};
+#pragma unroll
+            for (int t = 0; t < W / 2; ++t) {
+              if constexpr (DT == SELAS_BF16) {
+                v[g][2 * t] = __uint_as_float(w[t] << 16) + v[g][2 * t];
+                v[g][2 * t + 1] = __uint_as_float(w[t] & 0xffff0000u) + v[g][2 * t + 1];
+              } else {
+                v[g][2 * t] = f16_bits_to_f32(w[t] & 0xffffu) + v[g][2 * t];
+                v[g][2 * t + 1] = f16_bits_to_f32(w[t] >> 16) + v[g][2 * t + 1];
+              }
+            }
+          }
+        }
+        if (e + 1 < MB / 2) load_res(e + 1);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!on[u]) continue;
-        if (P.gate) {
-          float g[W];
-          load_cols<DT, W>(P.gate, bs[u] * P.gate_sb + n, P.gate_f32, g);
+      for (int g = 0; g < G; ++g) {
+        const uint32_t at = e * ER + g * RPI + row < rows && n < N ? yv : kOut, so = (e * ER + g * RPI) * ys;
+        uint32_t w[4];
 #pragma unroll
-          for (int j = 0; j < W; ++j) v[u][j] *= g[j];
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (W == 4) w[j] = __float_as_uint(v[g][j]);
+          else if constexpr (DT == SELAS_BF16) w[j] = pack_bf16x2(v[g][2 * j], v[g][2 * j + 1]);
+          else w[j] = f16_bits_rne(v[g][2 * j]) | (static_cast<uint32_t>(f16_bits_rne(v[g][2 * j + 1])) << 16);
         }
-        if (P.residual) {
-#pragma unroll
-          for (int j = 0; j < W; ++j) v[u][j] = res[u][j] + v[u][j];
-        }
-        store_cols<DT, W>(P.y, bs[u] * P.y_sb + ls[u] * P.y_sl + n, v[u]);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{w[0], w[1], w[2], w[3]}, yr, at, so, 0);
       }
     }
   };
@@ -525,12 +563,16 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
         finish_one<DT>(P, b, l, nw + i, *reinterpret_cast<const float *>(st + r * (NB * 64) + (((i >> 2) ^ (r & 15)) << 4) + (i & 3) * 4));
     }
   };
+  if (P.vec && P.y_f32) {
+    finish(std::integral_constant<int, 4>{});
+  } else if (P.vec) {
+    finish(std::integral_constant<int, 8>{});
+  } else {
 #pragma unroll 1
-  for (int e = 0; e < MB / 2; ++e) {
-    stage(e);
-    if (!P.vec) finish_columns(e);
-    else if (P.y_f32) finish(std::integral_constant<int, 4>{}, e);
-    else finish(std::integral_constant<int, 8>{}, e);
+    for (int e = 0; e < MB / 2; ++e) {
+      stage(e);
+      finish_columns(e);
+    }
   }
 }
 
@@ -571,9 +613,10 @@ bool rows_ok(const void *p, int64_t sb, int64_t s, int size) {
 
 bool epilogue_vec(const selas_raw_linear_problem &p) {
   auto size = [](int dt) { return dt == SELAS_F32 ? 4 : 2; };
-  return p.N % 8 == 0 && rows_ok(p.y, p.y_sb, p.y_sl, size(p.y_dtype)) && (!p.bias || aligned(p.bias, 16)) &&
-         (!p.gate || rows_ok(p.gate, p.gate_sb, 0, size(p.gate_dtype))) &&
-         (!p.residual || rows_ok(p.residual, p.r_sb, p.r_sl, size(p.residual_dtype)));
+  auto even = [&](int64_t sb, int64_t sl) { return (p.B == 1 || sb == p.L * sl) && sl < (1ll << 20); };
+  return p.N % 8 == 0 && rows_ok(p.y, p.y_sb, p.y_sl, size(p.y_dtype)) && even(p.y_sb, p.y_sl) &&
+         (!p.bias || aligned(p.bias, 16)) && (!p.gate || rows_ok(p.gate, p.gate_sb, 0, size(p.gate_dtype))) &&
+         (!p.residual || (rows_ok(p.residual, p.r_sb, p.r_sl, size(p.residual_dtype)) && even(p.r_sb, p.r_sl)));
 }
 
 RawProblem make_problem(const selas_raw_linear_problem &p) {
@@ -588,6 +631,7 @@ RawProblem make_problem(const selas_raw_linear_problem &p) {
   r.bias_f32 = p.bias_dtype == SELAS_F32; r.gate_f32 = p.gate_dtype == SELAS_F32;
   r.residual_f32 = p.residual_dtype == SELAS_F32; r.y_f32 = p.y_dtype == SELAS_F32;
   r.vec = epilogue_vec(p);
+  r.one_gate = p.B == 1 || p.gate_sb == 0;
   return r;
 }
 
@@ -625,9 +669,16 @@ int launch_tiled(RawBatch &batch, TileShape shape, hipStream_t s) {
   }
   batch.per_xcd = static_cast<int>(cdiv(batch.tiles, 8));
   const dim3 grid(static_cast<uint32_t>(batch.per_xcd * 8)), blk(256);
-  if (shape.tm == 256 && shape.tn == 256) raw_tile_kernel<DT, 2, 2, 8, 8, 1><<<grid, blk, 0, s>>>(batch);
-  else if (shape.tm == 256) raw_tile_kernel<DT, 2, 2, 8, 4, 1><<<grid, blk, 0, s>>>(batch);
-  else raw_tile_kernel<DT, 2, 2, 4, 4, 2><<<grid, blk, 0, s>>>(batch);
+  bool tail = false;
+  for (int i = 0; i < batch.count; ++i) tail = tail || batch.p[i].K % 64;
+#define SELAS_TILE(MB, NB, OCC)                                                      \
+  do {                                                                               \
+    if (tail) raw_tile_kernel<DT, 2, 2, MB, NB, OCC, true><<<grid, blk, 0, s>>>(batch); \
+    else raw_tile_kernel<DT, 2, 2, MB, NB, OCC, false><<<grid, blk, 0, s>>>(batch);     \
+  } while (0)
+  if (shape.tm == 256) SELAS_TILE(8, 8, 1);
+  else SELAS_TILE(4, 4, 2);
+#undef SELAS_TILE
   return check_launch("raw_linear");
 }
 
