@@ -81,12 +81,133 @@ __device__ __forceinline__ void finish_one(const RawProblem &P, int b, int l, in
   else store_f<DT>(P.y, o, v);
 }
 
+// f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>): a loop over register arrays that cannot stay rolled.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void for_each_index(F &&f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    for_each_index<N, I + 1>(f);
+  }
+}
+
+// W consecutive columns of a row as fp32, from 16-byte aligned addresses (8-byte for four 16-bit ones).
+template <int DT, int W>
+__device__ __forceinline__ void load_cols(const void *p, int64_t i, bool f32, float (&v)[W]) {
+  if (f32) {
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const float4 u = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + j);
+      v[j] = u.x; v[j + 1] = u.y; v[j + 2] = u.z; v[j + 3] = u.w;
+    }
+  } else {
+    uint32_t w[W / 2];
+    const uint16_t *q = static_cast<const uint16_t *>(p) + i;
+    if constexpr (W == 8) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(q);
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+      const uint2 u = *reinterpret_cast<const uint2 *>(q);
+      w[0] = u.x; w[1] = u.y;
+    }
+#pragma unroll
+    for (int t = 0; t < W / 2; ++t) {
+      if constexpr (DT == SELAS_BF16) {
+        v[2 * t] = __uint_as_float(w[t] << 16);
+        v[2 * t + 1] = __uint_as_float(w[t] & 0xffff0000u);
+      } else {
+        v[2 * t] = f16_bits_to_f32(w[t] & 0xffffu);
+        v[2 * t + 1] = f16_bits_to_f32(w[t] >> 16);
+      }
+    }
+  }
+}
+
+// Four outputs of row (b, l) from column n on, from their sums.
+template <int DT>
+__device__ __forceinline__ void finish_four(const RawProblem &P, int b, int l, int n, f32x4 s) {
+  if (!P.vec) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < P.N) finish_one<DT>(P, b, l, n + j, s[j]);
+    return;
+  }
+  if (n >= P.N) return;
+  float v[4] = {s[0], s[1], s[2], s[3]}, u[4];
+  if (P.bias) {
+    load_cols<DT, 4>(P.bias, n, P.bias_f32, u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += u[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = activate(v[j], P.act);
+  if (P.gate) {
+    load_cols<DT, 4>(P.gate, b * P.gate_sb + n, P.gate_f32, u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= u[j];
+  }
+  if (P.residual) {
+    load_cols<DT, 4>(P.residual, b * P.r_sb + l * P.r_sl + n, P.residual_f32, u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = u[j] + v[j];
+  }
+  const int64_t o = b * P.y_sb + l * P.y_sl + n;
+  if (P.y_f32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(P.y) + o) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint2 w;
+    if constexpr (DT == SELAS_BF16) {
+      w.x = pack_bf16x2(v[0], v[1]);
+      w.y = pack_bf16x2(v[2], v[3]);
+    } else {
+      w.x = f16_bits_rne(v[0]) | (static_cast<uint32_t>(f16_bits_rne(v[1])) << 16);
+      w.y = f16_bits_rne(v[2]) | (static_cast<uint32_t>(f16_bits_rne(v[3])) << 16);
+    }
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(P.y) + o) = w;
+  }
+}
+
+// The problem whose outputs are the plain fp32 sums, [M, N] contiguous at `part`: one range of K of a split launch.
+__device__ __forceinline__ void to_partial(RawProblem &P, float *part) {
+  P.bias = P.gate = P.residual = nullptr;
+  P.act = SELAS_ACT_NONE;
+  P.y = part;
+  P.y_sl = P.N;
+  P.y_sb = static_cast<int64_t>(P.L) * P.N;
+  P.y_f32 = true;
+  P.vec = P.N % 8 == 0;
+}
+
+// y = epilogue(sum over the K ranges, in their order): four columns per thread.
+template <int DT>
+__global__ __launch_bounds__(256) void raw_merge_kernel(RawProblem P, const float *__restrict__ part, int split) {
+  const int groups = (P.N + 3) / 4;
+  const int64_t size = static_cast<int64_t>(P.M) * P.N;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= static_cast<int64_t>(P.M) * groups) return;
+  const int m = static_cast<int>(i / groups), n = static_cast<int>(i - static_cast<int64_t>(m) * groups) * 4;
+  const float *src = part + static_cast<int64_t>(m) * P.N + n;
+  f32x4 v = {};
+  if (P.N % 4 == 0) {
+    for (int s = 0; s < split; ++s) v += *reinterpret_cast<const f32x4 *>(src + s * size);
+  } else {
+    for (int s = 0; s < split; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < P.N) v[j] += src[s * size + j];
+  }
+  const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l));
+  finish_four<DT>(P, b, m - b * P.L, n, v);
+}
+
 // Eight elements of a row from k on, zeros from K on. The address need not be aligned: global loads may start at any
 // element.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
+__device__ __forceinline__ uint4 load_any(const uint16_t *p) {
+  return __builtin_bit_cast(uint4, static_cast<u32x4>(*reinterpret_cast<const u32x4_any *>(p)));
+}
 __device__ __forceinline__ uint4 load_chunk(const uint16_t *row, int k, int K) {
-  if (k + 8 <= K) return __builtin_bit_cast(uint4, static_cast<u32x4>(*reinterpret_cast<const u32x4_any *>(row + k)));
+  if (k + 8 <= K) return load_any(row + k);
   uint32_t w[4] = {};
 #pragma unroll
   for (int j = 0; j < 8; ++j)
@@ -168,60 +289,205 @@ __global__ __launch_bounds__(256) void raw_any_kernel(RawProblem P) {
   }
 }
 
+// ------------------------------------------------------------------ few rows
+//
+// One operand of at most 64 rows (x of a modulation or an embedding; the weight of the final layer): HBM-bound by the
+// other, the streamed one. A workgroup takes NT x 16 of its rows; its 8 waves share K in ranges, each lane loading 16
+// bytes of row lane % 16 straight into the fragments of v_mfma_f32_16x16x32 (two loads cover a 128-byte line), and the
+// few rows' fragments from the caches. The waves' sums are added in LDS, in wave order.
+// SWAP: x is the streamed operand.
+constexpr int kFewWaves = 8;
+
+// The epilogue of the kernels for few rows: the waves' sums red[wave][few row][streamed row] are added in wave order, a
+// thread per four adjacent columns n of a row m.
+template <int DT, int NT, int MT, bool SWAP, int WAVES>
+__device__ __forceinline__ void finish_few(const RawProblem &P, int r0, const float *red) {
+  constexpr int BIG = NT * 16, FEW = MT * 16, LD = BIG + 4;
+  constexpr int ROWS = SWAP ? BIG : FEW, COLS = SWAP ? FEW : BIG;
+  for (int i = threadIdx.x; i < ROWS * COLS / 4; i += 64 * WAVES) {
+    const int rm = i / (COLS / 4), cn = i % (COLS / 4) * 4;
+    const int m = (SWAP ? r0 : 0) + rm, n = (SWAP ? 0 : r0) + cn;
+    if (m >= P.M || n >= P.N) continue;
+    f32x4 v = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float *p = red + w * FEW * LD;
+      if constexpr (SWAP) v += f32x4{p[cn * LD + rm], p[(cn + 1) * LD + rm], p[(cn + 2) * LD + rm], p[(cn + 3) * LD + rm]};
+      else v += *reinterpret_cast<const f32x4 *>(p + rm * LD + cn);
+    }
+    const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l));
+    finish_four<DT>(P, b, m - b * P.L, n, v);
+  }
+}
+
+template <int DT, int NT, int MT, bool SWAP>
+__global__ __launch_bounds__(64 * kFewWaves) void raw_few_kernel(RawProblem P, float *part, int split) {
+  constexpr int BIG = NT * 16, FEW = MT * 16, LD = BIG + 4, U = 4;
+  __shared__ float red[kFewWaves][FEW][LD];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int r0 = blockIdx.x * BIG, c = lane & 15, g = lane >> 4;
+  // Steps of 32 columns, dealt in contiguous ranges to the launch's splits and to the waves.
+  const int steps = (P.K + 31) / 32, ways = split * kFewWaves, way = blockIdx.y * kFewWaves + wave;
+  const int s0 = static_cast<int>(static_cast<int64_t>(steps) * way / ways);
+  const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (way + 1) / ways);
+  auto x_row = [&](int m) {
+    m = min(m, P.M - 1);
+    const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l));
+    return static_cast<const uint16_t *>(P.x) + b * P.x_sb + (m - b * P.L) * P.x_sl;
+  };
+  auto w_row = [&](int n) { return static_cast<const uint16_t *>(P.w) + min(n, P.N - 1) * P.ldw; };
+  const uint16_t *big[NT], *few[MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) big[i] = (SWAP ? x_row(r0 + 16 * i + c) : w_row(r0 + 16 * i + c)) + 8 * g;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) few[j] = (SWAP ? w_row(16 * j + c) : x_row(16 * j + c)) + 8 * g;
+  f32x4 acc[NT][MT] = {};
+  int s = s0;
+  for (; s + U <= s1 && 32 * (s + U) <= P.K; s += U) {  // no column of these steps is past K
+    uint4 a[U][NT], b[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) a[u][i] = load_any(big[i] + 32 * (s + u));
+#pragma unroll
+      for (int j = 0; j < MT; ++j) b[u][j] = load_any(few[j] + 32 * (s + u));
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all loads ahead of the products: the compiler would pair them up again
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = mfma16<DT>(a[u][i], b[u][j], acc[i][j]);
+  }
+  for (; s < s1; ++s) {
+    uint4 a[NT], b[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) a[i] = load_chunk(big[i], 32 * s, P.K - 8 * g);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) b[j] = load_chunk(few[j], 32 * s, P.K - 8 * g);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[i][j] = mfma16<DT>(a[i], b[j], acc[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+      *reinterpret_cast<f32x4 *>(&red[wave][16 * j + c][16 * i + 4 * g]) = acc[i][j];
+  __syncthreads();
+  if (split > 1) to_partial(P, part + static_cast<int64_t>(blockIdx.y) * P.M * P.N);
+  finish_few<DT, NT, MT, SWAP, kFewWaves>(P, r0, &red[0][0][0]);
+}
+
+// The same for operands whose rows are 16-byte aligned (tiled_ok): the fragments' lane order takes each of 16 adjacent
+// lanes to another row, 64 cache lines looked up per load, which held the loads above at 16 bytes per clock and CU (28 x
+// 18432 x 3072 36 us). Here each wave copies its range of K to LDS of its own by DMA, 8 rows of 128 bytes per
+// instruction, ST steps of 64 columns ahead, and reads the fragments there; no barrier until the sums are added.
+constexpr int kStreamWaves = 4;
+constexpr int stream_stages(int blocks) { return blocks <= 2 ? 4 : blocks == 3 ? 3 : 2; }
+
+template <int DT, int NT, int MT, bool SWAP>
+__global__ __launch_bounds__(64 * kStreamWaves) void raw_stream_kernel(RawProblem P, float *part, int split) {
+  constexpr int NB = NT + MT, ST = stream_stages(NB), SB = NB * 2048;  // blocks of 16 rows, stages, bytes of one
+  constexpr int D = 2 * NB;                                            // DMAs per stage
+  constexpr int BIG = NT * 16, FEW = MT * 16, LD = BIG + 4;
+  constexpr int RED = kStreamWaves * FEW * LD * 4, ALL = kStreamWaves * SB;
+  static_assert(RED <= ALL, "the sums take the place of a stage");
+  __shared__ __attribute__((aligned(1024))) uint8_t st0[ALL], st1[ALL], st2[ST > 2 ? ALL : 16], st3[ST > 3 ? ALL : 16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r0 = blockIdx.x * BIG;
+  const int steps = (P.K + 63) / 64, ways = split * kStreamWaves, way = blockIdx.y * kStreamWaves + wave;
+  const int lo = static_cast<int>(static_cast<int64_t>(steps) * way / ways);
+  const int hi = static_cast<int>(static_cast<int64_t>(steps) * (way + 1) / ways);
+  // Row offsets from the lowest row's address (as in the tiled kernel); rows past the end load zeros.
+  constexpr uint32_t kOut = 0x80000000u;
+  const int xm0 = SWAP ? r0 : 0, b0 = static_cast<int>(div31(static_cast<uint32_t>(xm0), P.by_l)), l0 = xm0 - b0 * P.L;
+  int64_t x_base = b0 * P.x_sb + l0 * P.x_sl;
+  if (l0 + min(SWAP ? BIG : FEW, P.M - xm0) > P.L) x_base = min(x_base, (b0 + 1) * P.x_sb);
+  const int64_t w_base = SWAP ? 0 : r0 * P.ldw;
+  auto x_off = [&](int m) {
+    const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l));
+    return m < P.M ? static_cast<uint32_t>((b * P.x_sb + (m - b * P.L) * P.x_sl - x_base) * 2) : kOut;
+  };
+  auto w_off = [&](int n) { return n < P.N ? static_cast<uint32_t>((n * P.ldw - w_base) * 2) : kOut; };
+  uint32_t off[D];
+  int kc[2];
+#pragma unroll
+  for (int j = 0; j < D; ++j) {
+    const int r = 8 * j + (lane >> 3);  // streamed rows, then the few
+    const int c = (lane & 7) ^ (4 * (j & 1) + (lane >> 4));
+    uint32_t o;
+    if (j < 2 * NT) o = SWAP ? x_off(r0 + r) : w_off(r0 + r);
+    else o = SWAP ? w_off(r - BIG) : x_off(r - BIG);
+    off[j] = o == kOut ? kOut : o + 16 * c;
+    kc[j & 1] = 8 * c;
+  }
+  const uint16_t *const xb = static_cast<const uint16_t *>(P.x) + x_base, *const wb = static_cast<const uint16_t *>(P.w) + w_base;
+  auto issue = [&](uint8_t *stage, int step) __attribute__((always_inline)) {
+    const uint32_t range = step < hi ? 0x7fffffffu : 0u;
+    const __amdgpu_buffer_rsrc_t big = make_rsrc(SWAP ? xb : wb, range), few = make_rsrc(SWAP ? wb : xb, range);
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+      load_lds16(j < 2 * NT ? big : few, stage + wave * SB + j * 1024, kc[j & 1] + 64 * step < P.K ? off[j] : kOut, 128u * step);
+  };
+  f32x4 acc[NT][MT] = {};
+  auto step = [&](uint8_t *stage, int s) __attribute__((always_inline)) {
+    wait_vmcnt<(ST - 1) * D>();
+    uint4 f[NB][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        f[i][h] = *reinterpret_cast<const uint4 *>(stage + wave * SB + i * 2048 + (lane & 15) * 128 +
+                                                   (((4 * h + (lane >> 4)) ^ ((lane & 15) >> 1)) << 4));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next DMA writes there
+    issue(stage, s + ST);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = mfma16<DT>(f[i][h], f[NT + j][h], acc[i][j]);
+  };
+  issue(st0, lo);
+  issue(st1, lo + 1);
+  if constexpr (ST > 2) issue(st2, lo + 2);
+  if constexpr (ST > 3) issue(st3, lo + 3);
+  for (int s = lo; s < hi; s += ST) {  // steps past hi multiply zeros
+    step(st0, s);
+    step(st1, s + 1);
+    if constexpr (ST > 2) step(st2, s + 2);
+    if constexpr (ST > 3) step(st3, s + 3);
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+  float *const red = reinterpret_cast<float *>(st0);
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+      *reinterpret_cast<f32x4 *>(red + (wave * FEW + 16 * j + (lane & 15)) * LD + 16 * i + 4 * (lane >> 4)) = acc[i][j];
+  __syncthreads();
+  if (split > 1) to_partial(P, part + static_cast<int64_t>(blockIdx.y) * P.M * P.N);
+  finish_few<DT, NT, MT, SWAP, kStreamWaves>(P, r0, red);
+}
+
 // ------------------------------------------------------------------ tiled
 
 constexpr int kMaxProblems = SELAS_MAX_BATCHED_LINEARS;
 
-// The problems of one launch. Problem i's tiles are [tile0[i], tile0[i + 1]) of the whole ones followed by its split ones'
-// K ranges: see plan_tiles.
+// The problems of one launch; problem i's tiles are [tile0[i], tile0[i + 1]) of all.
 struct RawBatch {
   RawProblem p[kMaxProblems];
   int tiles_m[kMaxProblems], tiles_n[kMaxProblems], tile0[kMaxProblems];
+  float *part[kMaxProblems];
   int count, tiles, per_xcd;
+  int split;  // K ranges per tile: item r * tiles + t is range r of tile t
 };
 
 __device__ __forceinline__ void wait_lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
-// f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>): a loop over register arrays that cannot stay rolled.
-template <int N, int I = 0, typename F>
-__device__ __forceinline__ void for_each_index(F &&f) {
-  if constexpr (I < N) {
-    f(std::integral_constant<int, I>{});
-    for_each_index<N, I + 1>(f);
-  }
-}
-
-// W consecutive columns of a row as fp32, from 16-byte aligned addresses (8-byte for four 16-bit ones).
-template <int DT, int W>
-__device__ __forceinline__ void load_cols(const void *p, int64_t i, bool f32, float (&v)[W]) {
-  if (f32) {
-#pragma unroll
-    for (int j = 0; j < W; j += 4) {
-      const float4 u = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + j);
-      v[j] = u.x; v[j + 1] = u.y; v[j + 2] = u.z; v[j + 3] = u.w;
-    }
-  } else {
-    uint32_t w[W / 2];
-    const uint16_t *q = static_cast<const uint16_t *>(p) + i;
-    if constexpr (W == 8) {
-      const uint4 u = *reinterpret_cast<const uint4 *>(q);
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2 *>(q);
-      w[0] = u.x; w[1] = u.y;
-    }
-#pragma unroll
-    for (int t = 0; t < W / 2; ++t) {
-      if constexpr (DT == SELAS_BF16) {
-        v[2 * t] = __uint_as_float(w[t] << 16);
-        v[2 * t + 1] = __uint_as_float(w[t] & 0xffff0000u);
-      } else {
-        v[2 * t] = f16_bits_to_f32(w[t] & 0xffffu);
-        v[2 * t + 1] = f16_bits_to_f32(w[t] >> 16);
-      }
-    }
-  }
-}
 
 // 4 waves (WM x WN), each with MB x NB blocks of 16 x 16 outputs: tiles of TM rows of x by TN rows of w, K in steps of 64.
 //
@@ -246,11 +512,13 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
   static_assert((kStageX ? XB : WB) >= EB && (NW <= 4 || XB == WB), "epilogue");
   __shared__ __attribute__((aligned(1024))) uint8_t x00[XB], x01[XB], x10[XB], x11[XB], w00[WB], w01[WB], w10[WB], w11[WB];
 
-  const int t = (blockIdx.x & 7) * batch.per_xcd + (blockIdx.x >> 3);
-  if (t >= batch.tiles) return;
+  const int item = (blockIdx.x & 7) * batch.per_xcd + (blockIdx.x >> 3);
+  if (item >= batch.tiles * batch.split) return;
+  const int range = item / batch.tiles, t = item - range * batch.tiles;
   // The tile's problem (uniform: scalar selects over the kernel arguments).
   RawProblem P = batch.p[0];
   int tile0 = 0, tn = batch.tiles_n[0], tm = batch.tiles_m[0];
+  float *part = batch.part[0];
 #pragma unroll
   for (int i = 1; i < kMaxProblems; ++i)
     if (i < batch.count && t >= batch.tile0[i]) {
@@ -258,7 +526,16 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
       tile0 = batch.tile0[i];
       tn = batch.tiles_n[i];
       tm = batch.tiles_m[i];
+      part = batch.part[i];
     }
+  if (batch.split > 1) {
+    const int steps = (P.K + 63) / 64;
+    const int lo = steps * range / batch.split * 64, hi = steps * (range + 1) / batch.split * 64;
+    P.x = static_cast<const uint16_t *>(P.x) + lo;
+    P.w = static_cast<const uint16_t *>(P.w) + lo;
+    P.K = min(P.K, hi) - lo;
+    to_partial(P, part + static_cast<int64_t>(range) * P.M * P.N);
+  }
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
   int m0, n0;
@@ -651,41 +928,127 @@ int cu_count() {
   return n;
 }
 
-struct TileShape {
-  int tm, tn;
+// How a problem runs. kFew, kStream and kAny are launches of their own; the tiled problems of a call share one.
+enum class Route { kEmpty, kFew, kStream, kTiled, kAny };
+
+struct Plan {
+  Route route[kMaxProblems];
+  int few_split[kMaxProblems];  // K ranges of a kFew or kStream problem
+  int tm, tn, split;            // of the tiled launch
+  int64_t part[kMaxProblems];   // floats of each problem's partial sums
+  int64_t floats;
 };
 
-template <int DT>
-int launch_tiled(RawBatch &batch, TileShape shape, hipStream_t s) {
-  batch.tiles = 0;
-  for (int i = 0; i < batch.count; ++i) {
-    const RawProblem &P = batch.p[i];
-    batch.tiles_m[i] = static_cast<int>(cdiv(P.M, shape.tm));
-    batch.tiles_n[i] = static_cast<int>(cdiv(P.N, shape.tn));
-    batch.tile0[i] = batch.tiles;
-    if (static_cast<int64_t>(batch.tiles_m[i]) * batch.tiles_n[i] >= (1ll << 30) - batch.tiles)
-      return set_error(SELAS_EUNSUPPORTED, "raw_linear: too many tiles");
-    batch.tiles += batch.tiles_m[i] * batch.tiles_n[i];
+constexpr int kFewRows = 64;
+
+Plan make_plan(const selas_raw_linear_problem *problems, int64_t count) {
+  Plan plan{};
+  const int cus = cu_count();
+  int64_t wide = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const selas_raw_linear_problem &p = problems[i];
+    const int64_t M = p.B * p.L;
+    if (M == 0 || p.N == 0) {
+      plan.route[i] = Route::kEmpty;
+    } else if (M <= kFewRows || p.N <= kFewRows) {
+      plan.route[i] = tiled_ok(p) ? Route::kStream : Route::kFew;
+      plan.few_split[i] = 1;
+    } else if (tiled_ok(p)) {
+      plan.route[i] = Route::kTiled;
+      wide += cdiv(M, 256) * cdiv(p.N, 256);
+    } else {
+      plan.route[i] = Route::kAny;
+    }
   }
-  batch.per_xcd = static_cast<int>(cdiv(batch.tiles, 8));
-  const dim3 grid(static_cast<uint32_t>(batch.per_xcd * 8)), blk(256);
-  bool tail = false;
-  for (int i = 0; i < batch.count; ++i) tail = tail || batch.p[i].K % 64;
-#define SELAS_TILE(MB, NB, OCC)                                                      \
-  do {                                                                               \
-    if (tail) raw_tile_kernel<DT, 2, 2, MB, NB, OCC, true><<<grid, blk, 0, s>>>(batch); \
-    else raw_tile_kernel<DT, 2, 2, MB, NB, OCC, false><<<grid, blk, 0, s>>>(batch);     \
-  } while (0)
-  if (shape.tm == 256) SELAS_TILE(8, 8, 1);
-  else SELAS_TILE(4, 4, 2);
-#undef SELAS_TILE
+  plan.tm = plan.tn = wide >= cus / 2 ? 256 : 128;
+  plan.split = 1;
+  for (int64_t i = 0; i < count; ++i) {
+    const int split = plan.route[i] == Route::kFew || plan.route[i] == Route::kStream ? plan.few_split[i] : plan.route[i] == Route::kTiled ? plan.split : 1;
+    plan.part[i] = split > 1 ? split * problems[i].B * problems[i].L * problems[i].N : 0;
+    plan.floats += (plan.part[i] + 3) / 4 * 4;
+  }
+  return plan;
+}
+
+template <int DT>
+int launch_merge(const RawProblem &P, const float *part, int split, hipStream_t s) {
+  const int64_t groups = static_cast<int64_t>(P.M) * ((P.N + 3) / 4);
+  raw_merge_kernel<DT><<<dim3(static_cast<uint32_t>(cdiv(groups, 256))), dim3(256), 0, s>>>(P, part, split);
   return check_launch("raw_linear");
 }
 
-TileShape pick_tile(const RawBatch &batch) {
-  int64_t wide = 0;
-  for (int i = 0; i < batch.count; ++i) wide += cdiv(batch.p[i].M, 256) * cdiv(batch.p[i].N, 256);
-  return wide >= cu_count() / 2 ? TileShape{256, 256} : TileShape{128, 128};
+template <int DT>
+int launch_few(const RawProblem &P, bool stream, float *part, int split, hipStream_t s) {
+  const bool swap = P.M > kFewRows;
+  const int few = swap ? P.N : P.M, big = swap ? P.M : P.N;
+  const int nt = big > 16 * cu_count() * 2 ? 2 : 1, mt = few <= 16 ? 1 : few <= 32 ? 2 : 4;
+  const dim3 grid(static_cast<uint32_t>(cdiv(big, 16 * nt)), static_cast<uint32_t>(split)), blk(64 * kFewWaves), sblk(64 * kStreamWaves);
+#define SELAS_FEW(NT, MT)                                                                       \
+  do {                                                                                          \
+    if (stream && swap) raw_stream_kernel<DT, NT, MT, true><<<grid, sblk, 0, s>>>(P, part, split); \
+    else if (stream) raw_stream_kernel<DT, NT, MT, false><<<grid, sblk, 0, s>>>(P, part, split);   \
+    else if (swap) raw_few_kernel<DT, NT, MT, true><<<grid, blk, 0, s>>>(P, part, split);       \
+    else raw_few_kernel<DT, NT, MT, false><<<grid, blk, 0, s>>>(P, part, split);                \
+  } while (0)
+  if (nt == 2 && mt == 1) SELAS_FEW(2, 1);
+  else if (nt == 2 && mt == 2) SELAS_FEW(2, 2);
+  else if (nt == 2) SELAS_FEW(2, 4);
+  else if (mt == 1) SELAS_FEW(1, 1);
+  else if (mt == 2) SELAS_FEW(1, 2);
+  else SELAS_FEW(1, 4);
+#undef SELAS_FEW
+  if (int e = check_launch("raw_linear")) return e;
+  return split > 1 ? launch_merge<DT>(P, part, split, s) : ok();
+}
+
+template <int DT>
+int launch_tiled(RawBatch &batch, const Plan &plan, hipStream_t s) {
+  batch.tiles = 0;
+  batch.split = plan.split;
+  bool tail = false;
+  for (int i = 0; i < batch.count; ++i) {
+    const RawProblem &P = batch.p[i];
+    batch.tiles_m[i] = static_cast<int>(cdiv(P.M, plan.tm));
+    batch.tiles_n[i] = static_cast<int>(cdiv(P.N, plan.tn));
+    batch.tile0[i] = batch.tiles;
+    if (static_cast<int64_t>(batch.tiles_m[i]) * batch.tiles_n[i] >= (1ll << 24) - batch.tiles)
+      return set_error(SELAS_EUNSUPPORTED, "raw_linear: too many tiles");
+    batch.tiles += batch.tiles_m[i] * batch.tiles_n[i];
+    tail = tail || P.K % 64;
+  }
+  batch.per_xcd = static_cast<int>(cdiv(batch.tiles * batch.split, 8));
+  const dim3 grid(static_cast<uint32_t>(batch.per_xcd * 8)), blk(256);
+#define SELAS_TILE(MB, NB, OCC)                                                         \
+  do {                                                                                  \
+    if (tail) raw_tile_kernel<DT, 2, 2, MB, NB, OCC, true><<<grid, blk, 0, s>>>(batch); \
+    else raw_tile_kernel<DT, 2, 2, MB, NB, OCC, false><<<grid, blk, 0, s>>>(batch);     \
+  } while (0)
+  if (plan.tm == 256) SELAS_TILE(8, 8, 1);
+  else SELAS_TILE(4, 4, 2);
+#undef SELAS_TILE
+  if (int e = check_launch("raw_linear")) return e;
+  if (plan.split > 1)
+    for (int i = 0; i < batch.count; ++i)
+      if (int e = launch_merge<DT>(batch.p[i], batch.part[i], plan.split, s)) return e;
+  return ok();
+}
+
+template <int DT>
+int launch_plan(const selas_raw_linear_problem *problems, int64_t count, const Plan &plan, float *ws, hipStream_t s) {
+  RawBatch batch{};
+  for (int64_t i = 0; i < count; ++i) {
+    if (plan.route[i] == Route::kEmpty) continue;
+    const RawProblem P = make_problem(problems[i]);
+    float *part = plan.part[i] ? ws : nullptr;
+    ws += (plan.part[i] + 3) / 4 * 4;
+    if (plan.route[i] == Route::kTiled) {
+      batch.part[batch.count] = part;
+      batch.p[batch.count++] = P;
+    } else if (int e = plan.route[i] != Route::kAny ? launch_few<DT>(P, plan.route[i] == Route::kStream, part, plan.few_split[i], s) : launch_any<DT>(P, s)) {
+      return e;
+    }
+  }
+  return batch.count ? launch_tiled<DT>(batch, plan, s) : ok();
 }
 
 int check_call(const selas_raw_linear_problem *problems, int64_t count, int dtype) {
@@ -709,6 +1072,7 @@ extern "C" int selas_raw_linear_workspace_bytes(const selas_raw_linear_problem *
   if (!bytes) return set_error(SELAS_EINVAL, "raw_linear: null result");
   *bytes = 0;
   if (int e = check_call(problems, count, dtype)) return e;
+  *bytes = make_plan(problems, count).floats * 4;
   return ok();
 }
 
@@ -720,20 +1084,12 @@ extern "C" int selas_raw_linear(const selas_raw_linear_problem *problems, int64_
     if (p.B * p.L == 0 || p.N == 0) continue;
     if (!p.y || (p.K && (!p.x || !p.w))) return set_error(SELAS_EINVAL, "raw_linear[%lld]: null pointer", (long long)i);
   }
-  (void)workspace, (void)workspace_bytes;
+  const Plan plan = make_plan(problems, count);
+  if (plan.floats && (!workspace || workspace_bytes < plan.floats * 4 || !aligned(workspace, 16)))
+    return set_error(SELAS_EINVAL, "raw_linear: needs a 16-byte aligned workspace of %lld bytes",
+                     (long long)(plan.floats * 4));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  RawBatch batch{};
-  for (int64_t i = 0; i < count; ++i) {
-    const selas_raw_linear_problem &p = problems[i];
-    if (p.B * p.L == 0 || p.N == 0) continue;
-    const RawProblem P = make_problem(p);
-    if (P.M > 64 && tiled_ok(p)) {
-      batch.p[batch.count++] = P;
-      continue;
-    }
-    if (int e = dtype == SELAS_BF16 ? launch_any<SELAS_BF16>(P, s) : launch_any<SELAS_F16>(P, s)) return e;
-  }
-  if (batch.count == 0) return ok();
-  const TileShape shape = pick_tile(batch);
-  return dtype == SELAS_BF16 ? launch_tiled<SELAS_BF16>(batch, shape, s) : launch_tiled<SELAS_F16>(batch, shape, s);
+  float *ws = static_cast<float *>(workspace);
+  return dtype == SELAS_BF16 ? launch_plan<SELAS_BF16>(problems, count, plan, ws, s)
+                             : launch_plan<SELAS_F16>(problems, count, plan, ws, s);
 }
