@@ -5,6 +5,8 @@
 // it in a block: the GELU or SiLU (flux.py:150-151, 194-195) and the gated residual add
 // (flux.py:169-171). The sum, the activation, the gate and the residual stay in fp32 and
 // are rounded once, to the output's type.
+#include <atomic>
+
 #include "common.h"
 
 namespace selas {
@@ -259,6 +261,7 @@ __global__ __launch_bounds__(256) void raw_any_kernel(RawProblem P) {
     for (int i = 0; i < 2; ++i) xs[dst[i]] = xv[i], ws[dst[i]] = wv[i];
     __syncthreads();
     if (k + 64 < P.K) load(k + 64);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       uint4 a[2], b[2];
@@ -921,11 +924,24 @@ bool tiled_ok(const selas_raw_linear_problem &p) {
   return (span + p.K) * 2 < (1ll << 31) - 4096 && (rows * p.ldw + p.K) * 2 < (1ll << 31) - 4096;
 }
 
+// The current device's CU count (asked once per device).
 int cu_count() {
-  int dev = 0, n = 0;
-  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+  constexpr int kDevices = 64;
+  static std::atomic<int> counts[kDevices];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) {
+    (void)hipGetLastError();
     return 256;
-  return n;
+  }
+  const int slot = dev >= 0 && dev < kDevices ? dev : 0;
+  int v = counts[slot].load(std::memory_order_relaxed);
+  if (v > 0) return v;
+  if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) {
+    (void)hipGetLastError();
+    v = 256;
+  }
+  counts[slot].store(v, std::memory_order_relaxed);
+  return v;
 }
 
 // How a problem runs. kFew, kStream and kAny are launches of their own; the tiled problems of a call share one.
@@ -934,36 +950,90 @@ enum class Route { kEmpty, kFew, kStream, kTiled, kAny };
 struct Plan {
   Route route[kMaxProblems];
   int few_split[kMaxProblems];  // K ranges of a kFew or kStream problem
-  int tm, tn, split;            // of the tiled launch
+  int tile, split;              // of the tiled launch
   int64_t part[kMaxProblems];   // floats of each problem's partial sums
   int64_t floats;
 };
 
-constexpr int kFewRows = 64;
+// Few rows: 32 of x (33 to 64 run faster as tiles: 60 x 9216 x 3072 25 us against 29), 64 of the weight (1024 x 64 x
+// 3072 9.6 us against 12).
+constexpr int kFewX = 32, kFewW = 64;
+
+// Streamed rows of 16 per workgroup: two blocks where that still gives every CU two workgroups, for half the loads of the
+// few rows (28 x 18432 x 3072 29.9 us against 34.3), one block otherwise (28 x 3072 x 3072 9.5 us against 11.4).
+int few_blocks(int64_t big) { return big > 16 * 2 * cu_count() ? 2 : 1; }
+
+// K ranges of a few-row launch: doubled while its workgroups leave CUs idle and a wave keeps 3 steps of 64 (1024 x 64 x
+// 3072 11.0 us whole, 9.6 us in four; with 192 workgroups, 28 x 3072 x 3072, two ranges cost 9.5 -> 13 us).
+int few_split(int64_t big, int64_t K) {
+  const int64_t units = cdiv(big, 16 * few_blocks(big)), steps = cdiv(K, 64);
+  int split = 1;
+  while (units * split * 2 <= cu_count() && steps / (kStreamWaves * split * 2) >= 3) split *= 2;
+  return split;
+}
+
+// Tile and K ranges of the tiled launch: the fastest by this model of a launch in us, fitted to 108 shapes (40 to 4608
+// rows, 64 to 21504 columns, K 512 to 12288, every tile and split timed), where its choices are within 1.5 % of the
+// fastest in the mean and 16 % at worst. A round is one tile on every CU; a step of K costs the more the more CUs are
+// busy (the power limit); a split launch pays for its second kernel and for writing and reading the partial sums.
+struct TileChoice {
+  int tile, split;
+};
+TileChoice pick_tile(const selas_raw_linear_problem *problems, const Plan &plan, int64_t count) {
+  const int cus = cu_count();
+  TileChoice best{256, 1};
+  double best_us = 1e30;
+  for (int tile : {256, 128})
+    for (int split : {1, 2, 3, 4, 6, 8, 12}) {
+      int64_t tiles = 0, steps = 0, sums = 0, merges = 0;
+      for (int64_t i = 0; i < count; ++i) {
+        if (plan.route[i] != Route::kTiled) continue;
+        const selas_raw_linear_problem &p = problems[i];
+        tiles += cdiv(p.B * p.L, tile) * cdiv(p.N, tile);
+        steps = steps > cdiv(p.K, 64) ? steps : cdiv(p.K, 64);
+        sums += p.B * p.L * p.N;
+        ++merges;
+      }
+      const int64_t items = tiles * split, rounds = cdiv(items, cus);
+      if (split > 1 && (steps < 3 * split || items > 2 * cus)) continue;
+      const double busy = items < cus ? static_cast<double>(items) / cus : 1.0, per = static_cast<double>(cdiv(steps, split));
+      double us = tile == 256 ? 13.0 + (0.67 + 0.30 * busy) * per * rounds + 4.0 * (rounds - 1)
+                              : 6.5 + (0.315 + 0.13 * busy) * per * rounds + 0.7 * (rounds - 1);
+      if (split > 1) us += 3.4 * merges + 1e-6 * split * sums;
+      if (us < best_us) {
+        best_us = us;
+        best = TileChoice{tile, split};
+      }
+    }
+  return best;
+}
 
 Plan make_plan(const selas_raw_linear_problem *problems, int64_t count) {
   Plan plan{};
-  const int cus = cu_count();
-  int64_t wide = 0;
+  bool tiled = false;
   for (int64_t i = 0; i < count; ++i) {
     const selas_raw_linear_problem &p = problems[i];
     const int64_t M = p.B * p.L;
+    plan.few_split[i] = 1;
     if (M == 0 || p.N == 0) {
       plan.route[i] = Route::kEmpty;
-    } else if (M <= kFewRows || p.N <= kFewRows) {
+    } else if (M <= kFewX || p.N <= kFewW) {
       plan.route[i] = tiled_ok(p) ? Route::kStream : Route::kFew;
-      plan.few_split[i] = 1;
+      plan.few_split[i] = few_split(M <= kFewX ? p.N : M, p.K);
     } else if (tiled_ok(p)) {
       plan.route[i] = Route::kTiled;
-      wide += cdiv(M, 256) * cdiv(p.N, 256);
+      tiled = true;
     } else {
       plan.route[i] = Route::kAny;
     }
   }
-  plan.tm = plan.tn = wide >= cus / 2 ? 256 : 128;
-  plan.split = 1;
+  if (tiled) {
+    const TileChoice c = pick_tile(problems, plan, count);
+    plan.tile = c.tile;
+    plan.split = c.split;
+  }
   for (int64_t i = 0; i < count; ++i) {
-    const int split = plan.route[i] == Route::kFew || plan.route[i] == Route::kStream ? plan.few_split[i] : plan.route[i] == Route::kTiled ? plan.split : 1;
+    const int split = plan.route[i] == Route::kTiled ? plan.split : plan.few_split[i];
     plan.part[i] = split > 1 ? split * problems[i].B * problems[i].L * problems[i].N : 0;
     plan.floats += (plan.part[i] + 3) / 4 * 4;
   }
@@ -979,23 +1049,26 @@ int launch_merge(const RawProblem &P, const float *part, int split, hipStream_t 
 
 template <int DT>
 int launch_few(const RawProblem &P, bool stream, float *part, int split, hipStream_t s) {
-  const bool swap = P.M > kFewRows;
+  const bool swap = P.M > kFewX;
   const int few = swap ? P.N : P.M, big = swap ? P.M : P.N;
-  const int nt = big > 16 * cu_count() * 2 ? 2 : 1, mt = few <= 16 ? 1 : few <= 32 ? 2 : 4;
+  const int nt = few_blocks(big), mt = few <= 16 ? 1 : few <= 32 ? 2 : 4;
   const dim3 grid(static_cast<uint32_t>(cdiv(big, 16 * nt)), static_cast<uint32_t>(split)), blk(64 * kFewWaves), sblk(64 * kStreamWaves);
-#define SELAS_FEW(NT, MT)                                                                       \
-  do {                                                                                          \
-    if (stream && swap) raw_stream_kernel<DT, NT, MT, true><<<grid, sblk, 0, s>>>(P, part, split); \
-    else if (stream) raw_stream_kernel<DT, NT, MT, false><<<grid, sblk, 0, s>>>(P, part, split);   \
-    else if (swap) raw_few_kernel<DT, NT, MT, true><<<grid, blk, 0, s>>>(P, part, split);       \
-    else raw_few_kernel<DT, NT, MT, false><<<grid, blk, 0, s>>>(P, part, split);                \
+#define SELAS_FEW(NT, MT, SWAP)                                                                  \
+  do {                                                                                           \
+    if (stream) raw_stream_kernel<DT, NT, MT, SWAP><<<grid, sblk, 0, s>>>(P, part, split);       \
+    else raw_few_kernel<DT, NT, MT, SWAP><<<grid, blk, 0, s>>>(P, part, split);                  \
   } while (0)
-  if (nt == 2 && mt == 1) SELAS_FEW(2, 1);
-  else if (nt == 2 && mt == 2) SELAS_FEW(2, 2);
-  else if (nt == 2) SELAS_FEW(2, 4);
-  else if (mt == 1) SELAS_FEW(1, 1);
-  else if (mt == 2) SELAS_FEW(1, 2);
-  else SELAS_FEW(1, 4);
+#define SELAS_FEW_NT(MT, SWAP)            \
+  do {                                    \
+    if (nt == 2) SELAS_FEW(2, MT, SWAP);  \
+    else SELAS_FEW(1, MT, SWAP);          \
+  } while (0)
+  if (swap && mt == 4) SELAS_FEW_NT(4, true);
+  else if (swap && mt == 2) SELAS_FEW_NT(2, true);
+  else if (swap) SELAS_FEW_NT(1, true);
+  else if (mt == 2) SELAS_FEW_NT(2, false);
+  else SELAS_FEW_NT(1, false);
+#undef SELAS_FEW_NT
 #undef SELAS_FEW
   if (int e = check_launch("raw_linear")) return e;
   return split > 1 ? launch_merge<DT>(P, part, split, s) : ok();
@@ -1008,8 +1081,8 @@ int launch_tiled(RawBatch &batch, const Plan &plan, hipStream_t s) {
   bool tail = false;
   for (int i = 0; i < batch.count; ++i) {
     const RawProblem &P = batch.p[i];
-    batch.tiles_m[i] = static_cast<int>(cdiv(P.M, plan.tm));
-    batch.tiles_n[i] = static_cast<int>(cdiv(P.N, plan.tn));
+    batch.tiles_m[i] = static_cast<int>(cdiv(P.M, plan.tile));
+    batch.tiles_n[i] = static_cast<int>(cdiv(P.N, plan.tile));
     batch.tile0[i] = batch.tiles;
     if (static_cast<int64_t>(batch.tiles_m[i]) * batch.tiles_n[i] >= (1ll << 24) - batch.tiles)
       return set_error(SELAS_EUNSUPPORTED, "raw_linear: too many tiles");
@@ -1023,7 +1096,7 @@ int launch_tiled(RawBatch &batch, const Plan &plan, hipStream_t s) {
     if (tail) raw_tile_kernel<DT, 2, 2, MB, NB, OCC, true><<<grid, blk, 0, s>>>(batch); \
     else raw_tile_kernel<DT, 2, 2, MB, NB, OCC, false><<<grid, blk, 0, s>>>(batch);     \
   } while (0)
-  if (plan.tm == 256) SELAS_TILE(8, 8, 1);
+  if (plan.tile == 256) SELAS_TILE(8, 8, 1);
   else SELAS_TILE(4, 4, 2);
 #undef SELAS_TILE
   if (int e = check_launch("raw_linear")) return e;
