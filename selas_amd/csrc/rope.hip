@@ -8,14 +8,19 @@
 // HBM-bound: q and k (and v, when it is laid out on the way) are read and written
 // once. A thread takes one unit of a token, two vectors of V channels that hold
 // V whole pairs, forms the V angles once and applies them to its share of the
-// heads, so the angles cost a few percent of the traffic's time and no table is
-// read. The G adjacent lanes of a token (its units, rounded up to a power of two)
-// hold a whole head, so the RMS sum is a short cross-lane reduction.
+// heads, the next head's vectors in flight while one is turned; no table is read.
+// The G adjacent lanes of a token (its units, rounded up to a power of two) hold a
+// whole head, so the RMS sum is a short cross-lane reduction.
+//
+// Measured (bytes read and written at the 5.1 TB/s of a large copy: the floor): q and
+// k of two clips of 20280 tokens, 24 heads of 128, fp16: 197 us (195.5, 5.06 TB/s);
+// q, k and v of 4608 tokens with norms 41 us (33); one token 5.1 us. What lies between is
+// the 5 to 8 us of a launch, the positions' loads and the angles ahead of the first store.
 //
 // Angles: pos * theta^(-2j/d) / 2 pi in fp64 (exact to 1e-11 turns at a position of
 // 10^5), reduced to the nearest quarter turn there; the remainder, at most 1/8 turn,
-// goes to fp32, where sin and cos are their Taylor sums (terms up to x^11 and x^12 / the
-// next one is below 2^-30 of the value).
+// goes to fp32, where sin and cos are their Taylor sums up to x^11 and x^12: on |x| <=
+// pi / 4 the next terms are below 2^-36.
 #include <cmath>
 
 #include "common.h"
@@ -26,17 +31,19 @@ namespace {
 constexpr int kMaxPairs = 128;  // Dh <= 256
 constexpr float kRmsEps = 1e-6f;
 
-// theta^(-2j / axis_dim) / (2 pi) and the axis of every pair.
+// theta^(-2j / axis_dim) / (2 pi) of every pair.
 struct Turns {
   double per_pos[kMaxPairs];
-  uint8_t axis[kMaxPairs];
 };
 
 struct RopeArgs {
   selas_rope_part part[SELAS_ROPE_MAX_PARTS];
   int count, heads;  // heads: of all parts
-  int B, L, Dh;
+  int tokens, L, Dh;
+  FastDiv by_l;
   int pairs;         // rotated pairs, R / 2
+  int axes;
+  int axis_end[SELAS_ROPE_MAX_AXES];  // the pair after each axis's last
   int units, group;  // units of a token, and the lanes that hold them
   int heads_per_block;
   const void *ids;
@@ -67,6 +74,22 @@ __device__ __forceinline__ void sincos_turns(double t, float &s, float &c) {
   const float a = (k & 1) ? pc : ps, b = (k & 1) ? ps : pc;
   s = (k & 2) ? -a : a;
   c = (k == 1 || k == 2) ? -b : b;
+}
+
+// Sum over the `group` lanes (a power of two) of a token: swaps inside quads, then mirrors of 8 and 16 lanes (each half's
+// lanes are equal by then), all on the vector unit; only wider groups go through the cross-lane network.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float group_sum(float v, int group) {
+  if (group > 1) v = dpp_add<0xB1>(v);    // quad_perm 1 0 3 2
+  if (group > 2) v = dpp_add<0x4E>(v);    // quad_perm 2 3 0 1
+  if (group > 4) v = dpp_add<0x141>(v);   // row_half_mirror
+  if (group > 8) v = dpp_add<0x140>(v);   // row_mirror
+  if (group > 16) v += __shfl_xor(v, 16, 64);
+  if (group > 32) v += __shfl_xor(v, 32, 64);
+  return v;
 }
 
 template <int DT, int V>
@@ -131,10 +154,9 @@ template <int DT, int V, bool HALVES>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, Turns turns) {
   const int group = a.group;
   const int u = threadIdx.x & (group - 1);
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * (256 / group) + threadIdx.x / group;
-  const bool live = token < static_cast<int64_t>(a.B) * a.L && u < a.units;
-  const int b = live ? static_cast<int>(token / a.L) : 0;
-  const int l = live ? static_cast<int>(token - static_cast<int64_t>(b) * a.L) : 0;
+  const uint32_t token = blockIdx.x * (256 / group) + threadIdx.x / group;
+  const bool live = token < static_cast<uint32_t>(a.tokens) && u < a.units;
+  const int b = live ? static_cast<int>(div31(token, a.by_l)) : 0, l = live ? static_cast<int>(token) - b * a.L : 0;
   const int R = 2 * a.pairs, rot_units = a.pairs / V;
   const bool rotated = live && u < rot_units;
   int c0, c1;
@@ -148,22 +170,32 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, Turns turns) {
   const bool two = live && c1 < a.Dh;
 
   float sn[V], cs[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) sn[j] = 0.0f, cs[j] = 1.0f;
   if (rotated) {
+    // All of the token's positions at once: an axis looked up first would put two loads in a row.
+    double pos[SELAS_ROPE_MAX_AXES] = {};
+    const int64_t at = b * a.ids_sb + l * a.ids_sl;
+#pragma unroll
+    for (int i = 0; i < SELAS_ROPE_MAX_AXES; ++i)
+      if (i < a.axes)
+        pos[i] = a.ids_dtype == SELAS_F32   ? static_cast<double>(static_cast<const float *>(a.ids)[at + i])
+                 : a.ids_dtype == SELAS_I32 ? static_cast<double>(static_cast<const int32_t *>(a.ids)[at + i])
+                                            : static_cast<double>(static_cast<const int64_t *>(a.ids)[at + i]);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       // Pair j of this unit: of its two vectors' adjacent pairs, or of its halves.
       const int i = (V == 1 || HALVES) ? u * V + j : (j < V / 2 ? c0 / 2 + j : c1 / 2 + j - V / 2);
-      const int64_t at = b * a.ids_sb + l * a.ids_sl + turns.axis[i];
-      const double pos = a.ids_dtype == SELAS_F32   ? static_cast<double>(static_cast<const float *>(a.ids)[at])
-                         : a.ids_dtype == SELAS_I32 ? static_cast<double>(static_cast<const int32_t *>(a.ids)[at])
-                                                    : static_cast<double>(static_cast<const int64_t *>(a.ids)[at]);
-      sincos_turns(pos * turns.per_pos[i], sn[j], cs[j]);
+      double p = pos[0];
+#pragma unroll
+      for (int e = 1; e < SELAS_ROPE_MAX_AXES; ++e) p = i >= a.axis_end[e - 1] ? pos[e] : p;
+      sincos_turns(p * turns.per_pos[i], sn[j], cs[j]);
       if (a.inverse) sn[j] = -sn[j];
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) sn[j] = 0.0f, cs[j] = 1.0f;
   }
 
+  const float inv_dh = 1.0f / static_cast<float>(a.Dh);
   const int h_lo = blockIdx.y * a.heads_per_block, h_hi = min(a.heads, h_lo + a.heads_per_block);
   int first = 0;  // of the part, in the heads of all parts
   for (int p = 0; p < a.count; ++p) {
@@ -182,16 +214,23 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, Turns turns) {
         if (two) s1[j] = part.scale[c1 + j];
       }
     }
+    // The next head's vectors are in flight while one is turned and stored.
+    float n0[V] = {}, n1[V] = {};
+    auto load = [&](int h) {
+      if (live) load_vec<DT, V>(part.x, xo + h * part.x_sh + c0, n0);
+      if (two) load_vec<DT, V>(part.x, xo + h * part.x_sh + c1, n1);
+    };
+    load(lo);
     for (int h = lo; h < hi; ++h) {
-      float v0[V] = {}, v1[V] = {};
-      if (live) load_vec<DT, V>(part.x, xo + h * part.x_sh + c0, v0);
-      if (two) load_vec<DT, V>(part.x, xo + h * part.x_sh + c1, v1);
+      float v0[V], v1[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v0[j] = n0[j], v1[j] = n1[j];
+      if (h + 1 < hi) load(h + 1);
       if (part.scale) {
         float ss = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) ss += v0[j] * v0[j] + v1[j] * v1[j];
-        for (int o = 1; o < group; o <<= 1) ss += __shfl_xor(ss, o, 64);
-        const float r = 1.0f / sqrtf(ss / static_cast<float>(a.Dh) + kRmsEps);
+        const float r = __builtin_amdgcn_rsqf(group_sum(ss, group) * inv_dh + kRmsEps);  // within 1 ulp
 #pragma unroll
         for (int j = 0; j < V; ++j) v0[j] = (v0[j] * r) * s0[j], v1[j] = (v1[j] * r) * s1[j];
       }
@@ -280,8 +319,9 @@ extern "C" int selas_rope(const selas_rope_part *parts, int64_t count, int64_t B
   if (B >= (1ll << 31) || L >= (1ll << 31) || B * L >= (1ll << 31) || heads >= (1ll << 16))
     return set_error(SELAS_EUNSUPPORTED, "rope: too many tokens or heads");
   a.heads = static_cast<int>(heads);
-  a.B = static_cast<int>(B);
+  a.tokens = static_cast<int>(B * L);
   a.L = static_cast<int>(L);
+  a.by_l = fast_div(static_cast<uint32_t>(L));
   a.Dh = static_cast<int>(Dh);
   a.pairs = static_cast<int>(R / 2);
   a.ids = ids;
@@ -290,11 +330,14 @@ extern "C" int selas_rope(const selas_rope_part *parts, int64_t count, int64_t B
   a.ids_dtype = ids_dtype;
   a.inverse = inverse != 0;
   Turns turns{};
-  for (int64_t i = 0, at = 0; i < axes; ++i)
-    for (int64_t j = 0; j < axis_dim[i]; j += 2, ++at) {
-      turns.per_pos[at] = std::pow(theta, -static_cast<double>(j) / static_cast<double>(axis_dim[i])) / 6.283185307179586;
-      turns.axis[at] = static_cast<uint8_t>(i);
-    }
+  a.axes = static_cast<int>(axes);
+  int pairs = 0;
+  for (int i = 0; i < SELAS_ROPE_MAX_AXES; ++i) {
+    for (int64_t j = 0; i < axes && j < axis_dim[i]; j += 2)
+      turns.per_pos[pairs++] =
+          std::pow(theta, -static_cast<double>(j) / static_cast<double>(axis_dim[i])) / 6.283185307179586;
+    a.axis_end[i] = pairs;
+  }
   const int esize = dtype == SELAS_F32 ? 4 : 2;
   const int V = dtype != SELAS_F32 && rope_vec_ok(a, 8, esize) ? 8 : rope_vec_ok(a, 4, esize) ? 4 : 1;
   a.units = static_cast<int>(R / 2 / V + cdiv(Dh - R, 2 * V));
@@ -302,11 +345,12 @@ extern "C" int selas_rope(const selas_rope_part *parts, int64_t count, int64_t B
   while (a.group < a.units) a.group *= 2;
   if (a.group > 64)
     return set_error(SELAS_EUNSUPPORTED, "rope: heads of %lld channels off 4-element alignment", (long long)Dh);
-  // Heads per thread: 8 share a thread's angles while that leaves 8 waves per SIMD (2048 workgroups), else fewer, so
-  // that short sequences still spread over the CUs.
+  // Heads per thread: the fewest that leave no more than 4 workgroups per CU of 256, which are resident at once (90
+  // registers allow 5). A thread's positions, angles and scales then serve as many heads as possible, and no second round
+  // pays for them again (image of 4608 tokens, us: 41.3 with 1152 workgroups, 46 with 1728, 50 with 1296 of which 16 wait).
   const int64_t blocks = cdiv(B * L, 256 / a.group);
-  int64_t hpb = 8;
-  while (hpb > 1 && blocks * cdiv(heads, hpb) < 2048) hpb /= 2;
+  int64_t hpb = 1;
+  while (hpb < heads && blocks * cdiv(heads, hpb) > 4 * 256) ++hpb;
   a.heads_per_block = static_cast<int>(hpb);
   const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(cdiv(heads, hpb))), blk(256);
   hipStream_t s = static_cast<hipStream_t>(stream);

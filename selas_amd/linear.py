@@ -377,15 +377,21 @@ def _raw_vector(v: torch.Tensor, b: int, n: int) -> tuple[torch.Tensor, int]:
 
 
 def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
-    if not problems:
-        return []
     dt = problems[0].x.dtype
-    arr = (_lib.RawLinearProblem * len(problems))()
-    outs, keep, given = [], [], []
-    dev = _lib.require_gpu(*(t for p in problems for t in p if isinstance(t, torch.Tensor)))
-    if dt not in (torch.bfloat16, torch.float16):
+    dev = _lib.require_gpu(*(t for p in problems for t in (p.x, p.weight, p.bias, p.gate, p.residual, p.out)))
+    if dt != torch.bfloat16 and dt != torch.float16:
         raise _lib.Unsupported(f"raw_linear: takes bf16 or fp16, got {dt}")
-    for i, (x, w, bias, act, gate, residual, out, out_dtype) in enumerate(problems):
+    code = _lib.DTYPE_CODES[dt]
+    outs, keep, packed = [], [], []
+
+    def dtype_of(name: str, d: torch.dtype) -> int:
+        if d == dt:
+            return code
+        if d == torch.float32:
+            return _lib.F32
+        raise ValueError(f"raw_linear: {name} is {d}, takes {dt} or float32")
+
+    for x, w, bias, act, gate, residual, out, out_dtype in problems:
         if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
             raise ValueError(f"raw_linear: x {tuple(x.shape)} does not go with weight {tuple(w.shape)}")
         if x.dtype != dt or w.dtype != dt:
@@ -394,51 +400,61 @@ def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
             raise ValueError(f"raw_linear: act must be None, 'gelu' or 'silu', got {act!r}")
         n, k = w.shape
         shape = (*x.shape[:-1], n)
-        _check_bias(bias, n)
-        if residual is not None and residual.shape != shape:
-            raise ValueError(f"raw_linear: residual {tuple(residual.shape)} is not {shape}")
-        ydt = out.dtype if out is not None else out_dtype or (dt if residual is None else residual.dtype)
-        for name, d in (("out", ydt), *((m, t.dtype) for m, t in (("bias", bias), ("gate", gate), ("residual", residual))
-                                        if t is not None)):
-            if d != dt and d != torch.float32:
-                raise ValueError(f"raw_linear: {name} is {d}, takes {dt} or float32")
-        if out is not None and out_dtype not in (None, out.dtype):
-            raise ValueError(f"raw_linear: out is {out.dtype}, out_dtype {out_dtype}")
         x3, x_sb, x_sl = _raw_rows(x)
-        if w.shape[1] > 1 and w.stride(1) != 1:
+        if k > 1 and w.stride(1) != 1:
             w = w.contiguous()
         b, l = (x3.shape[0], x3.shape[1]) if x3.dim() == 3 else (1, x3.shape[0] if x3.dim() == 2 else 1)
-        if bias is not None and not bias.is_contiguous():
-            bias = bias.contiguous()
-        g, g_sb = (None, 0) if gate is None else _raw_vector(gate, b, n)
-        r, r_sb, r_sl = (None, 0, 0) if residual is None else _raw_rows(residual)
+        bias_p = gate_p = g_sb = res_p = r_sb = r_sl = bias_dt = gate_dt = res_dt = 0
+        if bias is not None:
+            _check_bias(bias, n)
+            if not bias.is_contiguous():
+                bias = bias.contiguous()
+            bias_p, bias_dt = bias.data_ptr(), dtype_of("bias", bias.dtype)
+        g = r = None
+        if gate is not None:
+            g, g_sb = _raw_vector(gate, b, n)
+            gate_p, gate_dt = g.data_ptr(), dtype_of("gate", g.dtype)
+        if residual is not None:
+            if residual.shape != shape:
+                raise ValueError(f"raw_linear: residual {tuple(residual.shape)} is not {shape}")
+            r, r_sb, r_sl = _raw_rows(residual)
+            res_p, res_dt = r.data_ptr(), dtype_of("residual", r.dtype)
         if out is None:
-            out = torch.empty(shape, dtype=ydt, device=dev)
-            y, y_sb, y_sl = out, l * n, n
+            ydt = out_dtype or (dt if residual is None else residual.dtype)
+            y_dt = dtype_of("out", ydt)
+            out = y = torch.empty(shape, dtype=ydt, device=dev)
+            y_sb, y_sl = l * n, n
         else:
+            if out_dtype not in (None, out.dtype):
+                raise ValueError(f"raw_linear: out is {out.dtype}, out_dtype {out_dtype}")
+            y_dt = dtype_of("out", out.dtype)
             y = _check_raw_out(out, shape, (x, w, bias, gate), residual)
             y_sb, y_sl = (y.stride(0) if y.dim() == 3 else 0), (y.stride(-2) if y.dim() > 1 else 0)
-            given.append(i)
         outs.append(out)
         keep += (x3, w, bias, g, r)
-        code = _lib.DTYPE_CODES
-        arr[i] = _lib.RawLinearProblem(
-            x3.data_ptr(), x_sb, x_sl, w.data_ptr(), w.stride(0), _lib.ptr(bias), _lib.ptr(g), g_sb, _lib.ptr(r), r_sb,
-            r_sl, y.data_ptr(), y_sb, y_sl, b, l, n, k, code[bias.dtype] if bias is not None else 0,
-            code[g.dtype] if g is not None else 0, code[r.dtype] if r is not None else 0, code[ydt], ACTS[act], 0)
-    for i in given if len(problems) > 1 else ():
-        for j, p in enumerate(problems):
-            if j != i and any(t is not None and may_meet(outs[i], t) for t in (*p[:3], *p[4:6], outs[j])):
-                raise ValueError(f"raw_linear: out of problem {i} overlaps a tensor of problem {j}")
+        packed.append(_lib.RAW_LINEAR_PROBLEM.pack(
+            x3.data_ptr(), x_sb, x_sl, w.data_ptr(), w.stride(0), bias_p, gate_p, g_sb, res_p, r_sb, r_sl, y.data_ptr(),
+            y_sb, y_sl, b, l, n, k, bias_dt, gate_dt, res_dt, y_dt, ACTS[act], 0))
+    if len(problems) > 1:
+        _check_raw_disjoint(problems, outs)
+    arr, count = b"".join(packed), len(packed)
     size = ctypes.c_int64()
-    with torch.cuda.device(dev):
-        _lib.call("selas_raw_linear_workspace_bytes", ctypes.addressof(arr), len(problems), _lib.DTYPE_CODES[dt],
-                  ctypes.byref(size))
+    with _lib.on(dev):
+        _lib.call("selas_raw_linear_workspace_bytes", arr, count, code, ctypes.byref(size))
         ws = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-        _lib.call("selas_raw_linear", ctypes.addressof(arr), len(problems), _lib.DTYPE_CODES[dt], _lib.ptr(ws), size.value,
-                  _lib.stream(dev))
+        _lib.call("selas_raw_linear", arr, count, code, _lib.ptr(ws), size.value, _lib.stream(dev))
     del keep  # the launch is queued on the stream that later reuses this memory
     return outs
+
+
+def _check_raw_disjoint(problems: list[RawLinear], outs: list[torch.Tensor]) -> None:
+    for i, p in enumerate(problems):
+        if p.out is None:
+            continue
+        for j, q in enumerate(problems):
+            others = (q.x, q.weight, q.bias, q.gate, q.residual, outs[j])
+            if j != i and any(t is not None and may_meet(p.out, t) for t in others):
+                raise ValueError(f"raw_linear: out of problem {i} overlaps a tensor of problem {j}")
 
 
 def _check_raw_out(out: torch.Tensor, shape, inputs, residual) -> torch.Tensor:

@@ -9,7 +9,7 @@ heads that precedes the rotation (flux.py:124-126) and the layout of v run in th
 
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
@@ -61,38 +61,39 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, ids: torch.Tensor, axes_dim, theta
     if pairs not in PAIRS:
         raise ValueError(f"rope_qk: pairs must be one of {PAIRS}, got {pairs!r}")
     b, _, l, dh = q.shape
-    axes = tuple(int(d) for d in axes_dim)
+    axes = tuple(axes_dim)
     if not 1 <= len(axes) <= _lib.ROPE_MAX_AXES:
         raise ValueError(f"rope_qk: takes 1 to {_lib.ROPE_MAX_AXES} axes, got {len(axes)}")
-    if q.dtype not in _lib.DTYPE_CODES:
+    dtype = _lib.DTYPE_CODES.get(q.dtype)
+    if dtype is None:
         raise _lib.Unsupported(f"rope_qk: dtype {q.dtype}")
     dev = _lib.require_gpu(q, k, v, ids, q_scale, k_scale)
     xs = [_check_heads("q", q, q), _check_heads("k", k, q)]
     if v is not None:
         xs.append(_check_heads("v", v, q))
-    if ids.dim() not in (2, 3) or ids.shape[-1] != len(axes) or ids.shape[-2] != l or (ids.dim() == 3
-                                                                                      and ids.shape[0] not in (1, b)):
+    lead = ids.shape[:-2]
+    if (ids.dim() not in (2, 3) or ids.shape[-1] != len(axes) or ids.shape[-2] != l
+            or (len(lead) == 1 and lead[0] not in (1, b))):
         raise ValueError(f"rope_qk: positions {tuple(ids.shape)} are not [{l}, {len(axes)}] or [{b}, {l}, {len(axes)}]")
-    if ids.dtype not in _ID_CODES:
+    id_code = _ID_CODES.get(ids.dtype)
+    if id_code is None:
         raise ValueError(f"rope_qk: positions are float32, int32 or int64, got {ids.dtype}")
     if ids.stride(-1) != 1 and len(axes) > 1:
         ids = ids.contiguous()
-    ids_sb = ids.stride(0) if ids.dim() == 3 and ids.shape[0] > 1 else 0
-    scales = [_check_scale("q_scale", q_scale, dh), _check_scale("k_scale", k_scale, dh), None]
+    ids_sb = ids.stride(0) if lead and lead[0] > 1 else 0
+    scales = (_check_scale("q_scale", q_scale, dh), _check_scale("k_scale", k_scale, dh), None)
     if out is None:
         ys = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in xs]
     else:
         ys = list(out)
         _check_out(xs, ys, dev)
-    parts = (_lib.RopePart * len(xs))()
-    for i, (x, y) in enumerate(zip(xs, ys)):
-        parts[i] = _lib.RopePart(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), y.data_ptr(), y.stride(0),
-                                 y.stride(1), y.stride(2), _lib.ptr(scales[i]), x.shape[1], i < 2)
-    dims = (ctypes.c_int64 * len(axes))(*axes)
-    with torch.cuda.device(dev):
-        _lib.call("selas_rope", ctypes.addressof(parts), len(xs), b, l, dh, ids.data_ptr(), _ID_CODES[ids.dtype], ids_sb,
-                  ids.stride(-2), len(axes), dims, float(theta), int(pairs == "halves"), int(bool(inverse)),
-                  _lib.dtype_code(q.dtype), _lib.stream(dev))
+    parts = b"".join([_lib.ROPE_PART.pack(x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3],
+                                          0 if scale is None else scale.data_ptr(), x.shape[1], i < 2)
+                      for i, (x, y, scale) in enumerate(zip(xs, ys, scales))])
+    with _lib.on(dev):
+        _lib.call("selas_rope", parts, len(xs), b, l, dh, ids.data_ptr(), id_code, ids_sb, ids.stride(-2), len(axes),
+                  struct.pack(f"@{len(axes)}q", *axes), float(theta), pairs == "halves", bool(inverse), dtype,
+                  _lib.stream(dev))
     return tuple(ys)
 
 
