@@ -27,6 +27,10 @@ struct RawProblem {
   bool one_gate;  // one gate row for all batches
 };
 
+// Four dwords, and the same at the address of any 16-bit element (global accesses may start there).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
 // v_mfma_f32_16x16x32 of two 16-bit fragments: D(16x16) += A(16x32) B(32x16). Lane l supplies A[l % 16][8 (l / 16) ..
 // +8] and B[8 (l / 16) .. +8][l % 16] and holds D[4 (l / 16) + r][l % 16] in register r.
 template <int DT>
@@ -45,7 +49,6 @@ __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
 // same a comes again 16 calls (4 in the 128 x 128 tile) later at the earliest.
 template <int DT>
 __device__ __forceinline__ void mfma16_inplace(uint4 a, uint4 b, f32x4 &c) {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   const u32x4 av = {a.x, a.y, a.z, a.w}, bv = {b.x, b.y, b.z, b.w};
   if constexpr (DT == SELAS_BF16) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(av), "v"(bv));
   else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(av), "v"(bv));
@@ -64,6 +67,21 @@ __device__ __forceinline__ float silu_fast(float x) {
 
 __device__ __forceinline__ float activate(float v, int act) {
   return act == SELAS_ACT_GELU ? gelu_tanh_fast(v) : act == SELAS_ACT_SILU ? silu_fast(v) : v;
+}
+
+template <int A, int B>
+__device__ __forceinline__ void activate_all(float (&v)[A][B], int act) {  // one branch for all
+  if (act == SELAS_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) v[i][j] = gelu_tanh_fast(v[i][j]);
+  } else if (act == SELAS_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) v[i][j] = silu_fast(v[i][j]);
+  }
 }
 
 template <int DT>
@@ -121,6 +139,71 @@ __device__ __forceinline__ void load_cols(const void *p, int64_t i, bool f32, fl
         v[2 * t + 1] = f16_bits_to_f32(w[t] >> 16);
       }
     }
+  }
+}
+
+// W consecutive columns from any element on, of which the first `live` exist (the others hold any of them, or zeros).
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+template <int DT, int W>
+__device__ __forceinline__ void load_cols_any(const void *p, int64_t i, bool f32, int live, float (&v)[W]) {
+  if (live <= 0) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = 0.0f;
+  } else if (live < W) {
+    // The last column stands in for the ones past it: loads under a condition each would wait for one another.
+    if (f32) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] = static_cast<const float *>(p)[i + min(j, live - 1)];
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] = load_f<DT>(p, i + min(j, live - 1));
+    }
+  } else if (f32) {
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const f32x4 u = *reinterpret_cast<const f32x4_any *>(static_cast<const float *>(p) + i + j);
+      v[j] = u[0]; v[j + 1] = u[1]; v[j + 2] = u[2]; v[j + 3] = u[3];
+    }
+  } else {
+    const uint16_t *q = static_cast<const uint16_t *>(p) + i;
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const u32x2_any u = *reinterpret_cast<const u32x2_any *>(q + j);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (DT == SELAS_BF16) {
+          v[j + 2 * t] = __uint_as_float(u[t] << 16);
+          v[j + 2 * t + 1] = __uint_as_float(u[t] & 0xffff0000u);
+        } else {
+          v[j + 2 * t] = f16_bits_to_f32(u[t] & 0xffffu);
+          v[j + 2 * t + 1] = f16_bits_to_f32(u[t] >> 16);
+        }
+      }
+    }
+  }
+}
+
+// W == 4: fp32 outputs; W == 8: 16-bit ones.
+template <int DT, int W>
+__device__ __forceinline__ void store_cols_any(void *y, int64_t i, int live, const float (&v)[W]) {
+  if (live < W) {
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if (j < live) {
+        if constexpr (W == 4) static_cast<float *>(y)[i + j] = v[j];
+        else store_f<DT>(y, i + j, v[j]);
+      }
+  } else if constexpr (W == 4) {
+    *reinterpret_cast<f32x4_any *>(static_cast<float *>(y) + i) = f32x4{v[0], v[1], v[2], v[3]};
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == SELAS_BF16) w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+      else w[j] = f16_bits_rne(v[2 * j]) | (static_cast<uint32_t>(f16_bits_rne(v[2 * j + 1])) << 16);
+    }
+    *reinterpret_cast<u32x4_any *>(static_cast<uint16_t *>(y) + i) = u32x4{w[0], w[1], w[2], w[3]};
   }
 }
 
@@ -203,8 +286,6 @@ __global__ __launch_bounds__(256) void raw_merge_kernel(RawProblem P, const floa
 
 // Eight elements of a row from k on, zeros from K on. The address need not be aligned: global loads may start at any
 // element.
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
 __device__ __forceinline__ uint4 load_any(const uint16_t *p) {
   return __builtin_bit_cast(uint4, static_cast<u32x4>(*reinterpret_cast<const u32x4_any *>(p)));
 }
@@ -217,79 +298,29 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t *row, int k, int K) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// ------------------------------------------------------------------ any layout
+// ------------------------------------------------------------------ operands off alignment
 //
-// 4 waves, 64 x 64 outputs, 64 columns of K per step, staged through registers (the next step's loads are in flight
-// during this step's products). Rows of 128 bytes in LDS, their 16-byte chunks XOR-swizzled by (row / 2) % 8 so that the
-// 16 rows of a fragment read lie in distinct groups of the 64 banks.
-constexpr int kAnyT = 64;
-
+// The tiled kernel's DMA takes whole 16-byte chunks. An operand whose rows are not made of them (K not a multiple of 8, an
+// odd stride or address) or span too much is copied first, to rows of K rounded up to 64 that end in zeros: one more pass
+// over it against a kernel that loads such rows through registers (1386 x 1431 x 667 26 us in 64 x 64 tiles).
 template <int DT>
-__global__ __launch_bounds__(256) void raw_any_kernel(RawProblem P) {
-  __shared__ uint4 xs[kAnyT * 8], ws[kAnyT * 8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int m0 = blockIdx.y * kAnyT, n0 = blockIdx.x * kAnyT;
-  // Thread t loads chunks t % 8 of rows t / 8 and t / 8 + 32 of each operand.
-  const int c = tid & 7;
-  const uint16_t *xr[2], *wr[2];
-  int dst[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = (tid >> 3) + 32 * i;
-    const int m = m0 + r, n = n0 + r;
-    const int b = static_cast<int>(div31(static_cast<uint32_t>(min(m, P.M - 1)), P.by_l));
-    const int l = min(m, P.M - 1) - b * P.L;
-    xr[i] = static_cast<const uint16_t *>(P.x) + b * P.x_sb + l * P.x_sl;
-    wr[i] = static_cast<const uint16_t *>(P.w) + static_cast<int64_t>(min(n, P.N - 1)) * P.ldw;
-    dst[i] = r * 8 + (c ^ ((r >> 1) & 7));
+__global__ __launch_bounds__(256) void raw_pack_kernel(RawProblem P, uint16_t *xp, uint16_t *wp, int kp) {
+  const int per_row = kp / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / per_row;
+  const int k = static_cast<int>(i - row * per_row) * 8;
+  const int64_t xrows = xp ? P.M : 0;
+  if (row >= xrows + (wp ? P.N : 0)) return;
+  const uint16_t *src;
+  uint16_t *dst;
+  if (row < xrows) {
+    const int m = static_cast<int>(row), b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l));
+    src = static_cast<const uint16_t *>(P.x) + b * P.x_sb + (m - b * P.L) * P.x_sl;
+    dst = xp + row * kp;
+  } else {
+    src = static_cast<const uint16_t *>(P.w) + (row - xrows) * P.ldw;
+    dst = wp + (row - xrows) * kp;
   }
-  uint4 xv[2], wv[2];
-  auto load = [&](int k) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      xv[i] = load_chunk(xr[i], k + 8 * c, P.K);
-      wv[i] = load_chunk(wr[i], k + 8 * c, P.K);
-    }
-  };
-  f32x4 acc[2][2] = {};
-  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-  auto frag = [&](const uint4 *s, int r, int kc) { return s[r * 8 + (kc ^ ((r >> 1) & 7))]; };
-  if (P.K > 0) load(0);
-  for (int k = 0; k < P.K; k += 64) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) xs[dst[i]] = xv[i], ws[dst[i]] = wv[i];
-    __syncthreads();
-    if (k + 64 < P.K) load(k + 64);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      uint4 a[2], b[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        a[i] = frag(ws, wn + 16 * i + (lane & 15), 4 * s + (lane >> 4));
-        b[i] = frag(xs, wm + 16 * i + (lane & 15), 4 * s + (lane >> 4));
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<DT>(a[i], b[j], acc[i][j]);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int m = m0 + wm + 16 * j + (lane & 15);
-    if (m >= P.M) continue;
-    const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l)), l = m - b * P.L;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = n0 + wn + 16 * i + 4 * (lane >> 4) + r;
-        if (n >= P.N) continue;
-        finish_one<DT>(P, b, l, n, acc[i][j][r]);
-      }
-  }
+  *reinterpret_cast<uint4 *>(dst + k) = load_chunk(src, k, P.K);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -384,7 +415,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void raw_few_kernel(RawProblem P, f
   finish_few<DT, NT, MT, SWAP, kFewWaves>(P, r0, &red[0][0][0]);
 }
 
-// The same for operands whose rows are 16-byte aligned (tiled_ok): the fragments' lane order takes each of 16 adjacent
+// The same for operands whose rows the DMA can read (dma_ok_x, dma_ok_w): the fragments' lane order takes each of 16 adjacent
 // lanes to another row, 64 cache lines looked up per load, which held the loads above at 16 bytes per clock and CU (28 x
 // 18432 x 3072 36 us). Here each wave copies its range of K to LDS of its own by DMA, 8 rows of 128 bytes per
 // instruction, ST steps of 64 columns ahead, and reads the fragments there; no barrier until the sums are added.
@@ -767,17 +798,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[g][4 * q + j] = f[j] + bias[4 * q + j];
         }
-      if (P.act == SELAS_ACT_GELU) {
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int j = 0; j < W; ++j) v[g][j] = gelu_tanh_fast(v[g][j]);
-      } else if (P.act == SELAS_ACT_SILU) {
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int j = 0; j < W; ++j) v[g][j] = silu_fast(v[g][j]);
-      }
+      activate_all(v, P.act);
       if (P.gate) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -832,28 +853,63 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
       }
     }
   };
-  auto finish_columns = [&](int e) __attribute__((always_inline)) {  // no vectors: a lane per column
-#pragma unroll 1
-    for (int r = 0; r < ER; ++r) {
-      const int m = m0 + wm * MB * 16 + e * ER + r;
-      if (m >= M) return;
-      const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l)), l = m - b * P.L;
-#pragma unroll 1
-      for (int i = lane; i < NB * 16 && nw + i < N; i += 64)
-        finish_one<DT>(P, b, l, nw + i, *reinterpret_cast<const float *>(st + r * (NB * 64) + (((i >> 2) ^ (r & 15)) << 4) + (i & 3) * 4));
-    }
-  };
-  if (P.vec && P.y_f32) {
-    finish(std::integral_constant<int, 4>{});
-  } else if (P.vec) {
-    finish(std::integral_constant<int, 8>{});
-  } else {
+  // The same for outputs off alignment, N not a multiple of 8 or batches with spacing of their own: addresses per row, and
+  // vector accesses that may start at any element, except in the columns that N cuts.
+  auto finish_any = [&](auto width) __attribute__((always_inline)) {
+    constexpr int W = decltype(width)::value, LPR = NB * 16 / W, RPI = 64 / LPR, U = 4;
+    const int n = nw + (lane % LPR) * W, row = lane / LPR, live = N - n;
+    const int mw = m0 + wm * MB * 16;
+    float bias[W] = {}, gate[W];
+    if (P.bias) load_cols_any<DT, W>(P.bias, n, P.bias_f32, live, bias);
+    if (P.gate && P.one_gate) load_cols_any<DT, W>(P.gate, n, P.gate_f32, live, gate);
 #pragma unroll 1
     for (int e = 0; e < MB / 2; ++e) {
       stage(e);
-      finish_columns(e);
+#pragma unroll 1
+      for (int g = 0; g < ER / RPI; g += U) {
+        float v[U][W], res[U][W];
+        int bs[U], ls[U];
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int m = mw + e * ER + (g + u) * RPI + row;
+          on[u] = m < M;
+          bs[u] = static_cast<int>(div31(static_cast<uint32_t>(min(m, M - 1)), P.by_l));
+          ls[u] = m - bs[u] * P.L;
+          if (P.residual && on[u])
+            load_cols_any<DT, W>(P.residual, bs[u] * P.r_sb + ls[u] * P.r_sl + n, P.residual_f32, live, res[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int q = 0; q < W / 4; ++q) {
+            const int r = (g + u) * RPI + row, c = (lane % LPR) * (W / 4) + q;
+            const f32x4 f = *reinterpret_cast<const f32x4 *>(st + r * (NB * 64) + ((c ^ (r & 15)) << 4));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[u][4 * q + j] = f[j] + bias[4 * q + j];
+          }
+        }
+        activate_all(v, P.act);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (P.gate) {
+            if (!P.one_gate) load_cols_any<DT, W>(P.gate, bs[u] * P.gate_sb + n, P.gate_f32, live, gate);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[u][j] *= gate[j];
+          }
+          if (P.residual) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[u][j] = res[u][j] + v[u][j];
+          }
+          if (on[u]) store_cols_any<DT, W>(P.y, bs[u] * P.y_sb + ls[u] * P.y_sl + n, live, v[u]);
+        }
+      }
     }
-  }
+  };
+  if (P.vec && P.y_f32) finish(std::integral_constant<int, 4>{});
+  else if (P.vec) finish(std::integral_constant<int, 8>{});
+  else if (P.y_f32) finish_any(std::integral_constant<int, 4>{});
+  else finish_any(std::integral_constant<int, 8>{});
 }
 
 // ------------------------------------------------------------------ host side
@@ -876,14 +932,6 @@ int check_problem(const selas_raw_linear_problem &p, int64_t i, int dtype) {
       p.K >= (1ll << 31) - 256)
     return set_error(SELAS_EUNSUPPORTED, "raw_linear[%lld]: rows, columns or K above 2^31", at);
   return SELAS_OK;
-}
-
-template <int DT>
-int launch_any(const RawProblem &P, hipStream_t s) {
-  const int64_t tn = cdiv(P.N, kAnyT), tm = cdiv(P.M, kAnyT);
-  if (tm > 65535) return set_error(SELAS_EUNSUPPORTED, "raw_linear: too many rows (%d)", P.M);
-  raw_any_kernel<DT><<<dim3(static_cast<uint32_t>(tn), static_cast<uint32_t>(tm)), dim3(256), 0, s>>>(P);
-  return check_launch("raw_linear");
 }
 
 // Whether rows of p (stride s, batch stride sb, in elements of `size` bytes) take 16-byte accesses at every 8th element.
@@ -915,13 +963,16 @@ RawProblem make_problem(const selas_raw_linear_problem &p) {
   return r;
 }
 
-// Whether the tiled kernel's DMA can read the operands: whole 16-byte chunks, and a tile's rows within 31 bits of bytes.
-bool tiled_ok(const selas_raw_linear_problem &p) {
-  if (p.K % 8 || p.K == 0 || !rows_ok(p.x, p.x_sb, p.x_sl, 2) || !rows_ok(p.w, 0, p.ldw, 2)) return false;
+// Whether the kernels' DMA can read an operand where it is: whole 16-byte chunks, and the rows of a tile within 31 bits
+// of bytes.
+bool dma_ok_w(const selas_raw_linear_problem &p) {
+  return p.K % 8 == 0 && rows_ok(p.w, 0, p.ldw, 2) && p.ldw < (1ll << 40) && (256 * p.ldw + p.K) * 2 < (1ll << 31) - 4096;
+}
+bool dma_ok_x(const selas_raw_linear_problem &p) {
+  if (p.K % 8 || !rows_ok(p.x, p.x_sb, p.x_sl, 2) || p.x_sl >= (1ll << 40) || p.x_sb >= (1ll << 40)) return false;
   const int64_t rows = 256, gap = p.x_sb - (p.L - 1) * p.x_sl, crossings = p.B > 1 ? rows / p.L + 1 : 0;
-  if (p.x_sl >= (1ll << 40) || p.x_sb >= (1ll << 40) || p.ldw >= (1ll << 40)) return false;
   const int64_t span = gap >= 0 || p.B == 1 ? rows * p.x_sl + crossings * gap : p.L * p.x_sl + crossings * p.x_sb;
-  return (span + p.K) * 2 < (1ll << 31) - 4096 && (rows * p.ldw + p.K) * 2 < (1ll << 31) - 4096;
+  return (span + p.K) * 2 < (1ll << 31) - 4096;
 }
 
 // The current device's CU count (asked once per device).
@@ -944,15 +995,16 @@ int cu_count() {
   return v;
 }
 
-// How a problem runs. kFew, kStream and kAny are launches of their own; the tiled problems of a call share one.
-enum class Route { kEmpty, kFew, kStream, kTiled, kAny };
+// How a problem runs. kFew and kStream are launches of their own; the tiled problems of a call share one.
+enum class Route { kEmpty, kFew, kStream, kTiled };
 
 struct Plan {
   Route route[kMaxProblems];
   int few_split[kMaxProblems];  // K ranges of a kFew or kStream problem
   int tile, split;              // of the tiled launch
-  int64_t part[kMaxProblems];   // floats of each problem's partial sums
-  int64_t floats;
+  // The workspace, in 16-byte units: each problem's partial sums, then its packed x and w (0: none).
+  int64_t part[kMaxProblems], pack_x[kMaxProblems], pack_w[kMaxProblems];
+  int64_t units;
 };
 
 // Few rows: 32 of x (33 to 64 run faster as tiles: 60 x 9216 x 3072 25 us against 29), 64 of the weight (1024 x 64 x
@@ -1018,13 +1070,14 @@ Plan make_plan(const selas_raw_linear_problem *problems, int64_t count) {
     if (M == 0 || p.N == 0) {
       plan.route[i] = Route::kEmpty;
     } else if (M <= kFewX || p.N <= kFewW) {
-      plan.route[i] = tiled_ok(p) ? Route::kStream : Route::kFew;
+      plan.route[i] = dma_ok_x(p) && dma_ok_w(p) ? Route::kStream : Route::kFew;
       plan.few_split[i] = few_split(M <= kFewX ? p.N : M, p.K);
-    } else if (tiled_ok(p)) {
+    } else {
       plan.route[i] = Route::kTiled;
       tiled = true;
-    } else {
-      plan.route[i] = Route::kAny;
+      const int64_t chunks = cdiv(p.K, 64) * 8;
+      if (!dma_ok_x(p)) plan.pack_x[i] = M * chunks;
+      if (!dma_ok_w(p)) plan.pack_w[i] = p.N * chunks;
     }
   }
   if (tiled) {
@@ -1034,8 +1087,8 @@ Plan make_plan(const selas_raw_linear_problem *problems, int64_t count) {
   }
   for (int64_t i = 0; i < count; ++i) {
     const int split = plan.route[i] == Route::kTiled ? plan.split : plan.few_split[i];
-    plan.part[i] = split > 1 ? split * problems[i].B * problems[i].L * problems[i].N : 0;
-    plan.floats += (plan.part[i] + 3) / 4 * 4;
+    plan.part[i] = split > 1 ? cdiv(split * problems[i].B * problems[i].L * problems[i].N, 4) : 0;
+    plan.units += plan.part[i] + plan.pack_x[i] + plan.pack_w[i];
   }
   return plan;
 }
@@ -1107,17 +1160,42 @@ int launch_tiled(RawBatch &batch, const Plan &plan, hipStream_t s) {
 }
 
 template <int DT>
-int launch_plan(const selas_raw_linear_problem *problems, int64_t count, const Plan &plan, float *ws, hipStream_t s) {
+int launch_pack(RawProblem &P, uint4 *xp, uint4 *wp, hipStream_t s) {
+  const int kp = static_cast<int>(cdiv(P.K, 64)) * 64;
+  const int64_t chunks = (static_cast<int64_t>(xp ? P.M : 0) + (wp ? P.N : 0)) * (kp / 8);
+  if (chunks == 0) return ok();
+  if (cdiv(chunks, 256) >= (1ll << 31)) return set_error(SELAS_EUNSUPPORTED, "raw_linear: operands too large to copy");
+  raw_pack_kernel<DT><<<dim3(static_cast<uint32_t>(cdiv(chunks, 256))), dim3(256), 0, s>>>(
+      P, reinterpret_cast<uint16_t *>(xp), reinterpret_cast<uint16_t *>(wp), kp);
+  if (xp) {
+    P.x = xp;
+    P.x_sl = kp;
+    P.x_sb = static_cast<int64_t>(P.L) * kp;
+  }
+  if (wp) {
+    P.w = wp;
+    P.ldw = kp;
+  }
+  // An operand that stays where it is has no columns past K, so K grows only where both were copied.
+  if (xp && wp) P.K = kp;
+  return check_launch("raw_linear");
+}
+
+template <int DT>
+int launch_plan(const selas_raw_linear_problem *problems, int64_t count, const Plan &plan, uint4 *ws, hipStream_t s) {
   RawBatch batch{};
   for (int64_t i = 0; i < count; ++i) {
     if (plan.route[i] == Route::kEmpty) continue;
-    const RawProblem P = make_problem(problems[i]);
-    float *part = plan.part[i] ? ws : nullptr;
-    ws += (plan.part[i] + 3) / 4 * 4;
+    RawProblem P = make_problem(problems[i]);
+    float *const part = plan.part[i] ? reinterpret_cast<float *>(ws) : nullptr;
+    uint4 *const xp = plan.pack_x[i] ? ws + plan.part[i] : nullptr;
+    uint4 *const wp = plan.pack_w[i] ? ws + plan.part[i] + plan.pack_x[i] : nullptr;
+    ws += plan.part[i] + plan.pack_x[i] + plan.pack_w[i];
     if (plan.route[i] == Route::kTiled) {
+      if (int e = launch_pack<DT>(P, xp, wp, s)) return e;
       batch.part[batch.count] = part;
       batch.p[batch.count++] = P;
-    } else if (int e = plan.route[i] != Route::kAny ? launch_few<DT>(P, plan.route[i] == Route::kStream, part, plan.few_split[i], s) : launch_any<DT>(P, s)) {
+    } else if (int e = launch_few<DT>(P, plan.route[i] == Route::kStream, part, plan.few_split[i], s)) {
       return e;
     }
   }
@@ -1145,7 +1223,7 @@ extern "C" int selas_raw_linear_workspace_bytes(const selas_raw_linear_problem *
   if (!bytes) return set_error(SELAS_EINVAL, "raw_linear: null result");
   *bytes = 0;
   if (int e = check_call(problems, count, dtype)) return e;
-  *bytes = make_plan(problems, count).floats * 4;
+  *bytes = make_plan(problems, count).units * 16;
   return ok();
 }
 
@@ -1158,11 +1236,11 @@ extern "C" int selas_raw_linear(const selas_raw_linear_problem *problems, int64_
     if (!p.y || (p.K && (!p.x || !p.w))) return set_error(SELAS_EINVAL, "raw_linear[%lld]: null pointer", (long long)i);
   }
   const Plan plan = make_plan(problems, count);
-  if (plan.floats && (!workspace || workspace_bytes < plan.floats * 4 || !aligned(workspace, 16)))
+  if (plan.units && (!workspace || workspace_bytes < plan.units * 16 || !aligned(workspace, 16)))
     return set_error(SELAS_EINVAL, "raw_linear: needs a 16-byte aligned workspace of %lld bytes",
-                     (long long)(plan.floats * 4));
+                     (long long)(plan.units * 16));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  float *ws = static_cast<float *>(workspace);
+  uint4 *ws = static_cast<uint4 *>(workspace);
   return dtype == SELAS_BF16 ? launch_plan<SELAS_BF16>(problems, count, plan, ws, s)
                              : launch_plan<SELAS_F16>(problems, count, plan, ws, s);
 }
