@@ -16,9 +16,19 @@ def distinct(t: torch.Tensor) -> bool:
     return True
 
 
+def _as_rows(t: torch.Tensor) -> torch.Tensor:
+    """A tensor of at most four dims as [B, heads, L, C]."""
+    if t.dim() == 3:
+        return t.unsqueeze(1)
+    while t.dim() < 4:
+        t = t.unsqueeze(0)
+    return t
+
+
 def may_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors (non-negative strides) may share an element. False for address ranges apart, and for two
-    [B, heads, L, Dh] tensors at different columns of one matrix of rows: the q, k and v of one linear's output."""
+    [..., L, C] or [B, heads, L, C] tensors at different columns of one matrix of rows: the q, k and v of one linear's
+    output, the two halves of a linear's input."""
     if a.numel() == 0 or b.numel() == 0:
         return False
     size = a.element_size()
@@ -26,11 +36,12 @@ def may_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
             for t in (a, b)]
     if ends[0] <= b.data_ptr() or ends[1] <= a.data_ptr():
         return False
-    if a.dim() != 4 or b.dim() != 4 or b.element_size() != size:
+    gap = b.data_ptr() - a.data_ptr()
+    if a.dim() > 4 or b.dim() > 4 or b.element_size() != size or gap % size:
         return True
-    row, gap = a.stride(2), b.data_ptr() - a.data_ptr()
-    if (row <= 0 or row != b.stride(2) or a.stride(0) != b.stride(0) or gap % size
-            or (a.shape[0] > 1 or b.shape[0] > 1) and a.stride(0) % row):
+    a, b = _as_rows(a), _as_rows(b)
+    row = a.stride(2)
+    if row <= 0 or row != b.stride(2) or any(t.shape[0] > 1 and t.stride(0) % row for t in (a, b)):
         return True
     # Each tensor keeps to columns [at, at + width) of every row, counted from a's first.
     width = [(t.shape[1] - 1) * t.stride(1) + (t.shape[3] - 1) * t.stride(3) + 1 for t in (a, b)]

@@ -26,6 +26,7 @@ import torch.nn.functional as F
 from .codecs import EncodedTensor, encode_int8_row, encode_nf4, encode_raw
 from .kernels import FUSED, Kernels
 from .linear import UnitView, linear_grouped_into
+from .rope import rope_qk
 
 
 @dataclass
@@ -126,9 +127,40 @@ def _linear_pair(w, a, b):
     return ya, yb
 
 
+def _fused_raw(w, k) -> bool:
+    """Whether the unit's raw weights run through raw_linear, with the activation, gate and residual in its epilogue."""
+    return isinstance(k, Kernels) and getattr(w, "fused_raw", False)
+
+
+def _qkv_rope(qkv, q_scale, k_scale, ids, cfg: FluxConfig, out=None):
+    """(q, k, v) [B, H, L, Dh] of a linear's qkv columns, normed and turned by positions of each image's own."""
+    q, k, v = qkv.unflatten(-1, (3, cfg.heads, cfg.head_dim)).permute(2, 0, 3, 1, 4)
+    return rope_qk(q, k, ids, cfg.axes_dim, cfg.theta, v=v, q_scale=q_scale, k_scale=k_scale, out=out)
+
+
+def _qkv_double(w, k, tqkv, iqkv, cos, sin, ids, cfg: FluxConfig, dt):
+    scales = [w.get(f"{s}_attn.norm.{n}_norm.scale", torch.float32) for s in ("txt", "img") for n in ("query", "key")]
+    if ids is None:
+        return k.qkv_double(tqkv, iqkv, *scales, cos, sin, cfg.heads, dt)
+    b, lt, li = tqkv.shape[0], tqkv.shape[1], iqkv.shape[1]
+    joint = [torch.empty(b, cfg.heads, lt + li, cfg.head_dim, dtype=dt, device=tqkv.device) for _ in range(3)]
+    _qkv_rope(tqkv, scales[0], scales[1], ids[:, :lt], cfg, [t[:, :, :lt] for t in joint])
+    _qkv_rope(iqkv, scales[2], scales[3], ids[:, lt:], cfg, [t[:, :, lt:] for t in joint])
+    return joint
+
+
+def _qkv_single(w, k, qkv, cos, sin, ids, cfg: FluxConfig, dt):
+    qs, ks = (w.get(f"norm.{n}_norm.scale", torch.float32) for n in ("query", "key"))
+    if ids is None:
+        return k.qkv_single(qkv, qs, ks, cos, sin, cfg.heads, dt)
+    return _qkv_rope(qkv, qs, ks, ids, cfg)
+
+
 def double_block(w, img, txt, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k: Kernels = FUSED, h=None,
-                 next_mod=None):
+                 next_mod=None, ids=None):
     """img [B, Li, D] fp32, txt [B, Lt, D] fp32, mod [B, 12D] (img 6D | txt 6D).
+
+    ``ids`` [B, Lt + Li, axes]: the positions of every image's tokens, in place of cos and sin (then None).
 
     ``h``: the (img, txt) inputs of the attention linears, mod_in of img and txt with this block's first
     shift and scale, when the previous block computed them. With ``next_mod`` (the next double block's
@@ -138,14 +170,29 @@ def double_block(w, img, txt, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k
     i_sh1, i_sc1, i_g1, i_sh2, i_sc2, i_g2 = m[:6]
     t_sh1, t_sc1, t_g1, t_sh2, t_sc2, t_g2 = m[6:]
     lt = txt.shape[1]
-    f32 = torch.float32
     if h is None:
         h = (k.mod_in(img, i_sh1, i_sc1, dt), k.mod_in(txt, t_sh1, t_sc1, dt))
+    if _fused_raw(w, k):
+        # Raw weights: the gated residual adds and the GELU in the linears' epilogues, in fp32 (no 16-bit rounding of the
+        # linear's output, so nothing for the fp16 guard to clamp); the next mod_in is its own kernel.
+        iqkv, tqkv = w.raw_linear_many([(h[0], "img_attn.qkv"), (h[1], "txt_attn.qkv")])
+        del h
+        a = attention(*_qkv_double(w, k, tqkv, iqkv, cos, sin, ids, cfg, dt))
+        del iqkv, tqkv
+        img, txt = w.raw_linear_many([(a[:, lt:], "img_attn.proj", {"gate": i_g1, "residual": img}),
+                                      (a[:, :lt], "txt_attn.proj", {"gate": t_g1, "residual": txt})])
+        del a
+        hi, ht = k.mod_in(img, i_sh2, i_sc2, dt), k.mod_in(txt, t_sh2, t_sc2, dt)
+        hi, ht = w.raw_linear_many([(hi, "img_mlp.0", {"act": "gelu"}), (ht, "txt_mlp.0", {"act": "gelu"})])
+        img, txt = w.raw_linear_many([(hi, "img_mlp.2", {"gate": i_g2, "residual": img}),
+                                      (ht, "txt_mlp.2", {"gate": t_g2, "residual": txt})])
+        if next_mod is None:
+            return img, txt
+        n = next_mod.float().unsqueeze(1).chunk(12, dim=-1)
+        return img, txt, (k.mod_in(img, n[0], n[1], dt), k.mod_in(txt, n[6], n[7], dt))
     iqkv, tqkv = _linear_pair(w, (h[0], "img_attn.qkv"), (h[1], "txt_attn.qkv"))
     del h
-    q, kk, v = k.qkv_double(tqkv, iqkv, w.get("txt_attn.norm.query_norm.scale", f32),
-                            w.get("txt_attn.norm.key_norm.scale", f32), w.get("img_attn.norm.query_norm.scale", f32),
-                            w.get("img_attn.norm.key_norm.scale", f32), cos, sin, cfg.heads, dt)
+    q, kk, v = _qkv_double(w, k, tqkv, iqkv, cos, sin, ids, cfg, dt)
     del iqkv, tqkv
     a = attention(q, kk, v)
     del q, kk, v
@@ -173,16 +220,29 @@ def double_block(w, img, txt, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k
 
 
 def single_block(w, x, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k: Kernels = FUSED, h=None,
-                 next_mod=None):
-    """x [B, Lt+Li, D] fp32, mod [B, 3D].
+                 next_mod=None, ids=None):
+    """x [B, Lt+Li, D] fp32, mod [B, 3D]; ``ids`` as for double_block.
 
     ``h``: linear1's input, mod_in(x) with this block's shift and scale, when the previous block computed
     it. With ``next_mod`` (the next single block's [B, 3D]) the closing residual add also computes the next
     block's ``h`` in the same pass (gated_add_mod) and the result is ``(x, h_next)``."""
     sh, sc, g = mod.float().unsqueeze(1).chunk(3, dim=-1)
-    f32 = torch.float32
     if h is None:
         h = k.mod_in(x, sh, sc, dt)
+
+    if _fused_raw(w, k):
+        b, l, d = x.shape
+        cat = torch.empty(b, l, d + cfg.mlp_hidden, dtype=dt, device=x.device)
+        qkv, _ = w.raw_linear_many([(h, "linear1", {"rows": slice(0, 3 * d)}),
+                                    (h, "linear1", {"rows": slice(3 * d, None), "act": "gelu", "out": cat[..., d:]})])
+        del h
+        attention(*_qkv_single(w, k, qkv, cos, sin, ids, cfg, dt), out=cat[..., :d])
+        del qkv
+        (x,) = w.raw_linear_many([(cat, "linear2", {"gate": g, "residual": x})])
+        if next_mod is None:
+            return x
+        nsh, nsc, _ = next_mod.float().unsqueeze(1).chunk(3, dim=-1)
+        return x, k.mod_in(x, nsh, nsc, dt)
 
     def close(out):
         if next_mod is None:
@@ -197,8 +257,7 @@ def single_block(w, x, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k: Kerne
         cat = torch.empty(b, l, d + cfg.mlp_hidden, dtype=dt, device=x.device)
         ((qkv, _),) = w.linear_gelu_many([(h, "linear1", cfg.mlp_hidden, cat[..., d:])])
         del h
-        q, kk, v = k.qkv_single(qkv, w.get("norm.query_norm.scale", f32), w.get("norm.key_norm.scale", f32), cos,
-                                sin, cfg.heads, dt)
+        q, kk, v = _qkv_single(w, k, qkv, cos, sin, ids, cfg, dt)
         del qkv
         attention(q, kk, v, out=cat[..., :d])
         del q, kk, v
@@ -207,8 +266,7 @@ def single_block(w, x, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k: Kerne
         return close(out)
     h = w.linear(h, "linear1")
     qkv, mlp = h.split([3 * cfg.hidden, cfg.mlp_hidden], dim=-1)
-    q, kk, v = k.qkv_single(qkv, w.get("norm.query_norm.scale", f32), w.get("norm.key_norm.scale", f32), cos, sin,
-                            cfg.heads, dt)
+    q, kk, v = _qkv_single(w, k, qkv, cos, sin, ids, cfg, dt)
     a = attention(q, kk, v)
     del q, kk, v, qkv
     out = w.linear(k.attn_mlp(a, mlp), "linear2")
@@ -218,6 +276,8 @@ def single_block(w, x, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k: Kerne
 
 def final_layer(w, img, fmod, dt, k: Kernels = FUSED):
     sh, sc = fmod.float().unsqueeze(1).chunk(2, dim=-1)
+    if _fused_raw(w, k):
+        return w.raw_linear_many([(k.mod_in(img, sh, sc, dt), "final_layer.linear", {"out_dtype": torch.float32})])[0]
     return w.linear(k.mod_in(img, sh, sc, dt), "final_layer.linear").float()
 
 
@@ -274,14 +334,16 @@ def _linear_parts(gen: _Gen, name: str, n_in: int, n_out: int, dt, quant, std: f
 
 
 class RandomFlux:
-    """A FLUX-shaped transformer with random weights, quantized blocks resident on one GPU.
+    """A FLUX-shaped transformer with random weights, its blocks resident on one GPU.
 
-    ``quant``: "nf4" (default) or "int8" (int8_row) for the block and modulation linears."""
+    ``quant``: "nf4" (default) or "int8" (int8_row) for the block and modulation linears, or "raw" for weights in
+    ``dtype`` (selas's convert without --quant), which run through ``raw_linear`` in bf16 and fp16."""
 
     def __init__(self, cfg: FluxConfig, device, dtype=torch.bfloat16, seed: int = 0, n_double=None, n_single=None,
                  with_mods: bool = True, quant: str = "nf4"):
-        if quant not in ("nf4", "int8"):
-            raise ValueError(f"quant must be 'nf4' or 'int8', got {quant!r}")
+        if quant not in ("nf4", "int8", "raw"):
+            raise ValueError(f"quant must be 'nf4', 'int8' or 'raw', got {quant!r}")
+        raw, quant = quant == "raw", False if quant == "raw" else quant
         self.cfg, self.device, self.dt = cfg, torch.device(device), dtype
         nd = cfg.depth_double if n_double is None else n_double
         ns = cfg.depth_single if n_single is None else n_single
@@ -325,6 +387,8 @@ class RandomFlux:
             if with_mods:
                 self.mods.append(UnitView(_linear_parts(gen, "modulation.lin", d, 3 * d, dtype, quant), dtype))
         del gen
+        for u in (self.globals, *self.doubles, *self.singles, *self.mods):
+            u.fused_raw = raw and dtype in (torch.bfloat16, torch.float16)
 
     def nf4_bytes(self) -> int:
         units = self.doubles + self.singles + self.mods
@@ -365,6 +429,14 @@ class RandomFlux:
                 per.append(len(ps))
             linear_grouped_into(codec, sv, ws, out, per)
             return out
+        if self.mods and all(u.fused_raw for u in self.mods):
+            out = []
+            for j, u in enumerate(self.mods):
+                ps = ("img_mod.lin", "txt_mod.lin") if j < nd else ("modulation.lin",)
+                widths = [u.tensors[p + ".weight"].shape[0] for p in ps]
+                out.append(torch.empty(*sv.shape[:-1], sum(widths), dtype=sv.dtype, device=sv.device))
+                u.raw_linear_many([(sv, p, {"out": o}) for p, o in zip(ps, out[-1].split(widths, dim=-1))])
+            return out
         ys = [u.linear(sv, p) for u, p in pre]
         out, i = [], 0
         for j in range(len(self.mods)):
@@ -378,15 +450,19 @@ class RandomFlux:
 
     @torch.no_grad()
     def step(self, latents, txt, mods_s, final_mod_s, cos, sin, k: Kernels = FUSED,
-             micro_batch: int | None = None) -> torch.Tensor:
+             micro_batch: int | None = None, ids: torch.Tensor | None = None) -> torch.Tensor:
         """Velocity for one step (flux.py:527-582). latents [B, Li, 64] fp32, txt [B, Lt, D] fp32,
         mods_s: per block [B, kD] for this step, final_mod_s [B, 2D]. ``micro_batch``: each block runs
-        the batch in chunks of at most that many images, block by block (flux.py:492-524)."""
+        the batch in chunks of at most that many images, block by block (flux.py:492-524). ``ids`` [B, L, axes]:
+        positions of each image's own, in place of cos and sin."""
         cfg, dt, guard = self.cfg, self.dt, self.dt == torch.float16
         # The blocks use their modulation vectors in fp32 (each block converts its own, flux.py:302, 327):
         # one conversion of all of them is exact and saves a small kernel per block.
         *mods_s, final_mod_s = _fp32_vectors([*mods_s, final_mod_s])
-        img = self.globals.linear(latents.to(dt), "img_in").float()
+        if _fused_raw(self.globals, k):
+            (img,) = self.globals.raw_linear_many([(latents.to(dt), "img_in", {"out_dtype": torch.float32})])
+        else:
+            img = self.globals.linear(latents.to(dt), "img_in").float()
         lt = txt.shape[1]
         nd, ns = len(self.doubles), len(self.singles)
         # Between blocks of one kind, the closing residual add and the next block's mod_in run as one
@@ -399,12 +475,13 @@ class RandomFlux:
         for i, w in enumerate(self.doubles):
             nxt = mods_s[i + 1] if chain and i + 1 < nd else None
             if len(chunks) == 1:
-                r = double_block(w, img, txt, mods_s[i], cos, sin, cfg, dt, guard, k, h, nxt)
+                r = double_block(w, img, txt, mods_s[i], cos, sin, cfg, dt, guard, k, h, nxt, ids)
                 img, txt, h = r if nxt is not None else (*r, None)
                 continue
             outs = [double_block(w, img[a:e], txt[a:e], mods_s[i][a:e], cos, sin, cfg, dt, guard, k,
                                  None if h is None else (h[0][a:e], h[1][a:e]),
-                                 None if nxt is None else nxt[a:e]) for a, e in chunks]
+                                 None if nxt is None else nxt[a:e], None if ids is None else ids[a:e])
+                    for a, e in chunks]
             img, txt = torch.cat([o[0] for o in outs]), torch.cat([o[1] for o in outs])
             h = (torch.cat([o[2][0] for o in outs]), torch.cat([o[2][1] for o in outs])) if nxt is not None else None
             del outs
@@ -414,11 +491,12 @@ class RandomFlux:
         for j, w in enumerate(self.singles):
             nxt = mods_s[nd + j + 1] if chain and j + 1 < ns else None
             if len(chunks) == 1:
-                r = single_block(w, x, mods_s[nd + j], cos, sin, cfg, dt, guard, k, h, nxt)
+                r = single_block(w, x, mods_s[nd + j], cos, sin, cfg, dt, guard, k, h, nxt, ids)
                 x, h = r if nxt is not None else (r, None)
                 continue
             outs = [single_block(w, x[a:e], mods_s[nd + j][a:e], cos, sin, cfg, dt, guard, k,
-                                 None if h is None else h[a:e], None if nxt is None else nxt[a:e]) for a, e in chunks]
+                                 None if h is None else h[a:e], None if nxt is None else nxt[a:e],
+                                 None if ids is None else ids[a:e]) for a, e in chunks]
             if nxt is not None:
                 x, h = torch.cat([o[0] for o in outs]), torch.cat([o[1] for o in outs])
             else:
@@ -445,6 +523,9 @@ def timestep_embedding(t: torch.Tensor, dim: int = 256, max_period: float = 1000
 
 def mlp_embed(w, prefix: str, x: torch.Tensor) -> torch.Tensor:
     """in_layer, SiLU, out_layer (flux.py:150-151)."""
+    if getattr(w, "fused_raw", False):
+        (h,) = w.raw_linear_many([(x, prefix + ".in_layer", {"act": "silu"})])
+        return w.raw_linear_many([(h, prefix + ".out_layer")])[0]
     return w.linear(F.silu(w.linear(x, prefix + ".in_layer")), prefix + ".out_layer")
 
 
@@ -476,15 +557,17 @@ def get_schedule(num_steps: int, image_seq_len: int, base_shift: float = 0.5, ma
 @dataclass
 class FluxConditioning:
     """Everything a step needs besides the latents (flux.py:365-373): per block [S, B, kD] modulations,
-    the final layer's [S, B, 2D], the text stream after txt_in [B, Lt, D] fp32 and the RoPE tables."""
+    the final layer's [S, B, 2D], the text stream after txt_in [B, Lt, D] fp32 and the RoPE tables, or, where
+    the images of the batch stand at positions of their own, those positions ``ids`` [B, L, axes]."""
 
     sigmas: list
     mods: dict
     final_mod: torch.Tensor
     txt: torch.Tensor
-    cos: torch.Tensor
-    sin: torch.Tensor
+    cos: torch.Tensor | None
+    sin: torch.Tensor | None
     l_txt: int
+    ids: torch.Tensor | None = None
 
 
 @dataclass
@@ -539,14 +622,26 @@ class FluxRunner:
     def prepare(self, sigmas, guidance: float, pooled: torch.Tensor, txt: torch.Tensor, img_ids: torch.Tensor,
                 txt_ids: torch.Tensor, mods: dict[str, torch.Tensor] | None = None) -> FluxConditioning:
         """Everything that does not depend on the latents, once per batch (flux.py:448-465). ``mods``: the
-        batch's modulation vectors {block: [S, B, kD]} when already known."""
+        batch's modulation vectors {block: [S, B, kD]} when already known. ``img_ids`` [Li, axes], or
+        [B, Li, axes] for images of other shapes or offsets with the same number of tokens (a portrait and a
+        landscape, windows of one canvas)."""
         cfg, g, dt, dev = self.cfg, self.g, self.dt, self.model.device
         svecs = [self.svec(sigmas, guidance, pooled[i:i + 1]) for i in range(pooled.shape[0])]
         if mods is None:
             per_image = self.modulations(svecs)
             mods = {n: torch.cat([m[n] for m in per_image], dim=1) for n in self.main}
-        final_mod = torch.cat([g.linear(sv, "final_layer.adaLN_modulation.1") for sv in svecs], dim=1)
-        txt_h = g.linear(txt.to(dev, dt), "txt_in").float()
+        if getattr(g, "fused_raw", False):
+            final_mod = torch.cat([g.raw_linear_many([(sv, "final_layer.adaLN_modulation.1")])[0] for sv in svecs], dim=1)
+            (txt_h,) = g.raw_linear_many([(txt.to(dev, dt), "txt_in", {"out_dtype": torch.float32})])
+        else:
+            final_mod = torch.cat([g.linear(sv, "final_layer.adaLN_modulation.1") for sv in svecs], dim=1)
+            txt_h = g.linear(txt.to(dev, dt), "txt_in").float()
+        if img_ids.dim() == 3:
+            b = pooled.shape[0]
+            if img_ids.shape[0] not in (1, b):
+                raise ValueError(f"img_ids {tuple(img_ids.shape)} for a batch of {b}")
+            each = torch.cat([t.to(dev).expand(b, *t.shape[-2:]) for t in (txt_ids.to(img_ids.dtype), img_ids)], dim=1)
+            return FluxConditioning(list(sigmas), mods, final_mod, txt_h, None, None, txt.shape[1], each)
         ids = torch.cat((txt_ids, img_ids), dim=0).to(dev)
         cos, sin = rope_tables(ids, cfg.axes_dim, cfg.theta)
         return FluxConditioning(list(sigmas), mods, final_mod, txt_h, cos, sin, txt.shape[1])
@@ -559,7 +654,7 @@ class FluxRunner:
             raise NotImplementedError("the step cache is not supported by selas_amd's runner")
         mods_s = [cond.mods[n][s] for n in self.main]
         out = self.model.step(latents, cond.txt, mods_s, cond.final_mod[s], cond.cos, cond.sin, self.k,
-                              self.micro_batch)
+                              self.micro_batch, cond.ids)
         return out, StepInfo()
 
     @torch.no_grad()

@@ -626,13 +626,16 @@ class UnitView:
     and ``buf`` is the unit's 1-D uint8 device buffer; parts are viewed in place (part_view), never
     copied. ``UnitView(tensors, dtype)`` takes a dict of :class:`EncodedTensor` with device parts
     instead. ``get`` decodes (raw tensors in the compute dtype are returned as zero-copy views and
-    cached), ``linear`` is the quantized-linear forward.
+    cached), ``linear`` is the quantized-linear forward. With ``fused_raw`` set, the callers in
+    ``selas_amd.flux`` run a unit of raw weights through ``raw_linear_many`` (bf16 or fp16 weights in the compute
+    dtype) instead of ``F.linear`` and separate kernels after it.
     """
 
-    __slots__ = ("tensors", "dtype", "_views", "spec", "buf")
+    __slots__ = ("tensors", "dtype", "_views", "spec", "buf", "fused_raw")
 
     def __init__(self, spec_or_tensors, buf_or_dtype, dtype: torch.dtype | None = None):
         self._views: dict[tuple, torch.Tensor] = {}
+        self.fused_raw = False
         if dtype is None:  # (tensors, dtype)
             self.spec, self.buf = None, None
             self.tensors: dict[str, EncodedTensor] = spec_or_tensors
@@ -721,3 +724,16 @@ class UnitView:
         if codec is not None:
             return _single(codec, prob)
         return F.linear(x, self.get(prefix + ".weight", dtype), prob)
+
+    def raw_linear_many(self, items) -> list[torch.Tensor]:
+        """``raw_linear`` of each (x, prefix) or (x, prefix, options) item with this unit's raw weights, up to four
+        independent ones per launch. ``options``: the keyword arguments of ``raw_linear``, and "rows", a slice of
+        the weight's (and bias's) rows."""
+        problems = []
+        for x, prefix, *rest in items:
+            options = dict(rest[0]) if rest else {}
+            rows = options.pop("rows", slice(None))
+            bname = prefix + ".bias"
+            problems.append(RawLinear(x, self.get(prefix + ".weight")[rows],
+                                      self.get(bname)[rows] if bname in self.tensors else None, **options))
+        return raw_linear_batched(problems)
