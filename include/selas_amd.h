@@ -519,6 +519,14 @@ int selas_raw_linear(const selas_raw_linear_problem *problems, int64_t count, in
 int selas_raw_linear_workspace_bytes(const selas_raw_linear_problem *problems, int64_t count, int dtype,
                                      int64_t *bytes);
 
+/*
+ * Rows of x and of w per output tile of that launch, and its K ranges per tile (0, 0, 0 where
+ * no problem is tiled: at most 32 rows, or 64 columns). It says which kernel a size runs, for
+ * measurements and tests.
+ */
+int selas_raw_linear_tile(const selas_raw_linear_problem *problems, int64_t count, int dtype, int64_t *rows,
+                          int64_t *cols, int64_t *ranges);
+
 #ifdef __cplusplus
 }
 #endif

@@ -60,6 +60,7 @@ SIGNATURES: dict[str, list] = {
     "selas_rope": [_P, _I64, _I64, _I64, _I64, _P, _INT, _I64, _I64, _I64, _P, ctypes.c_double, _INT, _INT, _INT, _P],
     "selas_raw_linear": [_P, _I64, _INT, _P, _I64, _P],
     "selas_raw_linear_workspace_bytes": [_P, _I64, _INT, ctypes.POINTER(ctypes.c_int64)],
+    "selas_raw_linear_tile": [_P, _I64, _INT] + [ctypes.POINTER(ctypes.c_int64)] * 3,
 }
 
 

@@ -998,10 +998,15 @@ int cu_count() {
 // How a problem runs. kFew and kStream are launches of their own; the tiled problems of a call share one.
 enum class Route { kEmpty, kFew, kStream, kTiled };
 
+// Rows of x and of w per tile, K ranges per tile.
+struct TileChoice {
+  int tm, tn, split;
+};
+
 struct Plan {
   Route route[kMaxProblems];
   int few_split[kMaxProblems];  // K ranges of a kFew or kStream problem
-  int tile, split;              // of the tiled launch
+  TileChoice tile;              // of the tiled launch
   // The workspace, in 16-byte units: each problem's partial sums, then its packed x and w (0: none).
   int64_t part[kMaxProblems], pack_x[kMaxProblems], pack_w[kMaxProblems];
   int64_t units;
@@ -1024,37 +1029,43 @@ int few_split(int64_t big, int64_t K) {
   return split;
 }
 
-// Tile and K ranges of the tiled launch: the fastest by this model of a launch in us, fitted to 108 shapes (40 to 4608
-// rows, 64 to 21504 columns, K 512 to 12288, every tile and split timed), where its choices are within 1.5 % of the
-// fastest in the mean and 16 % at worst. A round is one tile on every CU; a step of K costs the more the more CUs are
-// busy (the power limit); a split launch pays for its second kernel and for writing and reading the partial sums.
-struct TileChoice {
-  int tile, split;
+// Tile and K ranges of the tiled launch: the fastest by this model of a launch in us, fitted to 272 shapes (40 to 4608
+// rows, 256 to 21504 columns, K 256 to 12288, every tile and split timed); its choices are within 1.2 % of the fastest in
+// the mean and 23 % at worst (square tiles alone: 1.5 % and 16 %, of a best that is up to 18 % slower: 1536 x 3072 x 3072
+// 40.7 us against 34.8). A round is one tile on every CU; a step of K costs the more the more CUs are busy (the power
+// limit); a split launch pays for its second kernel and for writing and reading the partial sums.
+struct TileCost {
+  int tm, tn;
+  double start, step, busy, round;
 };
+constexpr TileCost kTiles[] = {{256, 256, 15.1, 0.51, 0.34, 6.0},
+                               {256, 128, 8.7, 0.36, 0.23, 4.0},
+                               {128, 256, 8.7, 0.36, 0.23, 4.0},
+                               {128, 128, 7.1, 0.29, 0.11, 0.34}};
+
 TileChoice pick_tile(const selas_raw_linear_problem *problems, const Plan &plan, int64_t count) {
   const int cus = cu_count();
-  TileChoice best{256, 1};
+  TileChoice best{256, 256, 1};
   double best_us = 1e30;
-  for (int tile : {256, 128})
+  for (const TileCost &t : kTiles)
     for (int split : {1, 2, 3, 4, 6, 8, 12}) {
       int64_t tiles = 0, steps = 0, sums = 0, merges = 0;
       for (int64_t i = 0; i < count; ++i) {
         if (plan.route[i] != Route::kTiled) continue;
         const selas_raw_linear_problem &p = problems[i];
-        tiles += cdiv(p.B * p.L, tile) * cdiv(p.N, tile);
+        tiles += cdiv(p.B * p.L, t.tm) * cdiv(p.N, t.tn);
         steps = steps > cdiv(p.K, 64) ? steps : cdiv(p.K, 64);
         sums += p.B * p.L * p.N;
         ++merges;
       }
       const int64_t items = tiles * split, rounds = cdiv(items, cus);
       if (split > 1 && (steps < 3 * split || items > 2 * cus)) continue;
-      const double busy = items < cus ? static_cast<double>(items) / cus : 1.0, per = static_cast<double>(cdiv(steps, split));
-      double us = tile == 256 ? 13.0 + (0.67 + 0.30 * busy) * per * rounds + 4.0 * (rounds - 1)
-                              : 6.5 + (0.315 + 0.13 * busy) * per * rounds + 0.7 * (rounds - 1);
-      if (split > 1) us += 3.4 * merges + 1e-6 * split * sums;
+      const double busy = items < cus ? static_cast<double>(items) / cus : 1.0;
+      double us = t.start + (t.step + t.busy * busy) * cdiv(steps, split) * rounds + t.round * (rounds - 1);
+      if (split > 1) us += 3.35 * merges + 1.15e-6 * split * sums;
       if (us < best_us) {
         best_us = us;
-        best = TileChoice{tile, split};
+        best = TileChoice{t.tm, t.tn, split};
       }
     }
   return best;
@@ -1080,13 +1091,9 @@ Plan make_plan(const selas_raw_linear_problem *problems, int64_t count) {
       if (!dma_ok_w(p)) plan.pack_w[i] = p.N * chunks;
     }
   }
-  if (tiled) {
-    const TileChoice c = pick_tile(problems, plan, count);
-    plan.tile = c.tile;
-    plan.split = c.split;
-  }
+  if (tiled) plan.tile = pick_tile(problems, plan, count);
   for (int64_t i = 0; i < count; ++i) {
-    const int split = plan.route[i] == Route::kTiled ? plan.split : plan.few_split[i];
+    const int split = plan.route[i] == Route::kTiled ? plan.tile.split : plan.few_split[i];
     plan.part[i] = split > 1 ? cdiv(split * problems[i].B * problems[i].L * problems[i].N, 4) : 0;
     plan.units += plan.part[i] + plan.pack_x[i] + plan.pack_w[i];
   }
@@ -1130,12 +1137,12 @@ int launch_few(const RawProblem &P, bool stream, float *part, int split, hipStre
 template <int DT>
 int launch_tiled(RawBatch &batch, const Plan &plan, hipStream_t s) {
   batch.tiles = 0;
-  batch.split = plan.split;
+  batch.split = plan.tile.split;
   bool tail = false;
   for (int i = 0; i < batch.count; ++i) {
     const RawProblem &P = batch.p[i];
-    batch.tiles_m[i] = static_cast<int>(cdiv(P.M, plan.tile));
-    batch.tiles_n[i] = static_cast<int>(cdiv(P.N, plan.tile));
+    batch.tiles_m[i] = static_cast<int>(cdiv(P.M, plan.tile.tm));
+    batch.tiles_n[i] = static_cast<int>(cdiv(P.N, plan.tile.tn));
     batch.tile0[i] = batch.tiles;
     if (static_cast<int64_t>(batch.tiles_m[i]) * batch.tiles_n[i] >= (1ll << 24) - batch.tiles)
       return set_error(SELAS_EUNSUPPORTED, "raw_linear: too many tiles");
@@ -1149,13 +1156,15 @@ int launch_tiled(RawBatch &batch, const Plan &plan, hipStream_t s) {
     if (tail) raw_tile_kernel<DT, 2, 2, MB, NB, OCC, true><<<grid, blk, 0, s>>>(batch); \
     else raw_tile_kernel<DT, 2, 2, MB, NB, OCC, false><<<grid, blk, 0, s>>>(batch);     \
   } while (0)
-  if (plan.tile == 256) SELAS_TILE(8, 8, 1);
+  if (plan.tile.tm == 256 && plan.tile.tn == 256) SELAS_TILE(8, 8, 1);
+  else if (plan.tile.tm == 256) SELAS_TILE(8, 4, 1);
+  else if (plan.tile.tn == 256) SELAS_TILE(4, 8, 1);
   else SELAS_TILE(4, 4, 2);
 #undef SELAS_TILE
   if (int e = check_launch("raw_linear")) return e;
-  if (plan.split > 1)
+  if (batch.split > 1)
     for (int i = 0; i < batch.count; ++i)
-      if (int e = launch_merge<DT>(batch.p[i], batch.part[i], plan.split, s)) return e;
+      if (int e = launch_merge<DT>(batch.p[i], batch.part[i], batch.split, s)) return e;
   return ok();
 }
 
@@ -1224,6 +1233,18 @@ extern "C" int selas_raw_linear_workspace_bytes(const selas_raw_linear_problem *
   *bytes = 0;
   if (int e = check_call(problems, count, dtype)) return e;
   *bytes = make_plan(problems, count).units * 16;
+  return ok();
+}
+
+extern "C" int selas_raw_linear_tile(const selas_raw_linear_problem *problems, int64_t count, int dtype, int64_t *rows,
+                                     int64_t *cols, int64_t *ranges) {
+  if (!rows || !cols || !ranges) return set_error(SELAS_EINVAL, "raw_linear: null result");
+  *rows = *cols = *ranges = 0;
+  if (int e = check_call(problems, count, dtype)) return e;
+  const Plan plan = make_plan(problems, count);
+  *rows = plan.tile.tm;
+  *cols = plan.tile.tn;
+  *ranges = plan.tile.split;
   return ok();
 }
 

@@ -9,6 +9,7 @@ half a step of the output's type."""
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -107,6 +108,30 @@ def test_each_part_of_the_epilogue_alone(dev, which):
     y = raw_linear(x.to(dev), w.to(dev), **{n: t.to(dev) for n, t in kw.items()})
     assert y.dtype == BF
     check(y, reference(x, w, **kw))
+
+
+def tile(m, n, k):
+    out = [ctypes.c_int64() for _ in range(3)]
+    p = _lib.RAW_LINEAR_PROBLEM.pack(4096, 0, k, 4096, k, 0, 0, 0, 0, 0, 0, 4096, 0, n, 1, m, n, k, 0, 0, 0, 2, 0, 0)
+    _lib.call("selas_raw_linear_tile", p, 1, _lib.BF16, *map(ctypes.byref, out))
+    return tuple(o.value for o in out)
+
+
+# Every tile and both kinds of K (whole steps of 64 or not), whole and split, with sizes that fill no tile.
+@pytest.mark.parametrize("m,n,k,want", [(700, 12280, 1088, (256, 256, 1)), (700, 12279, 1352, (256, 256, 1)),
+                                        (2040, 2056, 8200, (256, 256, 3)), (2040, 2056, 320, (256, 128, 1)),
+                                        (2040, 2056, 1352, (256, 128, 1)), (130, 6008, 6152, (256, 128, 4)),
+                                        (300, 12280, 320, (128, 256, 1)), (300, 12279, 1352, (128, 256, 1)),
+                                        (100, 12280, 6152, (128, 256, 4)), (300, 500, 640, (128, 128, 1)),
+                                        (300, 1000, 1352, (128, 128, 1)), (100, 300, 1352, (128, 128, 6))])
+def test_every_tile_on_whole_numbers(dev, m, n, k, want):
+    if torch.cuda.get_device_properties(dev).multi_processor_count == 256:  # the choice goes by the CU count
+        assert tile(m, n, k) == want
+    x, w = ints((m, k), 1).to(dev), ints((n, k), 2).to(dev)
+    bias, gate, res = ints((n,), 3, dtype=F32).to(dev), ints((n,), 4, dtype=F32).to(dev), ints((m, n), 5, dtype=F32).to(dev)
+    z = x.double() @ w.double().t() + bias.double()
+    assert torch.equal(raw_linear(x, w, bias, gate=gate, residual=res).double(), res.double() + gate.double() * z)
+    assert torch.equal(raw_linear(x, w, bias), z.to(BF))
 
 
 def test_gate_shapes(dev):

@@ -163,3 +163,22 @@ def test_python_refusals_before_any_device_work():
             rope_qk(*args)
     with pytest.raises(ValueError, match="pairs"):
         rope_qk(q, q, torch.zeros(3, 1), (8,), pairs="both")
+
+
+def tile(m, n, k, *more):
+    ps = [problem(L=m, N=n, K=k, x_sl=k, ldw=k, y_sl=n) for m, n, k in ((m, n, k), *more)]
+    out = [ctypes.c_int64(-1) for _ in range(3)]
+    _lib.call("selas_raw_linear_tile", b"".join(ps), len(ps), _lib.BF16, *map(ctypes.byref, out))
+    return tuple(o.value for o in out)
+
+
+def test_tiles_and_ranges():
+    # Full grids run whole wide tiles, narrow ones fill the CUs of smaller grids, long K of few tiles is split.
+    assert tile(4608, 3072, 15360) == (256, 256, 1) and tile(4096, 12288, 3072) == (256, 256, 1)
+    rows, cols, ranges = tile(1536, 3072, 3072)
+    assert {rows, cols} == {128, 256} and ranges == 1
+    assert tile(512, 3072, 3072)[:2] == (128, 128) and tile(512, 3072, 12288)[2] > 1
+    assert tile(32, 3072, 3072) == tile(4096, 64, 3072) == tile(0, 64, 64) == (0, 0, 0)
+    assert tile(28, 96, 64, (4608, 3072, 15360)) == (256, 256, 1)  # the few rows do not count
+    with pytest.raises(ValueError, match="null"):
+        _lib.call("selas_raw_linear_tile", problem(), 1, _lib.BF16, None, None, None)
