@@ -541,9 +541,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
   constexpr int DX = XB / (1024 * NW), DW = WB / (1024 * NW);  // DMAs of a wave per half
   constexpr int ER = 32;                                   // rows that the epilogue stages at once
   constexpr int EB = ER * NB * 16 * 4;                     // bytes of them
-  static_assert(DX >= 1 && DW >= 1 && NW <= 8 && XB <= 16384 && WB <= 16384, "tile");
-  constexpr bool kStageX = XB >= EB;
-  static_assert((kStageX ? XB : WB) >= EB && (NW <= 4 || XB == WB), "epilogue");
+  static_assert(NW == 4 && DX >= 1 && DW >= 1 && XB <= 16384 && WB <= 16384 && XB >= EB, "tile");
   __shared__ __attribute__((aligned(1024))) uint8_t x00[XB], x01[XB], x10[XB], x11[XB], w00[WB], w01[WB], w10[WB], w11[WB];
 
   const int item = (blockIdx.x & 7) * batch.per_xcd + (blockIdx.x >> 3);
@@ -724,13 +722,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
 
   // Epilogue: each wave passes its outputs, 32 rows at a time, through its own part of LDS, so that a lane owns W
   // adjacent columns and a row leaves in whole lines.
-  uint8_t *st;
-  {
-    uint8_t *const a0 = kStageX ? x00 : w00, *const a1 = kStageX ? x01 : w01, *const a2 = kStageX ? x10 : w10,
-                   *const a3 = kStageX ? x11 : w11;
-    st = wave == 0 ? a0 : wave == 1 ? a1 : wave == 2 ? a2 : wave == 3 ? a3 : wave == 4 ? w00 : wave == 5 ? w01
-         : wave == 6 ? w10 : w11;
-  }
+  uint8_t *const st = wave == 0 ? x00 : wave == 1 ? x01 : wave == 2 ? x10 : x11;
   const int nw = n0 + wn * NB * 16;  // first column of this wave
   auto stage = [&](int e) __attribute__((always_inline)) {
     for_each_index<MB / 2>([&](auto part) __attribute__((always_inline)) {
@@ -1029,19 +1021,19 @@ int few_split(int64_t big, int64_t K) {
   return split;
 }
 
-// Tile and K ranges of the tiled launch: the fastest by this model of a launch in us, fitted to 272 shapes (40 to 4608
-// rows, 256 to 21504 columns, K 256 to 12288, every tile and split timed); its choices are within 1.2 % of the fastest in
-// the mean and 23 % at worst (square tiles alone: 1.5 % and 16 %, of a best that is up to 18 % slower: 1536 x 3072 x 3072
-// 40.7 us against 34.8). A round is one tile on every CU; a step of K costs the more the more CUs are busy (the power
-// limit); a split launch pays for its second kernel and for writing and reading the partial sums.
+// Tile and K ranges of the tiled launch: the fastest by this model of a launch in us, fitted to 288 shapes (40 to 4608
+// rows, 256 to 21504 columns, K 256 to 12288, weights from HBM; every tile and split timed). Its choices are within 1 %
+// of the fastest in the mean and 18 % at worst (384 x 12288 x 3072: 40 us in tiles of 256 x 128, 54 of 128 x 128; 1024 x
+// 12288 x 3072: 67 us of 256 x 256, 84 of 128 x 128; tiles of 128 x 256 were ahead in 13 shapes, by 0.3 % over all, and
+// are left out). A round is one tile on every CU; a step of K costs the more the more CUs are busy (the power limit); a
+// split launch pays for its second kernel and for writing and reading the partial sums.
 struct TileCost {
   int tm, tn;
   double start, step, busy, round;
 };
-constexpr TileCost kTiles[] = {{256, 256, 15.1, 0.51, 0.34, 6.0},
-                               {256, 128, 8.7, 0.36, 0.23, 4.0},
-                               {128, 256, 8.7, 0.36, 0.23, 4.0},
-                               {128, 128, 7.1, 0.29, 0.11, 0.34}};
+constexpr TileCost kTiles[] = {{256, 256, 10.6, 0.682, 0.263, 4.7},
+                               {256, 128, 9.7, 0.440, 0.185, 2.3},
+                               {128, 128, 6.5, 0.315, 0.138, 0.56}};
 
 TileChoice pick_tile(const selas_raw_linear_problem *problems, const Plan &plan, int64_t count) {
   const int cus = cu_count();
@@ -1062,7 +1054,7 @@ TileChoice pick_tile(const selas_raw_linear_problem *problems, const Plan &plan,
       if (split > 1 && (steps < 3 * split || items > 2 * cus)) continue;
       const double busy = items < cus ? static_cast<double>(items) / cus : 1.0;
       double us = t.start + (t.step + t.busy * busy) * cdiv(steps, split) * rounds + t.round * (rounds - 1);
-      if (split > 1) us += 3.35 * merges + 1.15e-6 * split * sums;
+      if (split > 1) us += 3.7 * merges + 0.81e-6 * split * sums;
       if (us < best_us) {
         best_us = us;
         best = TileChoice{t.tm, t.tn, split};
@@ -1158,7 +1150,6 @@ int launch_tiled(RawBatch &batch, const Plan &plan, hipStream_t s) {
   } while (0)
   if (plan.tile.tm == 256 && plan.tile.tn == 256) SELAS_TILE(8, 8, 1);
   else if (plan.tile.tm == 256) SELAS_TILE(8, 4, 1);
-  else if (plan.tile.tn == 256) SELAS_TILE(4, 8, 1);
   else SELAS_TILE(4, 4, 2);
 #undef SELAS_TILE
   if (int e = check_launch("raw_linear")) return e;

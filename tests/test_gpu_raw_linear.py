@@ -118,12 +118,11 @@ def tile(m, n, k):
 
 
 # Every tile and both kinds of K (whole steps of 64 or not), whole and split, with sizes that fill no tile.
-@pytest.mark.parametrize("m,n,k,want", [(700, 12280, 1088, (256, 256, 1)), (700, 12279, 1352, (256, 256, 1)),
-                                        (2040, 2056, 8200, (256, 256, 3)), (2040, 2056, 320, (256, 128, 1)),
-                                        (2040, 2056, 1352, (256, 128, 1)), (130, 6008, 6152, (256, 128, 4)),
-                                        (300, 12280, 320, (128, 256, 1)), (300, 12279, 1352, (128, 256, 1)),
-                                        (100, 12280, 6152, (128, 256, 4)), (300, 500, 640, (128, 128, 1)),
-                                        (300, 1000, 1352, (128, 128, 1)), (100, 300, 1352, (128, 128, 6))])
+@pytest.mark.parametrize("m,n,k,want", [(1030, 12280, 320, (256, 256, 1)), (700, 12279, 1352, (256, 256, 1)),
+                                        (130, 6008, 8200, (256, 256, 8)), (300, 12280, 640, (256, 128, 1)),
+                                        (300, 12279, 1352, (256, 128, 1)), (130, 6008, 6152, (256, 128, 4)),
+                                        (300, 500, 640, (128, 128, 1)), (130, 3064, 1352, (128, 128, 1)),
+                                        (70, 300, 1352, (128, 128, 6))])
 def test_every_tile_on_whole_numbers(dev, m, n, k, want):
     if torch.cuda.get_device_properties(dev).multi_processor_count == 256:  # the choice goes by the CU count
         assert tile(m, n, k) == want
