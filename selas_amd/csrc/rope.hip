@@ -333,9 +333,16 @@ extern "C" int selas_rope(const selas_rope_part *parts, int64_t count, int64_t B
   a.axes = static_cast<int>(axes);
   int pairs = 0;
   for (int i = 0; i < SELAS_ROPE_MAX_AXES; ++i) {
-    for (int64_t j = 0; i < axes && j < axis_dim[i]; j += 2)
-      turns.per_pos[pairs++] =
-          std::pow(theta, -static_cast<double>(j) / static_cast<double>(axis_dim[i])) / 6.283185307179586;
+    // The power of theta of pair j: pow where j is a power of two, otherwise the product of j's lowest bit's and the
+    // rest's, at most six roundings of 64 bits from it (a call of pow per pair took 2 us of a launch).
+    double *const t = turns.per_pos + pairs;
+    const int n = i < axes ? static_cast<int>(axis_dim[i] / 2) : 0;
+    for (int j = 0; j < n; ++j) {
+      const int low = j & -j;
+      t[j] = j == 0 ? 1.0 : j == low ? std::pow(theta, -2.0 * j / static_cast<double>(axis_dim[i])) : t[j - low] * t[low];
+    }
+    for (int j = 0; j < n; ++j) t[j] /= 6.283185307179586;
+    pairs += n;
     a.axis_end[i] = pairs;
   }
   const int esize = dtype == SELAS_F32 ? 4 : 2;

@@ -422,7 +422,7 @@ def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
         if out is None:
             ydt = out_dtype or (dt if residual is None else residual.dtype)
             y_dt = dtype_of("out", ydt)
-            out = y = torch.empty(shape, dtype=ydt, device=dev)
+            out = y = x.new_empty(shape, dtype=ydt)
             y_sb, y_sl = l * n, n
         else:
             if out_dtype not in (None, out.dtype):
@@ -438,11 +438,17 @@ def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
     if len(problems) > 1:
         _check_raw_disjoint(problems, outs)
     arr, count = b"".join(packed), len(packed)
-    size = ctypes.c_int64()
     with _lib.on(dev):
-        _lib.call("selas_raw_linear_workspace_bytes", arr, count, code, ctypes.byref(size))
-        ws = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-        _lib.call("selas_raw_linear", arr, count, code, _lib.ptr(ws), size.value, _lib.stream(dev))
+        stream = _lib.stream(dev)
+        try:
+            _lib.call("selas_raw_linear", arr, count, code, None, 0, stream)
+        except ValueError:  # most launches need no workspace: asked for only where one without was refused
+            size = ctypes.c_int64()
+            _lib.call("selas_raw_linear_workspace_bytes", arr, count, code, ctypes.byref(size))
+            if size.value == 0:
+                raise
+            ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+            _lib.call("selas_raw_linear", arr, count, code, ws.data_ptr(), size.value, stream)
     del keep  # the launch is queued on the stream that later reuses this memory
     return outs
 

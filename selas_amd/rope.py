@@ -83,7 +83,7 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, ids: torch.Tensor, axes_dim, theta
     ids_sb = ids.stride(0) if lead and lead[0] > 1 else 0
     scales = (_check_scale("q_scale", q_scale, dh), _check_scale("k_scale", k_scale, dh), None)
     if out is None:
-        ys = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in xs]
+        ys = [t.new_empty(t.shape) for t in xs]
     else:
         ys = list(out)
         _check_out(xs, ys, dev)
