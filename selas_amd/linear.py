@@ -12,6 +12,7 @@ GPU, by the bit-exact decode kernel) and a library GEMM runs.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import NamedTuple
 
 import torch
@@ -358,7 +359,7 @@ def raw_linear_batched(problems) -> list[torch.Tensor]:
 def _raw_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """(t, batch stride, row stride) of a [..., L, C] tensor seen as [B, L, C] with unit column stride."""
     if t.dim() > 3:
-        t = t.reshape(-1, *t.shape[-2:])
+        t = t.reshape(math.prod(t.shape[:-2]), *t.shape[-2:])  # -1 has no value where a dim is 0
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         t = t.contiguous()
     return t, (t.stride(0) if t.dim() == 3 else 0), (t.stride(-2) if t.dim() > 1 else 0)
@@ -474,7 +475,7 @@ def _check_raw_out(out: torch.Tensor, shape, inputs, residual) -> torch.Tensor:
     if out.dim() <= 3:
         return out
     try:
-        return out.view(-1, *out.shape[-2:])
+        return out.view(math.prod(out.shape[:-2]), *out.shape[-2:])
     except RuntimeError:
         raise ValueError(f"raw_linear: out's leading dims do not fold into one, strides {out.stride()}") from None
 

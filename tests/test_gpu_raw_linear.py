@@ -216,6 +216,14 @@ def test_empty_sizes(dev):
     assert raw_linear_batched([]) == []
 
 
+@pytest.mark.parametrize("lead", [(2, 3, 0), (2, 0, 4), (0, 3, 4), (2, 0, 0, 5)])
+def test_empty_higher_dims(dev, lead):
+    x, w = torch.zeros(*lead, 16, dtype=BF, device=dev), ints((24, 16), 73).to(dev)
+    r = torch.zeros(*lead, 24, dtype=BF, device=dev)
+    assert raw_linear(x, w, residual=r).shape == (*lead, 24)
+    assert raw_linear(x, w, residual=r, out=r).shape == (*lead, 24)
+
+
 def test_higher_dims(dev):
     x, w = ints((2, 3, 4, 64), 81).to(dev), ints((40, 64), 82).to(dev)
     ref = (x.cpu().double() @ w.cpu().double().t()).to(BF)
