@@ -86,7 +86,7 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, ids: torch.Tensor, axes_dim, theta
         ys = [t.new_empty(t.shape) for t in xs]
     else:
         ys = list(out)
-        _check_out(xs, ys, dev)
+        _check_out(xs, ys, dev, [t for t in (ids, *scales) if t is not None])
     parts = b"".join([_lib.ROPE_PART.pack(x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3],
                                           0 if scale is None else scale.data_ptr(), x.shape[1], i < 2)
                       for i, (x, y, scale) in enumerate(zip(xs, ys, scales))])
@@ -97,7 +97,7 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, ids: torch.Tensor, axes_dim, theta
     return tuple(ys)
 
 
-def _check_out(xs, ys, dev) -> None:
+def _check_out(xs, ys, dev, read) -> None:
     if len(ys) != len(xs):
         raise ValueError(f"rope_qk: out has {len(ys)} tensors for {len(xs)}")
     for i, (x, y) in enumerate(zip(xs, ys)):
@@ -107,6 +107,6 @@ def _check_out(xs, ys, dev) -> None:
         if not distinct(y):
             raise ValueError(f"rope_qk: out[{i}] has elements at one address (strides {y.stride()})")
         others = [t for j, t in enumerate(xs) if j != i or not same_elements(x, y)]
-        others += [t for j, t in enumerate(ys) if j != i]
+        others += [t for j, t in enumerate(ys) if j != i] + read
         if any(may_meet(y, t) for t in others):
             raise ValueError(f"rope_qk: out[{i}] overlaps another tensor of the call")

@@ -205,6 +205,17 @@ def test_streams_and_a_captured_graph(dev):
         assert torch.equal(y[0], want[0]) and torch.equal(y[1], want[1])
 
 
+def test_a_destination_over_the_positions_or_a_scale_is_refused(dev):
+    x, buf = torch.ones(1, 2, 8, 64, device=dev), torch.ones(2048, device=dev)
+    over, free = buf[:1024].view(1, 2, 8, 64), torch.empty(1, 2, 8, 64, device=dev)
+    for kw in ({"ids": buf[1000:1008].view(8, 1)}, {"ids": buf[2000:2008].view(8, 1), "q_scale": buf[960:1024]},
+               {"ids": buf[2000:2008].view(8, 1), "k_scale": buf[:64]}):
+        with pytest.raises(ValueError, match="overlaps"):
+            rope_qk(x, x, axes_dim=(64,), out=(free, over), **kw)
+    rope_qk(x, x, buf[2000:2008].view(8, 1), (64,), q_scale=buf[1024:1088], out=(free, over))
+    assert bool(buf[1024:].eq(1).all())
+
+
 def test_refusals(dev):
     q = torch.zeros(2, 3, 5, 64, dtype=BF, device=dev)
     ids = torch.zeros(5, 2, device=dev)
