@@ -5,6 +5,13 @@
 // it in a block: the GELU or SiLU (flux.py:150-151, 194-195) and the gated residual add
 // (flux.py:169-171). The sum, the activation, the gate and the residual stay in fp32 and
 // are rounded once, to the output's type.
+//
+// 2 M N K operations against the operands and the output moved once (eo bytes per output): products of 32 or fewer rows or 64
+// or fewer columns are bound by HBM and run in kernels that stream the large operand (raw_stream_kernel, raw_few_kernel);
+// the others are tiles of MFMAs (raw_tile_kernel), with K in ranges where the tiles leave CUs idle (raw_merge_kernel adds
+// them), and with operands off the DMA's alignment copied first (raw_pack_kernel). Every route adds in a fixed order.
+//
+// Times below: a large copy reaches 5.1 TB/s on the card, a library product of 8192^3 in bf16 1,590 TFLOP/s.
 #include <atomic>
 
 #include "common.h"
@@ -262,7 +269,9 @@ __device__ __forceinline__ void to_partial(RawProblem &P, float *part) {
   P.vec = P.N % 8 == 0;
 }
 
-// y = epilogue(sum over the K ranges, in their order): four columns per thread.
+// y = epilogue(sum over the K ranges, in their order): four columns per thread. Bound by the partial sums' reads, from the
+// Infinity Cache: 512 x 3072 of 8 ranges with an fp32 residual 11.6 us (63 MB, 5.4 TB/s). A pass of its own: tiles that
+// wait for one another need an order of workgroups that a launch does not promise, and atomic adds change the sum's order.
 template <int DT>
 __global__ __launch_bounds__(256) void raw_merge_kernel(RawProblem P, const float *__restrict__ part, int split) {
   const int groups = (P.N + 3) / 4;
@@ -301,8 +310,10 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t *row, int k, int K) {
 // ------------------------------------------------------------------ operands off alignment
 //
 // The tiled kernel's DMA takes whole 16-byte chunks. An operand whose rows are not made of them (K not a multiple of 8, an
-// odd stride or address) or span too much is copied first, to rows of K rounded up to 64 that end in zeros: one more pass
-// over it against a kernel that loads such rows through registers (1386 x 1431 x 667 26 us in 64 x 64 tiles).
+// odd stride or address) or span too much is copied first, to rows of K rounded up to 64 that end in zeros, a thread per
+// 16-byte chunk. The copy of 1386 x 667 and 1431 x 667 is 6.2 us (7.6 MB: a launch, and one load's latency), the tiles after
+// it 20 us; tiles of 64 x 64 that load such rows through registers took 26 us without it, and 4001 x 5999 x 5003
+// ran at 500 TFLOP/s there against 948.
 template <int DT>
 __global__ __launch_bounds__(256) void raw_pack_kernel(RawProblem P, uint16_t *xp, uint16_t *wp, int kp) {
   const int per_row = kp / 8;
@@ -330,6 +341,10 @@ __global__ __launch_bounds__(256) void raw_pack_kernel(RawProblem P, uint16_t *x
 // bytes of row lane % 16 straight into the fragments of v_mfma_f32_16x16x32 (two loads cover a 128-byte line), and the
 // few rows' fragments from the caches. The waves' sums are added in LDS, in wave order.
 // SWAP: x is the streamed operand.
+//
+// A workgroup reads the few rows again for its 16 or 32 streamed ones, so up to as many bytes come from the caches as
+// from HBM; that, not HBM, is the bound (28 x 18432 x 3072: 29.8 us, 3.95 TB/s of weight, the few rows' 99 MB beside it;
+// 8 waves in the kernel below where rows are off the DMA's alignment, 36 us).
 constexpr int kFewWaves = 8;
 
 // The epilogue of the kernels for few rows: the waves' sums red[wave][few row][streamed row] are added in wave order, a
@@ -418,7 +433,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void raw_few_kernel(RawProblem P, f
 // The same for operands whose rows the DMA can read (dma_ok_x, dma_ok_w): the fragments' lane order takes each of 16 adjacent
 // lanes to another row, 64 cache lines looked up per load, which held the loads above at 16 bytes per clock and CU (28 x
 // 18432 x 3072 36 us). Here each wave copies its range of K to LDS of its own by DMA, 8 rows of 128 bytes per
-// instruction, ST steps of 64 columns ahead, and reads the fragments there; no barrier until the sums are added.
+// instruction, ST steps of 64 columns ahead, and reads the fragments there; no barrier until the sums are added. 28 x 18432 x
+// 3072 29.8 us (the floor is 22.5); 1 x 3072 x 768 4.2 us and 4096 x 64 x 3072 11.0 us, where a launch, one chain of loads
+// per wave and the sum over the waves are what is left.
 constexpr int kStreamWaves = 4;
 constexpr int stream_stages(int blocks) { return blocks <= 2 ? 4 : blocks == 3 ? 3 : 2; }
 
@@ -534,6 +551,17 @@ __device__ __forceinline__ void wait_lds_barrier() { asm volatile("s_waitcnt lgk
 //   any more), and multiplies.
 // A half is read 7 phases after its DMA was issued, so 6 newer halves' loads may be pending at each wait. Past the end
 // of K the loads are out of range: they bring zeros and no traffic, and the counts stay the same.
+//
+// Why so: 256 x 256 is the largest tile whose sums (256 registers a lane) and fragments fit one wave per SIMD, and the
+// fewest LDS bytes per product (one fragment read for 8 MFMAs); 16x16x32 MFMAs draw less power per product than 32x32x16,
+// and power sets the clock. A half's 16 KB per DMA wave and the XOR of chunk and row (row / 2) % 8 leave no bank conflict
+// (counted: 0). Two barriers a step instead of four, and the reads and DMAs pinned between the products, took the
+// MFMAs from 72 to 83 % busy at 8192^3 (709 us, 1,550 TFLOP/s; the library's 692). Of the block's linears,
+// 4096 x 12288 x 3072 with GELU is 227-234 us (1,320-1,360 TFLOP/s, floor 194: three rounds of 256 tiles whose
+// prologue and epilogue, 11 us each, nothing overlaps at one workgroup per CU), 4608 x 3072 x 15360 with an fp32
+// residual 316-322 us (1,350-1,375; floor 273: 216 tiles for 256 CUs, and all residual traffic at the end); 66 and 65 %
+// MFMA busy. HBM traffic is 1.0 of the output written, and of the operands read 2.3 and 1.7 times (the XCDs' L2s
+// each load what their tiles share).
 template <int DT, int WM, int WN, int MB, int NB, int OCC, bool TAIL>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch batch) {
   constexpr int TM = WM * MB * 16, TN = WN * NB * 16, HM = MB / 2, HN = NB / 2, NW = WM * WN;
@@ -1021,7 +1049,7 @@ int few_split(int64_t big, int64_t K) {
   return split;
 }
 
-// Tile and K ranges of the tiled launch: the fastest by this model of a launch in us, fitted to 288 shapes (40 to 4608
+// Tile and K ranges of the tiled launch: the fastest by this model of a launch in us, fitted to 275 shapes (40 to 4608
 // rows, 256 to 21504 columns, K 256 to 12288, weights from HBM; every tile and split timed). Its choices are within 1 %
 // of the fastest in the mean and 18 % at worst (384 x 12288 x 3072: 40 us in tiles of 256 x 128, 54 of 128 x 128; 1024 x
 // 12288 x 3072: 67 us of 256 x 256, 84 of 128 x 128; tiles of 128 x 256 were ahead in 13 shapes, by 0.3 % over all, and
