@@ -149,45 +149,64 @@ __device__ __forceinline__ void load_cols(const void *p, int64_t i, bool f32, fl
   }
 }
 
-// W consecutive columns from any element on, of which the first `live` exist (the others hold any of them, or zeros).
+// W consecutive columns of U rows, row u from element at[u] on, of which the first `live` exist (0 or fewer: none; the
+// others repeat the last). Whether all exist is asked for a whole wave and the type for all rows, so that every row's loads
+// are in flight before the first one's values are used: asked per row, each row waited for the one before.
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
-template <int DT, int W>
-__device__ __forceinline__ void load_cols_any(const void *p, int64_t i, bool f32, int live, float (&v)[W]) {
-  if (live <= 0) {
+template <int DT, int U, int W>
+__device__ __forceinline__ void load_rows_any(const void *p, const int64_t (&at)[U], bool f32, bool whole, int live,
+                                              float (&v)[U][W]) {
+  const float *const pf = static_cast<const float *>(p);
+  const uint16_t *const ph = static_cast<const uint16_t *>(p);
+  if (whole && f32) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = 0.0f;
-  } else if (live < W) {
-    // The last column stands in for the ones past it: loads under a condition each would wait for one another.
-    if (f32) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < W; ++j) v[j] = static_cast<const float *>(p)[i + min(j, live - 1)];
-    } else {
+      for (int j = 0; j < W; j += 4) {
+        const f32x4 q = *reinterpret_cast<const f32x4_any *>(pf + at[u] + j);
+        v[u][j] = q[0]; v[u][j + 1] = q[1]; v[u][j + 2] = q[2]; v[u][j + 3] = q[3];
+      }
+  } else if (whole) {
+    uint32_t w[U][W / 2];
 #pragma unroll
-      for (int j = 0; j < W; ++j) v[j] = load_f<DT>(p, i + min(j, live - 1));
-    }
-  } else if (f32) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int j = 0; j < W; j += 4) {
-      const f32x4 u = *reinterpret_cast<const f32x4_any *>(static_cast<const float *>(p) + i + j);
-      v[j] = u[0]; v[j + 1] = u[1]; v[j + 2] = u[2]; v[j + 3] = u[3];
-    }
-  } else {
-    const uint16_t *q = static_cast<const uint16_t *>(p) + i;
+      for (int j = 0; j < W; j += 4) {
+        const auto q = *reinterpret_cast<const u32x2_any *>(ph + at[u] + j);
+        w[u][j / 2] = q[0]; w[u][j / 2 + 1] = q[1];
+      }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < W; j += 4) {
-      const u32x2_any u = *reinterpret_cast<const u32x2_any *>(q + j);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < W / 2; ++t) {
         if constexpr (DT == SELAS_BF16) {
-          v[j + 2 * t] = __uint_as_float(u[t] << 16);
-          v[j + 2 * t + 1] = __uint_as_float(u[t] & 0xffff0000u);
+          v[u][2 * t] = __uint_as_float(w[u][t] << 16);
+          v[u][2 * t + 1] = __uint_as_float(w[u][t] & 0xffff0000u);
         } else {
-          v[j + 2 * t] = f16_bits_to_f32(u[t] & 0xffffu);
-          v[j + 2 * t + 1] = f16_bits_to_f32(u[t] >> 16);
+          v[u][2 * t] = f16_bits_to_f32(w[u][t] & 0xffffu);
+          v[u][2 * t + 1] = f16_bits_to_f32(w[u][t] >> 16);
         }
       }
-    }
+  } else if (f32) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[u][j] = pf[at[u] + min(j, live - 1)];
+  } else {
+    uint16_t w[U][W];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[u][j] = ph[at[u] + min(j, live - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        if constexpr (DT == SELAS_BF16) v[u][j] = __uint_as_float(static_cast<uint32_t>(w[u][j]) << 16);
+        else v[u][j] = f16_bits_to_f32(w[u][j]);
+      }
   }
 }
 
@@ -312,8 +331,8 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t *row, int k, int K) {
 // The tiled kernel's DMA takes whole 16-byte chunks. An operand whose rows are not made of them (K not a multiple of 8, an
 // odd stride or address) or span too much is copied first, to rows of K rounded up to 64 that end in zeros, a thread per
 // 16-byte chunk. The copy of 1386 x 667 and 1431 x 667 is 6.2 us (7.6 MB: a launch, and one load's latency), the tiles after
-// it 20 us; tiles of 64 x 64 that load such rows through registers took 26 us without it, and 4001 x 5999 x 5003
-// ran at 500 TFLOP/s there against 948.
+// it 15 us; tiles of 64 x 64 that load such rows through registers took 26 us without it, and 4001 x 5999 x 5003
+// ran at 500 TFLOP/s there against 1,060 (the copy included).
 template <int DT>
 __global__ __launch_bounds__(256) void raw_pack_kernel(RawProblem P, uint16_t *xp, uint16_t *wp, int kp) {
   const int per_row = kp / 8;
@@ -874,31 +893,34 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
     }
   };
   // The same for outputs off alignment, N not a multiple of 8 or batches with spacing of their own: addresses per row, and
-  // vector accesses that may start at any element, except in the columns that N cuts.
+  // vector accesses that may start at any element, except in the columns that N cuts. Columns past N and rows past M read
+  // the last one (live - 1 is then negative: the column N - 1). Two rows at once in the tile of two workgroups per CU, whose
+  // registers do not hold four (1386 x 1431 x 667 with GELU and residual 21.5 us; four 24.1, one after another 25.5).
   auto finish_any = [&](auto width) __attribute__((always_inline)) {
-    constexpr int W = decltype(width)::value, LPR = NB * 16 / W, RPI = 64 / LPR, U = 4;
+    constexpr int W = decltype(width)::value, LPR = NB * 16 / W, RPI = 64 / LPR, U = OCC == 1 ? 4 : 2;
     const int n = nw + (lane % LPR) * W, row = lane / LPR, live = N - n;
     const int mw = m0 + wm * MB * 16;
-    float bias[W] = {}, gate[W];
-    if (P.bias) load_cols_any<DT, W>(P.bias, n, P.bias_f32, live, bias);
-    if (P.gate && P.one_gate) load_cols_any<DT, W>(P.gate, n, P.gate_f32, live, gate);
+    const bool whole = nw + NB * 16 <= N;
+    float bias[1][W] = {}, gate[1][W] = {};
+    const int64_t only[1] = {n};
+    if (P.bias) load_rows_any<DT, 1, W>(P.bias, only, P.bias_f32, whole, live, bias);
+    if (P.gate && P.one_gate) load_rows_any<DT, 1, W>(P.gate, only, P.gate_f32, whole, live, gate);
 #pragma unroll 1
     for (int e = 0; e < MB / 2; ++e) {
       stage(e);
 #pragma unroll 1
       for (int g = 0; g < ER / RPI; g += U) {
         float v[U][W], res[U][W];
-        int bs[U], ls[U];
-        bool on[U];
+        int64_t ga[U], ra[U], ya[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int m = mw + e * ER + (g + u) * RPI + row;
-          on[u] = m < M;
-          bs[u] = static_cast<int>(div31(static_cast<uint32_t>(min(m, M - 1)), P.by_l));
-          ls[u] = m - bs[u] * P.L;
-          if (P.residual && on[u])
-            load_cols_any<DT, W>(P.residual, bs[u] * P.r_sb + ls[u] * P.r_sl + n, P.residual_f32, live, res[u]);
+          const int m = min(mw + e * ER + (g + u) * RPI + row, M - 1);
+          const int b = static_cast<int>(div31(static_cast<uint32_t>(m), P.by_l)), l = m - b * P.L;
+          ga[u] = b * P.gate_sb + n;
+          ra[u] = b * P.r_sb + l * P.r_sl + n;
+          ya[u] = b * P.y_sb + l * P.y_sl + n;
         }
+        if (P.residual) load_rows_any<DT, U, W>(P.residual, ra, P.residual_f32, whole, live, res);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -906,22 +928,30 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
             const int r = (g + u) * RPI + row, c = (lane % LPR) * (W / 4) + q;
             const f32x4 f = *reinterpret_cast<const f32x4 *>(st + r * (NB * 64) + ((c ^ (r & 15)) << 4));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[u][4 * q + j] = f[j] + bias[4 * q + j];
+            for (int j = 0; j < 4; ++j) v[u][4 * q + j] = f[j] + bias[0][4 * q + j];
           }
         }
         activate_all(v, P.act);
+        if (P.gate && P.one_gate) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[u][j] *= gate[0][j];
+        } else if (P.gate) {
+          float gates[U][W];
+          load_rows_any<DT, U, W>(P.gate, ga, P.gate_f32, whole, live, gates);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[u][j] *= gates[u][j];
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (P.gate) {
-            if (!P.one_gate) load_cols_any<DT, W>(P.gate, bs[u] * P.gate_sb + n, P.gate_f32, live, gate);
-#pragma unroll
-            for (int j = 0; j < W; ++j) v[u][j] *= gate[j];
-          }
           if (P.residual) {
 #pragma unroll
             for (int j = 0; j < W; ++j) v[u][j] = res[u][j] + v[u][j];
           }
-          if (on[u]) store_cols_any<DT, W>(P.y, bs[u] * P.y_sb + ls[u] * P.y_sl + n, live, v[u]);
+          if (mw + e * ER + (g + u) * RPI + row < M) store_cols_any<DT, W>(P.y, ya[u], live, v[u]);
         }
       }
     }
