@@ -179,6 +179,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 # The handle of torch's current stream without the Stream object around it (0.1 us instead of 3), where torch has it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# The current device without the look at whether torch.cuda has started (a GPU tensor shows that it has): 0.1 us instead of 0.8.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def stream(device: torch.device) -> int:
@@ -203,7 +205,7 @@ _HERE = _Here()
 
 def on(device: torch.device):
     """``torch.cuda.device(device)``, at a tenth of its cost where that device is current."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if _current_device() == device.index else torch.cuda.device(device)
 
 
 def code_array(code) -> ctypes.Array:

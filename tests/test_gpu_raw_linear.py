@@ -133,6 +133,25 @@ def test_every_tile_on_whole_numbers(dev, m, n, k, want):
     assert torch.equal(raw_linear(x, w, bias), z.to(BF))
 
 
+# Outputs off every alignment (odd N; a residual and a result that start at an odd element), tiles across images.
+@pytest.mark.parametrize("b,l,n,k", [(3, 100, 129, 72), (4, 33, 1431, 667), (2, 350, 12279, 200), (2, 150, 12279, 1352)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("gates,gate_t,res_t", [("image", "w", F32), ("image", F32, "w"), ("one", "w", "w"), ("one", F32, F32),
+                                                ("none", F32, "w")])
+def test_epilogues_off_alignment(dev, b, l, n, k, dtype, gates, gate_t, res_t):
+    gate_t, res_t = dtype if gate_t == "w" else gate_t, dtype if res_t == "w" else res_t
+    x, w, bias = ints((b, l, k), 31, dtype=dtype).to(dev), ints((n, k), 32, dtype=dtype).to(dev), ints((n,), 33, dtype=dtype).to(dev)
+    gate = {"image": ints((b, 1, n), 34, dtype=gate_t).to(dev), "one": ints((n,), 34, dtype=gate_t).to(dev), "none": None}[gates]
+    buf = ints((b * l * n + 2 * n,), 35, dtype=res_t).to(dev)
+    res = buf[1:1 + b * l * n].view(b, l, n)
+    z = x.double() @ w.double().t() + bias.double()
+    want = (res.double() + (z if gate is None else gate.double() * z)).to(res_t)
+    ends = buf[0].clone(), buf[1 + b * l * n:].clone()
+    assert torch.equal(raw_linear(x, w, bias, gate=gate, residual=res), want)
+    assert torch.equal(raw_linear(x, w, bias, gate=gate, residual=res, out=res), want)
+    assert torch.equal(res, want) and torch.equal(buf[0], ends[0]) and torch.equal(buf[1 + b * l * n:], ends[1])
+
+
 def test_gate_shapes(dev):
     x, w, g = normal((3, 9, 64), 31), normal((40, 64), 32), normal((3, 40), 33, dtype=F32)
     a = raw_linear(x.to(dev), w.to(dev), gate=g.to(dev))
