@@ -362,8 +362,8 @@ __global__ __launch_bounds__(256) void raw_pack_kernel(RawProblem P, uint16_t *x
 // SWAP: x is the streamed operand.
 //
 // A workgroup reads the few rows again for its 16 or 32 streamed ones, so up to as many bytes come from the caches as
-// from HBM; that, not HBM, is the bound (28 x 18432 x 3072: 29.8 us, 3.95 TB/s of weight, the few rows' 99 MB beside it;
-// 8 waves in the kernel below where rows are off the DMA's alignment, 36 us).
+// from HBM; that, not HBM, is the bound (28 x 18432 x 3072: 26.7 us, 4.24 TB/s of weight, the few rows' 45 MB beside it;
+// in the kernel right below, for rows off the DMA's alignment, 36 us).
 constexpr int kFewWaves = 8;
 
 // The epilogue of the kernels for few rows: the waves' sums red[wave][few row][streamed row] are added in wave order, a
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void raw_few_kernel(RawProblem P, f
 // lanes to another row, 64 cache lines looked up per load, which held the loads above at 16 bytes per clock and CU (28 x
 // 18432 x 3072 36 us). Here each wave copies its range of K to LDS of its own by DMA, 8 rows of 128 bytes per
 // instruction, ST steps of 64 columns ahead, and reads the fragments there; no barrier until the sums are added. 28 x 18432 x
-// 3072 29.8 us (the floor is 22.5); 1 x 3072 x 768 4.2 us and 4096 x 64 x 3072 11.0 us, where a launch, one chain of loads
+// 3072 26.7 us (the floor is 22.5); 1 x 3072 x 768 4.2 us and 4096 x 64 x 3072 11.0 us, where a launch, one chain of loads
 // per wave and the sum over the waves are what is left.
 constexpr int kStreamWaves = 4;
 constexpr int stream_stages(int blocks) { return blocks <= 2 ? 4 : blocks == 3 ? 3 : 2; }
@@ -1066,14 +1066,21 @@ struct Plan {
 // 3072 9.6 us against 12).
 constexpr int kFewX = 32, kFewW = 64;
 
-// Streamed rows of 16 per workgroup: two blocks where that still gives every CU two workgroups, for half the loads of the
-// few rows (28 x 18432 x 3072 29.9 us against 34.3), one block otherwise (28 x 3072 x 3072 9.5 us against 11.4).
-int few_blocks(int64_t big) { return big > 16 * 2 * cu_count() ? 2 : 1; }
+// Blocks of 16 streamed rows per workgroup. Streamed weights: as many as make one round of one workgroup per CU, up to six,
+// for fewer reads of the few rows and no second round (us against two blocks: 28 x 18432 x 3072, five, 26.7 against 29.9;
+// 28 x 9216 x 3072, three, 16.8 against 20.2; 28 x 21504 x 3072, six, 30.3 against 32.1). Two instead of four are one round of two
+// workgroups per CU (4 x 16384 x 4096 25.2 against 28.7), and two past six (28 x 40000 x 1024 22.7 us, five 24.6).
+// Streamed x, and rows off the DMA's alignment: two blocks where that gives every CU two workgroups, else one.
+int few_blocks(int64_t big, bool weights) {
+  const int64_t blocks = cdiv(cdiv(big, 16), cu_count());  // per CU
+  if (!weights) return blocks > 2 ? 2 : 1;
+  return blocks == 4 || blocks > 6 ? 2 : static_cast<int>(blocks);
+}
 
 // K ranges of a few-row launch: doubled while its workgroups leave CUs idle and a wave keeps 3 steps of 64 (1024 x 64 x
 // 3072 11.0 us whole, 9.6 us in four; with 192 workgroups, 28 x 3072 x 3072, two ranges cost 9.5 -> 13 us).
 int few_split(int64_t big, int64_t K) {
-  const int64_t units = cdiv(big, 16 * few_blocks(big)), steps = cdiv(K, 64);
+  const int64_t units = cdiv(big, 16), steps = cdiv(K, 64);
   int split = 1;
   while (units * split * 2 <= cu_count() && steps / (kStreamWaves * split * 2) >= 3) split *= 2;
   return split;
@@ -1161,7 +1168,7 @@ template <int DT>
 int launch_few(const RawProblem &P, bool stream, float *part, int split, hipStream_t s) {
   const bool swap = P.M > kFewX;
   const int few = swap ? P.N : P.M, big = swap ? P.M : P.N;
-  const int nt = few_blocks(big), mt = few <= 16 ? 1 : few <= 32 ? 2 : 4;
+  const int nt = few_blocks(big, stream && !swap), mt = few <= 16 ? 1 : few <= 32 ? 2 : 4;
   const dim3 grid(static_cast<uint32_t>(cdiv(big, 16 * nt)), static_cast<uint32_t>(split)), blk(64 * kFewWaves), sblk(64 * kStreamWaves);
 #define SELAS_FEW(NT, MT, SWAP)                                                                  \
   do {                                                                                           \
@@ -1173,11 +1180,16 @@ int launch_few(const RawProblem &P, bool stream, float *part, int split, hipStre
     if (nt == 2) SELAS_FEW(2, MT, SWAP);  \
     else SELAS_FEW(1, MT, SWAP);          \
   } while (0)
+#define SELAS_WIDE(NT)                                                                                     \
+  else if (nt == NT && mt == 2) raw_stream_kernel<DT, NT, 2, false><<<grid, sblk, 0, s>>>(P, part, split); \
+  else if (nt == NT) raw_stream_kernel<DT, NT, 1, false><<<grid, sblk, 0, s>>>(P, part, split);
   if (swap && mt == 4) SELAS_FEW_NT(4, true);
   else if (swap && mt == 2) SELAS_FEW_NT(2, true);
   else if (swap) SELAS_FEW_NT(1, true);
+  SELAS_WIDE(3) SELAS_WIDE(5) SELAS_WIDE(6)
   else if (mt == 2) SELAS_FEW_NT(2, false);
   else SELAS_FEW_NT(1, false);
+#undef SELAS_WIDE
 #undef SELAS_FEW_NT
 #undef SELAS_FEW
   if (int e = check_launch("raw_linear")) return e;

@@ -133,6 +133,17 @@ def test_every_tile_on_whole_numbers(dev, m, n, k, want):
     assert torch.equal(raw_linear(x, w, bias), z.to(BF))
 
 
+# Few rows against weights of one to seven blocks of 16 rows per CU of 256, the last block and round not full.
+@pytest.mark.parametrize("n", [4000, 5000, 9208, 12283, 16376, 18424, 21499, 24568, 29000])
+@pytest.mark.parametrize("m,k", [(1, 72), (16, 640), (28, 1352), (32, 64)])
+def test_few_rows_on_whole_numbers(dev, m, n, k):
+    x, w = ints((m, k), 1).to(dev), ints((n, k), 2).to(dev)
+    bias, gate, res = ints((n,), 3, dtype=F32).to(dev), ints((n,), 4, dtype=F32).to(dev), ints((m, n), 5, dtype=F32).to(dev)
+    z = x.double() @ w.double().t() + bias.double()
+    assert torch.equal(raw_linear(x, w, bias, gate=gate, residual=res).double(), res.double() + gate.double() * z)
+    assert torch.equal(raw_linear(x, w, bias), z.to(BF))
+
+
 # Outputs off every alignment (odd N; a residual and a result that start at an odd element), tiles across images.
 @pytest.mark.parametrize("b,l,n,k", [(3, 100, 129, 72), (4, 33, 1431, 667), (2, 350, 12279, 200), (2, 150, 12279, 1352)])
 @pytest.mark.parametrize("dtype", [BF, FP])
