@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libselas_amd.so"
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 OK, EINVAL, EUNSUPPORTED, EHIP = 0, 1, 2, 3
 F32, F16, BF16 = 0, 1, 2
@@ -84,7 +84,7 @@ class GemvDesc(ctypes.Structure):
 # the time of filling a ctypes structure.
 ROPE_PART = struct.Struct("@P3qP3qP2q")
 # One selas_raw_linear_problem: x and strides, w and stride, bias, gate and stride, residual and strides, y and strides;
-# B, L, N, K; the dtypes of bias, gate, residual and y, the activation, a reserved int.
+# B, L, N, K; the dtypes of bias, gate, residual and y, the activation, the guard.
 RAW_LINEAR_PROBLEM = struct.Struct("@P2qPqPPqP2qP2q4q6i")
 ROPE_MAX_PARTS, ROPE_MAX_AXES = 3, 4
 STATIC_MAX_WEIGHTS = 1023

@@ -52,6 +52,12 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// The fp16 guard of a residual add: into the fp16 range.
+constexpr float kFp16Max = 65504.0f;
+__device__ __forceinline__ float clamp_guard(float v) {
+  return v < -kFp16Max ? -kFp16Max : (v > kFp16Max ? kFp16Max : v);  // NaN passes through
+}
+
 __device__ __forceinline__ uint32_t perm(uint32_t s0, uint32_t s1, uint32_t sel) {
   return __builtin_amdgcn_perm(s0, s1, sel);
 }

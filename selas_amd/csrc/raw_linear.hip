@@ -1,5 +1,6 @@
 // Linear with an unquantized weight and the block's epilogue, on gfx950:
 //   y[b, l, n] = residual[b, l, n] + gate[b, n] * act(sum_k x[b, l, k] w[n, k] + bias[n])
+// with act(..) clamped to the fp16 range where the fp16 guard is on.
 //
 // UnitView.linear for raw weights (selas/store.py:289-293) together with what follows
 // it in a block: the GELU or SiLU (flux.py:150-151, 194-195) and the gated residual add
@@ -32,6 +33,7 @@ struct RawProblem {
   // of the residual are equally spaced over the batches, a tile of them within 31 bits of bytes.
   bool vec;
   bool one_gate;  // one gate row for all batches
+  bool guard;     // the fp16 guard
 };
 
 // Four dwords, and the same at the address of any 16-bit element (global accesses may start there).
@@ -76,8 +78,15 @@ __device__ __forceinline__ float activate(float v, int act) {
   return act == SELAS_ACT_GELU ? gelu_tanh_fast(v) : act == SELAS_ACT_SILU ? silu_fast(v) : v;
 }
 
+// The activation and the fp16 guard. The sums are fp32, but fp16 inputs may be infinite (a hidden value stored past 65504),
+// and an infinite sum would stay in the residual stream.
+__device__ __forceinline__ float activate(float v, int act, bool guard) {
+  v = activate(v, act);
+  return guard ? clamp_guard(v) : v;
+}
+
 template <int A, int B>
-__device__ __forceinline__ void activate_all(float (&v)[A][B], int act) {  // one branch for all
+__device__ __forceinline__ void activate_all(float (&v)[A][B], int act, bool guard) {  // one branch for all
   if (act == SELAS_ACT_GELU) {
 #pragma unroll
     for (int i = 0; i < A; ++i)
@@ -88,6 +97,12 @@ __device__ __forceinline__ void activate_all(float (&v)[A][B], int act) {  // on
     for (int i = 0; i < A; ++i)
 #pragma unroll
       for (int j = 0; j < B; ++j) v[i][j] = silu_fast(v[i][j]);
+  }
+  if (guard) {
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) v[i][j] = clamp_guard(v[i][j]);
   }
 }
 
@@ -100,7 +115,7 @@ __device__ __forceinline__ float load_either(const void *p, int64_t i, bool f32)
 template <int DT>
 __device__ __forceinline__ void finish_one(const RawProblem &P, int b, int l, int n, float v) {
   if (P.bias) v += load_either<DT>(P.bias, n, P.bias_f32);
-  v = activate(v, P.act);
+  v = activate(v, P.act, P.guard);
   if (P.gate) v *= load_either<DT>(P.gate, b * P.gate_sb + n, P.gate_f32);
   if (P.residual) v = load_either<DT>(P.residual, b * P.r_sb + l * P.r_sl + n, P.residual_f32) + v;
   const int64_t o = b * P.y_sb + l * P.y_sl + n;
@@ -250,7 +265,7 @@ __device__ __forceinline__ void finish_four(const RawProblem &P, int b, int l, i
     for (int j = 0; j < 4; ++j) v[j] += u[j];
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = activate(v[j], P.act);
+  for (int j = 0; j < 4; ++j) v[j] = activate(v[j], P.act, P.guard);
   if (P.gate) {
     load_cols<DT, 4>(P.gate, b * P.gate_sb + n, P.gate_f32, u);
 #pragma unroll
@@ -281,6 +296,7 @@ __device__ __forceinline__ void finish_four(const RawProblem &P, int b, int l, i
 __device__ __forceinline__ void to_partial(RawProblem &P, float *part) {
   P.bias = P.gate = P.residual = nullptr;
   P.act = SELAS_ACT_NONE;
+  P.guard = false;
   P.y = part;
   P.y_sl = P.N;
   P.y_sb = static_cast<int64_t>(P.L) * P.N;
@@ -837,7 +853,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[g][4 * q + j] = f[j] + bias[4 * q + j];
         }
-      activate_all(v, P.act);
+      activate_all(v, P.act, P.guard);
       if (P.gate) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -931,7 +947,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
             for (int j = 0; j < 4; ++j) v[u][4 * q + j] = f[j] + bias[0][4 * q + j];
           }
         }
-        activate_all(v, P.act);
+        activate_all(v, P.act, P.guard);
         if (P.gate && P.one_gate) {
 #pragma unroll
           for (int u = 0; u < U; ++u)
@@ -1006,6 +1022,7 @@ RawProblem make_problem(const selas_raw_linear_problem &p) {
   r.N = static_cast<int>(p.N); r.K = static_cast<int>(p.K);
   r.by_l = fast_div(static_cast<uint32_t>(p.L));
   r.act = p.act;
+  r.guard = p.guard != 0;
   r.bias_f32 = p.bias_dtype == SELAS_F32; r.gate_f32 = p.gate_dtype == SELAS_F32;
   r.residual_f32 = p.residual_dtype == SELAS_F32; r.y_f32 = p.y_dtype == SELAS_F32;
   r.vec = epilogue_vec(p);

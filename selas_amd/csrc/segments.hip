@@ -20,7 +20,6 @@ namespace {
 
 constexpr int kRowThreads = 256;
 constexpr int kMaxVec = 4;  // float4 groups per thread: D <= 256 * 4 * 4 = 4096
-constexpr float kFp16Max = 65504.0f;
 constexpr float kLnEps = 1e-6f;
 constexpr float kRmsEps = 1e-6f;
 
@@ -31,10 +30,6 @@ __device__ __forceinline__ float block_sum(float v, float *slot) {
   if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
   __syncthreads();
   return ((slot[0] + slot[1]) + slot[2]) + slot[3];
-}
-
-__device__ __forceinline__ float clamp_guard(float v) {
-  return v < -kFp16Max ? -kFp16Max : (v > kFp16Max ? kFp16Max : v);  // NaN passes through
 }
 
 // Loads 4 consecutive elements (d multiple of 4) of a 16/32-bit float row.

@@ -173,19 +173,20 @@ def double_block(w, img, txt, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k
     if h is None:
         h = (k.mod_in(img, i_sh1, i_sc1, dt), k.mod_in(txt, t_sh1, t_sc1, dt))
     if _fused_raw(w, k):
-        # Raw weights: the gated residual adds and the GELU in the linears' epilogues, in fp32 (no 16-bit rounding of the
-        # linear's output, so nothing for the fp16 guard to clamp); the next mod_in is its own kernel.
+        # Raw weights: the gated residual adds and the GELU in the linears' epilogues, in fp32, with no 16-bit
+        # rounding of the linear's output; the fp16 guard clamps it there (hidden values stored in fp16 may be infinite).
+        # The next mod_in is its own kernel.
         iqkv, tqkv = w.raw_linear_many([(h[0], "img_attn.qkv"), (h[1], "txt_attn.qkv")])
         del h
         a = attention(*_qkv_double(w, k, tqkv, iqkv, cos, sin, ids, cfg, dt))
         del iqkv, tqkv
-        img, txt = w.raw_linear_many([(a[:, lt:], "img_attn.proj", {"gate": i_g1, "residual": img}),
-                                      (a[:, :lt], "txt_attn.proj", {"gate": t_g1, "residual": txt})])
+        img, txt = w.raw_linear_many([(a[:, lt:], "img_attn.proj", {"gate": i_g1, "residual": img, "guard": guard}),
+                                      (a[:, :lt], "txt_attn.proj", {"gate": t_g1, "residual": txt, "guard": guard})])
         del a
         hi, ht = k.mod_in(img, i_sh2, i_sc2, dt), k.mod_in(txt, t_sh2, t_sc2, dt)
         hi, ht = w.raw_linear_many([(hi, "img_mlp.0", {"act": "gelu"}), (ht, "txt_mlp.0", {"act": "gelu"})])
-        img, txt = w.raw_linear_many([(hi, "img_mlp.2", {"gate": i_g2, "residual": img}),
-                                      (ht, "txt_mlp.2", {"gate": t_g2, "residual": txt})])
+        img, txt = w.raw_linear_many([(hi, "img_mlp.2", {"gate": i_g2, "residual": img, "guard": guard}),
+                                      (ht, "txt_mlp.2", {"gate": t_g2, "residual": txt, "guard": guard})])
         if next_mod is None:
             return img, txt
         n = next_mod.float().unsqueeze(1).chunk(12, dim=-1)
@@ -238,7 +239,7 @@ def single_block(w, x, mod, cos, sin, cfg: FluxConfig, dt, guard: bool, k: Kerne
         del h
         attention(*_qkv_single(w, k, qkv, cos, sin, ids, cfg, dt), out=cat[..., :d])
         del qkv
-        (x,) = w.raw_linear_many([(cat, "linear2", {"gate": g, "residual": x})])
+        (x,) = w.raw_linear_many([(cat, "linear2", {"gate": g, "residual": x, "guard": guard})])
         if next_mod is None:
             return x
         nsh, nsc, _ = next_mod.float().unsqueeze(1).chunk(3, dim=-1)

@@ -324,6 +324,7 @@ class RawLinear(NamedTuple):
     residual: torch.Tensor | None = None
     out: torch.Tensor | None = None
     out_dtype: torch.dtype | None = None
+    guard: bool = False
 
 
 ACTS = {None: 0, "gelu": 1, "silu": 2}  # SELAS_ACT_*
@@ -331,18 +332,20 @@ ACTS = {None: 0, "gelu": 1, "silu": 2}  # SELAS_ACT_*
 
 def raw_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, act: str | None = None,
                gate: torch.Tensor | None = None, residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
-               out_dtype: torch.dtype | None = None) -> torch.Tensor:
+               out_dtype: torch.dtype | None = None, guard: bool = False) -> torch.Tensor:
     """``residual + gate * act(x @ weight.T + bias)`` with an unquantized weight, in one kernel.
 
     x [..., K] and weight [N, K] (bf16 or fp16, unit column stride or copied); ``act``: None, "gelu" (tanh
     approximation, flux.py:194-195) or "silu" (flux.py:150-151); ``gate``: one row per image, [B, 1, N], or one
     for all ([N], [1, N], [1, 1, N]), where x is [B, L, K]; ``residual``: [..., N]. Bias, gate, residual and the
     result are each fp32 or x's dtype; the result has ``out``'s dtype, or ``out_dtype``, or the residual's, or x's.
-    The sum, the activation, the gate and the residual are fp32, rounded once.
+    The sum, the activation, the gate and the residual are fp32, rounded once. ``guard``: act(..) is clamped to the
+    fp16 range ahead of the gate and the residual, NaN passing through, as ``Kernels.gated_add`` clamps the linear's
+    output (flux.py:169-171): an fp16 x may hold infinities, which would stay in the residual.
 
     ``out``: optional [..., N] destination with unit column stride (returned); it may be the residual itself
     (the residual stream updated in place), any other overlap is refused. Other dtypes raise ``Unsupported``."""
-    return raw_linear_batched([RawLinear(x, weight, bias, act, gate, residual, out, out_dtype)])[0]
+    return raw_linear_batched([RawLinear(x, weight, bias, act, gate, residual, out, out_dtype, guard)])[0]
 
 
 def raw_linear_batched(problems) -> list[torch.Tensor]:
@@ -392,7 +395,7 @@ def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
             return _lib.F32
         raise ValueError(f"raw_linear: {name} is {d}, takes {dt} or float32")
 
-    for x, w, bias, act, gate, residual, out, out_dtype in problems:
+    for x, w, bias, act, gate, residual, out, out_dtype, guard in problems:
         if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
             raise ValueError(f"raw_linear: x {tuple(x.shape)} does not go with weight {tuple(w.shape)}")
         if x.dtype != dt or w.dtype != dt:
@@ -435,7 +438,7 @@ def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
         keep += (x3, w, bias, g, r)
         packed.append(_lib.RAW_LINEAR_PROBLEM.pack(
             x3.data_ptr(), x_sb, x_sl, w.data_ptr(), w.stride(0), bias_p, gate_p, g_sb, res_p, r_sb, r_sl, y.data_ptr(),
-            y_sb, y_sl, b, l, n, k, bias_dt, gate_dt, res_dt, y_dt, ACTS[act], 0))
+            y_sb, y_sl, b, l, n, k, bias_dt, gate_dt, res_dt, y_dt, ACTS[act], bool(guard)))
     if len(problems) > 1:
         _check_raw_disjoint(problems, outs)
     arr, count = b"".join(packed), len(packed)
