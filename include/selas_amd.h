@@ -505,7 +505,9 @@ typedef struct selas_raw_linear_problem {
 /*
  * Up to SELAS_MAX_BATCHED_LINEARS independent linears with unquantized weights,
  * x and w in dtype (bf16 or fp16, otherwise SELAS_EUNSUPPORTED), fp32 accumulation
- * and epilogue, one rounding at the end. K may be 0 (act(bias) remains).
+ * and epilogue, one rounding at the end. K may be 0 (act(bias) remains). With more than
+ * 32 rows and 64 columns, min(256, rows) rows of K elements of each operand, K rounded up to 64, must take less
+ * than 2^31 - 4096 bytes (K to 4,194,240 at 256 rows; otherwise SELAS_EUNSUPPORTED).
  * workspace: device memory of at least selas_raw_linear_workspace_bytes for
  * these problems, 16-byte aligned, not used by anything else until the call has
  * run; NULL and 0 where that size is 0, otherwise SELAS_EINVAL. The kernels, tiles

@@ -1042,6 +1042,9 @@ bool dma_ok_x(const selas_raw_linear_problem &p) {
   return (span + p.K) * 2 < (1ll << 31) - 4096;
 }
 
+// Whether the rows of a tile of a copied operand of `rows` rows (raw_pack_kernel) span less than 31 bits of bytes.
+bool pack_ok(int64_t rows, int64_t K) { return (rows < 256 ? rows : 256) * cdiv(K, 64) * 128 < (1ll << 31) - 4096; }
+
 // The current device's CU count (asked once per device).
 int cu_count() {
   constexpr int kDevices = 64;
@@ -1295,8 +1298,14 @@ int check_call(const selas_raw_linear_problem *problems, int64_t count, int dtyp
                      (long long)count);
   if (!valid_dtype(dtype)) return set_error(SELAS_EINVAL, "raw_linear: bad dtype %d", dtype);
   if (dtype == SELAS_F32) return set_error(SELAS_EUNSUPPORTED, "raw_linear: takes bf16 or fp16 weights");
-  for (int64_t i = 0; i < count; ++i)
-    if (int e = check_problem(problems[i], i, dtype)) return e;
+  for (int64_t i = 0; i < count; ++i) {
+    const selas_raw_linear_problem &p = problems[i];
+    if (int e = check_problem(p, i, dtype)) return e;
+    const int64_t M = p.B * p.L;
+    if (M > kFewX && p.N > kFewW && ((!dma_ok_x(p) && !pack_ok(M, p.K)) || (!dma_ok_w(p) && !pack_ok(p.N, p.K))))
+      return set_error(SELAS_EUNSUPPORTED, "raw_linear[%lld]: K = %lld: the rows of a tile span 2^31 bytes", (long long)i,
+                       (long long)p.K);
+  }
   return SELAS_OK;
 }
 

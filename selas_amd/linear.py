@@ -344,7 +344,8 @@ def raw_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     output (flux.py:169-171): an fp16 x may hold infinities, which would stay in the residual.
 
     ``out``: optional [..., N] destination with unit column stride (returned); it may be the residual itself
-    (the residual stream updated in place), any other overlap is refused. Other dtypes raise ``Unsupported``."""
+    (the residual stream updated in place), any other overlap is refused. Other dtypes, and K above 4 million
+    against more than 32 rows and 64 columns, raise ``Unsupported``."""
     return raw_linear_batched([RawLinear(x, weight, bias, act, gate, residual, out, out_dtype, guard)])[0]
 
 
