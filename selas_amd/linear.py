@@ -352,8 +352,10 @@ def raw_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 def raw_linear_batched(problems) -> list[torch.Tensor]:
     """``[raw_linear(...) for each]`` of independent ``RawLinear`` problems of one dtype, up to four per launch (e.g.
     the image and text streams of a double block, selas/models/flux.py:300-324). No problem's ``out`` may overlap
-    another problem's tensors."""
+    another problem's tensors, in whichever launch."""
     problems = [RawLinear(*p) for p in problems]
+    if len(problems) > 1:
+        _check_raw_disjoint(problems)
     outs: list[torch.Tensor] = []
     for i in range(0, len(problems), _lib.MAX_BATCHED_LINEARS):
         outs += _raw_chunk(problems[i:i + _lib.MAX_BATCHED_LINEARS])
@@ -440,8 +442,6 @@ def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
         packed.append(_lib.RAW_LINEAR_PROBLEM.pack(
             x3.data_ptr(), x_sb, x_sl, w.data_ptr(), w.stride(0), bias_p, gate_p, g_sb, res_p, r_sb, r_sl, y.data_ptr(),
             y_sb, y_sl, b, l, n, k, bias_dt, gate_dt, res_dt, y_dt, ACTS[act], bool(guard)))
-    if len(problems) > 1:
-        _check_raw_disjoint(problems, outs)
     arr, count = b"".join(packed), len(packed)
     with _lib.on(dev):
         stream = _lib.stream(dev)
@@ -458,12 +458,12 @@ def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
     return outs
 
 
-def _check_raw_disjoint(problems: list[RawLinear], outs: list[torch.Tensor]) -> None:
+def _check_raw_disjoint(problems: list[RawLinear]) -> None:
     for i, p in enumerate(problems):
         if p.out is None:
             continue
         for j, q in enumerate(problems):
-            others = (q.x, q.weight, q.bias, q.gate, q.residual, outs[j])
+            others = (q.x, q.weight, q.bias, q.gate, q.residual, q.out)
             if j != i and any(t is not None and may_meet(p.out, t) for t in others):
                 raise ValueError(f"raw_linear: out of problem {i} overlaps a tensor of problem {j}")
 
