@@ -352,13 +352,17 @@ def raw_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 def raw_linear_batched(problems) -> list[torch.Tensor]:
     """``[raw_linear(...) for each]`` of independent ``RawLinear`` problems of one dtype, up to four per launch (e.g.
     the image and text streams of a double block, selas/models/flux.py:300-324). No problem's ``out`` may overlap
-    another problem's tensors, in whichever launch."""
+    another problem's tensors, in whichever launch. Nothing is launched where one of the problems is refused."""
     problems = [RawLinear(*p) for p in problems]
     if len(problems) > 1:
         _check_raw_disjoint(problems)
+    # Every launch is prepared and checked ahead of the first: a problem that is refused leaves all results as they were.
+    most = _lib.MAX_BATCHED_LINEARS
+    chunks = [_raw_chunk(problems[i:i + most], len(problems) > most) for i in range(0, len(problems), most)]
     outs: list[torch.Tensor] = []
-    for i in range(0, len(problems), _lib.MAX_BATCHED_LINEARS):
-        outs += _raw_chunk(problems[i:i + _lib.MAX_BATCHED_LINEARS])
+    for chunk_outs, launch in chunks:
+        launch()
+        outs += chunk_outs
     return outs
 
 
@@ -383,7 +387,8 @@ def _raw_vector(v: torch.Tensor, b: int, n: int) -> tuple[torch.Tensor, int]:
     return v, (v.stride(0) if lead and lead[0] > 1 else 0)
 
 
-def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
+def _raw_chunk(problems: list[RawLinear], check: bool):
+    """(results, the call that launches them) of up to four problems. ``check``: what the library refuses is refused here."""
     dt = problems[0].x.dtype
     dev = _lib.require_gpu(*(t for p in problems for t in (p.x, p.weight, p.bias, p.gate, p.residual, p.out)))
     if dt != torch.bfloat16 and dt != torch.float16:
@@ -443,19 +448,31 @@ def _raw_chunk(problems: list[RawLinear]) -> list[torch.Tensor]:
             x3.data_ptr(), x_sb, x_sl, w.data_ptr(), w.stride(0), bias_p, gate_p, g_sb, res_p, r_sb, r_sl, y.data_ptr(),
             y_sb, y_sl, b, l, n, k, bias_dt, gate_dt, res_dt, y_dt, ACTS[act], bool(guard)))
     arr, count = b"".join(packed), len(packed)
-    with _lib.on(dev):
-        stream = _lib.stream(dev)
-        try:
-            _lib.call("selas_raw_linear", arr, count, code, None, 0, stream)
-        except ValueError:  # most launches need no workspace: asked for only where one without was refused
-            size = ctypes.c_int64()
-            _lib.call("selas_raw_linear_workspace_bytes", arr, count, code, ctypes.byref(size))
-            if size.value == 0:
-                raise
-            ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
-            _lib.call("selas_raw_linear", arr, count, code, ws.data_ptr(), size.value, stream)
-    del keep  # the launch is queued on the stream that later reuses this memory
-    return outs
+
+    def workspace_bytes() -> int:
+        size = ctypes.c_int64()
+        _lib.call("selas_raw_linear_workspace_bytes", arr, count, code, ctypes.byref(size))
+        return size.value
+
+    if check:
+        with _lib.on(dev):
+            workspace_bytes()
+
+    def launch():
+        nonlocal keep
+        with _lib.on(dev):
+            stream = _lib.stream(dev)
+            try:
+                _lib.call("selas_raw_linear", arr, count, code, None, 0, stream)
+            except ValueError:  # most launches need no workspace: asked for only where one without was refused
+                size = workspace_bytes()
+                if size == 0:
+                    raise
+                ws = torch.empty(size, dtype=torch.uint8, device=dev)
+                _lib.call("selas_raw_linear", arr, count, code, ws.data_ptr(), size, stream)
+        keep = None  # the launch is queued on the stream that later reuses this memory
+
+    return outs, launch
 
 
 def _check_raw_disjoint(problems: list[RawLinear]) -> None:
