@@ -555,6 +555,22 @@ def get_schedule(num_steps: int, image_seq_len: int, base_shift: float = 0.5, ma
     return [shifted(t) for t in ts]
 
 
+def _positions_of_each(txt_ids: torch.Tensor, img_ids: torch.Tensor, b: int, dev) -> torch.Tensor:
+    """Positions [b, Lt + Li, axes] of every image's tokens, text first, in a type that rope_qk takes and that holds
+    them: the image positions' own where it is one of those, or fp32. Positions that fp32 does not hold are refused."""
+    if img_ids.shape[0] not in (1, b):
+        raise ValueError(f"img_ids {tuple(img_ids.shape)} for a batch of {b}")
+
+    def holds(dtype: torch.dtype, t: torch.Tensor) -> bool:
+        return t.dtype == dtype or bool(((t.to(dtype).to(t.dtype) == t) | (t != t)).all())
+
+    own = img_ids.dtype if img_ids.dtype in (torch.int32, torch.int64) else torch.float32
+    for dtype in dict.fromkeys((own, torch.float32)):
+        if holds(dtype, txt_ids) and holds(dtype, img_ids):
+            return torch.cat([t.to(dev, dtype).expand(b, *t.shape[-2:]) for t in (txt_ids, img_ids)], dim=1)
+    raise ValueError(f"img_ids {img_ids.dtype} and txt_ids {txt_ids.dtype}: positions that float32 does not hold")
+
+
 @dataclass
 class FluxConditioning:
     """Everything a step needs besides the latents (flux.py:365-373): per block [S, B, kD] modulations,
@@ -625,8 +641,9 @@ class FluxRunner:
         """Everything that does not depend on the latents, once per batch (flux.py:448-465). ``mods``: the
         batch's modulation vectors {block: [S, B, kD]} when already known. ``img_ids`` [Li, axes], or
         [B, Li, axes] for images of other shapes or offsets with the same number of tokens (a portrait and a
-        landscape, windows of one canvas)."""
+        landscape, windows of one canvas); of any type there, with values that int32, int64 or fp32 hold."""
         cfg, g, dt, dev = self.cfg, self.g, self.dt, self.model.device
+        each = _positions_of_each(txt_ids, img_ids, pooled.shape[0], dev) if img_ids.dim() == 3 else None
         svecs = [self.svec(sigmas, guidance, pooled[i:i + 1]) for i in range(pooled.shape[0])]
         if mods is None:
             per_image = self.modulations(svecs)
@@ -637,11 +654,7 @@ class FluxRunner:
         else:
             final_mod = torch.cat([g.linear(sv, "final_layer.adaLN_modulation.1") for sv in svecs], dim=1)
             txt_h = g.linear(txt.to(dev, dt), "txt_in").float()
-        if img_ids.dim() == 3:
-            b = pooled.shape[0]
-            if img_ids.shape[0] not in (1, b):
-                raise ValueError(f"img_ids {tuple(img_ids.shape)} for a batch of {b}")
-            each = torch.cat([t.to(dev).expand(b, *t.shape[-2:]) for t in (txt_ids.to(img_ids.dtype), img_ids)], dim=1)
+        if each is not None:
             return FluxConditioning(list(sigmas), mods, final_mod, txt_h, None, None, txt.shape[1], each)
         ids = torch.cat((txt_ids, img_ids), dim=0).to(dev)
         cos, sin = rope_tables(ids, cfg.axes_dim, cfg.theta)
