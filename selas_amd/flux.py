@@ -128,8 +128,9 @@ def _linear_pair(w, a, b):
 
 
 def _fused_raw(w, k) -> bool:
-    """Whether the unit's raw weights run through raw_linear, with the activation, gate and residual in its epilogue."""
-    return isinstance(k, Kernels) and getattr(w, "fused_raw", False)
+    """Whether the unit's raw weights run through raw_linear, with the activation, gate and residual in its epilogue:
+    asked for, possible for all of its linears, and the segments are this package's kernels."""
+    return isinstance(k, Kernels) and getattr(w, "fused_raw", False) and w.takes_raw_linear()
 
 
 def _qkv_rope(qkv, q_scale, k_scale, ids, cfg: FluxConfig, out=None):
@@ -389,7 +390,7 @@ class RandomFlux:
                 self.mods.append(UnitView(_linear_parts(gen, "modulation.lin", d, 3 * d, dtype, quant), dtype))
         del gen
         for u in (self.globals, *self.doubles, *self.singles, *self.mods):
-            u.fused_raw = raw and dtype in (torch.bfloat16, torch.float16)
+            u.fused_raw = raw
 
     def nf4_bytes(self) -> int:
         units = self.doubles + self.singles + self.mods
@@ -403,7 +404,7 @@ class RandomFlux:
         return out
 
     @torch.no_grad()
-    def modulations(self, sv: torch.Tensor, grouped: bool = True) -> list[torch.Tensor]:
+    def modulations(self, sv: torch.Tensor, grouped: bool = True, k: Kernels = FUSED) -> list[torch.Tensor]:
         """Every block's modulation vectors [S, 1, kD] from silu(vec) [S, 1, D] (flux.py:428-445).
 
         ``grouped`` runs all modulation linears in one launch (same bits as one call per linear)."""
@@ -430,7 +431,7 @@ class RandomFlux:
                 per.append(len(ps))
             linear_grouped_into(codec, sv, ws, out, per)
             return out
-        if self.mods and all(u.fused_raw for u in self.mods):
+        if self.mods and all(_fused_raw(u, k) for u in self.mods):
             out = []
             for j, u in enumerate(self.mods):
                 ps = ("img_mod.lin", "txt_mod.lin") if j < nd else ("modulation.lin",)
@@ -522,9 +523,9 @@ def timestep_embedding(t: torch.Tensor, dim: int = 256, max_period: float = 1000
     return emb
 
 
-def mlp_embed(w, prefix: str, x: torch.Tensor) -> torch.Tensor:
+def mlp_embed(w, prefix: str, x: torch.Tensor, k: Kernels = FUSED) -> torch.Tensor:
     """in_layer, SiLU, out_layer (flux.py:150-151)."""
-    if getattr(w, "fused_raw", False):
+    if _fused_raw(w, k):
         (h,) = w.raw_linear_many([(x, prefix + ".in_layer", {"act": "silu"})])
         return w.raw_linear_many([(h, prefix + ".out_layer")])[0]
     return w.linear(F.silu(w.linear(x, prefix + ".in_layer")), prefix + ".out_layer")
@@ -623,17 +624,17 @@ class FluxRunner:
         embeddings (flux.py:411-425)."""
         cfg, g, dt, dev = self.cfg, self.g, self.dt, self.model.device
         t = torch.tensor(list(sigmas[:-1]), dtype=torch.float32, device=dev)
-        vec = mlp_embed(g, "time_in", timestep_embedding(t, 256).to(dt)).float()[:, None, :]
+        vec = mlp_embed(g, "time_in", timestep_embedding(t, 256).to(dt), self.k).float()[:, None, :]
         if cfg.guidance_embed:
             gv = torch.full((1,), float(guidance), dtype=torch.float32, device=dev)
-            vec = vec + mlp_embed(g, "guidance_in", timestep_embedding(gv, 256).to(dt)).float()[None]
-        vec = vec + mlp_embed(g, "vector_in", pooled.to(dev, dt)).float()[None]
+            vec = vec + mlp_embed(g, "guidance_in", timestep_embedding(gv, 256).to(dt), self.k).float()[None]
+        vec = vec + mlp_embed(g, "vector_in", pooled.to(dev, dt), self.k).float()[None]
         return F.silu(vec).to(dt)
 
     @torch.no_grad()
     def modulations(self, svecs: list[torch.Tensor]) -> list[dict[str, torch.Tensor]]:
         """Every block's modulation vectors [S, 1, kD] for each image's svec (flux.py:428-445)."""
-        return [dict(zip(self.main, self.model.modulations(sv))) for sv in svecs]
+        return [dict(zip(self.main, self.model.modulations(sv, k=self.k))) for sv in svecs]
 
     @torch.no_grad()
     def prepare(self, sigmas, guidance: float, pooled: torch.Tensor, txt: torch.Tensor, img_ids: torch.Tensor,
@@ -648,7 +649,7 @@ class FluxRunner:
         if mods is None:
             per_image = self.modulations(svecs)
             mods = {n: torch.cat([m[n] for m in per_image], dim=1) for n in self.main}
-        if getattr(g, "fused_raw", False):
+        if _fused_raw(g, self.k):
             final_mod = torch.cat([g.raw_linear_many([(sv, "final_layer.adaLN_modulation.1")])[0] for sv in svecs], dim=1)
             (txt_h,) = g.raw_linear_many([(txt.to(dev, dt), "txt_in", {"out_dtype": torch.float32})])
         else:

@@ -655,8 +655,8 @@ class UnitView:
     copied. ``UnitView(tensors, dtype)`` takes a dict of :class:`EncodedTensor` with device parts
     instead. ``get`` decodes (raw tensors in the compute dtype are returned as zero-copy views and
     cached), ``linear`` is the quantized-linear forward. With ``fused_raw`` set, the callers in
-    ``selas_amd.flux`` run a unit of raw weights through ``raw_linear_many`` (bf16 or fp16 weights in the compute
-    dtype) instead of ``F.linear`` and separate kernels after it.
+    ``selas_amd.flux`` run a unit that ``takes_raw_linear`` through ``raw_linear_many`` instead of ``F.linear`` and
+    separate kernels after it; other units (fp32, quantized weights) run as without it.
     """
 
     __slots__ = ("tensors", "dtype", "_views", "spec", "buf", "fused_raw")
@@ -752,6 +752,12 @@ class UnitView:
         if codec is not None:
             return _single(codec, prob)
         return F.linear(x, self.get(prefix + ".weight", dtype), prob)
+
+    def takes_raw_linear(self) -> bool:
+        """Whether ``raw_linear_many`` takes every linear of this unit as it is: computed in bf16 or fp16, all matrices
+        raw (a quantized one would be decoded whole for each call)."""
+        return self.dtype in (torch.bfloat16, torch.float16) and all(
+            e.codec == "raw" for e in self.tensors.values() if len(e.shape) == 2)
 
     def raw_linear_many(self, items) -> list[torch.Tensor]:
         """``raw_linear`` of each (x, prefix) or (x, prefix, options) item with this unit's raw weights, up to four
