@@ -463,8 +463,8 @@ typedef struct selas_rope_part {
  * even, R <= Dh. Angles are formed and reduced in fp64, the rest is fp32 and
  * rounded once. dtype is the tensors' type. y may be x (same address and strides);
  * otherwise no y may overlap an x or another y. Dh <= 256 where the tensors can be read
- * in vectors (4 elements or 8 bytes: addresses, strides, Dh, R and, with halves, R/2),
- * Dh <= 128 otherwise (SELAS_EUNSUPPORTED).
+ * in vectors of 4 elements (strides, Dh, R and, with halves, R/2 multiples of 4, addresses
+ * of 16 bytes in fp32 and of 8 otherwise), Dh <= 128 elsewhere (SELAS_EUNSUPPORTED).
  * Next to selas_qkv_single and selas_qkv_double, which take cos/sin tables that a
  * batch shares. Restates qk_rms, apply_rope and rope_tables (flux.py:106-126).
  */

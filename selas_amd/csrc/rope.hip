@@ -147,9 +147,9 @@ __device__ __forceinline__ void store_vec(void *p, int64_t i, const float (&v)[V
 }
 
 // V channels per vector: 8 (16-bit types) or 4 where everything is aligned to that, else 1. With V = 1 a unit is
-// one pair; otherwise the first vector of a rotated unit u starts at channel u V, the second at R/2 + u V (V divides
-// R/2), which are halves of the same pairs or, for adjacent pairs, V/2 pairs each. Unrotated channels follow in pairs
-// of vectors, the last without its second where (Dh - R) / V is odd.
+// one pair; otherwise the first vector of a rotated unit u of U starts at channel u V, the second at (U + u) V, which are
+// halves of the same pairs (V divides R/2 = U V) or, for adjacent pairs, V/2 pairs each, the last unit without its second
+// where R / V is odd. Unrotated channels follow in pairs of vectors, the last without its second where (Dh - R) / V is odd.
 template <int DT, int V, bool HALVES>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, Turns turns) {
   const int group = a.group;
@@ -157,17 +157,17 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, Turns turns) {
   const uint32_t token = blockIdx.x * (256 / group) + threadIdx.x / group;
   const bool live = token < static_cast<uint32_t>(a.tokens) && u < a.units;
   const int b = live ? static_cast<int>(div31(token, a.by_l)) : 0, l = live ? static_cast<int>(token) - b * a.L : 0;
-  const int R = 2 * a.pairs, rot_units = a.pairs / V;
+  const int R = 2 * a.pairs, rot_units = (R + 2 * V - 1) / (2 * V);
   const bool rotated = live && u < rot_units;
   int c0, c1;
   if (u < rot_units) {
     c0 = (V == 1 && !HALVES) ? 2 * u : u * V;
-    c1 = (V == 1 && !HALVES) ? 2 * u + 1 : a.pairs + u * V;
+    c1 = (V == 1 && !HALVES) ? 2 * u + 1 : (rot_units + u) * V;
   } else {
     c0 = R + 2 * (u - rot_units) * V;
     c1 = c0 + V;
   }
-  const bool two = live && c1 < a.Dh;
+  const bool two = live && c1 < (u < rot_units ? R : a.Dh);
 
   float sn[V], cs[V];
   if (rotated) {
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, Turns turns) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       // Pair j of this unit: of its two vectors' adjacent pairs, or of its halves.
-      const int i = (V == 1 || HALVES) ? u * V + j : (j < V / 2 ? c0 / 2 + j : c1 / 2 + j - V / 2);
+      const int i = (V == 1 || HALVES) ? u * V + j : (j < V / 2 ? c0 / 2 + j : min(c1 / 2 + j - V / 2, a.pairs - 1));
       double p = pos[0];
 #pragma unroll
       for (int e = 1; e < SELAS_ROPE_MAX_AXES; ++e) p = i >= a.axis_end[e - 1] ? pos[e] : p;
@@ -260,9 +260,10 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, Turns turns) {
   }
 }
 
-// Whether every vector of `bytes` bytes (V elements) that the kernel would access is aligned.
-bool rope_vec_ok(const RopeArgs &a, int V, int esize) {
-  if (a.Dh % V || a.pairs % V) return false;
+// Whether every vector of `bytes` bytes (V elements) that the kernel would access is aligned, and the rotated channels are
+// whole vectors: two for each unit with halves, and with vectors of 8 (where that fails for 8, it holds for 4).
+bool rope_vec_ok(const RopeArgs &a, int V, int esize, bool halves) {
+  if (a.Dh % V || (halves || V == 8 ? a.pairs : 2 * a.pairs) % V) return false;
   const uintptr_t bytes = static_cast<uintptr_t>(V) * esize > 16 ? 16 : static_cast<uintptr_t>(V) * esize;
   for (int i = 0; i < a.count; ++i) {
     const selas_rope_part &p = a.part[i];
@@ -346,12 +347,13 @@ extern "C" int selas_rope(const selas_rope_part *parts, int64_t count, int64_t B
     a.axis_end[i] = pairs;
   }
   const int esize = dtype == SELAS_F32 ? 4 : 2;
-  const int V = dtype != SELAS_F32 && rope_vec_ok(a, 8, esize) ? 8 : rope_vec_ok(a, 4, esize) ? 4 : 1;
-  a.units = static_cast<int>(R / 2 / V + cdiv(Dh - R, 2 * V));
+  const int V = dtype != SELAS_F32 && rope_vec_ok(a, 8, esize, halves != 0) ? 8 : rope_vec_ok(a, 4, esize, halves != 0) ? 4 : 1;
+  a.units = static_cast<int>(cdiv(R, 2 * V) + cdiv(Dh - R, 2 * V));
   a.group = 1;
   while (a.group < a.units) a.group *= 2;
   if (a.group > 64)
-    return set_error(SELAS_EUNSUPPORTED, "rope: heads of %lld channels off 4-element alignment", (long long)Dh);
+    return set_error(SELAS_EUNSUPPORTED, "rope: heads of %lld channels off 4-element alignment (%lld rotated%s)", (long long)Dh,
+                     (long long)R, halves ? " in halves" : "");
   // Heads per thread: the fewest that leave no more than 4 workgroups per CU of 256, which are resident at once (90
   // registers allow 5). A thread's positions, angles and scales then serve as many heads as possible, and no second round
   // pays for them again (image of 4608 tokens, us: 41.3 with 1152 workgroups, 46 with 1728, 50 with 1296 of which 16 wait).

@@ -54,8 +54,9 @@ def rope_qk(q: torch.Tensor, k: torch.Tensor, ids: torch.Tensor, axes_dim, theta
     arithmetic is fp32 with one rounding.
 
     ``out``: destinations (q_out, k_out[, v_out]) of the same shapes with unit channel stride; a tensor may be its
-    own destination, any other overlap is refused. Heads above 256 channels, or above 128 whose addresses, strides or
-    axes are not multiples of 4 elements, raise ``Unsupported``."""
+    own destination, any other overlap is refused. Heads above 256 channels raise ``Unsupported``, and so
+    do those above 128 that are not read in vectors of 4 elements: addresses, strides, Dh and sum(axes_dim) (half of it with
+    ``pairs="halves"``) are multiples of 4 elements there."""
     if q.dim() != 4:
         raise ValueError(f"rope_qk: q must be [B, heads, L, Dh], got shape {tuple(q.shape)}")
     if pairs not in PAIRS:
