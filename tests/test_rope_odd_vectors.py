@@ -52,3 +52,16 @@ def test_adjacent_pairs(dev, dh, axes, dtype, norm):
         rope_qk(x, kk, to(ids), axes, out=(x, kk))
         assert torch.equal(x, y[0]) and torch.equal(kk, y[1])
         assert bool((buf[:at] == 5.0).all()) and bool((buf[at + q.numel():] == 5.0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_channels_that_are_not_turned_keep_what_is_not_finite(dev, dtype):
+    # 12 of 20 channels turned: the third vector's unit also holds the first vector that is not.
+    q = normal((1, 2, 9, 20), 1, 1, dtype)
+    q[..., 12], q[..., 14], q[..., 19] = float("inf"), float("nan"), float("-inf")
+    y = rope_qk(q.to(dev), q.to(dev), grid(1, 9, 1, 2).to(dev), (12,))[0].cpu()
+    assert bool(y[..., :12].isfinite().all())
+    for c in (13, 15, 16, 17, 18):
+        assert torch.equal(y[..., c], q[..., c])
+    assert torch.equal(y[..., 12], q[..., 12]) and torch.equal(y[..., 19], q[..., 19]) and bool(y[..., 14].isnan().all())
