@@ -305,8 +305,9 @@ __device__ __forceinline__ void to_partial(RawProblem &P, float *part) {
 }
 
 // y = epilogue(sum over the K ranges, in their order): four columns per thread. Bound by the partial sums' reads, from the
-// Infinity Cache: 512 x 3072 of 8 ranges with an fp32 residual 11.6 us (63 MB, 5.4 TB/s). A pass of its own: tiles that
-// wait for one another need an order of workgroups that a launch does not promise, and atomic adds change the sum's order.
+// Infinity Cache: 512 x 3072 of 8 ranges with an fp32 residual 11.6 us (63 MB, 5.4 TB/s). A pass of its own, on all CUs.
+// Not tried: the last workgroup of a tile to count itself in adds the ranges, in the same order and without anyone waiting.
+// That saves the launch; the sums of these 24 tiles would be read by 24 CUs.
 template <int DT>
 __global__ __launch_bounds__(256) void raw_merge_kernel(RawProblem P, const float *__restrict__ part, int split) {
   const int groups = (P.N + 3) / 4;
@@ -346,9 +347,9 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t *row, int k, int K) {
 //
 // The tiled kernel's DMA takes whole 16-byte chunks. An operand whose rows are not made of them (K not a multiple of 8, an
 // odd stride or address) or span too much is copied first, to rows of K rounded up to 64 that end in zeros, a thread per
-// 16-byte chunk. The copy of 1386 x 667 and 1431 x 667 is 6.2 us (7.6 MB: a launch, and one load's latency), the tiles after
-// it 15 us; tiles of 64 x 64 that load such rows through registers took 26 us without it, and 4001 x 5999 x 5003
-// ran at 500 TFLOP/s there against 1,060 (the copy included).
+// 16-byte chunk. The copy of 1386 x 667 and 1431 x 667 is 6.3 us (7.6 MB: a launch, and one load's latency), the tiles after
+// it 16.3 us with GELU, gate and residual; tiles of 64 x 64 that load such rows through registers took 26 us without it, and
+// 4001 x 5999 x 5003 ran at 500 TFLOP/s there against 1,060 (the copy included).
 template <int DT>
 __global__ __launch_bounds__(256) void raw_pack_kernel(RawProblem P, uint16_t *xp, uint16_t *wp, int kp) {
   const int per_row = kp / 8;
@@ -377,9 +378,9 @@ __global__ __launch_bounds__(256) void raw_pack_kernel(RawProblem P, uint16_t *x
 // few rows' fragments from the caches. The waves' sums are added in LDS, in wave order.
 // SWAP: x is the streamed operand.
 //
-// A workgroup reads the few rows again for its 16 or 32 streamed ones, so up to as many bytes come from the caches as
-// from HBM; that, not HBM, is the bound (28 x 18432 x 3072: 26.7 us, 4.24 TB/s of weight, the few rows' 45 MB beside it;
-// in the kernel right below, for rows off the DMA's alignment, 36 us).
+// A workgroup reads the few rows again for its 16 or 32 streamed ones (28 x 18432 x 3072: 576 workgroups, 99 MB from the
+// caches beside the weight's 113 MB), and 16 adjacent lanes load from 16 rows: rows that the DMA could read take 36 us here,
+// rows of the weight that start at odd elements 81.
 constexpr int kFewWaves = 8;
 
 // The epilogue of the kernels for few rows: the waves' sums red[wave][few row][streamed row] are added in wave order, a
@@ -469,7 +470,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void raw_few_kernel(RawProblem P, f
 // lanes to another row, 64 cache lines looked up per load, which held the loads above at 16 bytes per clock and CU (28 x
 // 18432 x 3072 36 us). Here each wave copies its range of K to LDS of its own by DMA, 8 rows of 128 bytes per
 // instruction, ST steps of 64 columns ahead, and reads the fragments there; no barrier until the sums are added. 28 x 18432 x
-// 3072 26.7 us (the floor is 22.5); 1 x 3072 x 768 4.2 us and 4096 x 64 x 3072 11.0 us, where a launch, one chain of loads
+// 3072 26.7 us (the floor is 22.5): 231 workgroups of five blocks (80 rows) on 256 CUs, 4.24 TB/s of weight, and the few
+// rows' 40 MB from the caches beside it. 1 x 3072 x 768 4.5 us and 4096 x 64 x 3072 10.8 us, where a launch, one chain of loads
 // per wave and the sum over the waves are what is left.
 constexpr int kStreamWaves = 4;
 constexpr int stream_stages(int blocks) { return blocks <= 2 ? 4 : blocks == 3 ? 3 : 2; }
@@ -588,15 +590,16 @@ __device__ __forceinline__ void wait_lds_barrier() { asm volatile("s_waitcnt lgk
 // of K the loads are out of range: they bring zeros and no traffic, and the counts stay the same.
 //
 // Why so: 256 x 256 is the largest tile whose sums (256 registers a lane) and fragments fit one wave per SIMD, and the
-// fewest LDS bytes per product (one fragment read for 8 MFMAs); 16x16x32 MFMAs draw less power per product than 32x32x16,
-// and power sets the clock. A half's 16 KB per DMA wave and the XOR of chunk and row (row / 2) % 8 leave no bank conflict
-// (counted: 0). Two barriers a step instead of four, and the reads and DMAs pinned between the products, took the
-// MFMAs from 72 to 83 % busy at 8192^3 (709 us, 1,550 TFLOP/s; the library's 692). Of the block's linears,
-// 4096 x 12288 x 3072 with GELU is 227-234 us (1,320-1,360 TFLOP/s, floor 194: three rounds of 256 tiles whose
-// prologue and epilogue, 11 us each, nothing overlaps at one workgroup per CU), 4608 x 3072 x 15360 with an fp32
-// residual 316-322 us (1,350-1,375; floor 273: 216 tiles for 256 CUs, and all residual traffic at the end); 66 and 65 %
-// MFMA busy. HBM traffic is 1.0 of the output written, and of the operands read 2.3 and 1.7 times (the XCDs' L2s
-// each load what their tiles share).
+// fewest LDS bytes per product (one fragment read for 8 MFMAs). A half's 16 KB per DMA wave and the XOR of chunk and row
+// (row / 2) % 8 leave no bank conflict (counted: 0). Two barriers a step instead of four, and the reads and DMAs pinned
+// between the products, took the MFMAs from 72 to 83 % busy at 8192^3 (708-787 us back to back on several cards, the
+// library's product 710-735).
+// Of the block's linears, 4096 x 12288 x 3072 with GELU is 227-244 us where other kernels run in between and 244-268 back
+// to back (1,154-1,362 TFLOP/s, floor 194; the library's product with its bias 220-261 back to back): three rounds of 256
+// tiles whose prologue and epilogue, 11 us each, nothing overlaps at one workgroup per CU. 4608 x 3072 x 15360 with an
+// fp32 residual is 316-333 and 325-354 us (1,228-1,376 TFLOP/s, floor 273; the library's product 526): 216 tiles for 256
+// CUs, and all residual traffic at the end. MFMAs 65 and 66 % busy. HBM traffic is 1.0 of the output written, and of the
+// operands read 2.3 and 1.7 times (the XCDs' L2s each load what their tiles share).
 template <int DT, int WM, int WN, int MB, int NB, int OCC, bool TAIL>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch batch) {
   constexpr int TM = WM * MB * 16, TN = WN * NB * 16, HM = MB / 2, HN = NB / 2, NW = WM * WN;
@@ -1083,13 +1086,14 @@ struct Plan {
 };
 
 // Few rows: 32 of x (33 to 64 run faster as tiles: 60 x 9216 x 3072 25 us against 29), 64 of the weight (1024 x 64 x
-// 3072 9.6 us against 12).
+// 3072 9.6 us against 12). Each of these problems is a launch of its own.
 constexpr int kFewX = 32, kFewW = 64;
 
 // Blocks of 16 streamed rows per workgroup. Streamed weights: as many as make one round of one workgroup per CU, up to six,
 // for fewer reads of the few rows and no second round (us against two blocks: 28 x 18432 x 3072, five, 26.7 against 29.9;
 // 28 x 9216 x 3072, three, 16.8 against 20.2; 28 x 21504 x 3072, six, 30.3 against 32.1). Two instead of four are one round of two
-// workgroups per CU (4 x 16384 x 4096 25.2 against 28.7), and two past six (28 x 40000 x 1024 22.7 us, five 24.6).
+// workgroups per CU (4 x 16384 x 4096 25.2 against 28.7; with 17 to 32 rows, 27.0, four were not measured), and two past six
+// (28 x 40000 x 1024 22.7 us, five 24.6).
 // Streamed x, and rows off the DMA's alignment: two blocks where that gives every CU two workgroups, else one.
 int few_blocks(int64_t big, bool weights) {
   const int64_t blocks = cdiv(cdiv(big, 16), cu_count());  // per CU
@@ -1110,8 +1114,8 @@ int few_split(int64_t big, int64_t K) {
 // rows, 256 to 21504 columns, K 256 to 12288, weights from HBM; every tile and split timed). Its choices are within 1 %
 // of the fastest in the mean and 18 % at worst (384 x 12288 x 3072: 40 us in tiles of 256 x 128, 54 of 128 x 128; 1024 x
 // 12288 x 3072: 67 us of 256 x 256, 84 of 128 x 128; tiles of 128 x 256 were ahead in 13 shapes, by 0.3 % over all, and
-// are left out). A round is one tile on every CU; a step of K costs the more the more CUs are busy (the power limit); a
-// split launch pays for its second kernel and for writing and reading the partial sums.
+// are left out). Other ranges than the seven were not timed. A round is one tile on every CU; a step of K costs the more
+// the more CUs are busy; a split launch pays for its second kernel and for writing and reading the partial sums.
 struct TileCost {
   int tm, tn;
   double start, step, busy, round;

@@ -336,7 +336,7 @@ def raw_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     """``residual + gate * act(x @ weight.T + bias)`` with an unquantized weight, in one kernel.
 
     x [..., K] and weight [N, K] (bf16 or fp16, unit column stride or copied); ``act``: None, "gelu" (tanh
-    approximation, flux.py:194-195) or "silu" (flux.py:150-151); ``gate``: one row per image, [B, 1, N], or one
+    approximation, flux.py:194-195) or "silu" (flux.py:150-151); ``gate``: one row per image, [B, 1, N] or [B, N], or one
     for all ([N], [1, N], [1, 1, N]), where x is [B, L, K]; ``residual``: [..., N]. Bias, gate, residual and the
     result are each fp32 or x's dtype; the result has ``out``'s dtype, or ``out_dtype``, or the residual's, or x's.
     The sum, the activation, the gate and the residual are fp32, rounded once. ``guard``: act(..) is clamped to the
@@ -350,8 +350,9 @@ def raw_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
 
 def raw_linear_batched(problems) -> list[torch.Tensor]:
-    """``[raw_linear(...) for each]`` of independent ``RawLinear`` problems of one dtype, up to four per launch (e.g.
-    the image and text streams of a double block, selas/models/flux.py:300-324). No problem's ``out`` may overlap
+    """``[raw_linear(...) for each]`` of independent ``RawLinear`` problems of one dtype (e.g. the image and text
+    streams of a double block, selas/models/flux.py:300-324). Up to four tiled ones share a launch; one with at most 32 rows
+    or 64 columns is a launch of its own. No problem's ``out`` may overlap
     another problem's tensors, in whichever launch. Nothing is launched where one of the problems is refused."""
     problems = [RawLinear(*p) for p in problems]
     if len(problems) > 1:
@@ -760,8 +761,8 @@ class UnitView:
             e.codec == "raw" for e in self.tensors.values() if len(e.shape) == 2)
 
     def raw_linear_many(self, items) -> list[torch.Tensor]:
-        """``raw_linear`` of each (x, prefix) or (x, prefix, options) item with this unit's raw weights, up to four
-        independent ones per launch. ``options``: the keyword arguments of ``raw_linear``, and "rows", a slice of
+        """``raw_linear`` of each (x, prefix) or (x, prefix, options) item with this unit's raw weights, as
+        ``raw_linear_batched`` runs them. ``options``: the keyword arguments of ``raw_linear``, and "rows", a slice of
         the weight's (and bias's) rows."""
         problems = []
         for x, prefix, *rest in items:
