@@ -563,7 +563,8 @@ def _positions_of_each(txt_ids: torch.Tensor, img_ids: torch.Tensor, b: int, dev
         raise ValueError(f"img_ids {tuple(img_ids.shape)} for a batch of {b}")
 
     def holds(dtype: torch.dtype, t: torch.Tensor) -> bool:
-        return t.dtype == dtype or bool(((t.to(dtype).to(t.dtype) == t) | (t != t)).all())
+        same = t.to(dtype).to(t.dtype) == t
+        return t.dtype == dtype or bool((same | (t != t) if dtype.is_floating_point else same).all())  # NaN: no whole number
 
     own = img_ids.dtype if img_ids.dtype in (torch.int32, torch.int64) else torch.float32
     for dtype in dict.fromkeys((own, torch.float32)):

@@ -47,6 +47,13 @@ def test_values_that_no_type_holds_are_refused(txt, img):
         prepared(txt, img)
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_positions_that_are_not_finite_are_no_whole_numbers(value):
+    ids = prepared(torch.tensor([[0.0, value, 1.0]]), torch.ones(1, 2, 3, dtype=I64), 1)
+    assert ids.dtype == F32 and torch.equal(ids[0, 0, 1].isnan(), torch.tensor(value != value))
+    assert value != value or ids[0, 0, 1] == value
+
+
 def test_a_batch_of_another_size_is_refused():
     with pytest.raises(ValueError, match="batch of 2"):
         prepared(torch.zeros(1, 3), torch.zeros(3, 1, 3))
