@@ -913,12 +913,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
   };
   // The same for outputs off alignment, N not a multiple of 8 or batches with spacing of their own: addresses per row, and
   // vector accesses that may start at any element, except in the columns that N cuts. Columns past N and rows past M read
-<<<<<<< Updated upstream
   // the last one (live - 1 is then negative: the column N - 1). Two rows at once in the tile of two workgroups per CU, whose
   // registers do not hold four (1386 x 1431 x 667 with GELU and residual 21.5 us; four 24.1, one after another 25.5).
-=======
-  // the last one (live - 1 is then negative: the column N - 1).
->>>>>>> Stashed changes
   auto finish_any = [&](auto width) __attribute__((always_inline)) {
     constexpr int W = decltype(width)::value, LPR = NB * 16 / W, RPI = 64 / LPR, U = OCC == 1 ? 4 : 2;
     const int n = nw + (lane % LPR) * W, row = lane / LPR, live = N - n;
@@ -954,11 +950,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void raw_tile_kernel(RawBatch ba
             for (int j = 0; j < 4; ++j) v[u][4 * q + j] = f[j] + bias[0][4 * q + j];
           }
         }
-<<<<<<< Updated upstream
         activate_all(v, P.act, P.guard);
-=======
-        activate_all(v, P.act);
->>>>>>> Stashed changes
         if (P.gate && P.one_gate) {
 #pragma unroll
           for (int u = 0; u < U; ++u)
