@@ -482,8 +482,8 @@ int selas_rope(const selas_rope_part *parts, int64_t count, int64_t B, int64_t L
 /* One linear of a selas_raw_linear call (host-memory array element):
  *   y[b, l, n] = residual[b, l, n] + gate[b, n] * act(sum_k x[b, l, k] w[n, k] + bias[n])
  * with act(..) clamped to the fp16 range (+-65504, NaN passes through) where guard != 0,
- * as selas_gated_add clamps the linear's output, and unit column strides, batch strides *_sb and row strides *_sl in elements,
- * and the rows of w ldw elements apart. bias, gate and residual may be NULL. The
+ * as selas_gated_add clamps the linear's output. Unit column strides, batch strides *_sb
+ * and row strides *_sl in elements, and the rows of w ldw elements apart. bias, gate and residual may be NULL. The
  * dtypes of bias, gate, residual and y are each SELAS_F32 or the call's dtype.
  * y may be the residual (same address, strides and dtype) and overlap nothing else. */
 typedef struct selas_raw_linear_problem {

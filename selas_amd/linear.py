@@ -351,9 +351,9 @@ def raw_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
 def raw_linear_batched(problems) -> list[torch.Tensor]:
     """``[raw_linear(...) for each]`` of independent ``RawLinear`` problems of one dtype (e.g. the image and text
-    streams of a double block, selas/models/flux.py:300-324). Up to four tiled ones share a launch; one with at most 32 rows
-    or 64 columns is a launch of its own. No problem's ``out`` may overlap
-    another problem's tensors, in whichever launch. Nothing is launched where one of the problems is refused."""
+    streams of a double block, selas/models/flux.py:300-324). Up to four tiled ones share a launch; one with at most 32
+    rows or 64 columns is a launch of its own. No problem's ``out`` may overlap another problem's tensors, in whichever
+    launch. Nothing is launched where one of the problems is refused."""
     problems = [RawLinear(*p) for p in problems]
     if len(problems) > 1:
         _check_raw_disjoint(problems)
