@@ -530,6 +530,62 @@ int selas_raw_linear_workspace_bytes(const selas_raw_linear_problem *problems, i
 int selas_raw_linear_tile(const selas_raw_linear_problem *problems, int64_t count, int dtype, int64_t *rows,
                           int64_t *cols, int64_t *ranges);
 
+/* ------------------------------------------------------------ attention of the text side */
+
+/* One call of selas_text_attention (host memory): q [B, H, Lq, Dh], k and v [B, Hk, Lk, Dh] with unit channel stride and
+ * any batch, head and row strides (*_sb, *_sh, *_sl, elements), H a multiple of Hk; query head h reads key head
+ * h / (H / Hk). out is [B, Lq, H*Dh] (o_sb, o_sl); lse [B, H, Lq] fp32, contiguous, or NULL.
+ * Key j of image b exists where j < lengths[b] (NULL: all Lk; values outside 0 .. Lk count as the nearer end) and
+ * mask[b * mask_sb + j] != 0 (NULL: all). start[b], or start0 where start is NULL, is the position of the image's first
+ * query among the keys' positions 0 .. Lk - 1: with causal != 0 query i sees the keys j <= start + i.
+ * table [buckets, H] (row stride table_sl, type table_dtype) is the learned bias, or NULL. Its buckets are those of
+ * selas_relative_buckets. */
+typedef struct selas_text_attention_problem {
+  const void *q;
+  int64_t q_sb, q_sh, q_sl;
+  const void *k;
+  int64_t k_sb, k_sh, k_sl;
+  const void *v;
+  int64_t v_sb, v_sh, v_sl;
+  void *out;
+  int64_t o_sb, o_sl;
+  float *lse;
+  const int32_t *lengths;
+  const uint8_t *mask;
+  int64_t mask_sb;
+  const int32_t *start;
+  int64_t start0;
+  const void *table;
+  int64_t table_sl;
+  int64_t B, H, Hk, Lq, Lk, Dh, buckets, max_distance;
+  double scale;
+  int table_dtype, bidirectional, causal, reserved; /* reserved: 0 */
+} selas_text_attention_problem;
+
+/*
+ * s_ij = scale * q_i . k_j + table[bucket(j - (start + i)), h];  out_i = sum_j softmax_j(s_ij) v_j over the keys
+ * that query i sees; lse_i = log(sum_j exp(s_ij)). A query that sees no key gets zeros and an lse of -inf. What
+ * masked keys and values hold (NaN, infinities) does not reach a result. dtype (bf16 or fp16, otherwise SELAS_EUNSUPPORTED)
+ * is that of q, k, v and out; scores, maxima and sums are fp32, the probabilities are rounded to dtype for the second product.
+ * Takes Dh a multiple of 8 up to 128, addresses of 16 bytes and strides of 8 elements (out: 8 bytes and 4 elements), row
+ * strides up to 2^23 elements; otherwise SELAS_EUNSUPPORTED. scale is in 1e-30 .. 1e30. out and lse overlap nothing.
+ * workspace: at least selas_text_attention_workspace_bytes, 16-byte aligned, not used by anything else until the call has
+ * run; NULL and 0 where that size is 0. Kernels and the split of the keys depend on the sizes, on which of lengths, mask and
+ * table are given and on the CU count only, so equal calls give equal bits.
+ * Next to selas_attention, for the attention of the text encoders (selas/models/t5.py:66, clip.py:34) and of image tokens
+ * to an encoder's states. */
+int selas_text_attention(const selas_text_attention_problem *problem, int dtype, void *workspace, int64_t workspace_bytes,
+                         void *stream);
+int selas_text_attention_workspace_bytes(const selas_text_attention_problem *problem, int dtype, int64_t *bytes);
+
+/*
+ * The buckets of one direction: bucket t begins at distance edges[t] (edges[0] = 0, ascending), as many as *count says (at
+ * most 128; edges has room for them). With n buckets a direction (all of them, or half when bidirectional != 0), e = n / 2
+ * and m = max_distance: distance a is in bucket a if a < e, else in e + floor((n - e) log(a / e) / log(m / e)), at most
+ * n - 1, in exact arithmetic (a distance on a border belongs to the bucket that begins there). Keys after the query have the
+ * buckets from n on when bidirectional != 0, bucket 0 otherwise. n is 2 to 128, e < m <= 1024 (above: SELAS_EUNSUPPORTED). */
+int selas_relative_buckets(int64_t buckets, int64_t max_distance, int bidirectional, int32_t *edges, int64_t *count);
+
 #ifdef __cplusplus
 }
 #endif

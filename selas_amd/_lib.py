@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libselas_amd.so"
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 OK, EINVAL, EUNSUPPORTED, EHIP = 0, 1, 2, 3
 F32, F16, BF16 = 0, 1, 2
@@ -61,6 +61,9 @@ SIGNATURES: dict[str, list] = {
     "selas_raw_linear": [_P, _I64, _INT, _P, _I64, _P],
     "selas_raw_linear_workspace_bytes": [_P, _I64, _INT, ctypes.POINTER(ctypes.c_int64)],
     "selas_raw_linear_tile": [_P, _I64, _INT] + [ctypes.POINTER(ctypes.c_int64)] * 3,
+    "selas_text_attention": [_P, _INT, _P, _I64, _P],
+    "selas_text_attention_workspace_bytes": [_P, _INT, ctypes.POINTER(ctypes.c_int64)],
+    "selas_relative_buckets": [_I64, _I64, _INT, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int64)],
 }
 
 

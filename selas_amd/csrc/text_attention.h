@@ -1,0 +1,289 @@
+// What the kernels of the text side's attention share: the arguments, which keys a tile has, the bias by buckets, and the
+// LDS tiles of 64 rows that feed 32x32x16 MFMAs both along the rows and, transposed by the reads, across them.
+#pragma once
+
+#include <math.h>
+
+#include "common.h"
+
+namespace selas {
+namespace textattn {
+
+constexpr int kRows = 64;              // rows (keys or queries) per LDS tile
+constexpr int kMaxSide = 128;          // buckets per direction
+constexpr int kMaxDistance = 1024;     // the table by distance has to fit LDS beside the tiles
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr uint32_t kPast = 0x80000000u;  // a byte offset past every buffer range here (ranges stay below 2^31): loads read 0
+
+// [B, heads, rows, channels] with unit channel stride; strides in elements.
+struct Side {
+  const uint16_t *p;
+  int64_t sb, sh, sl;
+};
+
+// The learned bias: bucket t of a direction begins at distance edge[t], and from `reach` = edge[n - 1] on the bias no
+// longer changes. Keys after the query have the buckets from `ahead` on, or bucket 0 where there is one direction only.
+struct Bias {
+  const void *table;  // [buckets, H], unit column stride; null: no bias
+  int64_t row;
+  int dtype, n, ahead, reach;
+  int16_t edge[kMaxSide];
+};
+
+struct Args {
+  Side q, k, v;
+  uint16_t *out;  // [B, Lq, H * dh], unit column stride
+  int64_t out_sb, out_sl;
+  float *lse;  // [B, H, Lq] or null
+  const int32_t *lengths;  // [B] or null
+  const uint8_t *mask;     // [B, Lk] or null
+  int64_t mask_sb;
+  const int32_t *start;  // position of each image's first query, [B], or null: start0 for all
+  int start0;
+  int B, H, Hk, group, Lq, Lk, dh, causal;
+  float c2;  // scale * log2(e)
+  Bias bias;
+};
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Keys of image b; the position of its first query. Both are uniform, and bounded so that sums with them stay in 32 bits.
+__device__ __forceinline__ int keys_of(const Args &a, int b) {
+  return a.lengths ? uniform(min(max(a.lengths[b], 0), a.Lk)) : a.Lk;
+}
+__device__ __forceinline__ int start_of(const Args &a, int b) {
+  const int s = a.start ? uniform(a.start[b]) : a.start0;
+  return min(max(s, -(1 << 29)), 1 << 29);
+}
+
+// ------------------------------------------------------------------ element types
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Two values, already in registers of their own, rounded to nearest even into a packed pair.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  if constexpr (BF) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+template <bool BF>
+__device__ __forceinline__ float lo_of(uint32_t w) {
+  return BF ? __uint_as_float(w << 16) : f16_bits_to_f32(static_cast<uint16_t>(w));
+}
+template <bool BF>
+__device__ __forceinline__ float hi_of(uint32_t w) {
+  return BF ? __uint_as_float(w & 0xffff0000u) : f16_bits_to_f32(static_cast<uint16_t>(w >> 16));
+}
+
+// The probabilities of a forward pass are 2^(s - m) with m this far below the maximum: fp16 has room for it, and then
+// holds weights down to 2^-21 of the largest at full precision instead of 2^-14.
+template <bool BF>
+__device__ constexpr float headroom() {
+  return BF ? 0.0f : 7.0f;
+}
+
+__device__ __forceinline__ float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ------------------------------------------------------------------ the bias by distance
+
+// The table of head `head` as a function of distance d = key - query, times log2(e). Beyond `reach` it is constant, so
+// d in [-reach - 8, reach + 8] is all of it: runs of 8 distances starting anywhere are entries of it once their start is
+// clamped to [-reach - 8, reach + 1]. Lanes read runs of 4 distances that start anywhere, in one 16-byte read each: copy c
+// (of 4) begins c entries later, so that a run starting at i is aligned in copy i % 4. The copies are `bias_pitch` floats
+// apart, 64 bytes past a multiple of 256: the 16 lanes of a read then meet 16 different groups of banks.
+__host__ __device__ inline int bias_pitch(int reach) { return (2 * reach + 20 + 47) / 64 * 64 + 16; }
+__host__ __device__ inline int bias_bytes(int reach) { return 4 * 4 * bias_pitch(reach); }
+
+__device__ __forceinline__ int bucket_of(const Bias &t, int d) {
+  const int side = t.ahead ? abs(d) : max(-d, 0);
+  int r = t.ahead && d > 0 ? t.ahead - 1 : -1;
+  for (int i = 0; i < t.n; ++i) r += side >= t.edge[i];  // edge[0] = 0
+  return r;
+}
+
+__device__ __forceinline__ float bias_at(const Bias &t, int head, int d) {
+  const int64_t i = bucket_of(t, d) * t.row + head;
+  const float v = t.dtype == SELAS_F32   ? load_f<SELAS_F32>(t.table, i)
+                  : t.dtype == SELAS_F16 ? load_f<SELAS_F16>(t.table, i)
+                                         : load_f<SELAS_BF16>(t.table, i);
+  return v * kLog2e;
+}
+
+// reversed: by query - key. The caller puts barriers around it.
+__device__ __forceinline__ void build_bias(float *lds, const Bias &t, int head, int tid, int threads, bool reversed) {
+  const int pitch = bias_pitch(t.reach), first = -t.reach - 8;
+  for (int i = tid; i < 2 * t.reach + 17; i += threads) {
+    const int d = first + i;
+    const float v = bias_at(t, head, reversed ? -d : d);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (i >= c) lds[c * pitch + i - c] = v;
+  }
+}
+
+// Eight entries from distance d on.
+__device__ __forceinline__ void bias_run(const float *lds, int pitch, int reach, int d, float (&v)[8]) {
+  const int i = min(max(d, -reach - 8), reach + 1) + reach + 8;
+  const float *p = lds + (i & 3) * pitch + (i & ~3);
+  const f32x4 x = *reinterpret_cast<const f32x4 *>(p), y = *reinterpret_cast<const f32x4 *>(p + 4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = x[e];
+    v[4 + e] = y[e];
+  }
+}
+
+// ------------------------------------------------------------------ LDS tiles
+
+// 64 rows of D channels (dh of them given, the rest zeros), in 16-byte chunks whose place in the row is XORed with a
+// function of the row, so that two kinds of read are free of bank conflicts: 16 rows at one chunk (a row-wise operand),
+// and 4 rows at 64 bytes (ds_read_b64_tr_b16, a transposed operand).
+template <int D>
+struct Tile {
+  static constexpr int kRow = 2 * D;        // bytes
+  static constexpr int kChunks = D / 8;     // per row
+  static constexpr int kBytes = kRows * kRow;
+  static constexpr int kLoads = kBytes / 1024;  // DMA instructions (a wave's 64 x 16 bytes)
+  __device__ static __forceinline__ int swizzle(int r) {
+    return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  }
+
+  // The offsets of a wave's share of the loads: instructions KJ * wave + j, whose lane fills row `row(j)`.
+  template <int KJ>
+  struct Loader {
+    uint32_t voff[KJ];
+    int wave, lane;
+    __device__ __forceinline__ int row(int j) const { return (KJ * wave + j) * (64 / kChunks) + lane / kChunks; }
+    __device__ __forceinline__ Loader(int wave_, int lane_, int64_t sl, int dh) : wave(wave_), lane(lane_) {
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) {
+        const int r = row(j), chunk = (lane & (kChunks - 1)) ^ swizzle(r);
+        voff[j] = 8 * chunk < dh ? static_cast<uint32_t>(r) * static_cast<uint32_t>(2 * sl) + 16 * chunk : kPast;
+      }
+    }
+    // The tile whose first row is at `p`, of which `rows` exist (the others read as zeros, and so do rows whose bit in
+    // `bits` is not set where PART is).
+    template <bool PART>
+    __device__ __forceinline__ void issue(uint8_t *lds, const uint16_t *p, int64_t sl, int dh, int rows, uint64_t bits) const {
+      rows = min(rows, kRows);
+      const uint32_t bytes = rows > 0 ? 2 * ((rows - 1) * static_cast<uint32_t>(sl) + dh) : 0;
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(p, bytes);
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) {
+        uint32_t off = voff[j];
+        if constexpr (PART) off = (bits >> row(j)) & 1 ? off : kPast;
+        load_lds16(r, lds + (KJ * wave + j) * 1024, off, 0);
+      }
+    }
+  };
+
+  // Row-wise operand: lane (c, h) reads channels 16 s + 8 h .. + 8 of row 32 blk + swap23(c).
+  struct RowReader {
+    uint32_t base, flip;
+    __device__ __forceinline__ RowReader(int lane) {
+      const int c = lane & 31, r = (c & ~12) | ((c & 4) << 1) | ((c & 8) >> 1);
+      base = r * kRow;
+      flip = (swizzle(r) ^ (lane >> 5)) << 4;
+    }
+    __device__ __forceinline__ uint4 read(const uint8_t *lds, int blk, int s) const {
+      return *reinterpret_cast<const uint4 *>(lds + base + blk * 32 * kRow + ((32 * s) ^ flip));
+    }
+  };
+
+  // Transposed operand: lane (c, h) receives channel 32 db + c of rows 32 blk + 16 t + 8 h .. + 8.
+  struct ColReader {
+    uint32_t off[D / 32][2];
+    __device__ __forceinline__ ColReader(int lane) {
+      const int h = lane >> 5, r4 = (lane >> 2) & 3, x = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = 8 * h + 4 * u + r4;
+          off[db][u] = r * kRow + (((4 * db + x) ^ swizzle(r)) << 4) + 8 * (lane & 1);
+        }
+    }
+    __device__ __forceinline__ uint4 read(uint8_t *lds, int db, int blk, int t) const {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      auto half = [&](int u) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4 *)(lds + off[db][u] + (32 * blk + 16 * t) * kRow));
+      };
+      const s16x4 lo = half(0), hi = half(1);
+      return __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
+};
+
+// A wave's 32 rows as the B operand, in registers for the whole loop: lane (c, h) holds channels 16 s + 8 h .. + 8 of row c.
+// Rows that do not exist and channels from dh on are zeros.
+template <int D>
+struct Held {
+  uint4 f[D / 16];
+  __device__ __forceinline__ void load(const uint16_t *p, int64_t sl, int dh, int rows, int lane, bool keep = true) {
+    rows = min(rows, 32);
+    const uint32_t bytes = rows > 0 ? 2 * ((rows - 1) * static_cast<uint32_t>(sl) + dh) : 0;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(p, bytes);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const int ch = 16 * s + 8 * (lane >> 5);
+      const uint32_t off = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(2 * sl) + 2 * ch;
+      f[s] = load_b128(r, ch < dh && keep ? off : kPast, 0);
+    }
+  }
+};
+
+// ------------------------------------------------------------------ which keys a tile has
+
+// Bit i of a tile's word: key 64 kt + i exists and is not masked. The mask's bytes are loaded a tile ahead of their use.
+struct KeyBits {
+  const uint8_t *mask;  // of this image, or null
+  int keys, lane;
+  __device__ __forceinline__ KeyBits(const Args &a, int b, int keys_, int lane_)
+      : mask(a.mask ? a.mask + b * a.mask_sb : nullptr), keys(keys_), lane(lane_) {}
+  __device__ __forceinline__ int load(int kt) const {
+    const int key = kt * kRows + lane;
+    return mask && key < keys ? mask[key] : 0;
+  }
+  __device__ __forceinline__ uint64_t word(int kt, int byte) const {
+    if (mask) return __builtin_amdgcn_ballot_w64(byte != 0);
+    const int rows = keys - kt * kRows;
+    return rows >= kRows ? ~0ull : rows > 0 ? ~0ull >> (kRows - rows) : 0ull;
+  }
+};
+
+// The low n + 1 bits (none below 0, all from 63 on): the keys at or before position n of a tile.
+__device__ __forceinline__ uint64_t up_to(int n) { return n < 0 ? 0ull : n >= 63 ? ~0ull : (2ull << n) - 1; }
+
+// ------------------------------------------------------------------ host side
+
+int cu_count();
+// Fills and checks the arguments; `pointers`: of a call, not only of a question about sizes.
+int check_args(const char *what, const selas_text_attention_problem *p, int dtype, bool pointers, Args &a);
+// Work item of block x (of 8 * per_xcd): each XCD takes a contiguous range.
+__device__ __forceinline__ int item_of(int per_xcd) { return (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3); }
+
+}  // namespace textattn
+}  // namespace selas

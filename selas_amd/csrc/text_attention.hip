@@ -1,0 +1,807 @@
+// Attention of the text side, forward, for gfx950: keys of another length than the queries, shared key heads, images whose
+// keys end early or are masked, a causal mask, and a learned bias by buckets of the distance. Per image b, head h and key
+// head g = h / (H / Hk):
+//   s_ij = scale q_i . k_j + table[bucket(j - (start_b + i)), h],   out_i = sum_j softmax_j(s_ij) v_j
+// over the keys that row i sees; a row that sees none gives zeros. Scores, maxima and sums are fp32; the running maximum and
+// sum make it one pass over the keys.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "text_attention.h"
+
+namespace selas {
+namespace textattn {
+namespace {
+
+// ------------------------------------------------------------------ few rows
+
+// Rows (query head in the group, query) that share one key head: R of them at most, `rows` = group * Lq. A row is
+// r = g * Lq + i.
+//
+// Bounded by the stream of k and v: 4 bytes a key and channel for 2 R multiply-adds, so plain vector instructions are
+// enough (MFMAs would fill 1 to 8 of their 32 columns). A lane holds 8 channels; D / 8 lanes make a key, 64 / (D / 8) key
+// slots a wave; each slot keeps a softmax of its own over the keys it meets, joined once at the end. k and v go from memory
+// to registers, the next unit's loads ahead of this one's arithmetic.
+template <int D, int R>
+struct Few {
+  static constexpr int kLanes = D / 8, kSlots = 64 / kLanes;
+  static constexpr int kU = R <= 2 ? 8 : 4;        // keys of a slot per unit
+  static constexpr int kUnit = kU * kSlots;        // keys per wave and step (at most 64)
+  static constexpr int kFloats = R * (D + 2);      // a part's result: R x D outputs, maxima, sums
+};
+
+// Sum over the D / 8 neighbouring lanes of a key.
+template <int LANES>
+__device__ __forceinline__ float key_sum(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  v += dpp(v, std::integral_constant<int, 0xB1>{});   // quad_perm 1 0 3 2
+  v += dpp(v, std::integral_constant<int, 0x4E>{});   // quad_perm 2 3 0 1
+  v += dpp(v, std::integral_constant<int, 0x141>{});  // row_half_mirror: the other four of 8
+  if constexpr (LANES == 16) v += dpp(v, std::integral_constant<int, 0x140>{});  // row_mirror: the other eight of 16
+  return v;
+}
+
+template <bool BF>
+__device__ __forceinline__ float dot8(uint4 a, uint4 b) {
+  float s = 0.0f;
+  const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = __builtin_fmaf(lo_of<BF>(x[i]), lo_of<BF>(y[i]), s);
+    s = __builtin_fmaf(hi_of<BF>(x[i]), hi_of<BF>(y[i]), s);
+  }
+  return s;
+}
+
+template <bool BF, int D, int R, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW) void few_kernel(Args a, int parts, float *__restrict__ partial) {
+  using F = Few<D, R>;
+  constexpr int kSlots = F::kSlots, kU = F::kU, kUnit = F::kUnit;
+  extern __shared__ __attribute__((aligned(16))) float table[];  // [group][2 reach + 1], by distance
+  __shared__ float red[NW][F::kFloats];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int part = blockIdx.x % parts, item = blockIdx.x / parts, b = item / a.Hk, hk = item - b * a.Hk;
+  const int rows = a.group * a.Lq;
+  const int keys = keys_of(a, b), start = start_of(a, b);
+  const int slot = lane / F::kLanes, ch = (lane % F::kLanes) * 8;
+  const bool given = ch < a.dh;
+
+  const int reach = a.bias.reach, span = 2 * reach + 1;
+  if constexpr (BIAS) {
+    for (int i = threadIdx.x; i < a.group * span; i += 64 * NW) {
+      const int g = i / span;
+      table[i] = bias_at(a.bias, hk * a.group + g, i - g * span - reach);
+    }
+    __syncthreads();
+  }
+
+  uint4 qf[R];
+  int at[R], head[R];  // position, head in the group
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    head[r] = r < rows ? r / a.Lq : 0;
+    const int i = r < rows ? r - head[r] * a.Lq : 0;
+    at[r] = start + i;
+    const uint16_t *p = a.q.p + b * a.q.sb + (hk * a.group + head[r]) * a.q.sh + i * a.q.sl + ch;
+    qf[r] = given && r < rows ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0);
+  }
+
+  const uint16_t *kp = a.k.p + b * a.k.sb + hk * a.k.sh, *vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+  const uint8_t *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
+  uint32_t koff[kU], voff[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const uint32_t r = u * kSlots + slot;
+    koff[u] = given ? r * static_cast<uint32_t>(2 * a.k.sl) + 2 * ch : kPast;
+    voff[u] = given ? r * static_cast<uint32_t>(2 * a.v.sl) + 2 * ch : kPast;
+  }
+  auto bytes_of = [&](int64_t sl, int n) {
+    n = min(n, kUnit);
+    return n > 0 ? 2 * ((n - 1) * static_cast<uint32_t>(sl) + a.dh) : 0u;
+  };
+  uint4 kf[kU], vf[kU];
+  auto load_k = [&](int unit) {
+    const int64_t key0 = static_cast<int64_t>(unit) * kUnit;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(kp + key0 * a.k.sl, bytes_of(a.k.sl, keys - static_cast<int>(key0)));
+#pragma unroll
+    for (int u = 0; u < kU; ++u) kf[u] = load_b128(r, koff[u], 0);
+  };
+  auto load_v = [&](int unit, uint64_t bits) {  // masked values read as zeros: what they hold must not reach a product
+    const int64_t key0 = static_cast<int64_t>(unit) * kUnit;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(vp + key0 * a.v.sl, bytes_of(a.v.sl, keys - static_cast<int>(key0)));
+#pragma unroll
+    for (int u = 0; u < kU; ++u) vf[u] = load_b128(r, (bits >> (u * kSlots + slot)) & 1 ? voff[u] : kPast, 0);
+  };
+  auto load_byte = [&](int unit) {
+    const int64_t key = static_cast<int64_t>(unit) * kUnit + lane;
+    return mask && lane < kUnit && key < keys ? mask[key] : 0;
+  };
+  auto word = [&](int unit, int byte) {
+    if (mask) return __builtin_amdgcn_ballot_w64(byte != 0);
+    return up_to(keys - unit * kUnit - 1);
+  };
+
+  // This part's units, dealt to the waves in turn.
+  int n = (keys + kUnit - 1) / kUnit;
+  if (a.causal) n = min(n, max(start + a.Lq + kUnit - 1, 0) / kUnit);
+  const int per = (n + parts - 1) / parts, end = min(n, (part + 1) * per);
+  int unit = uniform(part * per + wave);
+
+  float m[R], l[R], o[R][8];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = kLowest;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[r][e] = 0.0f;
+  }
+
+  uint64_t bits = 0, bits_next = 0;
+  int byte = 0;
+  if (unit < end) {
+    bits = word(unit, load_byte(unit));
+    load_k(unit);
+    load_v(unit, bits);
+    byte = load_byte(unit + NW);
+  }
+  for (; unit < end; unit += NW) {
+    const int next = unit + NW;
+    bits_next = word(next, byte);
+    float s[kU][R];
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[u][r] = key_sum<F::kLanes>(dot8<BF>(kf[u], qf[r]));
+    if (next < end) load_k(next);
+    byte = load_byte(next + NW);
+    float p[kU][R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mx = m[r];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int key = unit * kUnit + u * kSlots + slot, d = key - at[r];
+        float x = s[u][r] * a.c2;
+        if constexpr (BIAS) x += table[head[r] * span + min(max(d, -reach), reach) + reach];
+        const bool seen = ((bits >> (u * kSlots + slot)) & 1) && !(a.causal && d > 0);
+        s[u][r] = seen ? x : -__builtin_inff();
+        mx = fmaxf(mx, s[u][r]);
+      }
+      const float alpha = __builtin_amdgcn_exp2f(m[r] - mx);
+      m[r] = mx;
+      l[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[r][e] *= alpha;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        p[u][r] = __builtin_amdgcn_exp2f(s[u][r] - mx);
+        l[r] += p[u][r];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint32_t w[4] = {vf[u].x, vf[u].y, vf[u].z, vf[u].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float lo = lo_of<BF>(w[e]), hi = hi_of<BF>(w[e]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          o[r][2 * e] = __builtin_fmaf(p[u][r], lo, o[r][2 * e]);
+          o[r][2 * e + 1] = __builtin_fmaf(p[u][r], hi, o[r][2 * e + 1]);
+        }
+      }
+    }
+    bits = bits_next;
+    if (next < end) load_v(next, bits);
+  }
+
+  // The slots of a wave, then the waves.
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int x = F::kLanes; x < 64; x <<= 1) {
+      const float om = __shfl_xor(m[r], x, 64), ol = __shfl_xor(l[r], x, 64), mx = fmaxf(m[r], om);
+      const float f = __builtin_amdgcn_exp2f(m[r] - mx), g = __builtin_amdgcn_exp2f(om - mx);
+      l[r] = l[r] * f + ol * g;
+      m[r] = mx;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[r][e] = o[r][e] * f + __shfl_xor(o[r][e], x, 64) * g;
+    }
+    if (slot == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) red[wave][r * D + ch + e] = o[r][e];
+      if (ch == 0) {
+        red[wave][R * D + r] = m[r];
+        red[wave][R * D + R + r] = l[r];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * D; i += 64 * NW) {
+    const int r = i / D, c = i - r * D;
+    if (r >= rows) continue;
+    float mx = kLowest, sum = 0.0f, x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, red[w][R * D + r]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(red[w][R * D + r] - mx);
+      sum += red[w][R * D + R + r] * f;
+      x += red[w][i] * f;
+    }
+    if (parts > 1) {
+      float *out = partial + static_cast<int64_t>(blockIdx.x) * F::kFloats;
+      out[i] = x;
+      if (c == 0) {
+        out[R * D + r] = mx;
+        out[R * D + R + r] = sum;
+      }
+      continue;
+    }
+    const int g = r / a.Lq, q = r - g * a.Lq, h = hk * a.group + g;
+    if (c < a.dh)
+      store_f<BF ? SELAS_BF16 : SELAS_F16>(a.out + b * a.out_sb + q * a.out_sl + h * a.dh, c, sum == 0.0f ? 0.0f : x / sum);
+    if (a.lse && c == 0) a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + q] = (mx + __builtin_log2f(sum)) * kLn2;
+  }
+}
+
+// The parts of few_kernel, joined in their order: a workgroup per (image, key head, row).
+template <bool BF>
+__global__ __launch_bounds__(128) void few_merge_kernel(Args a, int parts, int D, int R, const float *__restrict__ partial) {
+  const int rows = a.group * a.Lq, item = blockIdx.x / rows, r = blockIdx.x - item * rows, c = threadIdx.x;
+  const int b = item / a.Hk, hk = item - b * a.Hk, step = R * (D + 2);
+  const float *w = partial + static_cast<int64_t>(item) * parts * step;
+  if (c >= a.dh) return;
+  float mx = kLowest, sum = 0.0f, x = 0.0f;
+  for (int p = 0; p < parts; ++p) mx = fmaxf(mx, w[p * step + R * D + r]);
+  for (int p = 0; p < parts; ++p) {
+    const float f = __builtin_amdgcn_exp2f(w[p * step + R * D + r] - mx);
+    sum += w[p * step + R * D + R + r] * f;
+    x += w[p * step + r * D + c] * f;
+  }
+  const int g = r / a.Lq, q = r - g * a.Lq, h = hk * a.group + g;
+  store_f<BF ? SELAS_BF16 : SELAS_F16>(a.out + b * a.out_sb + q * a.out_sl + h * a.dh, c, sum == 0.0f ? 0.0f : x / sum);
+  if (a.lse && c == 0) a.lse[(static_cast<int64_t>(b) * a.H + h) * a.Lq + q] = (mx + __builtin_log2f(sum)) * kLn2;
+}
+
+// ------------------------------------------------------------------ tiles
+
+// A call cut into work items: parts of the keys innermost but for the query tiles and the heads of a group, so that what
+// reads the same keys runs at the same time behind the same L2.
+struct Cut {
+  int qtiles, parts, total, per_xcd;
+  float *partial;
+};
+constexpr int partial_floats(int D) { return 64 * (D / 2) + 2 * 64; }  // per wave: outputs in register order, maxima, sums
+
+// One workgroup = NW waves = 32 NW queries of one (image, head); wave w owns queries 32 w .. + 32. The keys stream through
+// LDS in double-buffered tiles of 64 that all waves share. Per tile: S^T = K Q^T (K row-wise from LDS, Q held), the softmax
+// on the scores in registers, O^T += V^T P^T (V transposed by the LDS reads, the probabilities straight from the score
+// registers: the K rows of a block are read with bits 2 and 3 of the row exchanged, so that register r of a lane holds key
+// 16 (r / 8) + 8 h + r % 8 of it, as the second product's operand wants them).
+template <bool BF, int D, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void fwd_kernel(Args a, Cut cut) {
+  using T = Tile<D>;
+  constexpr int KJ = T::kLoads / NW;
+  static_assert(KJ * NW == T::kLoads, "loads per wave");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
+  extern __shared__ __attribute__((aligned(16))) float table[];
+  const int t = item_of(cut.per_xcd);
+  if (t >= cut.total) return;
+  int rest = t;
+  const int qt0 = rest % cut.qtiles;
+  rest /= cut.qtiles;
+  const int g = rest % a.group;
+  rest /= a.group;
+  const int part = rest % cut.parts;
+  rest /= cut.parts;
+  const int hk = rest % a.Hk, b = rest / a.Hk, head = hk * a.group + g;
+  const int qt = a.causal ? cut.qtiles - 1 - qt0 : qt0;  // the longest first
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+
+  const int keys = keys_of(a, b), start = start_of(a, b);
+  const int row0 = (qt * NW + wave) * 32;  // this wave's first query
+  const int first = start + row0, pos = first + c;
+  int ntiles = (keys + kRows - 1) / kRows;
+  if (a.causal) ntiles = min(ntiles, max(start + min((qt + 1) * NW * 32, a.Lq) + kRows - 1, 0) / kRows);
+  const int per = (ntiles + cut.parts - 1) / cut.parts;
+  int kt = part * per;
+  const int end = min(ntiles, kt + per);
+
+  Held<D> q;
+  q.load(a.q.p + b * a.q.sb + head * a.q.sh + row0 * a.q.sl, a.q.sl, a.dh, a.Lq - row0, lane);
+  const uint16_t *kp = a.k.p + b * a.k.sb + hk * a.k.sh, *vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+  const typename T::template Loader<KJ> kl(wave, lane, a.k.sl, a.dh), vl(wave, lane, a.v.sl, a.dh);
+  const typename T::RowReader rows(lane);
+  const typename T::ColReader cols(lane);
+  const KeyBits keybits(a, b, keys, lane);
+  auto issue = [&](int stage, int kt, uint64_t bits) {
+    uint8_t *base = stage ? smem1 : smem0;
+    const int64_t key0 = static_cast<int64_t>(kt) * kRows;
+    const int left = keys - kt * kRows;
+    if (keybits.mask) {
+      kl.template issue<true>(base, kp + key0 * a.k.sl, a.k.sl, a.dh, left, bits);
+      vl.template issue<true>(base + T::kBytes, vp + key0 * a.v.sl, a.v.sl, a.dh, left, bits);
+    } else {
+      kl.template issue<false>(base, kp + key0 * a.k.sl, a.k.sl, a.dh, left, bits);
+      vl.template issue<false>(base + T::kBytes, vp + key0 * a.v.sl, a.v.sl, a.dh, left, bits);
+    }
+  };
+
+  const int reach = a.bias.reach, pitch = bias_pitch(reach);
+  float far_behind = 0.0f, far_ahead = 0.0f;
+  if constexpr (BIAS) build_bias(table, a.bias, head, threadIdx.x, 64 * NW, false);
+
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) o[db] = f32x16{};
+  float m_run = kLowest, l_run = 0.0f;
+  constexpr float kRoom = headroom<BF>();
+
+  uint64_t bits = 0;
+  int byte = 0;
+  if (kt < end) {
+    bits = keybits.word(kt, keybits.load(kt));
+    issue(0, kt, bits);
+    byte = keybits.load(kt + 1);
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+  if constexpr (BIAS) {
+    far_behind = table[0];
+    far_ahead = table[2 * reach + 16];
+  }
+
+  // kMode 0: all 64 keys are seen by all of the wave's queries and the bias is one value (`bc`); 1: all are seen, the bias
+  // by distance; 2: whatever is seen, the bias by distance.
+  auto compute = [&](int stage, int kt, float bc, auto mode) {
+    constexpr int kMode = decltype(mode)::value;
+    constexpr bool kNear = BIAS && kMode > 0;
+    uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
+    f32x16 sc[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+    for (int i = 0; i < 2 * (D / 16); ++i) sc[i / (D / 16)] = mfma<BF>(rows.read(ks, i / (D / 16), i % (D / 16)), q.f[i % (D / 16)], sc[i / (D / 16)]);
+    if constexpr (kNear) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+          float bv[8];
+          bias_run(table, pitch, reach, kt * kRows + 32 * kb + 16 * t2 + 8 * h - pos, bv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sc[kb][8 * t2 + e] = __builtin_fmaf(sc[kb][8 * t2 + e], a.c2, bv[e]);
+        }
+    }
+    if constexpr (kMode == 2) {
+      const uint64_t seen = (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h);
+      const uint32_t w[2] = {static_cast<uint32_t>(seen), static_cast<uint32_t>(seen >> 32)};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          sc[kb][r] = (w[kb] >> (16 * (r >> 3) + (r & 7))) & 1 ? sc[kb][r] : -__builtin_inff();
+    }
+    float mx = sc[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kb][r]);
+    mx = pair_max(mx);
+    if constexpr (!kNear) mx = __builtin_fmaf(mx, a.c2, bc);
+    const bool raise = mx - kRoom > m_run + 8.0f;
+    if (__builtin_amdgcn_ballot_w64(raise)) {
+      const float to = mx - kRoom, alpha = raise ? __builtin_amdgcn_exp2f(m_run - to) : 1.0f;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) o[db] *= alpha;
+      l_run *= alpha;
+      m_run = raise ? to : m_run;
+    }
+    const float sub = kNear ? m_run : m_run - bc;
+    float ls = 0.0f;
+    uint4 pb[2][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          auto prob = [&](float s) {
+            return materialize(__builtin_amdgcn_exp2f(kNear ? s - sub : __builtin_fmaf(s, a.c2, -sub)));
+          };
+          const float p0 = prob(sc[kb][8 * t2 + 2 * e]), p1 = prob(sc[kb][8 * t2 + 2 * e + 1]);
+          ls += p0 + p1;
+          w[e] = pack<BF>(p0, p1);
+        }
+        pb[kb][t2] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    l_run += ls;
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+      o[i / 4] = mfma<BF>(cols.read(vs, i / 4, (i / 2) % 2, i % 2), pb[(i / 2) % 2][i % 2], o[i / 4]);
+  };
+  auto step = [&](int stage) {
+    const uint64_t bits_next = keybits.word(kt + 1, byte);
+    if (kt + 1 < end) issue(stage ^ 1, kt + 1, bits_next);
+    byte = keybits.load(kt + 2);
+    const int key0 = kt * kRows;
+    if (bits && !(a.causal && key0 > first + 31)) {
+      const bool all = bits == ~0ull && !(a.causal && key0 + kRows - 1 > first);
+      bool one = !BIAS;  // the bias is one value
+      float bc = 0.0f;
+      if constexpr (BIAS) {
+        if (key0 + kRows - 1 - first <= -reach) {
+          one = true;
+          bc = far_behind;
+        } else if (key0 - first - 31 >= (a.bias.ahead ? reach : 0)) {
+          one = true;
+          bc = far_ahead;
+        }
+      }
+      if (!all) compute(stage, kt, 0.0f, std::integral_constant<int, 2>{});
+      else if (one) compute(stage, kt, bc, std::integral_constant<int, 0>{});
+      else if constexpr (BIAS) compute(stage, kt, 0.0f, std::integral_constant<int, 1>{});
+    }
+    bits = bits_next;
+    wait_vmcnt<0>();
+    __syncthreads();
+  };
+  while (kt < end) {
+    step(0);
+    if (++kt >= end) break;
+    step(1);
+    ++kt;
+  }
+
+  const float l_all = pair_sum(l_run);
+  if (cut.parts > 1) {
+    float *w = cut.partial + (static_cast<int64_t>(t) * NW + wave) * partial_floats(D);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+      *reinterpret_cast<float4 *>(w + (i * 64 + lane) * 4) =
+          make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
+    *reinterpret_cast<float2 *>(w + 32 * D + 2 * lane) = make_float2(m_run, l_all);
+    return;
+  }
+  const int row = row0 + c;
+  if (row >= a.Lq) return;
+  const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
+  uint16_t *orow = a.out + b * a.out_sb + row * a.out_sl + head * a.dh;
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i) {
+    const int ch = 8 * i + 4 * h;
+    const f32x16 &x = o[i >> 2];
+    const int e = 4 * (i & 3);
+    if (8 * i < a.dh)
+      *reinterpret_cast<uint2 *>(orow + ch) =
+          make_uint2(pack<BF>(materialize(x[e] * inv), materialize(x[e + 1] * inv)),
+                     pack<BF>(materialize(x[e + 2] * inv), materialize(x[e + 3] * inv)));
+  }
+  if (a.lse && h == 0)
+    a.lse[(static_cast<int64_t>(b) * a.H + head) * a.Lq + row] = (m_run + __builtin_log2f(l_all)) * kLn2;
+}
+
+// The parts of fwd_kernel, joined in key order: a wave per 32 queries and 32 channels, in the lane order of that kernel.
+template <bool BF, int D>
+__global__ __launch_bounds__(64) void merge_kernel(Args a, Cut cut, int nw) {
+  const int lane = threadIdx.x, db = blockIdx.x % (D / 32);
+  int rest = blockIdx.x / (D / 32);
+  const int wave = rest % nw;
+  rest /= nw;
+  const int qt0 = rest % cut.qtiles;
+  rest /= cut.qtiles;
+  const int head = rest % a.H, b = rest / a.H, hk = head / a.group, g = head - hk * a.group;
+  const int qt = a.causal ? cut.qtiles - 1 - qt0 : qt0;
+  const int row = (qt * nw + wave) * 32 + (lane & 31);
+  const int64_t item = ((static_cast<int64_t>(b) * a.Hk + hk) * cut.parts * a.group + g) * cut.qtiles + qt0;
+  const int64_t step = static_cast<int64_t>(a.group) * cut.qtiles * nw * partial_floats(D);  // from one part to the next
+  const float *w = cut.partial + (item * nw + wave) * partial_floats(D);
+  if (row >= a.Lq) return;
+  float m = kLowest, l = 0.0f;
+  for (int p = 0; p < cut.parts; ++p) m = fmaxf(m, w[p * step + 32 * D + 2 * lane]);
+  float4 o[4] = {};
+  for (int p = 0; p < cut.parts; ++p) {
+    const float2 ml = *reinterpret_cast<const float2 *>(w + p * step + 32 * D + 2 * lane);
+    const float f = __builtin_amdgcn_exp2f(ml.x - m);
+    l += f * ml.y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 x = *reinterpret_cast<const float4 *>(w + p * step + ((4 * db + i) * 64 + lane) * 4);
+      o[i].x += f * x.x;
+      o[i].y += f * x.y;
+      o[i].z += f * x.z;
+      o[i].w += f * x.w;
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t *orow = a.out + b * a.out_sb + row * a.out_sl + head * a.dh;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int ch = 32 * db + 8 * i;
+    if (ch < a.dh)
+      *reinterpret_cast<uint2 *>(orow + ch + 4 * (lane >> 5)) =
+          make_uint2(pack<BF>(materialize(o[i].x * inv), materialize(o[i].y * inv)),
+                     pack<BF>(materialize(o[i].z * inv), materialize(o[i].w * inv)));
+  }
+  if (a.lse && db == 0 && lane < 32)
+    a.lse[(static_cast<int64_t>(b) * a.H + head) * a.Lq + row] = (m + __builtin_log2f(l)) * kLn2;
+}
+
+}  // namespace
+}  // namespace textattn
+}  // namespace selas
+
+// ------------------------------------------------------------------ host side
+
+namespace selas {
+namespace textattn {
+
+int cu_count() {
+  static std::atomic<int> counts[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
+    (void)hipGetLastError();
+    dev = 0;
+  }
+  int v = counts[dev].load(std::memory_order_relaxed);
+  if (v > 0) return v;
+  if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) {
+    (void)hipGetLastError();
+    v = 256;
+  }
+  counts[dev].store(v, std::memory_order_relaxed);
+  return v;
+}
+
+namespace {
+
+// Whole numbers of up to 40 words, for the borders of the buckets.
+struct Big {
+  uint32_t w[40] = {1};
+  int n = 1;
+  bool mul(uint32_t m) {
+    uint64_t carry = 0;
+    for (int i = 0; i < n; ++i) {
+      carry += static_cast<uint64_t>(w[i]) * m;
+      w[i] = static_cast<uint32_t>(carry);
+      carry >>= 32;
+    }
+    if (carry) {
+      if (n == 40) return false;
+      w[n++] = static_cast<uint32_t>(carry);
+    }
+    return true;
+  }
+  void pow(uint32_t m, int e) {
+    for (int i = 0; i < e; ++i) mul(m);
+  }
+  bool at_least(const Big &o) const {
+    if (n != o.n) return n > o.n;
+    for (int i = n - 1; i >= 0; --i)
+      if (w[i] != o.w[i]) return w[i] > o.w[i];
+    return true;
+  }
+};
+
+// Whether (a / e)^k >= (m / e)^t, that is a^k e^t >= m^t e^k: at most 10 bits times 64 + 63, 40 words hold it.
+bool past_border(int a, int e, int m, int k, int t) {
+  Big x, y;
+  x.pow(a, k);
+  x.pow(e, t);
+  y.pow(m, t);
+  y.pow(e, k);
+  return x.at_least(y);
+}
+
+int fill_buckets(const char *what, int64_t buckets, int64_t max_distance, int bidirectional, int16_t *edge, int &n) {
+  if (bidirectional && buckets % 2)
+    return set_error(SELAS_EINVAL, "%s: %lld buckets do not halve into two directions", what, (long long)buckets);
+  const int64_t side = bidirectional ? buckets / 2 : buckets;
+  if (side < 2) return set_error(SELAS_EINVAL, "%s: needs two buckets a direction, got %lld", what, (long long)side);
+  if (max_distance <= side / 2)
+    return set_error(SELAS_EINVAL, "%s: max_distance %lld is not above the %lld exact distances", what, (long long)max_distance,
+                     (long long)(side / 2));
+  if (side > kMaxSide || max_distance > kMaxDistance)
+    return set_error(SELAS_EUNSUPPORTED, "%s: takes up to %d buckets a direction and distances up to %d", what, kMaxSide,
+                     kMaxDistance);
+  n = static_cast<int>(side);
+  const int e = n / 2, m = static_cast<int>(max_distance), k = n - e;
+  for (int t = 0; t <= e; ++t) edge[t] = static_cast<int16_t>(t);
+  for (int t = 1; t < k; ++t) {
+    // The real border, and the distance at or after it: whole numbers decide where rounding could.
+    int a = std::max(static_cast<int>(e * pow(static_cast<double>(m) / e, static_cast<double>(t) / k)) - 1, e);
+    while (!past_border(a, e, m, k, t)) ++a;
+    edge[e + t] = static_cast<int16_t>(a);
+  }
+  return SELAS_OK;
+}
+
+int check_side(const char *what, const char *name, const void *p, int64_t sb, int64_t sh, int64_t sl, Side &side) {
+  if (!p) return set_error(SELAS_EINVAL, "%s: null pointer (%s)", what, name);
+  if (sb < 0 || sh < 0 || sl < 0) return set_error(SELAS_EINVAL, "%s: %s has a negative stride", what, name);
+  if (!aligned(p, 16) || sb % 8 || sh % 8 || sl % 8)
+    return set_error(SELAS_EUNSUPPORTED, "%s: %s must be 16-byte aligned with strides of whole 16 bytes", what, name);
+  if (sl > (1 << 23)) return set_error(SELAS_EUNSUPPORTED, "%s: %s has a row stride above 2^23 elements", what, name);
+  side = {static_cast<const uint16_t *>(p), sb, sh, sl};
+  return SELAS_OK;
+}
+
+}  // namespace
+
+int check_args(const char *what, const selas_text_attention_problem *p, int dtype, bool pointers, Args &a) {
+  if (!p) return set_error(SELAS_EINVAL, "%s: null problem", what);
+  if (p->B < 0 || p->H < 0 || p->Hk < 0 || p->Lq < 0 || p->Lk < 0 || p->Dh <= 0)
+    return set_error(SELAS_EINVAL, "%s: bad shape B=%lld H=%lld Hk=%lld Lq=%lld Lk=%lld Dh=%lld", what, (long long)p->B,
+                     (long long)p->H, (long long)p->Hk, (long long)p->Lq, (long long)p->Lk, (long long)p->Dh);
+  if (p->Hk == 0 ? p->H != 0 : p->H % p->Hk != 0)
+    return set_error(SELAS_EINVAL, "%s: %lld heads do not share %lld key heads evenly", what, (long long)p->H, (long long)p->Hk);
+  if (!valid_dtype(dtype)) return set_error(SELAS_EINVAL, "%s: bad dtype %d", what, dtype);
+  if (p->reserved != 0) return set_error(SELAS_EINVAL, "%s: reserved must be 0", what);
+  if (!(p->scale >= 1e-30 && p->scale <= 1e30))
+    return set_error(SELAS_EINVAL, "%s: scale %g is outside 1e-30 .. 1e30", what, p->scale);
+  if (p->table && !valid_dtype(p->table_dtype)) return set_error(SELAS_EINVAL, "%s: bad table dtype %d", what, p->table_dtype);
+  if (dtype == SELAS_F32 || p->Dh % 8 || p->Dh > 128)
+    return set_error(SELAS_EUNSUPPORTED, "%s: takes bf16 or fp16 and head dims of whole 8 up to 128 (got %s, %lld)", what,
+                     dtype_name(dtype), (long long)p->Dh);
+  if (p->Lq >= (1 << 28) || p->Lk >= (1 << 28) || p->B >= (1 << 28) || p->H >= (1 << 28) ||
+      p->B * p->H * cdiv(std::max<int64_t>(std::max(p->Lq, p->Lk), 1), 32) >= (1ll << 26))
+    return set_error(SELAS_EUNSUPPORTED, "%s: more than 2^26 blocks of 32 rows", what);
+  a = Args{};
+  a.bias.dtype = p->table_dtype;
+  if (p->table) {
+    if (int e = fill_buckets(what, p->buckets, p->max_distance, p->bidirectional, a.bias.edge, a.bias.n)) return e;
+    a.bias.ahead = p->bidirectional ? a.bias.n : 0;
+    a.bias.reach = a.bias.edge[a.bias.n - 1];
+    a.bias.row = p->table_sl;
+    a.bias.table = p->table;
+    if (p->table_sl < 0) return set_error(SELAS_EINVAL, "%s: the table has a negative stride", what);
+  }
+  a.B = static_cast<int>(p->B);
+  a.H = static_cast<int>(p->H);
+  a.Hk = static_cast<int>(p->Hk);
+  a.group = p->Hk ? static_cast<int>(p->H / p->Hk) : 0;
+  a.Lq = static_cast<int>(p->Lq);
+  a.Lk = static_cast<int>(p->Lk);
+  a.dh = static_cast<int>(p->Dh);
+  a.causal = p->causal != 0;
+  a.c2 = static_cast<float>(p->scale * 1.4426950408889634);
+  a.lse = p->lse;
+  a.lengths = p->lengths;
+  a.mask = p->mask;
+  a.mask_sb = p->mask_sb;
+  a.start = p->start;
+  a.start0 = static_cast<int>(std::min<int64_t>(std::max<int64_t>(p->start0, -(1 << 29)), 1 << 29));
+  if (!pointers || p->B == 0 || p->H == 0 || p->Lq == 0) return SELAS_OK;
+  if (int e = check_side(what, "q", p->q, p->q_sb, p->q_sh, p->q_sl, a.q)) return e;
+  if (p->Lk) {  // without keys there may be no memory
+    if (int e = check_side(what, "k", p->k, p->k_sb, p->k_sh, p->k_sl, a.k)) return e;
+    if (int e = check_side(what, "v", p->v, p->v_sb, p->v_sh, p->v_sl, a.v)) return e;
+  }
+  if (!p->out) return set_error(SELAS_EINVAL, "%s: null pointer (out)", what);
+  if (p->o_sb < 0 || p->o_sl < 0 || p->mask_sb < 0) return set_error(SELAS_EINVAL, "%s: negative stride", what);
+  if (!aligned(p->out, 8) || p->o_sb % 4 || p->o_sl % 4)
+    return set_error(SELAS_EUNSUPPORTED, "%s: out must be 8-byte aligned with strides of whole 8 bytes", what);
+  a.out = static_cast<uint16_t *>(p->out);
+  a.out_sb = p->o_sb;
+  a.out_sl = p->o_sl;
+  return SELAS_OK;
+}
+
+namespace {
+
+struct Plan {
+  int few = 0;  // rows held by the few-row kernel, 0: tiles
+  int D, nw, parts, qtiles;
+  int64_t bytes = 0;  // workspace
+};
+
+Plan plan_of(const Args &a) {
+  Plan p{};
+  p.D = a.dh <= 64 ? 64 : 128;
+  const int cu = cu_count();
+  const int64_t rows = static_cast<int64_t>(a.group) * a.Lq, items = static_cast<int64_t>(a.B) * a.Hk;
+  if (rows <= 8) {
+    p.few = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+    p.nw = 8;
+    const int unit = (p.few <= 2 ? 8 : 4) * (512 / p.D);
+    const int64_t units = cdiv(a.Lk, unit);
+    // Parts for two workgroups a CU, of four units a wave at least.
+    p.parts = static_cast<int>(std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(items, 1), units / (4 * p.nw))));
+    if (p.parts > 1) p.bytes = items * p.parts * p.few * (p.D + 2) * 4;
+    return p;
+  }
+  p.nw = a.Lq <= 32 ? 1 : a.Lq <= 64 ? 2 : 4;
+  p.qtiles = static_cast<int>(cdiv(a.Lq, 32 * p.nw));
+  const int64_t whole = static_cast<int64_t>(a.B) * a.H * p.qtiles, tiles = cdiv(a.Lk, kRows);
+  // Workgroups for two to a CU, of four tiles at least.
+  const int64_t room = 2 * cu * (4 / p.nw);
+  p.parts = static_cast<int>(std::max<int64_t>(1, std::min(room / std::max<int64_t>(whole, 1), tiles / 4)));
+  if (p.parts > 1) p.bytes = whole * p.parts * p.nw * partial_floats(p.D) * 4;
+  return p;
+}
+
+template <bool BF, int D, int R, bool BIAS>
+void launch_few(const Args &a, const Plan &p, float *ws, hipStream_t st) {
+  const int items = a.B * a.Hk;
+  const size_t lds = BIAS ? static_cast<size_t>(a.group) * (2 * a.bias.reach + 1) * 4 : 0;
+  few_kernel<BF, D, R, 8, BIAS><<<dim3(items * p.parts), dim3(512), lds, st>>>(a, p.parts, ws);
+  if (p.parts > 1) few_merge_kernel<BF><<<dim3(items * a.group * a.Lq), dim3(128), 0, st>>>(a, p.parts, D, R, ws);
+}
+
+template <bool BF, int D, int NW, bool BIAS>
+void launch_tiles(const Args &a, const Plan &p, float *ws, hipStream_t st) {
+  Cut cut{p.qtiles, p.parts, a.B * a.H * p.qtiles * p.parts, 0, ws};
+  cut.per_xcd = (cut.total + 7) / 8;
+  const size_t lds = BIAS ? bias_bytes(a.bias.reach) : 0;
+  fwd_kernel<BF, D, NW, BIAS><<<dim3(8 * cut.per_xcd), dim3(64 * NW), lds, st>>>(a, cut);
+  if (p.parts > 1)
+    merge_kernel<BF, D><<<dim3(a.B * a.H * p.qtiles * NW * (D / 32)), dim3(64), 0, st>>>(a, cut, NW);
+}
+
+template <bool BF, int D, bool BIAS>
+void launch(const Args &a, const Plan &p, float *ws, hipStream_t st) {
+  switch (p.few) {
+    case 1: return launch_few<BF, D, 1, BIAS>(a, p, ws, st);
+    case 2: return launch_few<BF, D, 2, BIAS>(a, p, ws, st);
+    case 4: return launch_few<BF, D, 4, BIAS>(a, p, ws, st);
+    case 8: return launch_few<BF, D, 8, BIAS>(a, p, ws, st);
+  }
+  switch (p.nw) {
+    case 1: return launch_tiles<BF, D, 1, BIAS>(a, p, ws, st);
+    case 2: return launch_tiles<BF, D, 2, BIAS>(a, p, ws, st);
+    default: return launch_tiles<BF, D, 4, BIAS>(a, p, ws, st);
+  }
+}
+
+}  // namespace
+}  // namespace textattn
+}  // namespace selas
+
+using namespace selas;
+using namespace selas::textattn;
+
+extern "C" int selas_relative_buckets(int64_t buckets, int64_t max_distance, int bidirectional, int32_t *edges,
+                                      int64_t *count) {
+  if (!edges || !count) return set_error(SELAS_EINVAL, "relative_buckets: null pointer");
+  int16_t edge[kMaxSide];
+  int n = 0;
+  if (int e = fill_buckets("relative_buckets", buckets, max_distance, bidirectional, edge, n)) return e;
+  for (int t = 0; t < n; ++t) edges[t] = edge[t];
+  *count = n;
+  return ok();
+}
+
+extern "C" int selas_text_attention_workspace_bytes(const selas_text_attention_problem *problem, int dtype, int64_t *bytes) {
+  if (!bytes) return set_error(SELAS_EINVAL, "text_attention_workspace_bytes: null pointer");
+  *bytes = 0;
+  Args a;
+  if (int e = check_args("text_attention_workspace_bytes", problem, dtype, false, a)) return e;
+  if (a.B && a.H && a.Lq) *bytes = plan_of(a).bytes;
+  return ok();
+}
+
+extern "C" int selas_text_attention(const selas_text_attention_problem *problem, int dtype, void *workspace,
+                                    int64_t workspace_bytes, void *stream) {
+  Args a;
+  if (int e = check_args("text_attention", problem, dtype, true, a)) return e;
+  if (!a.B || !a.H || !a.Lq) return ok();
+  const Plan p = plan_of(a);
+  if (p.bytes && (workspace_bytes < p.bytes || !workspace || !aligned(workspace, 16)))
+    return set_error(SELAS_EINVAL, "text_attention: needs a 16-byte aligned workspace of %lld bytes", (long long)p.bytes);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  float *ws = static_cast<float *>(workspace);
+  auto go = [&](auto bf, auto d) {
+    constexpr bool kBf = decltype(bf)::value;
+    constexpr int kD = decltype(d)::value;
+    if (a.bias.table) launch<kBf, kD, true>(a, p, ws, st);
+    else launch<kBf, kD, false>(a, p, ws, st);
+  };
+  using I64 = std::integral_constant<int, 64>;
+  using I128 = std::integral_constant<int, 128>;
+  if (dtype == SELAS_BF16) p.D == 64 ? go(std::true_type{}, I64{}) : go(std::true_type{}, I128{});
+  else p.D == 64 ? go(std::false_type{}, I64{}) : go(std::false_type{}, I128{});
+  return check_launch("text_attention");
+}
