@@ -579,11 +579,23 @@ int selas_text_attention(const selas_text_attention_problem *problem, int dtype,
 int selas_text_attention_workspace_bytes(const selas_text_attention_problem *problem, int dtype, int64_t *bytes);
 
 /*
+ * The gradients of that call for grad, the gradient of out ([B, Lq, H*Dh], g_sb, g_sl): problem is the forward call's, with
+ * the out and lse that it wrote (out may be a copy at other strides). dq [B, H, Lq, Dh], dk and dv [B, Hk, Lk, Dh] are
+ * contiguous, in dtype; dtable [buckets, H] contiguous, in table_dtype (unused where table is NULL). Keys that are not seen
+ * have gradients of 0, and so have queries that see none. grad's address and strides are as q's, dq, dk and dv 8-byte
+ * aligned. dk and dv are summed over the query heads that share a key head, dtable over everything, in fp32 and in one
+ * order: no atomics. workspace as in selas_text_attention, of selas_text_attention_backward_workspace_bytes. */
+int selas_text_attention_backward(const selas_text_attention_problem *problem, const void *grad, int64_t g_sb, int64_t g_sl,
+                                  void *dq, void *dk, void *dv, void *dtable, int dtype, void *workspace,
+                                  int64_t workspace_bytes, void *stream);
+int selas_text_attention_backward_workspace_bytes(const selas_text_attention_problem *problem, int dtype, int64_t *bytes);
+
+/*
  * The buckets of one direction: bucket t begins at distance edges[t] (edges[0] = 0, ascending), as many as *count says (at
  * most 128; edges has room for them). With n buckets a direction (all of them, or half when bidirectional != 0), e = n / 2
  * and m = max_distance: distance a is in bucket a if a < e, else in e + floor((n - e) log(a / e) / log(m / e)), at most
  * n - 1, in exact arithmetic (a distance on a border belongs to the bucket that begins there). Keys after the query have the
- * buckets from n on when bidirectional != 0, bucket 0 otherwise. n is 2 to 128, e < m <= 1024 (above: SELAS_EUNSUPPORTED). */
+ * buckets from n on when bidirectional != 0, bucket 0 otherwise. n is 2 to 128, e < m <= 512 (above: SELAS_EUNSUPPORTED). */
 int selas_relative_buckets(int64_t buckets, int64_t max_distance, int bidirectional, int32_t *edges, int64_t *count);
 
 #ifdef __cplusplus

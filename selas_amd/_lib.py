@@ -63,6 +63,8 @@ SIGNATURES: dict[str, list] = {
     "selas_raw_linear_tile": [_P, _I64, _INT] + [ctypes.POINTER(ctypes.c_int64)] * 3,
     "selas_text_attention": [_P, _INT, _P, _I64, _P],
     "selas_text_attention_workspace_bytes": [_P, _INT, ctypes.POINTER(ctypes.c_int64)],
+    "selas_text_attention_backward": [_P, _P, _I64, _I64, _P, _P, _P, _P, _INT, _P, _I64, _P],
+    "selas_text_attention_backward_workspace_bytes": [_P, _INT, ctypes.POINTER(ctypes.c_int64)],
     "selas_relative_buckets": [_I64, _I64, _INT, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int64)],
 }
 

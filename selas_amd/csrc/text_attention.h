@@ -11,7 +11,7 @@ namespace textattn {
 
 constexpr int kRows = 64;              // rows (keys or queries) per LDS tile
 constexpr int kMaxSide = 128;          // buckets per direction
-constexpr int kMaxDistance = 1024;     // the table by distance has to fit LDS beside the tiles
+constexpr int kMaxDistance = 512;      // tables and histograms by distance have to fit LDS beside the tiles
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kPast = 0x80000000u;  // a byte offset past every buffer range here (ranges stay below 2^31): loads read 0

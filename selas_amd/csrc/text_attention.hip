@@ -357,7 +357,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void fwd_kernel(Args a, C
 
   // kMode 0: all 64 keys are seen by all of the wave's queries and the bias is one value (`bc`); 1: all are seen, the bias
   // by distance; 2: whatever is seen, the bias by distance.
-  auto compute = [&](int stage, int kt, float bc, auto mode) {
+  auto compute = [&](int stage, int kt, float bc, auto mode) __attribute__((always_inline)) {
     constexpr int kMode = decltype(mode)::value;
     constexpr bool kNear = BIAS && kMode > 0;
     uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void fwd_kernel(Args a, C
     for (int i = 0; i < D / 8; ++i)
       o[i / 4] = mfma<BF>(cols.read(vs, i / 4, (i / 2) % 2, i % 2), pb[(i / 2) % 2][i % 2], o[i / 4]);
   };
-  auto step = [&](int stage) {
+  auto step = [&](int stage) __attribute__((always_inline)) {
     const uint64_t bits_next = keybits.word(kt + 1, byte);
     if (kt + 1 < end) issue(stage ^ 1, kt + 1, bits_next);
     byte = keybits.load(kt + 2);

@@ -1,0 +1,721 @@
+// The gradients of selas_text_attention, for gfx950. With dO the gradient of out and p the probabilities:
+//   D_i = dO_i . out_i,  dP_ij = dO_i . v_j,  dS_ij = p_ij (dP_ij - D_i)
+//   dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i,  dq_i = scale sum_j dS_ij k_j,  dtable[r, h] = sum of dS_ij over
+//   the pairs in bucket r; dk and dv sum over the query heads that share the key head.
+// p is formed again from q, k and the forward pass's lse. Three kernels: row_kernel leaves D and lse per row; key_kernel has
+// the keys as owners and streams queries past them (dk, dv); query_kernel has the queries as owners and streams keys (dq,
+// dtable). S and dP are formed in both: 7 products where one kernel would need 5 and floating-point atomics, whose order
+// would change the bits from call to call.
+#include <algorithm>
+#include <type_traits>
+
+#include "text_attention.h"
+
+namespace selas {
+namespace textattn {
+namespace {
+
+// fp16 operands of the second products. p <= 1 is stored times 2^15, and dS times a power of two (per image and key head)
+// that puts its bound, 2 max|dO| max|v|, at or below 2^15: nothing overflows, and what falls below fp16's normal numbers is
+// under 2^-29 of that bound. bf16 has fp32's range and needs neither.
+constexpr float kProbShift = 15.0f;
+template <bool BF>
+__device__ constexpr float prob_shift() {
+  return BF ? 0.0f : kProbShift;
+}
+
+struct Grads {
+  Side g;  // dO as [B, H, Lq, dh]
+  uint16_t *dq, *dk, *dv;  // contiguous [B, heads, L, dh]
+  float *neg_lse, *dot;    // [B, H, Lqp]: -lse log2(e) (-inf for rows that see nothing and rows past Lq), D (0 there)
+  int Lqp, qblocks, kblocks;  // rows padded to whole tiles; tiles of queries, of keys
+  float *g_norm, *v_norm;  // fp16: largest squared norms of the rows of dO and v, per tile
+  float *dtable_part;      // [B, H, qtiles * parts, buckets]
+  void *dtable;
+};
+
+// A kernel's work items: `parts` ranges of the streamed axis; sums of a part go to `partial` (fp32) where parts > 1.
+struct Cut {
+  int tiles, parts, total, per_xcd;
+  float *partial;
+};
+
+// D and lse of 64 rows, 4 lanes to a row. fp16: the tiles' largest norms of dO, and (blocks past the queries') of v.
+template <bool BF>
+__global__ __launch_bounds__(256) void row_kernel(Args a, Grads w) {
+  const int lane = threadIdx.x & 63, r = threadIdx.x >> 2, part = threadIdx.x & 3;
+  int t = blockIdx.x;
+  __shared__ float red[4];
+  float norm = 0.0f;
+  float *norm_out;
+  auto add4 = [](float v) {
+    v += __shfl_xor(v, 1, 64);
+    return v + __shfl_xor(v, 2, 64);
+  };
+  if (t < a.B * a.H * w.qblocks) {
+    const int qt = t % w.qblocks, bh = t / w.qblocks, b = bh / a.H, head = bh - b * a.H;
+    const int row = qt * kRows + r;
+    norm_out = w.g_norm + t;
+    float dot = 0.0f;
+    if (row < a.Lq) {
+      const uint16_t *g = w.g.p + b * w.g.sb + head * w.g.sh + row * w.g.sl;
+      const uint16_t *o = a.out + b * a.out_sb + row * a.out_sl + head * a.dh;
+      for (int ch = 8 * part; ch < a.dh; ch += 32) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(g + ch);
+        const uint2 y0 = *reinterpret_cast<const uint2 *>(o + ch), y1 = *reinterpret_cast<const uint2 *>(o + ch + 4);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y0.x, y0.y, y1.x, y1.y};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo = lo_of<BF>(xs[e]), hi = hi_of<BF>(xs[e]);
+          dot = __builtin_fmaf(lo, lo_of<BF>(ys[e]), dot);
+          dot = __builtin_fmaf(hi, hi_of<BF>(ys[e]), dot);
+          norm = __builtin_fmaf(lo, lo, norm);
+          norm = __builtin_fmaf(hi, hi, norm);
+        }
+      }
+    }
+    dot = add4(dot);
+    norm = add4(norm);
+    if (part == 0) {
+      const int64_t at = static_cast<int64_t>(bh) * w.Lqp + row;
+      const float lse = row < a.Lq ? a.lse[static_cast<int64_t>(bh) * a.Lq + row] : -__builtin_inff();
+      const bool none = lse == -__builtin_inff();
+      w.neg_lse[at] = none ? lse : -lse * kLog2e;
+      w.dot[at] = none ? 0.0f : dot;
+    }
+  } else {
+    t -= a.B * a.H * w.qblocks;
+    const int kt = t % w.kblocks, bh = t / w.kblocks, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int row = kt * kRows + r;
+    norm_out = w.v_norm + t;
+    if (row < keys_of(a, b) && (!a.mask || a.mask[b * a.mask_sb + row])) {
+      const uint16_t *v = a.v.p + b * a.v.sb + hk * a.v.sh + row * a.v.sl;
+      for (int ch = 8 * part; ch < a.dh; ch += 32) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(v + ch);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo = lo_of<BF>(xs[e]), hi = hi_of<BF>(xs[e]);
+          norm = __builtin_fmaf(lo, lo, norm);
+          norm = __builtin_fmaf(hi, hi, norm);
+        }
+      }
+    }
+    norm = add4(norm);
+  }
+  if constexpr (!BF) {
+#pragma unroll
+    for (int o = 4; o < 64; o <<= 1) norm = fmaxf(norm, __shfl_xor(norm, o, 64));
+    if (lane == 0) red[threadIdx.x >> 6] = norm;
+    __syncthreads();
+    if (threadIdx.x == 0) *norm_out = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+}
+
+// log2 of the factor that dS of image b and key head hk is stored with.
+template <bool BF>
+__device__ __forceinline__ float ds_shift(const Args &a, const Grads &w, int b, int hk, int lane) {
+  if constexpr (BF) return 0.0f;
+  float g = 0.0f, v = 0.0f;
+  const float *gn = w.g_norm + static_cast<int64_t>(b * a.H + hk * a.group) * w.qblocks;
+  const float *vn = w.v_norm + static_cast<int64_t>(b * a.Hk + hk) * w.kblocks;
+  for (int i = lane; i < a.group * w.qblocks; i += 64) g = fmaxf(g, gn[i]);
+  for (int i = lane; i < w.kblocks; i += 64) v = fmaxf(v, vn[i]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    g = fmaxf(g, __shfl_xor(g, o, 64));
+    v = fmaxf(v, __shfl_xor(v, o, 64));
+  }
+  // 0.5 log2(g v): of each, a product of squares might overflow. A step of 1 / 16 covers the logarithms' rounding.
+  const float bound = 0.5f * (__builtin_log2f(g) + __builtin_log2f(v)) + 1.0625f;
+  const float e = floorf(15.0f - bound);
+  return e >= -120.0f && e <= 120.0f ? e : 0.0f;  // zeros, infinities and NaN: as they are
+}
+
+// ------------------------------------------------------------------ dk, dv
+
+// One workgroup = NW waves = 32 NW keys of one (image, key head); wave w owns keys 32 w .. + 32 and holds their k and v.
+// Tiles of 64 queries (q and dO rows, lse and D), of all the heads of the group in turn, stream through LDS. Per block of 32
+// queries: S = Q K^T and dP = dO V^T with the query rows read row-wise, so that a lane's registers hold 16 queries of one
+// key, in runs of 8; then dV^T += dO^T P and dK^T += Q^T dS with the same tiles read transposed and P, dS straight from the
+// registers. A key's column depends on nothing of the other keys, so masked keys need no select: their results are zeroed at
+// the end.
+template <bool BF, int D, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, Grads w, Cut cut) {
+  using T = Tile<D>;
+  constexpr int KJ = T::kLoads / NW, kStats = 2 * kRows * 4;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes + kStats], smem1[2 * T::kBytes + kStats];
+  extern __shared__ __attribute__((aligned(16))) float table[];
+  const int t = item_of(cut.per_xcd);
+  if (t >= cut.total) return;
+  const int tile = t % cut.tiles, part = t / cut.tiles % cut.parts, bhk = t / cut.tiles / cut.parts;
+  const int b = bhk / a.Hk, hk = bhk - b * a.Hk;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+  const int keys = keys_of(a, b), start = start_of(a, b);
+  const int wg_key = tile * NW * 32, key0 = wg_key + wave * 32, key = key0 + c;
+
+  // The tiles of queries that see a key of this workgroup, for each head; this part's range of them all.
+  int qt0 = a.causal ? max(wg_key - start, 0) / kRows : 0;
+  const int each = wg_key < keys ? max(w.qblocks - qt0, 0) : 0, n = each * a.group;
+  const int per = (n + cut.parts - 1) / cut.parts;
+  int i = part * per;
+  const int end = min(n, i + per);
+  int g = each ? i / each : 0, qt = qt0 + (each ? i % each : 0);
+
+  bool valid = key < keys;
+  if (valid && a.mask) valid = a.mask[b * a.mask_sb + key] != 0;
+  Held<D> k, v;
+  k.load(a.k.p + b * a.k.sb + hk * a.k.sh + key0 * a.k.sl, a.k.sl, a.dh, keys - key0, lane, valid);
+  v.load(a.v.p + b * a.v.sb + hk * a.v.sh + key0 * a.v.sl, a.v.sl, a.dh, keys - key0, lane, valid);
+  const typename T::template Loader<KJ> ql(wave, lane, a.q.sl, a.dh), gl(wave, lane, w.g.sl, a.dh);
+  const typename T::RowReader rows(lane);
+  const typename T::ColReader cols(lane);
+  auto issue = [&](int stage, int g, int qt) {
+    uint8_t *base = stage ? smem1 : smem0;
+    const int head = hk * a.group + g, left = a.Lq - qt * kRows;
+    const int64_t row = static_cast<int64_t>(qt) * kRows;
+    ql.template issue<false>(base, a.q.p + b * a.q.sb + head * a.q.sh + row * a.q.sl, a.q.sl, a.dh, left, 0);
+    gl.template issue<false>(base + T::kBytes, w.g.p + b * w.g.sb + head * w.g.sh + row * w.g.sl, w.g.sl, a.dh, left, 0);
+    if (wave < 2) {  // 64 floats each
+      const float *p = (wave ? w.dot : w.neg_lse) + (static_cast<int64_t>(b) * a.H + head) * w.Lqp + row;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          make_rsrc(p, kRows * 4), (__attribute__((address_space(3))) void *)(base + 2 * T::kBytes + wave * kRows * 4), 4,
+          4 * lane, 0, 0, 0);
+    }
+  };
+  const int reach = a.bias.reach, pitch = bias_pitch(reach);
+  const float shift = ds_shift<BF>(a, w, b, hk, lane);
+  const float ds_mul = BF ? 1.0f : __builtin_exp2f(shift - kProbShift);
+
+  f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) dk[db] = dv[db] = f32x16{};
+
+  // kMode as in the forward pass: 0 one value of the bias and no mask, 1 by distance, 2 by distance and causal.
+  auto compute = [&](int stage, int qt, float bc, auto mode) __attribute__((always_inline)) {
+    constexpr int kMode = decltype(mode)::value;
+    constexpr bool kNear = BIAS && kMode > 0;
+    uint8_t *qs = stage ? smem1 : smem0, *gs = qs + T::kBytes;
+    const float *stats = reinterpret_cast<const float *>(qs + 2 * T::kBytes);
+    const int pos0 = start + qt * kRows;  // of the tile's first query
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) s = mfma<BF>(rows.read(qs, qb, x), k.f[x], s);
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) dp = mfma<BF>(rows.read(gs, qb, x), v.f[x], dp);
+      uint4 pb[2], sb[2];
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) {
+        const int at = 32 * qb + 16 * t2 + 8 * h;  // the first of this lane's 8 queries
+        float bv[8];
+        if constexpr (kNear) bias_run(table, pitch, reach, pos0 + at - key, bv);
+        const uint32_t seen = kMode == 2 ? static_cast<uint32_t>(~up_to(key - pos0 - at - 1)) : 0;  // queries at or after the key
+        float p[8], ds[8];
+#pragma unroll
+        for (int e4 = 0; e4 < 2; ++e4) {
+          const f32x4 nl = *reinterpret_cast<const f32x4 *>(stats + at + 4 * e4);
+          const f32x4 dd = *reinterpret_cast<const f32x4 *>(stats + kRows + at + 4 * e4);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int e = 4 * e4 + y, r = 8 * t2 + e;
+            float x = __builtin_fmaf(s[r], a.c2, nl[y] + prob_shift<BF>());
+            if constexpr (kNear) x += bv[e];
+            else if constexpr (BIAS) x += bc;
+            if constexpr (kMode == 2) x = (seen >> e) & 1 ? x : -__builtin_inff();
+            p[e] = materialize(__builtin_amdgcn_exp2f(x));
+            ds[e] = materialize(p[e] * (dp[r] - dd[y]) * ds_mul);
+          }
+        }
+        pb[t2] = make_uint4(pack<BF>(p[0], p[1]), pack<BF>(p[2], p[3]), pack<BF>(p[4], p[5]), pack<BF>(p[6], p[7]));
+        sb[t2] = make_uint4(pack<BF>(ds[0], ds[1]), pack<BF>(ds[2], ds[3]), pack<BF>(ds[4], ds[5]), pack<BF>(ds[6], ds[7]));
+      }
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) {
+          dv[db] = mfma<BF>(cols.read(gs, db, qb, t2), pb[t2], dv[db]);
+          dk[db] = mfma<BF>(cols.read(qs, db, qb, t2), sb[t2], dk[db]);
+        }
+    }
+  };
+
+  if (i < end) issue(0, g, qt);
+  float far_behind = 0.0f, far_ahead = 0.0f;
+  bool build = true;  // the table of a head that begins
+  auto step = [&](int stage) __attribute__((always_inline)) {
+    wait_vmcnt<0>();
+    __syncthreads();  // this tile has landed for all waves, and the other stage and the table are no longer read
+    if constexpr (BIAS) {
+      if (build) {
+        build_bias(table, a.bias, hk * a.group + g, threadIdx.x, 64 * NW, true);
+        __syncthreads();
+        far_ahead = table[0];
+        far_behind = table[2 * reach + 16];
+      }
+    }
+    const int at = qt;
+    build = false;
+    if (++qt == w.qblocks) {
+      qt = qt0;
+      ++g;
+      build = true;
+    }
+    if (i + 1 < end) issue(stage ^ 1, g, qt);
+    const int pos0 = start + at * kRows;
+    if (key0 < keys && !(a.causal && pos0 + kRows - 1 < key0)) {
+      bool one = !BIAS;
+      float bc = 0.0f;
+      if constexpr (BIAS) {
+        if (key0 + 31 - pos0 <= -reach) {
+          one = true;
+          bc = far_behind;
+        } else if (key0 - (pos0 + kRows - 1) >= (a.bias.ahead ? reach : 0)) {
+          one = true;
+          bc = far_ahead;
+        }
+      }
+      if (a.causal && pos0 < key0 + 31) compute(stage, at, 0.0f, std::integral_constant<int, 2>{});
+      else if (one) compute(stage, at, bc, std::integral_constant<int, 0>{});
+      else if constexpr (BIAS) compute(stage, at, 0.0f, std::integral_constant<int, 1>{});
+    }
+  };
+  while (i < end) {
+    step(0);
+    if (++i >= end) break;
+    step(1);
+    ++i;
+  }
+
+  if (key >= a.Lk) return;
+  const float k_mul = a.c2 * kLn2 * (BF ? 1.0f : __builtin_exp2f(-shift)), v_mul = BF ? 1.0f : __builtin_exp2f(-kProbShift);
+  const int64_t at = (static_cast<int64_t>(bhk) * a.Lk + key) * a.dh, all = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.dh;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int ch = 32 * db + 8 * y + 4 * h;
+      if (32 * db + 8 * y >= a.dh) continue;
+      float x[4], z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = materialize(valid ? dk[db][4 * y + e] * k_mul : 0.0f);
+        z[e] = materialize(valid ? dv[db][4 * y + e] * v_mul : 0.0f);
+      }
+      if (cut.parts > 1) {
+        float *p = cut.partial + 2 * part * all + at + ch;
+        *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4 *>(p + all) = make_float4(z[0], z[1], z[2], z[3]);
+      } else {
+        *reinterpret_cast<uint2 *>(w.dk + at + ch) = make_uint2(pack<BF>(x[0], x[1]), pack<BF>(x[2], x[3]));
+        *reinterpret_cast<uint2 *>(w.dv + at + ch) = make_uint2(pack<BF>(z[0], z[1]), pack<BF>(z[2], z[3]));
+      }
+    }
+}
+
+// ------------------------------------------------------------------ dq, dtable
+
+// One workgroup = NW waves = 32 NW queries of one (image, head), the keys in tiles of 64 as in the forward pass; q and dO are
+// held. S^T = K Q^T and dP^T = V dO^T leave a lane's registers with keys of one query, in runs of 8; dQ^T += K^T dS^T reads
+// the same K tile transposed.
+//
+// dtable: tiles that hold only one value of the bias add dS up in a register. In the others a lane adds its 8 keys' dS to a
+// histogram by distance in LDS, one for each half of each wave: within a half the 32 lanes are 32 queries at one key, 32
+// distances, so no two lanes of an instruction meet, a wave's instructions are in order, and the sums have one order. It
+// covers every distance that such a tile can hold (kSpill past `reach` on either side). At the end the histograms are summed
+// by bucket, and by dtable_kernel over workgroups.
+constexpr int kSpill = kRows + 32;
+__host__ __device__ inline int hist_floats(int reach) { return 2 * reach + 2 * kSpill + 1; }
+
+template <bool BF, int D, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut cut) {
+  using T = Tile<D>;
+  constexpr int KJ = T::kLoads / NW;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
+  extern __shared__ __attribute__((aligned(16))) float table[];
+  const int t = item_of(cut.per_xcd);
+  if (t >= cut.total) return;
+  int rest = t;
+  const int qt0 = rest % cut.tiles;
+  rest /= cut.tiles;
+  const int g = rest % a.group;
+  rest /= a.group;
+  const int part = rest % cut.parts;
+  rest /= cut.parts;
+  const int hk = rest % a.Hk, b = rest / a.Hk, head = hk * a.group + g;
+  const int qt = a.causal ? cut.tiles - 1 - qt0 : qt0;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
+  const int keys = keys_of(a, b), start = start_of(a, b);
+  const int row0 = (qt * NW + wave) * 32, first = start + row0, pos = first + c;
+  int ntiles = (keys + kRows - 1) / kRows;
+  if (a.causal) ntiles = min(ntiles, max(start + min((qt + 1) * NW * 32, a.Lq) + kRows - 1, 0) / kRows);
+  const int per = (ntiles + cut.parts - 1) / cut.parts;
+  int kt = part * per;
+  const int end = min(ntiles, kt + per);
+
+  Held<D> q, dO;
+  q.load(a.q.p + b * a.q.sb + head * a.q.sh + row0 * a.q.sl, a.q.sl, a.dh, a.Lq - row0, lane);
+  dO.load(w.g.p + b * w.g.sb + head * w.g.sh + row0 * w.g.sl, w.g.sl, a.dh, a.Lq - row0, lane);
+  const bool here = row0 + c < a.Lq;
+  const int64_t stat = (static_cast<int64_t>(b) * a.H + head) * w.Lqp + row0 + c;
+  const float nl = here ? w.neg_lse[stat] : -__builtin_inff(), dd = here ? w.dot[stat] : 0.0f;
+  const uint16_t *kp = a.k.p + b * a.k.sb + hk * a.k.sh, *vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+  const typename T::template Loader<KJ> kl(wave, lane, a.k.sl, a.dh), vl(wave, lane, a.v.sl, a.dh);
+  const typename T::RowReader rows(lane);
+  const typename T::ColReader cols(lane);
+  const KeyBits keybits(a, b, keys, lane);
+  auto issue = [&](int stage, int kt, uint64_t bits) {
+    uint8_t *base = stage ? smem1 : smem0;
+    const int64_t key0 = static_cast<int64_t>(kt) * kRows;
+    const int left = keys - kt * kRows;
+    if (keybits.mask) {
+      kl.template issue<true>(base, kp + key0 * a.k.sl, a.k.sl, a.dh, left, bits);
+      vl.template issue<true>(base + T::kBytes, vp + key0 * a.v.sl, a.v.sl, a.dh, left, bits);
+    } else {
+      kl.template issue<false>(base, kp + key0 * a.k.sl, a.k.sl, a.dh, left, bits);
+      vl.template issue<false>(base + T::kBytes, vp + key0 * a.v.sl, a.v.sl, a.dh, left, bits);
+    }
+  };
+
+  const int reach = a.bias.reach, pitch = bias_pitch(reach), span = hist_floats(reach);
+  float *hist = table + 4 * pitch;  // [2 NW][span]; after that [NW][2] sums
+  float *mine = hist + (2 * wave + h) * span;
+  float sum_behind = 0.0f, sum_ahead = 0.0f, far_behind = 0.0f, far_ahead = 0.0f;
+  if constexpr (BIAS) {
+    build_bias(table, a.bias, head, threadIdx.x, 64 * NW, false);
+    for (int i = threadIdx.x; i < 2 * NW * span; i += 64 * NW) hist[i] = 0.0f;
+  }
+  const float shift = ds_shift<BF>(a, w, b, hk, lane), ds_mul = BF ? 1.0f : __builtin_exp2f(shift);
+
+  f32x16 dq[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) dq[db] = f32x16{};
+  uint64_t bits = 0;
+  int byte = 0;
+  if (kt < end) {
+    bits = keybits.word(kt, keybits.load(kt));
+    issue(0, kt, bits);
+    byte = keybits.load(kt + 1);
+  }
+  wait_vmcnt<0>();
+  __syncthreads();
+  if constexpr (BIAS) {
+    far_behind = table[0];
+    far_ahead = table[2 * reach + 16];
+  }
+
+  // kMode 0: all keys seen, one value of the bias; 1: all seen, bias by distance; 2 and 3: whatever is seen, one value / by
+  // distance.
+  auto compute = [&](int stage, int kt, float bc, auto mode) __attribute__((always_inline)) {
+    constexpr int kMode = decltype(mode)::value;
+    constexpr bool kNear = BIAS && (kMode & 1), kPart = kMode >= 2;
+    uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
+    const uint64_t seen = kPart ? (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h) : 0;
+    const float base = nl + bc;
+    float add = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const uint32_t word = static_cast<uint32_t>(kb ? seen >> 32 : seen);
+      f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) s = mfma<BF>(rows.read(ks, kb, x), q.f[x], s);
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) dp = mfma<BF>(rows.read(vs, kb, x), dO.f[x], dp);
+      uint4 sb[2];
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) {
+        const int d = kt * kRows + 32 * kb + 16 * t2 + 8 * h - pos;  // distance of this lane's first key
+        float bv[8];
+        if constexpr (kNear) bias_run(table, pitch, reach, d, bv);
+        float ds[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int r = 8 * t2 + e;
+          float x = __builtin_fmaf(s[r], a.c2, base);
+          if constexpr (kNear) x += bv[e];
+          if constexpr (kPart) x = (word >> (16 * t2 + e)) & 1 ? x : -__builtin_inff();
+          ds[e] = __builtin_amdgcn_exp2f(x) * (dp[r] - dd);
+          if constexpr (kNear)
+            __hip_atomic_fetch_add(mine + d + e + reach + kSpill, ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          else if constexpr (BIAS)
+            add += ds[e];
+          ds[e] = materialize(BF ? ds[e] : ds[e] * ds_mul);
+        }
+        sb[t2] = make_uint4(pack<BF>(ds[0], ds[1]), pack<BF>(ds[2], ds[3]), pack<BF>(ds[4], ds[5]), pack<BF>(ds[6], ds[7]));
+      }
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) dq[db] = mfma<BF>(cols.read(ks, db, kb, t2), sb[t2], dq[db]);
+    }
+    return add;
+  };
+  auto step = [&](int stage) __attribute__((always_inline)) {
+    const uint64_t bits_next = keybits.word(kt + 1, byte);
+    if (kt + 1 < end) issue(stage ^ 1, kt + 1, bits_next);
+    byte = keybits.load(kt + 2);
+    const int key0 = kt * kRows;
+    if (bits && !(a.causal && key0 > first + 31)) {
+      const bool all = bits == ~0ull && !(a.causal && key0 + kRows - 1 > first);
+      const bool behind = BIAS && key0 + kRows - 1 - first <= -reach;
+      const bool ahead = BIAS && !behind && key0 - first - 31 >= (a.bias.ahead ? reach : 0);
+      const float bc = behind ? far_behind : far_ahead;
+      float add = 0.0f;
+      if (!BIAS || behind || ahead) {
+        if (all) add = compute(stage, kt, bc, std::integral_constant<int, 0>{});
+        else add = compute(stage, kt, bc, std::integral_constant<int, 2>{});
+      } else if constexpr (BIAS) {
+        if (all) compute(stage, kt, 0.0f, std::integral_constant<int, 1>{});
+        else compute(stage, kt, 0.0f, std::integral_constant<int, 3>{});
+      }
+      sum_behind += behind ? add : 0.0f;
+      sum_ahead += behind ? 0.0f : add;
+    }
+    bits = bits_next;
+    wait_vmcnt<0>();
+    __syncthreads();
+  };
+  while (kt < end) {
+    step(0);
+    if (++kt >= end) break;
+    step(1);
+    ++kt;
+  }
+
+  if constexpr (BIAS) {
+    // The histograms added up, then each bucket by one wave.
+    float *sums = hist + 2 * NW * span;
+    sum_behind = wave_sum(sum_behind);
+    sum_ahead = wave_sum(sum_ahead);
+    if (lane == 0) {
+      sums[2 * wave] = sum_behind;
+      sums[2 * wave + 1] = sum_ahead;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < span; i += 64 * NW) {
+      float x = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2 * NW; ++j) x += hist[j * span + i];
+      hist[i] = x;
+    }
+    __syncthreads();
+    const int n = a.bias.n, buckets = a.bias.ahead ? 2 * n : n;
+    float *out = w.dtable_part + ((static_cast<int64_t>(b) * a.H + head) * cut.tiles * cut.parts + qt * cut.parts + part) * buckets;
+    for (int r = wave; r < buckets; r += NW) {
+      const bool up = r >= n;  // keys after the query
+      const int bt = up ? r - n : r;
+      int lo = a.bias.edge[bt], hi = bt + 1 < n ? a.bias.edge[bt + 1] : reach + kSpill + 1;  // distances
+      if (up) lo = max(lo, 1);
+      float x = 0.0f;
+      for (int i = lo + lane; i < hi; i += 64) x += hist[(up ? i : -i) + reach + kSpill];
+      if (!a.bias.ahead && bt == 0)
+        for (int i = 1 + lane; i <= reach + kSpill; i += 64) x += hist[i + reach + kSpill];
+      x = wave_sum(x);
+      if (lane == 0) {
+        if (bt == n - 1 && !up)
+          for (int j = 0; j < NW; ++j) x += sums[2 * j];
+        if (a.bias.ahead ? up && bt == n - 1 : bt == 0)
+          for (int j = 0; j < NW; ++j) x += sums[2 * j + 1];
+        out[r] = x;
+      }
+    }
+  }
+
+  const int row = row0 + c;
+  if (row >= a.Lq) return;
+  const float mul = a.c2 * kLn2 * (BF ? 1.0f : __builtin_exp2f(-shift));
+  const int64_t at = ((static_cast<int64_t>(b) * a.H + head) * a.Lq + row) * a.dh;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int ch = 32 * db + 8 * y + 4 * h;
+      if (32 * db + 8 * y >= a.dh) continue;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = materialize(dq[db][4 * y + e] * mul);
+      if (cut.parts > 1)
+        *reinterpret_cast<float4 *>(cut.partial + static_cast<int64_t>(part) * a.B * a.H * a.Lq * a.dh + at + ch) =
+            make_float4(x[0], x[1], x[2], x[3]);
+      else
+        *reinterpret_cast<uint2 *>(w.dq + at + ch) = make_uint2(pack<BF>(x[0], x[1]), pack<BF>(x[2], x[3]));
+    }
+}
+
+// y = the sum of `parts` arrays of n floats, in their order; 4 values a thread. blockIdx.y: the second array of a pair.
+template <bool BF>
+__global__ __launch_bounds__(256) void sum_kernel(const float *__restrict__ partial, int parts, int64_t n, int arrays,
+                                                  uint16_t *y0, uint16_t *y1) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const float *p = partial + blockIdx.y * n + i;
+  float4 s = *reinterpret_cast<const float4 *>(p);
+  for (int j = 1; j < parts; ++j) {
+    const float4 x = *reinterpret_cast<const float4 *>(p + static_cast<int64_t>(j) * arrays * n);
+    s.x += x.x;
+    s.y += x.y;
+    s.z += x.z;
+    s.w += x.w;
+  }
+  *reinterpret_cast<uint2 *>((blockIdx.y ? y1 : y0) + i) =
+      make_uint2(pack<BF>(materialize(s.x), materialize(s.y)), pack<BF>(materialize(s.z), materialize(s.w)));
+}
+
+// dtable[r, head] = the sum over images and workgroups, in a fixed order. One workgroup per head.
+__global__ __launch_bounds__(256) void dtable_kernel(const float *__restrict__ part, int B, int H, int each, int buckets,
+                                                     void *dtable, int dtype) {
+  __shared__ float red[256];
+  const int head = blockIdx.x, rows = max(256 / buckets, 1), lane = threadIdx.x % buckets, row = threadIdx.x / buckets;
+  float x = 0.0f;
+  if (row < rows)
+    for (int i = row; i < B * each; i += rows) {
+      const int b = i / each, j = i - b * each;
+      x += part[((static_cast<int64_t>(b) * H + head) * each + j) * buckets + lane];
+    }
+  red[threadIdx.x] = x;
+  __syncthreads();
+  if (threadIdx.x >= buckets) return;
+  x = 0.0f;
+  for (int j = 0; j < rows; ++j) x += red[j * buckets + threadIdx.x];
+  const int64_t at = static_cast<int64_t>(threadIdx.x) * H + head;
+  if (dtype == SELAS_F32) store_f<SELAS_F32>(dtable, at, x);
+  else if (dtype == SELAS_F16) store_f<SELAS_F16>(dtable, at, x);
+  else store_f<SELAS_BF16>(dtable, at, x);
+}
+
+// ------------------------------------------------------------------ host side
+
+struct Plan {
+  int D, qblocks, kblocks, buckets;
+  Cut key, query;
+  int64_t neg_lse, dot, g_norm, v_norm, dtable, key_partial, query_partial, bytes;  // offsets into the workspace
+};
+constexpr int kNW = 4;
+
+Plan plan_of(const Args &a, bool bf) {
+  Plan p{};
+  p.D = a.dh <= 64 ? 64 : 128;
+  p.qblocks = static_cast<int>(cdiv(a.Lq, kRows));
+  p.kblocks = static_cast<int>(cdiv(a.Lk, kRows));
+  p.buckets = a.bias.ahead ? 2 * a.bias.n : a.bias.n;
+  const int64_t cu = cu_count();
+  auto cut = [&](int64_t heads, int tiles, int64_t streamed) {
+    const int64_t whole = heads * tiles;
+    // Workgroups for two to a CU, of four streamed tiles at least.
+    const int64_t parts = std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(whole, 1), streamed / 4));
+    return Cut{tiles, static_cast<int>(parts), static_cast<int>(whole * parts), static_cast<int>(cdiv(whole * parts, 8)), nullptr};
+  };
+  p.key = cut(static_cast<int64_t>(a.B) * a.Hk, static_cast<int>(cdiv(a.Lk, 32 * kNW)), static_cast<int64_t>(a.group) * p.qblocks);
+  p.query = cut(static_cast<int64_t>(a.B) * a.H, static_cast<int>(cdiv(a.Lq, 32 * kNW)), p.kblocks);
+  auto take = [&](int64_t floats) {
+    const int64_t at = p.bytes;
+    p.bytes += (floats * 4 + 255) / 256 * 256;
+    return at;
+  };
+  const int64_t stats = static_cast<int64_t>(a.B) * a.H * p.qblocks * kRows;
+  p.neg_lse = take(stats);
+  p.dot = take(stats);
+  if (!bf) {
+    p.g_norm = take(static_cast<int64_t>(a.B) * a.H * p.qblocks);
+    p.v_norm = take(static_cast<int64_t>(a.B) * a.Hk * p.kblocks);
+  }
+  if (a.bias.table) p.dtable = take(static_cast<int64_t>(a.B) * a.H * p.query.tiles * p.query.parts * p.buckets);
+  if (p.key.parts > 1) p.key_partial = take(2ll * p.key.parts * a.B * a.Hk * a.Lk * a.dh);
+  if (p.query.parts > 1) p.query_partial = take(static_cast<int64_t>(p.query.parts) * a.B * a.H * a.Lq * a.dh);
+  return p;
+}
+
+template <bool BF, int D, bool BIAS>
+void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
+  const int row_blocks = a.B * a.H * p.qblocks + (BF ? 0 : a.B * a.Hk * p.kblocks);
+  if (row_blocks) row_kernel<BF><<<dim3(row_blocks), dim3(256), 0, st>>>(a, w);
+  const int reach = a.bias.reach;
+  if (p.key.total) {
+    key_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.key.per_xcd), dim3(64 * kNW), BIAS ? bias_bytes(reach) : 0, st>>>(a, w, p.key);
+    if (p.key.parts > 1) {
+      const int64_t n = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.dh;
+      sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(n, 1024)), 2), dim3(256), 0, st>>>(p.key.partial, p.key.parts, n, 2, w.dk, w.dv);
+    }
+  }
+  if (p.query.total) {
+    const size_t lds = BIAS ? bias_bytes(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
+    query_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.query.per_xcd), dim3(64 * kNW), lds, st>>>(a, w, p.query);
+    if (p.query.parts > 1) {
+      const int64_t n = static_cast<int64_t>(a.B) * a.H * a.Lq * a.dh;
+      sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(n, 1024))), dim3(256), 0, st>>>(p.query.partial, p.query.parts, n, 1, w.dq, nullptr);
+    }
+  }
+  if constexpr (BIAS)
+    dtable_kernel<<<dim3(a.H), dim3(256), 0, st>>>(w.dtable_part, a.B, a.H, p.query.tiles * p.query.parts, p.buckets, w.dtable,
+                                                   a.bias.dtype);
+}
+
+}  // namespace
+}  // namespace textattn
+}  // namespace selas
+
+using namespace selas;
+using namespace selas::textattn;
+
+extern "C" int selas_text_attention_backward_workspace_bytes(const selas_text_attention_problem *problem, int dtype,
+                                                             int64_t *bytes) {
+  if (!bytes) return set_error(SELAS_EINVAL, "text_attention_backward_workspace_bytes: null pointer");
+  *bytes = 0;
+  Args a;
+  if (int e = check_args("text_attention_backward_workspace_bytes", problem, dtype, false, a)) return e;
+  if (a.H) *bytes = plan_of(a, dtype == SELAS_BF16).bytes;
+  return ok();
+}
+
+extern "C" int selas_text_attention_backward(const selas_text_attention_problem *problem, const void *grad, int64_t g_sb,
+                                             int64_t g_sl, void *dq, void *dk, void *dv, void *dtable, int dtype,
+                                             void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *what = "text_attention_backward";
+  Args a;
+  if (int e = check_args(what, problem, dtype, true, a)) return e;
+  if (!a.H) return ok();
+  const bool bf = dtype == SELAS_BF16;
+  Grads w{};
+  if (a.B && a.Lq) {
+    if (!grad || !a.lse || !dq) return set_error(SELAS_EINVAL, "%s: null pointer (grad, lse or dq)", what);
+    if (g_sb < 0 || g_sl < 0) return set_error(SELAS_EINVAL, "%s: grad has a negative stride", what);
+    if (!aligned(grad, 16) || g_sb % 8 || g_sl % 8 || g_sl > (1 << 23))
+      return set_error(SELAS_EUNSUPPORTED, "%s: grad must be 16-byte aligned with strides of whole 16 bytes, rows up to 2^23 elements", what);
+  }
+  if (a.B && a.Lk && (!dk || !dv)) return set_error(SELAS_EINVAL, "%s: null pointer (dk or dv)", what);
+  if (a.bias.table && !dtable) return set_error(SELAS_EINVAL, "%s: null pointer (dtable)", what);
+  if (!aligned(dq, 8) || !aligned(dk, 8) || !aligned(dv, 8))
+    return set_error(SELAS_EUNSUPPORTED, "%s: dq, dk and dv must be 8-byte aligned", what);
+  Plan p = plan_of(a, bf);
+  if (p.bytes && (workspace_bytes < p.bytes || !workspace || !aligned(workspace, 16)))
+    return set_error(SELAS_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)p.bytes);
+  auto at = [&](int64_t offset) { return reinterpret_cast<float *>(static_cast<char *>(workspace) + offset); };
+  w.g = {static_cast<const uint16_t *>(grad), g_sb, a.dh, g_sl};
+  w.dq = static_cast<uint16_t *>(dq);
+  w.dk = static_cast<uint16_t *>(dk);
+  w.dv = static_cast<uint16_t *>(dv);
+  w.neg_lse = at(p.neg_lse);
+  w.dot = at(p.dot);
+  w.Lqp = p.qblocks * kRows;
+  w.qblocks = p.qblocks;
+  w.kblocks = p.kblocks;
+  w.g_norm = at(p.g_norm);
+  w.v_norm = at(p.v_norm);
+  w.dtable_part = at(p.dtable);
+  w.dtable = dtable;
+  p.key.partial = at(p.key_partial);
+  p.query.partial = at(p.query_partial);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  auto go = [&](auto t, auto d) {
+    constexpr bool kBf = decltype(t)::value;
+    constexpr int kD = decltype(d)::value;
+    if (a.bias.table) launch<kBf, kD, true>(a, w, p, st);
+    else launch<kBf, kD, false>(a, w, p, st);
+  };
+  using I64 = std::integral_constant<int, 64>;
+  using I128 = std::integral_constant<int, 128>;
+  if (bf) p.D == 64 ? go(std::true_type{}, I64{}) : go(std::true_type{}, I128{});
+  else p.D == 64 ? go(std::false_type{}, I64{}) : go(std::false_type{}, I128{});
+  return check_launch(what);
+}

@@ -139,6 +139,35 @@ def _forward(what, q, k, v, table, max_distance, bidirectional, causal, q_start,
     return (out, lse) if return_lse else out
 
 
+def _backward(what, grad, q, k, v, out, lse, table, max_distance, bidirectional, causal, q_start, lengths, mask, scale):
+    call = _Call(what, q, k, v, table, max_distance, bidirectional, causal, q_start, lengths, mask, scale)
+    b, h, hk, lq, lk, dh = call.shape
+    _lib.require_gpu(q, grad, out, lse)
+    for name, t in (("grad", grad), ("out", out)):
+        if t.shape != (b, lq, h * dh) or t.dtype != q.dtype:
+            raise ValueError(f"{what}: {name} must be [{b}, {lq}, {h * dh}] {q.dtype}, got {tuple(t.shape)} {t.dtype}")
+    if lse.shape != (b, h, lq) or lse.dtype != torch.float32:
+        raise ValueError(f"{what}: lse must be float32 [{b}, {h}, {lq}], got {lse.dtype} {tuple(lse.shape)}")
+    s = grad.stride()
+    if s[2] != 1 or (s[0] | s[1]) & 7 or s[1] > 1 << 23 or grad.data_ptr() & 15:
+        grad = grad.clone(memory_format=torch.contiguous_format)
+    s = out.stride()
+    if s[2] != 1 or (s[0] | s[1]) & 3 or out.data_ptr() & 7:
+        out = out.clone(memory_format=torch.contiguous_format)
+    lse = lse.contiguous()
+    dq = torch.empty(b, h, lq, dh, dtype=q.dtype, device=call.dev)
+    dk, dv = (torch.empty(b, hk, lk, dh, dtype=q.dtype, device=call.dev) for _ in range(2))
+    dtable = None if table is None else torch.empty(table.shape, dtype=table.dtype, device=call.dev)
+    problem, size = call.problem(out, lse), _SIZES()
+    with _lib.on(call.dev):
+        _lib.call("selas_text_attention_backward_workspace_bytes", problem, call.dtype, ctypes.byref(size))
+        n = size.value
+        ws = torch.empty(n, dtype=torch.uint8, device=call.dev) if n else None
+        _lib.call("selas_text_attention_backward", problem, grad.data_ptr(), grad.stride(0), grad.stride(1), dq.data_ptr(),
+                  dk.data_ptr(), dv.data_ptr(), _lib.ptr(dtable), call.dtype, _lib.ptr(ws), n, _lib.stream(call.dev))
+    return dq, dk, dv, dtable
+
+
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, lengths: torch.Tensor | None = None,
                     mask: torch.Tensor | None = None, scale: float | None = None, out: torch.Tensor | None = None,
                     return_lse: bool = False):
@@ -167,8 +196,31 @@ def text_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: tor
     score. With n buckets a direction (half of them each with ``bidirectional``; otherwise all of them for the keys before
     the query, and bucket 0 for those after it) distance a has bucket a below n // 2, and above it
     n // 2 + floor((n - n // 2) log(a / (n // 2)) / log(max_distance / (n // 2))), at most n - 1; keys after the query
-    have the second half. Distances are compared in exact arithmetic. 2 to 128 buckets a direction, max_distance up to 1024.
+    have the second half. Distances are compared in exact arithmetic. 2 to 128 buckets a direction, max_distance up to 512.
     ``causal``: a query sees the keys up to its own position. For one more token over a cache give q [B, H, 1, Dh],
     ``lengths`` and ``q_start = lengths - 1`` (int32: no conversion)."""
     return _forward("text_attention", q, k, v, table, max_distance, bidirectional, causal, q_start, lengths, mask, scale, out,
                     return_lse)
+
+
+def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                             lse: torch.Tensor, *, lengths: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                             scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv), contiguous and in the type of q, for ``grad`` [B, Lq, H * Dh], the gradient of ``cross_attention``'s
+    output; ``out`` and ``lse`` are what that call returned, the other arguments what it was given.
+
+    Each is the gradient of the tensor as given: dk and dv are summed over the query heads that share a key head; a
+    broadcast input (an expanded batch) still has its own sum to take. Keys that are not seen and queries that see none
+    have zeros. Sums are fp32 in one order: equal calls give equal bits."""
+    return _backward("cross_attention_backward", grad, q, k, v, out, lse, None, 0, True, False, 0, lengths, mask, scale)[:3]
+
+
+def text_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                            lse: torch.Tensor, table: torch.Tensor | None = None, *, max_distance: int = 128,
+                            bidirectional: bool = True, causal: bool = False, q_start: int | torch.Tensor = 0,
+                            lengths: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                            scale: float | None = None):
+    """(dq, dk, dv, dtable) of ``text_attention``, as in ``cross_attention_backward``. dtable [buckets, H] is in the table's
+    type, summed in fp32 over images, queries and keys; None without a table."""
+    return _backward("text_attention_backward", grad, q, k, v, out, lse, table, max_distance, bidirectional, causal, q_start,
+                     lengths, mask, scale)

@@ -10,7 +10,8 @@ The bounds count roundings, element by element. With h half a step of the type (
   D        sum |dO| err(out) + (Dh + 2) u sum |dO out|;  dP: (Dh + 2) u sum |dO v|.
   dS       p (err(dP) + err(D)) + err(p) |dP - D| + 4 u |dS|, then rounded: h; fp16: scaled so that 2^-40 max|dO| max|v|
            bounds what falls below its normal numbers.
-  sums of n terms add n u of the sum of their magnitudes, and each result is rounded once."""
+  sums of n terms add n u of the sum of their magnitudes, and each result is rounded once. The table's sums run over trees
+  and rows of at most 4 sqrt(n) additions in a chain: 4 sqrt(n) u."""
 
 from __future__ import annotations
 
@@ -87,6 +88,43 @@ class Reference:
         self.oerr = self.oerr + self.h * (o.abs() + self.oerr) + torch.finfo(self.dtype).smallest_normal * 2 * self.h
         self.o = o
         self.out, self.out_bound = (t.transpose(1, 2).reshape(b, lq, h * dh) for t in (o, self.oerr))
+
+    def backward(self, grad):
+        """[(gradient, bound)] of q, k, v and the table (None without one)."""
+        b, h, lq, dh = self.q.shape
+        hk, lk, fp16 = h // max(self.group, 1), self.k.shape[2], self.dtype == torch.float16
+        step, tiny = self.h, torch.finfo(self.dtype).smallest_normal * 2 * self.h
+        g = grad.detach().cpu().double().view(b, lq, h, dh).transpose(1, 2)
+        dp = g @ self.v.mT
+        dot = (g * self.o).sum(-1, keepdim=True)
+        dot_err = (g.abs() * self.oerr).sum(-1, keepdim=True) + (dh + 2) * U * (g * self.o).abs().sum(-1, keepdim=True)
+        dp_err = (dh + 2) * U * (g.abs() @ self.v.abs().mT)
+        ds = self.p * (dp - dot)
+        ds_err = self.p * (dp_err + dot_err + (self.perr + 4 * U) * (dp - dot).abs())
+        # What fp16 drops below its normal numbers, per element (the norms' product bounds |dP|).
+        low = 0.0
+        if fp16 and self.v.numel() and g.numel():
+            low = torch.where(self.seen, 2.0 ** -37 * g.norm(dim=-1).amax() * self.v.norm(dim=-1).amax(), 0.0)
+        s_err = ds_err + step * (ds.abs() + ds_err) + low
+        p_err = self.p * (self.perr + step) + torch.where(self.seen, 2.0 ** -39 if fp16 else 0.0, 0.0)
+        u_q, u_k = (lk + 8) * U, (lq * max(self.group, 1) + 8) * U
+
+        def rounded(x, e):
+            return x, e + step * (x.abs() + e) + tiny
+
+        def heads(t):
+            return t.view(b, hk, self.group, lk, dh).sum(2) if h else t.view(b, hk, lk, dh)
+
+        dq = rounded(self.scale * ds @ self.k, self.scale * (s_err + u_q * ds.abs()) @ self.k.abs())
+        dk = rounded(heads(self.scale * ds.mT @ self.q), heads(self.scale * (s_err + u_k * ds.abs()).mT @ self.q.abs()))
+        dv = rounded(heads(self.p.mT @ g), heads((p_err + u_k * self.p).mT @ g.abs()))
+        if self.table is None:
+            return [dq, dk, dv, None]
+        hot = torch.nn.functional.one_hot(self.bucket.expand(b, lq, lk).reshape(-1), self.table.shape[0]).double()
+        flat = [x.transpose(0, 1).reshape(h, -1) @ hot for x in (ds, ds_err + (lq * lk + 64) ** 0.5 * 4 * U * ds.abs())]
+        half = torch.finfo(self.table.dtype).eps / 2
+        x, e = flat[0].t(), flat[1].t()
+        return [dq, dk, dv, (x, e + half * (x.abs() + e) + torch.finfo(self.table.dtype).smallest_normal * 2 * half)]
 
 
 def within(y: torch.Tensor, ref: torch.Tensor, bound: torch.Tensor) -> None:
