@@ -28,7 +28,7 @@ struct Bias {
   const void *table;  // [buckets, H], unit column stride; null: no bias
   int64_t row;
   int dtype, n, ahead, reach;
-  int16_t edge[kMaxSide];
+  int edge[kMaxSide];  // from n on: beyond every distance
 };
 
 struct Args {
@@ -119,7 +119,9 @@ __host__ __device__ inline int bias_bytes(int reach) { return 4 * 4 * bias_pitch
 __device__ __forceinline__ int bucket_of(const Bias &t, int d) {
   const int side = t.ahead ? abs(d) : max(-d, 0);
   int r = t.ahead && d > 0 ? t.ahead - 1 : -1;
-  for (int i = 0; i < t.n; ++i) r += side >= t.edge[i];  // edge[0] = 0
+  for (int i = 0; i < t.n; i += 8)  // edge[0] = 0; eight at a time, which are one scalar load
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r += side >= t.edge[i + j];
   return r;
 }
 

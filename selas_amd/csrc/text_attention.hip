@@ -596,7 +596,7 @@ bool past_border(int a, int e, int m, int k, int t) {
   return x.at_least(y);
 }
 
-int fill_buckets(const char *what, int64_t buckets, int64_t max_distance, int bidirectional, int16_t *edge, int &n) {
+int fill_buckets(const char *what, int64_t buckets, int64_t max_distance, int bidirectional, int32_t *edge, int &n) {
   if (bidirectional && buckets % 2)
     return set_error(SELAS_EINVAL, "%s: %lld buckets do not halve into two directions", what, (long long)buckets);
   const int64_t side = bidirectional ? buckets / 2 : buckets;
@@ -609,13 +609,14 @@ int fill_buckets(const char *what, int64_t buckets, int64_t max_distance, int bi
                      kMaxDistance);
   n = static_cast<int>(side);
   const int e = n / 2, m = static_cast<int>(max_distance), k = n - e;
-  for (int t = 0; t <= e; ++t) edge[t] = static_cast<int16_t>(t);
+  for (int t = 0; t <= e; ++t) edge[t] = t;
   for (int t = 1; t < k; ++t) {
     // The real border, and the distance at or after it: whole numbers decide where rounding could.
     int a = std::max(static_cast<int>(e * pow(static_cast<double>(m) / e, static_cast<double>(t) / k)) - 1, e);
     while (!past_border(a, e, m, k, t)) ++a;
-    edge[e + t] = static_cast<int16_t>(a);
+    edge[e + t] = a;
   }
+  for (int t = n; t < kMaxSide; ++t) edge[t] = INT32_MAX;
   return SELAS_OK;
 }
 
@@ -766,7 +767,7 @@ using namespace selas::textattn;
 extern "C" int selas_relative_buckets(int64_t buckets, int64_t max_distance, int bidirectional, int32_t *edges,
                                       int64_t *count) {
   if (!edges || !count) return set_error(SELAS_EINVAL, "relative_buckets: null pointer");
-  int16_t edge[kMaxSide];
+  int32_t edge[kMaxSide];
   int n = 0;
   if (int e = fill_buckets("relative_buckets", buckets, max_distance, bidirectional, edge, n)) return e;
   for (int t = 0; t < n; ++t) edges[t] = edge[t];

@@ -320,13 +320,50 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
 // held. S^T = K Q^T and dP^T = V dO^T leave a lane's registers with keys of one query, in runs of 8; dQ^T += K^T dS^T reads
 // the same K tile transposed.
 //
-// dtable: tiles that hold only one value of the bias add dS up in a register. In the others a lane adds its 8 keys' dS to a
-// histogram by distance in LDS, one for each half of each wave: within a half the 32 lanes are 32 queries at one key, 32
-// distances, so no two lanes of an instruction meet, a wave's instructions are in order, and the sums have one order. It
+// dtable: tiles that hold only one value of the bias add dS up in a register. In the others dS is summed along the diagonals
+// (one distance each): a lane's run of 8 keys moves a lane per key through the 16 lanes of its row (Diagonals), and what is
+// left, a value per lane and 16 distances, is added to a histogram by distance in LDS, one for each half of each wave. It
 // covers every distance that such a tile can hold (kSpill past `reach` on either side). At the end the histograms are summed
 // by bucket, and by dtable_kernel over workgroups.
-constexpr int kSpill = kRows + 32;
+constexpr int kSpill = 112;
 __host__ __device__ inline int hist_floats(int reach) { return 2 * reach + 2 * kSpill + 1; }
+
+// Sums along the diagonals of a wave's 64 keys x 32 queries. v[e] of lane q belongs to distance o + e - q. With
+// t_e[p] = v[e][p] + t_{e+1}[p + 1], the lanes' indices modulo 16, t_0[p] holds distance o - p and, from the lanes below e
+// that wrapped, o + 16 - p; the latter are summed apart and belong to the next 16 keys' first part.
+struct Diagonals {
+  float u[5] = {};  // u[m] of lane q: distance d0 + 16 m of that lane
+  __device__ __forceinline__ static float next_lane(float v) {  // row_ror:15
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x12F, 0xF, 0xF, false));
+  }
+  __device__ __forceinline__ void add(int m, const float (&v)[8], int lane) {
+    const int p = lane & 15;
+    float all = v[7], low = p < 7 ? v[7] : 0.0f;
+#pragma unroll
+    for (int e = 6; e >= 0; --e) {
+      all = v[e] + next_lane(all);
+      low = next_lane(low);
+      if (e) low += p < e ? v[e] : 0.0f;
+    }
+    u[m] += all - low;
+    u[m + 1] += low;
+  }
+  // u[m + 1] of the lanes 16 .. 31 meets u[m] of the lanes 0 .. 15: first the even ones, then the odd ones. LDS
+  // instructions of a wave are in order.
+  __device__ __forceinline__ void store(float *at) const {
+    float x[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) x[i] = at[32 * i];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) at[32 * i] = x[i] + u[2 * i];
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = at[32 * i + 16];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) at[32 * i + 16] = x[i] + u[2 * i + 1];
+    asm volatile("" ::: "memory");
+  }
+};
 
 template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut cut) {
@@ -414,6 +451,7 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
     const uint64_t seen = kPart ? (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h) : 0;
     const float base = nl + bc;
     float add = 0.0f;
+    Diagonals diagonals;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       const uint32_t word = static_cast<uint32_t>(kb ? seen >> 32 : seen);
@@ -435,13 +473,13 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
           float x = __builtin_fmaf(s[r], a.c2, base);
           if constexpr (kNear) x += bv[e];
           if constexpr (kPart) x = (word >> (16 * t2 + e)) & 1 ? x : -__builtin_inff();
-          ds[e] = __builtin_amdgcn_exp2f(x) * (dp[r] - dd);
-          if constexpr (kNear)
-            __hip_atomic_fetch_add(mine + d + e + reach + kSpill, ds[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          else if constexpr (BIAS)
-            add += ds[e];
-          ds[e] = materialize(BF ? ds[e] : ds[e] * ds_mul);
+          ds[e] = materialize(__builtin_amdgcn_exp2f(x) * (dp[r] - dd));
+          if constexpr (BIAS && !kNear) add += ds[e];
         }
+        if constexpr (kNear) diagonals.add(2 * kb + t2, ds, lane);
+        if constexpr (!BF)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ds[e] = materialize(ds[e] * ds_mul);
         sb[t2] = make_uint4(pack<BF>(ds[0], ds[1]), pack<BF>(ds[2], ds[3]), pack<BF>(ds[4], ds[5]), pack<BF>(ds[6], ds[7]));
       }
 #pragma unroll
@@ -449,6 +487,7 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) dq[db] = mfma<BF>(cols.read(ks, db, kb, t2), sb[t2], dq[db]);
     }
+    if constexpr (kNear) diagonals.store(mine + kt * kRows + 8 * h - pos + reach + kSpill);
     return add;
   };
   auto step = [&](int stage) __attribute__((always_inline)) {
