@@ -48,12 +48,16 @@ struct Args {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Keys of image b; the position of its first query. Both are uniform, and bounded so that sums with them stay in 32 bits.
+// Keys of image b; the position of its first query. Both are uniform (scalar loads: a vector load's wait would also wait
+// for the tiles in flight), and bounded so that sums with them stay in 32 bits.
+__device__ __forceinline__ int scalar_load(const int32_t *p, int i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(p))[uniform(i)];
+}
 __device__ __forceinline__ int keys_of(const Args &a, int b) {
-  return a.lengths ? uniform(min(max(a.lengths[b], 0), a.Lk)) : a.Lk;
+  return a.lengths ? min(max(scalar_load(a.lengths, b), 0), a.Lk) : a.Lk;
 }
 __device__ __forceinline__ int start_of(const Args &a, int b) {
-  const int s = a.start ? uniform(a.start[b]) : a.start0;
+  const int s = a.start ? scalar_load(a.start, b) : a.start0;
   return min(max(s, -(1 << 29)), 1 << 29);
 }
 
@@ -133,17 +137,23 @@ __device__ __forceinline__ float bias_at(const Bias &t, int head, int d) {
   return v * kLog2e;
 }
 
-// reversed: by query - key. The caller puts barriers around it.
-__device__ __forceinline__ void build_bias(float *lds, const Bias &t, int head, int tid, int threads, bool reversed) {
-  const int pitch = bias_pitch(t.reach), first = -t.reach - 8;
-  for (int i = tid; i < 2 * t.reach + 17; i += threads) {
-    const int d = first + i;
-    const float v = bias_at(t, head, reversed ? -d : d);
+// The four copies of a head's table, by a thread per distance, into global memory: workgroups then only copy them to LDS.
+// reversed: by query - key.
+__device__ __forceinline__ void write_bias(float *out, const Bias &t, int head, int i, bool reversed) {
+  const int pitch = bias_pitch(t.reach), d = i - t.reach - 8;
+  if (i >= 2 * t.reach + 17) return;
+  const float v = bias_at(t, head, reversed ? -d : d);
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (i >= c) lds[c * pitch + i - c] = v;
-  }
+  for (int c = 0; c < 4; ++c)
+    if (i >= c) out[c * pitch + i - c] = v;
 }
+
+// `bytes` (whole 16) from global memory to LDS, 1 KiB an instruction, dealt to the waves; LDS is written to the next KiB.
+__device__ __forceinline__ void load_bytes(uint8_t *lds, const void *p, int bytes, int wave, int waves, int lane) {
+  const __amdgpu_buffer_rsrc_t r = make_rsrc(p, bytes);
+  for (int i = wave; i * 1024 < bytes; i += waves) load_lds16(r, lds + i * 1024, i * 1024 + 16 * lane, 0);
+}
+__host__ __device__ inline int bias_lds(int reach) { return (bias_bytes(reach) + 1023) / 1024 * 1024; }
 
 // Eight entries from distance d on.
 __device__ __forceinline__ void bias_run(const float *lds, int pitch, int reach, int d, float (&v)[8]) {
@@ -159,31 +169,32 @@ __device__ __forceinline__ void bias_run(const float *lds, int pitch, int reach,
 
 // ------------------------------------------------------------------ LDS tiles
 
-// 64 rows of D channels (dh of them given, the rest zeros), in 16-byte chunks whose place in the row is XORed with a
-// function of the row, so that two kinds of read are free of bank conflicts: 16 rows at one chunk (a row-wise operand),
-// and 4 rows at 64 bytes (ds_read_b64_tr_b16, a transposed operand).
+// 64 rows of D channels (dh of them given, the rest zeros), in 16-byte chunks. A DMA instruction fills 1 KiB, a group of 4
+// (D = 128) or 8 rows; the groups are 16 bytes further apart than that, and within a group a chunk's place in its row is
+// XORed with a function of the row. So two kinds of read are free of bank conflicts: 16 rows at one chunk (a row-wise
+// operand), and 4 rows at 64 bytes (ds_read_b64_tr_b16, a transposed operand); and since the function is the same in every
+// group, a lane needs few addresses: the rest is in the instructions' offsets.
 template <int D>
 struct Tile {
   static constexpr int kRow = 2 * D;        // bytes
   static constexpr int kChunks = D / 8;     // per row
-  static constexpr int kBytes = kRows * kRow;
-  static constexpr int kLoads = kBytes / 1024;  // DMA instructions (a wave's 64 x 16 bytes)
-  __device__ static __forceinline__ int swizzle(int r) {
-    return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  static constexpr int kGroupRows = 1024 / kRow, kGroup = 1024 + 16;
+  static constexpr int kLoads = kRows / kGroupRows;
+  static constexpr int kBytes = kLoads * kGroup;
+  __device__ static __forceinline__ int swizzle(int r) {  // of row r of a group
+    return D == 128 ? r << 2 : (((r >> 1) & 1) << 2) | (((r >> 2) & 1) << 1);
   }
+  static constexpr int at(int r) { return r / kGroupRows * kGroup; }  // offset of the group that begins with row r
 
-  // The offsets of a wave's share of the loads: instructions KJ * wave + j, whose lane fills row `row(j)`.
+  // A wave's share of the loads: instructions KJ * wave + j, whose lane fills row `row(j)`.
   template <int KJ>
   struct Loader {
-    uint32_t voff[KJ];
+    uint32_t voff;
     int wave, lane;
-    __device__ __forceinline__ int row(int j) const { return (KJ * wave + j) * (64 / kChunks) + lane / kChunks; }
+    __device__ __forceinline__ int row(int j) const { return (KJ * wave + j) * kGroupRows + lane / kChunks; }
     __device__ __forceinline__ Loader(int wave_, int lane_, int64_t sl, int dh) : wave(wave_), lane(lane_) {
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) {
-        const int r = row(j), chunk = (lane & (kChunks - 1)) ^ swizzle(r);
-        voff[j] = 8 * chunk < dh ? static_cast<uint32_t>(r) * static_cast<uint32_t>(2 * sl) + 16 * chunk : kPast;
-      }
+      const int r = lane / kChunks, chunk = (lane & (kChunks - 1)) ^ swizzle(r);
+      voff = 8 * chunk < dh ? static_cast<uint32_t>(r) * static_cast<uint32_t>(2 * sl) + 16 * chunk : kPast;
     }
     // The tile whose first row is at `p`, of which `rows` exist (the others read as zeros, and so do rows whose bit in
     // `bits` is not set where PART is).
@@ -194,44 +205,47 @@ struct Tile {
       const __amdgpu_buffer_rsrc_t r = make_rsrc(p, bytes);
 #pragma unroll
       for (int j = 0; j < KJ; ++j) {
-        uint32_t off = voff[j];
+        const int J = KJ * wave + j;
+        uint32_t off = voff;
         if constexpr (PART) off = (bits >> row(j)) & 1 ? off : kPast;
-        load_lds16(r, lds + (KJ * wave + j) * 1024, off, 0);
+        load_lds16(r, lds + J * kGroup, off, static_cast<uint32_t>(J * kGroupRows) * static_cast<uint32_t>(2 * sl));
       }
     }
   };
 
-  // Row-wise operand: lane (c, h) reads channels 16 s + 8 h .. + 8 of row 32 blk + swap23(c).
+  // Row-wise operand: lane (c, h) reads channels 16 s + 8 h .. + 8 of row 32 blk + swap23(c) (bits 2 and 3 exchanged).
   struct RowReader {
-    uint32_t base, flip;
+    uint32_t off[4];
     __device__ __forceinline__ RowReader(int lane) {
-      const int c = lane & 31, r = (c & ~12) | ((c & 4) << 1) | ((c & 8) >> 1);
-      base = r * kRow;
-      flip = (swizzle(r) ^ (lane >> 5)) << 4;
+      const int c = lane & 31, r = (c & ~12) | ((c & 4) << 1) | ((c & 8) >> 1), r8 = r % kGroupRows;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int chunk = (D == 128 ? 4 * i : 2 * i) + (lane >> 5);
+        off[i] = r / kGroupRows * kGroup + r8 * kRow + ((chunk ^ swizzle(r8)) << 4);
+      }
     }
     __device__ __forceinline__ uint4 read(const uint8_t *lds, int blk, int s) const {
-      return *reinterpret_cast<const uint4 *>(lds + base + blk * 32 * kRow + ((32 * s) ^ flip));
+      return *reinterpret_cast<const uint4 *>(lds + (D == 128 ? off[s >> 1] + 32 * (s & 1) : off[s]) + at(32 * blk));
     }
   };
 
   // Transposed operand: lane (c, h) receives channel 32 db + c of rows 32 blk + 16 t + 8 h .. + 8.
   struct ColReader {
-    uint32_t off[D / 32][2];
+    uint32_t off[4];
     __device__ __forceinline__ ColReader(int lane) {
       const int h = lane >> 5, r4 = (lane >> 2) & 3, x = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = 8 * h + 4 * u + r4;
-          off[db][u] = r * kRow + (((4 * db + x) ^ swizzle(r)) << 4) + 8 * (lane & 1);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int db = D == 128 ? i : i >> 1, r = 8 * h + r4 + (D == 128 ? 0 : 4 * (i & 1)), r8 = r % kGroupRows;
+        off[i] = r / kGroupRows * kGroup + r8 * kRow + (((4 * db + x) ^ swizzle(r8)) << 4) + 8 * (lane & 1);
+      }
     }
     __device__ __forceinline__ uint4 read(uint8_t *lds, int db, int blk, int t) const {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       auto half = [&](int u) {
+        const uint32_t o = D == 128 ? off[db] + u * at(4) : off[2 * db + u];
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4 *)(lds + off[db][u] + (32 * blk + 16 * t) * kRow));
+            (__attribute__((address_space(3))) s16x4 *)(lds + o + at(32 * blk + 16 * t)));
       };
       const s16x4 lo = half(0), hi = half(1);
       return __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -278,6 +292,17 @@ struct KeyBits {
 
 // The low n + 1 bits (none below 0, all from 63 on): the keys at or before position n of a tile.
 __device__ __forceinline__ uint64_t up_to(int n) { return n < 0 ? 0ull : n >= 63 ? ~0ull : (2ull << n) - 1; }
+
+namespace {
+// Every head's table by distance, [orders][H][4 bias_pitch]; blockIdx = (distances / 256, head, order).
+__global__ __launch_bounds__(256) void bias_kernel(Bias t, float *out) {
+  const int64_t at = static_cast<int64_t>(blockIdx.z * gridDim.y + blockIdx.y) * 4 * bias_pitch(t.reach);
+  write_bias(out + at, t, blockIdx.y, blockIdx.x * 256 + threadIdx.x, blockIdx.z);
+}
+inline void launch_bias(const Bias &t, int H, int orders, float *out, hipStream_t st) {
+  bias_kernel<<<dim3((2 * t.reach + 17 + 255) / 256, H, orders), dim3(256), 0, st>>>(t, out);
+}
+}  // namespace
 
 // ------------------------------------------------------------------ host side
 

@@ -269,71 +269,99 @@ __global__ __launch_bounds__(128) void few_merge_kernel(Args a, int parts, int D
 
 // ------------------------------------------------------------------ tiles
 
-// A call cut into work items: parts of the keys innermost but for the query tiles and the heads of a group, so that what
-// reads the same keys runs at the same time behind the same L2.
+// A call cut into work items of NW blocks of 32 rows: the blocks of one query head, or (pack) of all the heads of a group one
+// after another, so that few queries of several heads share their key head's tiles. Parts of the keys are outside the blocks
+// and the heads of a group, so that what reads the same keys runs at the same time behind the same L2.
 struct Cut {
-  int qtiles, parts, total, per_xcd;
-  float *partial;
+  int qblocks;  // of 32 queries, per head
+  int tiles;    // items per head, or per group (pack)
+  int parts, pack, total, per_xcd;
+  float *partial, *tables;  // tables: every head's bias by distance
 };
 constexpr int partial_floats(int D) { return 64 * (D / 2) + 2 * 64; }  // per wave: outputs in register order, maxima, sums
 
-// One workgroup = NW waves = 32 NW queries of one (image, head); wave w owns queries 32 w .. + 32. The keys stream through
-// LDS in double-buffered tiles of 64 that all waves share. Per tile: S^T = K Q^T (K row-wise from LDS, Q held), the softmax
-// on the scores in registers, O^T += V^T P^T (V transposed by the LDS reads, the probabilities straight from the score
-// registers: the K rows of a block are read with bits 2 and 3 of the row exchanged, so that register r of a lane holds key
-// 16 (r / 8) + 8 h + r % 8 of it, as the second product's operand wants them).
+// What a workgroup has to know of an item. Uniform but for the wave's share.
+struct Item {
+  int b, hk, head;  // head: of this wave
+  int row0;         // this wave's first query (Lq: no rows)
+  int keys, start, kt, end;
+  const uint16_t *kp, *vp;
+};
+
+__device__ __forceinline__ Item item_at(const Args &a, const Cut &cut, int t, int nw, int wave) {
+  Item x;
+  const int tile0 = t % cut.tiles;
+  int rest = t / cut.tiles, g = 0;
+  if (!cut.pack) {
+    g = rest % a.group;
+    rest /= a.group;
+  }
+  const int part = rest % cut.parts;
+  rest /= cut.parts;
+  x.hk = rest % a.Hk;
+  x.b = rest / a.Hk;
+  const int tile = a.causal ? cut.tiles - 1 - tile0 : tile0;  // the longest first
+  int block = tile * nw + wave;
+  if (cut.pack) {
+    g = block / cut.qblocks;
+    block -= g * cut.qblocks;
+  }
+  x.row0 = g < a.group ? min(32 * block, a.Lq) : a.Lq;
+  x.head = x.hk * a.group + min(g, a.group - 1);
+  x.keys = keys_of(a, x.b);
+  x.start = start_of(a, x.b);
+  int n = (x.keys + kRows - 1) / kRows;
+  if (a.causal) n = min(n, max(x.start + min((tile + 1) * nw * 32, a.Lq) + kRows - 1, 0) / kRows);
+  const int per = (n + cut.parts - 1) / cut.parts;
+  x.kt = part * per;
+  x.end = max(min(n, x.kt + per), x.kt + 1);  // without keys: one tile of which nothing is seen
+  x.kp = a.k.p + x.b * a.k.sb + x.hk * a.k.sh;
+  x.vp = a.v.p + x.b * a.v.sb + x.hk * a.v.sh;
+  return x;
+}
+
+// One workgroup = NW waves = NW blocks of 32 queries. The keys stream through LDS in double-buffered tiles of 64 that all
+// waves share. Per tile: S^T = K Q^T (K row-wise from LDS, Q held), the softmax on the scores in registers, O^T += V^T P^T
+// (V transposed by the LDS reads, the probabilities straight from the score registers: the K rows of a block are read with
+// bits 2 and 3 of the row exchanged, so that register r of a lane holds key 16 (r / 8) + 8 h + r % 8 of it, as the second
+// product's operand wants them).
 template <bool BF, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void fwd_kernel(Args a, Cut cut) {
+__global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_kernel(Args a, Cut cut) {
   using T = Tile<D>;
   constexpr int KJ = T::kLoads / NW;
   static_assert(KJ * NW == T::kLoads, "loads per wave");
   __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
-  extern __shared__ __attribute__((aligned(16))) float table[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t tables[];  // the head's bias by distance
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const int t = item_of(cut.per_xcd);
   if (t >= cut.total) return;
-  int rest = t;
-  const int qt0 = rest % cut.qtiles;
-  rest /= cut.qtiles;
-  const int g = rest % a.group;
-  rest /= a.group;
-  const int part = rest % cut.parts;
-  rest /= cut.parts;
-  const int hk = rest % a.Hk, b = rest / a.Hk, head = hk * a.group + g;
-  const int qt = a.causal ? cut.qtiles - 1 - qt0 : qt0;  // the longest first
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
-
-  const int keys = keys_of(a, b), start = start_of(a, b);
-  const int row0 = (qt * NW + wave) * 32;  // this wave's first query
-  const int first = start + row0, pos = first + c;
-  int ntiles = (keys + kRows - 1) / kRows;
-  if (a.causal) ntiles = min(ntiles, max(start + min((qt + 1) * NW * 32, a.Lq) + kRows - 1, 0) / kRows);
-  const int per = (ntiles + cut.parts - 1) / cut.parts;
-  int kt = part * per;
-  const int end = min(ntiles, kt + per);
-
-  Held<D> q;
-  q.load(a.q.p + b * a.q.sb + head * a.q.sh + row0 * a.q.sl, a.q.sl, a.dh, a.Lq - row0, lane);
-  const uint16_t *kp = a.k.p + b * a.k.sb + hk * a.k.sh, *vp = a.v.p + b * a.v.sb + hk * a.v.sh;
+  const Item x = item_at(a, cut, t, NW, wave);
+  const KeyBits keybits(a, x.b, x.keys, lane);
   const typename T::template Loader<KJ> kl(wave, lane, a.k.sl, a.dh), vl(wave, lane, a.v.sl, a.dh);
   const typename T::RowReader rows(lane);
   const typename T::ColReader cols(lane);
-  const KeyBits keybits(a, b, keys, lane);
-  auto issue = [&](int stage, int kt, uint64_t bits) {
+  const int reach = a.bias.reach, pitch = bias_pitch(reach);
+
+  auto issue = [&](int stage, int kt, uint64_t bits) __attribute__((always_inline)) {
     uint8_t *base = stage ? smem1 : smem0;
     const int64_t key0 = static_cast<int64_t>(kt) * kRows;
-    const int left = keys - kt * kRows;
-    if (keybits.mask) {
-      kl.template issue<true>(base, kp + key0 * a.k.sl, a.k.sl, a.dh, left, bits);
-      vl.template issue<true>(base + T::kBytes, vp + key0 * a.v.sl, a.v.sl, a.dh, left, bits);
+    const int left = x.keys - kt * kRows;
+    const uint16_t *kp = x.kp + key0 * a.k.sl, *vp = x.vp + key0 * a.v.sl;
+    if (a.mask) {
+      kl.template issue<true>(base, kp, a.k.sl, a.dh, left, bits);
+      vl.template issue<true>(base + T::kBytes, vp, a.v.sl, a.dh, left, bits);
     } else {
-      kl.template issue<false>(base, kp + key0 * a.k.sl, a.k.sl, a.dh, left, bits);
-      vl.template issue<false>(base + T::kBytes, vp + key0 * a.v.sl, a.v.sl, a.dh, left, bits);
+      kl.template issue<false>(base, kp, a.k.sl, a.dh, left, bits);
+      vl.template issue<false>(base + T::kBytes, vp, a.v.sl, a.dh, left, bits);
     }
   };
-
-  const int reach = a.bias.reach, pitch = bias_pitch(reach);
-  float far_behind = 0.0f, far_ahead = 0.0f;
-  if constexpr (BIAS) build_bias(table, a.bias, head, threadIdx.x, 64 * NW, false);
+  int kt = x.kt;
+  uint64_t bits = keybits.word(kt, keybits.load(kt));
+  int byte = keybits.load(kt + 1);  // mask bytes a tile ahead of the loads that they are for
+  Held<D> q;
+  if constexpr (BIAS) load_bytes(tables, cut.tables + static_cast<int64_t>(x.head) * 4 * pitch, bias_bytes(reach), wave, NW, lane);
+  issue(0, kt, bits);
+  q.load(a.q.p + x.b * a.q.sb + x.head * a.q.sh + x.row0 * a.q.sl, a.q.sl, a.dh, a.Lq - x.row0, lane);
 
   f32x16 o[D / 32];
 #pragma unroll
@@ -341,30 +369,18 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void fwd_kernel(Args a, C
   float m_run = kLowest, l_run = 0.0f;
   constexpr float kRoom = headroom<BF>();
 
-  uint64_t bits = 0;
-  int byte = 0;
-  if (kt < end) {
-    bits = keybits.word(kt, keybits.load(kt));
-    issue(0, kt, bits);
-    byte = keybits.load(kt + 1);
-  }
-  wait_vmcnt<0>();
-  __syncthreads();
-  if constexpr (BIAS) {
-    far_behind = table[0];
-    far_ahead = table[2 * reach + 16];
-  }
-
   // kMode 0: all 64 keys are seen by all of the wave's queries and the bias is one value (`bc`); 1: all are seen, the bias
   // by distance; 2: whatever is seen, the bias by distance.
-  auto compute = [&](int stage, int kt, float bc, auto mode) __attribute__((always_inline)) {
+  auto compute = [&](int stage, float bc, auto mode) __attribute__((always_inline)) {
     constexpr int kMode = decltype(mode)::value;
     constexpr bool kNear = BIAS && kMode > 0;
     uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
+    const int pos = x.start + x.row0 + c;
     f32x16 sc[2] = {f32x16{}, f32x16{}};
 #pragma unroll
     for (int i = 0; i < 2 * (D / 16); ++i) sc[i / (D / 16)] = mfma<BF>(rows.read(ks, i / (D / 16), i % (D / 16)), q.f[i % (D / 16)], sc[i / (D / 16)]);
     if constexpr (kNear) {
+      const float *table = reinterpret_cast<const float *>(tables);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -423,87 +439,108 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 2 : 1) void fwd_kernel(Args a, C
     for (int i = 0; i < D / 8; ++i)
       o[i / 4] = mfma<BF>(cols.read(vs, i / 4, (i / 2) % 2, i % 2), pb[(i / 2) % 2][i % 2], o[i / 4]);
   };
+
   auto step = [&](int stage) __attribute__((always_inline)) {
-    const uint64_t bits_next = keybits.word(kt + 1, byte);
-    if (kt + 1 < end) issue(stage ^ 1, kt + 1, bits_next);
-    byte = keybits.load(kt + 2);
-    const int key0 = kt * kRows;
+    uint64_t bits_next = 0;
+    if (kt + 1 < x.end) {
+      bits_next = keybits.word(kt + 1, byte);
+      issue(stage ^ 1, kt + 1, bits_next);
+      byte = keybits.load(kt + 2);
+    }
+    const int key0 = kt * kRows, first = x.start + x.row0;
     if (bits && !(a.causal && key0 > first + 31)) {
       const bool all = bits == ~0ull && !(a.causal && key0 + kRows - 1 > first);
       bool one = !BIAS;  // the bias is one value
       float bc = 0.0f;
       if constexpr (BIAS) {
+        const float *table = reinterpret_cast<const float *>(tables);
         if (key0 + kRows - 1 - first <= -reach) {
           one = true;
-          bc = far_behind;
+          bc = table[0];
         } else if (key0 - first - 31 >= (a.bias.ahead ? reach : 0)) {
           one = true;
-          bc = far_ahead;
+          bc = table[2 * reach + 16];
         }
       }
-      if (!all) compute(stage, kt, 0.0f, std::integral_constant<int, 2>{});
-      else if (one) compute(stage, kt, bc, std::integral_constant<int, 0>{});
-      else if constexpr (BIAS) compute(stage, kt, 0.0f, std::integral_constant<int, 1>{});
+      if (!all) compute(stage, 0.0f, std::integral_constant<int, 2>{});
+      else if (one) compute(stage, bc, std::integral_constant<int, 0>{});
+      else if constexpr (BIAS) compute(stage, 0.0f, std::integral_constant<int, 1>{});
     }
     bits = bits_next;
     wait_vmcnt<0>();
-    __syncthreads();
+    __syncthreads();  // the next tile has landed for every wave, and no wave reads this stage any more
   };
-  while (kt < end) {
+  wait_vmcnt<0>();
+  __syncthreads();
+  while (true) {
     step(0);
-    if (++kt >= end) break;
+    if (++kt >= x.end) break;
     step(1);
-    ++kt;
+    if (++kt >= x.end) break;
   }
 
-  const float l_all = pair_sum(l_run);
-  if (cut.parts > 1) {
-    float *w = cut.partial + (static_cast<int64_t>(t) * NW + wave) * partial_floats(D);
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-      *reinterpret_cast<float4 *>(w + (i * 64 + lane) * 4) =
-          make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
-    *reinterpret_cast<float2 *>(w + 32 * D + 2 * lane) = make_float2(m_run, l_all);
-    return;
-  }
-  const int row = row0 + c;
-  if (row >= a.Lq) return;
-  const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
-  uint16_t *orow = a.out + b * a.out_sb + row * a.out_sl + head * a.dh;
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) {
-    const int ch = 8 * i + 4 * h;
-    const f32x16 &x = o[i >> 2];
-    const int e = 4 * (i & 3);
-    if (8 * i < a.dh)
-      *reinterpret_cast<uint2 *>(orow + ch) =
-          make_uint2(pack<BF>(materialize(x[e] * inv), materialize(x[e + 1] * inv)),
-                     pack<BF>(materialize(x[e + 2] * inv), materialize(x[e + 3] * inv)));
-  }
-  if (a.lse && h == 0)
-    a.lse[(static_cast<int64_t>(b) * a.H + head) * a.Lq + row] = (m_run + __builtin_log2f(l_all)) * kLn2;
+  // The result: divided by the sums, or as it is where the keys are in parts.
+      const float l_all = pair_sum(l_run);
+      const int row = x.row0 + c;
+      if (cut.parts > 1) {
+        float *w = cut.partial + (static_cast<int64_t>(t) * NW + wave) * partial_floats(D);
+  #pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<float4 *>(w + (i * 64 + lane) * 4) =
+              make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
+        *reinterpret_cast<float2 *>(w + 32 * D + 2 * lane) = make_float2(m_run, l_all);
+      } else {
+        const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
+        if (a.lse && h == 0 && row < a.Lq)
+          a.lse[(static_cast<int64_t>(x.b) * a.H + x.head) * a.Lq + row] = (m_run + __builtin_log2f(l_all)) * kLn2;
+        const int rows = min(a.Lq - x.row0, 32);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(a.out + x.b * a.out_sb + x.row0 * a.out_sl + x.head * a.dh,
+                                                   rows > 0 ? 2 * ((rows - 1) * static_cast<uint32_t>(a.out_sl) + a.dh) : 0);
+        const uint32_t at = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(2 * a.out_sl);
+        // Lanes c and c + 32 hold the halves of 8 channels: they exchange halves, and each stores 8 channels of row c.
+        // What does not exist is out of the buffer's range.
+  #pragma unroll
+        for (int i = 0; i < D / 8; i += 2) {
+          uint32_t w[2][2];
+  #pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const f32x16 &z = o[i >> 2];
+            const int e = 4 * (i & 3) + 2 * u;
+            const auto p = __builtin_amdgcn_permlane32_swap(pack<BF>(materialize(z[e] * inv), materialize(z[e + 1] * inv)),
+                                                            pack<BF>(materialize(z[e + 4] * inv), materialize(z[e + 5] * inv)), false, false);
+            w[0][u] = p[0];
+            w[1][u] = p[1];
+          }
+          typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+          const int ch = 8 * (i + h);
+          __builtin_amdgcn_raw_buffer_store_b128(u32x4{w[0][0], w[0][1], w[1][0], w[1][1]}, r, ch < a.dh ? at + 2 * ch : kPast, 0, 0);
+        }
+      }
 }
 
-// The parts of fwd_kernel, joined in key order: a wave per 32 queries and 32 channels, in the lane order of that kernel.
+// The parts of fwd_kernel, joined: a workgroup per 32 queries and 32 channels, whose four waves take parts in turn, in the lane
+// order of that kernel.
 template <bool BF, int D>
-__global__ __launch_bounds__(64) void merge_kernel(Args a, Cut cut, int nw) {
-  const int lane = threadIdx.x, db = blockIdx.x % (D / 32);
+__global__ __launch_bounds__(256) void merge_kernel(Args a, Cut cut, int nw) {
+  __shared__ float4 so[4][4][64];
+  __shared__ float2 sm[4][64];
+  const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6, db = blockIdx.x % (D / 32);
   int rest = blockIdx.x / (D / 32);
-  const int wave = rest % nw;
-  rest /= nw;
-  const int qt0 = rest % cut.qtiles;
-  rest /= cut.qtiles;
+  const int qb = rest % cut.qblocks;
+  rest /= cut.qblocks;
   const int head = rest % a.H, b = rest / a.H, hk = head / a.group, g = head - hk * a.group;
-  const int qt = a.causal ? cut.qtiles - 1 - qt0 : qt0;
-  const int row = (qt * nw + wave) * 32 + (lane & 31);
-  const int64_t item = ((static_cast<int64_t>(b) * a.Hk + hk) * cut.parts * a.group + g) * cut.qtiles + qt0;
-  const int64_t step = static_cast<int64_t>(a.group) * cut.qtiles * nw * partial_floats(D);  // from one part to the next
+  const int block = cut.pack ? g * cut.qblocks + qb : qb, tile = block / nw, wave = block - tile * nw;
+  const int tile0 = a.causal ? cut.tiles - 1 - tile : tile;
+  const int heads = cut.pack ? 1 : a.group;
+  const int64_t bhk = static_cast<int64_t>(b) * a.Hk + hk;
+  const int64_t item = cut.pack ? bhk * cut.parts * cut.tiles + tile0 : (bhk * cut.parts * a.group + g) * cut.tiles + tile0;
+  const int64_t step = static_cast<int64_t>(heads) * cut.tiles * nw * partial_floats(D);  // from one part to the next
   const float *w = cut.partial + (item * nw + wave) * partial_floats(D);
-  if (row >= a.Lq) return;
   float m = kLowest, l = 0.0f;
-  for (int p = 0; p < cut.parts; ++p) m = fmaxf(m, w[p * step + 32 * D + 2 * lane]);
+  for (int p = sub; p < cut.parts; p += 4) m = fmaxf(m, w[p * step + 32 * D + 2 * lane]);
   float4 o[4] = {};
-  for (int p = 0; p < cut.parts; ++p) {
+#pragma unroll 2
+  for (int p = sub; p < cut.parts; p += 4) {
     const float2 ml = *reinterpret_cast<const float2 *>(w + p * step + 32 * D + 2 * lane);
     const float f = __builtin_amdgcn_exp2f(ml.x - m);
     l += f * ml.y;
@@ -516,17 +553,34 @@ __global__ __launch_bounds__(64) void merge_kernel(Args a, Cut cut, int nw) {
       o[i].w += f * x.w;
     }
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t *orow = a.out + b * a.out_sb + row * a.out_sl + head * a.dh;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int ch = 32 * db + 8 * i;
-    if (ch < a.dh)
-      *reinterpret_cast<uint2 *>(orow + ch + 4 * (lane >> 5)) =
-          make_uint2(pack<BF>(materialize(o[i].x * inv), materialize(o[i].y * inv)),
-                     pack<BF>(materialize(o[i].z * inv), materialize(o[i].w * inv)));
+  for (int i = 0; i < 4; ++i) so[sub][i][lane] = o[i];
+  sm[sub][lane] = make_float2(m, l);
+  __syncthreads();
+  // Wave `sub` joins the channels 8 sub .. + 8.
+  float2 ml[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) ml[j] = sm[j][lane];
+  m = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+  l = 0.0f;
+  float4 x = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
+    const float4 z = so[j][sub][lane];
+    l += f * ml[j].y;
+    x.x += f * z.x;
+    x.y += f * z.y;
+    x.z += f * z.z;
+    x.w += f * z.w;
   }
-  if (a.lse && db == 0 && lane < 32)
+  const int row = 32 * qb + (lane & 31), ch = 32 * db + 8 * sub;
+  if (row >= a.Lq) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (ch < a.dh)
+    *reinterpret_cast<uint2 *>(a.out + b * a.out_sb + row * a.out_sl + head * a.dh + ch + 4 * (lane >> 5)) =
+        make_uint2(pack<BF>(materialize(x.x * inv), materialize(x.y * inv)), pack<BF>(materialize(x.z * inv), materialize(x.w * inv)));
+  if (a.lse && db == 0 && sub == 0 && lane < 32)
     a.lse[(static_cast<int64_t>(b) * a.H + head) * a.Lq + row] = (m + __builtin_log2f(l)) * kLn2;
 }
 
@@ -685,6 +739,7 @@ int check_args(const char *what, const selas_text_attention_problem *p, int dtyp
   if (p->o_sb < 0 || p->o_sl < 0 || p->mask_sb < 0) return set_error(SELAS_EINVAL, "%s: negative stride", what);
   if (!aligned(p->out, 8) || p->o_sb % 4 || p->o_sl % 4)
     return set_error(SELAS_EUNSUPPORTED, "%s: out must be 8-byte aligned with strides of whole 8 bytes", what);
+  if (p->o_sl > (1 << 23)) return set_error(SELAS_EUNSUPPORTED, "%s: out has a row stride above 2^23 elements", what);
   a.out = static_cast<uint16_t *>(p->out);
   a.out_sb = p->o_sb;
   a.out_sl = p->o_sl;
@@ -695,14 +750,16 @@ namespace {
 
 struct Plan {
   int few = 0;  // rows held by the few-row kernel, 0: tiles
-  int D, nw, parts, qtiles;
-  int64_t bytes = 0;  // workspace
+  int D, nw;
+  Cut cut{};
+  int few_parts;
+  int64_t partial = 0, tables = 0, bytes = 0;  // offsets into the workspace, its size
 };
 
 Plan plan_of(const Args &a) {
   Plan p{};
   p.D = a.dh <= 64 ? 64 : 128;
-  const int cu = cu_count();
+  const int64_t cu = cu_count();
   const int64_t rows = static_cast<int64_t>(a.group) * a.Lq, items = static_cast<int64_t>(a.B) * a.Hk;
   if (rows <= 8) {
     p.few = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
@@ -710,36 +767,50 @@ Plan plan_of(const Args &a) {
     const int unit = (p.few <= 2 ? 8 : 4) * (512 / p.D);
     const int64_t units = cdiv(a.Lk, unit);
     // Parts for two workgroups a CU, of four units a wave at least.
-    p.parts = static_cast<int>(std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(items, 1), units / (4 * p.nw))));
-    if (p.parts > 1) p.bytes = items * p.parts * p.few * (p.D + 2) * 4;
+    p.few_parts = static_cast<int>(std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(items, 1), units / (4 * p.nw))));
+    if (p.few_parts > 1) p.bytes = items * p.few_parts * p.few * (p.D + 2) * 4;
     return p;
   }
-  p.nw = a.Lq <= 32 ? 1 : a.Lq <= 64 ? 2 : 4;
-  p.qtiles = static_cast<int>(cdiv(a.Lq, 32 * p.nw));
-  const int64_t whole = static_cast<int64_t>(a.B) * a.H * p.qtiles, tiles = cdiv(a.Lk, kRows);
-  // Workgroups for two to a CU, of four tiles at least.
-  const int64_t room = 2 * cu * (4 / p.nw);
-  p.parts = static_cast<int>(std::max<int64_t>(1, std::min(room / std::max<int64_t>(whole, 1), tiles / 4)));
-  if (p.parts > 1) p.bytes = whole * p.parts * p.nw * partial_floats(p.D) * 4;
+  Cut &c = p.cut;
+  c.qblocks = static_cast<int>(cdiv(a.Lq, 32));
+  c.pack = a.group > 1 && !a.causal && !a.bias.table;
+  const int64_t blocks = c.pack ? static_cast<int64_t>(a.group) * c.qblocks : c.qblocks;
+  p.nw = blocks <= 1 ? 1 : blocks <= 2 ? 2 : 4;
+  c.tiles = static_cast<int>(cdiv(blocks, p.nw));
+  // Workgroups that are resident at once: two to a CU, of one or two waves with narrow heads four.
+  const int64_t resident = cu * (p.D == 128 ? 2 : p.nw < 4 ? 4 : 3);
+  const int64_t whole = items * (c.pack ? 1 : a.group) * c.tiles, tiles = cdiv(a.Lk, kRows);
+  // Parts where items are too few to fill the CUs, of four tiles at least.
+  c.parts = static_cast<int>(std::max<int64_t>(1, std::min(resident / std::max<int64_t>(whole, 1), tiles / 4)));
+  c.total = static_cast<int>(whole * c.parts);
+  c.per_xcd = static_cast<int>(cdiv(c.total, 8));
+  auto take = [&](int64_t bytes) {
+    const int64_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  if (c.parts > 1) p.partial = take(static_cast<int64_t>(c.total) * p.nw * partial_floats(p.D) * 4);
+  if (a.bias.table) p.tables = take(static_cast<int64_t>(a.H) * bias_bytes(a.bias.reach));
   return p;
 }
 
 template <bool BF, int D, int R, bool BIAS>
 void launch_few(const Args &a, const Plan &p, float *ws, hipStream_t st) {
-  const int items = a.B * a.Hk;
+  const int items = a.B * a.Hk, parts = p.few_parts;
   const size_t lds = BIAS ? static_cast<size_t>(a.group) * (2 * a.bias.reach + 1) * 4 : 0;
-  few_kernel<BF, D, R, 8, BIAS><<<dim3(items * p.parts), dim3(512), lds, st>>>(a, p.parts, ws);
-  if (p.parts > 1) few_merge_kernel<BF><<<dim3(items * a.group * a.Lq), dim3(128), 0, st>>>(a, p.parts, D, R, ws);
+  few_kernel<BF, D, R, 8, BIAS><<<dim3(items * parts), dim3(512), lds, st>>>(a, parts, ws);
+  if (parts > 1) few_merge_kernel<BF><<<dim3(items * a.group * a.Lq), dim3(128), 0, st>>>(a, parts, D, R, ws);
 }
 
 template <bool BF, int D, int NW, bool BIAS>
 void launch_tiles(const Args &a, const Plan &p, float *ws, hipStream_t st) {
-  Cut cut{p.qtiles, p.parts, a.B * a.H * p.qtiles * p.parts, 0, ws};
-  cut.per_xcd = (cut.total + 7) / 8;
-  const size_t lds = BIAS ? bias_bytes(a.bias.reach) : 0;
-  fwd_kernel<BF, D, NW, BIAS><<<dim3(8 * cut.per_xcd), dim3(64 * NW), lds, st>>>(a, cut);
-  if (p.parts > 1)
-    merge_kernel<BF, D><<<dim3(a.B * a.H * p.qtiles * NW * (D / 32)), dim3(64), 0, st>>>(a, cut, NW);
+  Cut cut = p.cut;
+  cut.partial = ws + p.partial / 4;
+  cut.tables = ws + p.tables / 4;
+  if constexpr (BIAS) launch_bias(a.bias, a.H, 1, cut.tables, st);
+  fwd_kernel<BF, D, NW, BIAS><<<dim3(8 * cut.per_xcd), dim3(64 * NW), BIAS ? bias_lds(a.bias.reach) : 0, st>>>(a, cut);
+  if (cut.parts > 1)
+    merge_kernel<BF, D><<<dim3(a.B * a.H * cut.qblocks * (D / 32)), dim3(256), 0, st>>>(a, cut, NW);
 }
 
 template <bool BF, int D, bool BIAS>

@@ -30,6 +30,7 @@ struct Grads {
   float *neg_lse, *dot;    // [B, H, Lqp]: -lse log2(e) (-inf for rows that see nothing and rows past Lq), D (0 there)
   int Lqp, qblocks, kblocks;  // rows padded to whole tiles; tiles of queries, of keys
   float *g_norm, *v_norm;  // fp16: largest squared norms of the rows of dO and v, per tile
+  float *tables;           // bias by distance, [2 (by key - query, by query - key)][H][4 bias_pitch]
   float *dtable_part;      // [B, H, qtiles * parts, buckets]
   void *dtable;
 };
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
   using T = Tile<D>;
   constexpr int KJ = T::kLoads / NW, kStats = 2 * kRows * 4;
   __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes + kStats], smem1[2 * T::kBytes + kStats];
-  extern __shared__ __attribute__((aligned(16))) float table[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t tables[];  // two heads' bias by distance
   const int t = item_of(cut.per_xcd);
   if (t >= cut.total) return;
   const int tile = t % cut.tiles, part = t / cut.tiles % cut.parts, bhk = t / cut.tiles / cut.parts;
@@ -184,6 +185,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
     }
   };
   const int reach = a.bias.reach, pitch = bias_pitch(reach);
+  auto load_table = [&](int g) {  // the heads of the group take the two buffers in turn
+    load_bytes(tables + (g & 1) * bias_lds(reach), w.tables + static_cast<int64_t>(a.H + hk * a.group + g) * 4 * pitch,
+               bias_bytes(reach), wave, NW, lane);
+  };
   const float shift = ds_shift<BF>(a, w, b, hk, lane);
   const float ds_mul = BF ? 1.0f : __builtin_exp2f(shift - kProbShift);
 
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
   for (int db = 0; db < D / 32; ++db) dk[db] = dv[db] = f32x16{};
 
   // kMode as in the forward pass: 0 one value of the bias and no mask, 1 by distance, 2 by distance and causal.
-  auto compute = [&](int stage, int qt, float bc, auto mode) __attribute__((always_inline)) {
+  auto compute = [&](int stage, int qt, const float *table, float bc, auto mode) __attribute__((always_inline)) {
     constexpr int kMode = decltype(mode)::value;
     constexpr bool kNear = BIAS && kMode > 0;
     uint8_t *qs = stage ? smem1 : smem0, *gs = qs + T::kBytes;
@@ -241,28 +246,24 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
     }
   };
 
-  if (i < end) issue(0, g, qt);
-  float far_behind = 0.0f, far_ahead = 0.0f;
-  bool build = true;  // the table of a head that begins
+  if (i < end) {
+    if constexpr (BIAS) load_table(g);
+    issue(0, g, qt);
+  }
   auto step = [&](int stage) __attribute__((always_inline)) {
     wait_vmcnt<0>();
-    __syncthreads();  // this tile has landed for all waves, and the other stage and the table are no longer read
-    if constexpr (BIAS) {
-      if (build) {
-        build_bias(table, a.bias, hk * a.group + g, threadIdx.x, 64 * NW, true);
-        __syncthreads();
-        far_ahead = table[0];
-        far_behind = table[2 * reach + 16];
-      }
-    }
+    __syncthreads();  // this tile has landed for every wave, and no wave reads the other stage any more
     const int at = qt;
-    build = false;
+    const float *table = reinterpret_cast<const float *>(tables + (g & 1) * bias_lds(reach));
     if (++qt == w.qblocks) {
       qt = qt0;
       ++g;
-      build = true;
     }
-    if (i + 1 < end) issue(stage ^ 1, g, qt);
+    if (i + 1 < end) {
+      if constexpr (BIAS)
+        if (qt == qt0) load_table(g);
+      issue(stage ^ 1, g, qt);
+    }
     const int pos0 = start + at * kRows;
     if (key0 < keys && !(a.causal && pos0 + kRows - 1 < key0)) {
       bool one = !BIAS;
@@ -270,15 +271,15 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
       if constexpr (BIAS) {
         if (key0 + 31 - pos0 <= -reach) {
           one = true;
-          bc = far_behind;
+          bc = table[2 * reach + 16];
         } else if (key0 - (pos0 + kRows - 1) >= (a.bias.ahead ? reach : 0)) {
           one = true;
-          bc = far_ahead;
+          bc = table[0];
         }
       }
-      if (a.causal && pos0 < key0 + 31) compute(stage, at, 0.0f, std::integral_constant<int, 2>{});
-      else if (one) compute(stage, at, bc, std::integral_constant<int, 0>{});
-      else if constexpr (BIAS) compute(stage, at, 0.0f, std::integral_constant<int, 1>{});
+      if (a.causal && pos0 < key0 + 31) compute(stage, at, table, 0.0f, std::integral_constant<int, 2>{});
+      else if (one) compute(stage, at, table, bc, std::integral_constant<int, 0>{});
+      else if constexpr (BIAS) compute(stage, at, table, 0.0f, std::integral_constant<int, 1>{});
     }
   };
   while (i < end) {
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
   using T = Tile<D>;
   constexpr int KJ = T::kLoads / NW;
   __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
-  extern __shared__ __attribute__((aligned(16))) float table[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t dynamic[];
   const int t = item_of(cut.per_xcd);
   if (t >= cut.total) return;
   int rest = t;
@@ -416,11 +417,12 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
   };
 
   const int reach = a.bias.reach, pitch = bias_pitch(reach), span = hist_floats(reach);
-  float *hist = table + 4 * pitch;  // [2 NW][span]; after that [NW][2] sums
+  const float *table = reinterpret_cast<const float *>(dynamic);
+  float *hist = reinterpret_cast<float *>(dynamic + bias_lds(reach));  // [2 NW][span]; after that [NW][2] sums
   float *mine = hist + (2 * wave + h) * span;
   float sum_behind = 0.0f, sum_ahead = 0.0f, far_behind = 0.0f, far_ahead = 0.0f;
   if constexpr (BIAS) {
-    build_bias(table, a.bias, head, threadIdx.x, 64 * NW, false);
+    load_bytes(dynamic, w.tables + static_cast<int64_t>(head) * 4 * pitch, bias_bytes(reach), wave, NW, lane);
     for (int i = threadIdx.x; i < 2 * NW * span; i += 64 * NW) hist[i] = 0.0f;
   }
   const float shift = ds_shift<BF>(a, w, b, hk, lane), ds_mul = BF ? 1.0f : __builtin_exp2f(shift);
@@ -628,7 +630,7 @@ __global__ __launch_bounds__(256) void dtable_kernel(const float *__restrict__ p
 struct Plan {
   int D, qblocks, kblocks, buckets;
   Cut key, query;
-  int64_t neg_lse, dot, g_norm, v_norm, dtable, key_partial, query_partial, bytes;  // offsets into the workspace
+  int64_t neg_lse, dot, g_norm, v_norm, tables, dtable, key_partial, query_partial, bytes;  // offsets into the workspace
 };
 constexpr int kNW = 4;
 
@@ -659,6 +661,7 @@ Plan plan_of(const Args &a, bool bf) {
     p.g_norm = take(static_cast<int64_t>(a.B) * a.H * p.qblocks);
     p.v_norm = take(static_cast<int64_t>(a.B) * a.Hk * p.kblocks);
   }
+  if (a.bias.table) p.tables = take(2ll * a.H * 4 * bias_pitch(a.bias.reach));
   if (a.bias.table) p.dtable = take(static_cast<int64_t>(a.B) * a.H * p.query.tiles * p.query.parts * p.buckets);
   if (p.key.parts > 1) p.key_partial = take(2ll * p.key.parts * a.B * a.Hk * a.Lk * a.dh);
   if (p.query.parts > 1) p.query_partial = take(static_cast<int64_t>(p.query.parts) * a.B * a.H * a.Lq * a.dh);
@@ -670,15 +673,16 @@ void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
   const int row_blocks = a.B * a.H * p.qblocks + (BF ? 0 : a.B * a.Hk * p.kblocks);
   if (row_blocks) row_kernel<BF><<<dim3(row_blocks), dim3(256), 0, st>>>(a, w);
   const int reach = a.bias.reach;
+  if constexpr (BIAS) launch_bias(a.bias, a.H, 2, w.tables, st);
   if (p.key.total) {
-    key_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.key.per_xcd), dim3(64 * kNW), BIAS ? bias_bytes(reach) : 0, st>>>(a, w, p.key);
+    key_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.key.per_xcd), dim3(64 * kNW), BIAS ? 2 * bias_lds(reach) : 0, st>>>(a, w, p.key);
     if (p.key.parts > 1) {
       const int64_t n = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.dh;
       sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(n, 1024)), 2), dim3(256), 0, st>>>(p.key.partial, p.key.parts, n, 2, w.dk, w.dv);
     }
   }
   if (p.query.total) {
-    const size_t lds = BIAS ? bias_bytes(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
+    const size_t lds = BIAS ? bias_lds(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
     query_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.query.per_xcd), dim3(64 * kNW), lds, st>>>(a, w, p.query);
     if (p.query.parts > 1) {
       const int64_t n = static_cast<int64_t>(a.B) * a.H * a.Lq * a.dh;
@@ -741,6 +745,7 @@ extern "C" int selas_text_attention_backward(const selas_text_attention_problem 
   w.kblocks = p.kblocks;
   w.g_norm = at(p.g_norm);
   w.v_norm = at(p.v_norm);
+  w.tables = at(p.tables);
   w.dtable_part = at(p.dtable);
   w.dtable = dtable;
   p.key.partial = at(p.key_partial);
