@@ -27,6 +27,7 @@ struct Side {
 struct Bias {
   const void *table;  // [buckets, H], unit column stride; null: no bias
   int64_t row;
+  float inv_scale;  // 1 / scale
   int dtype, n, ahead, reach;
   int edge[kMaxSide];  // from n on: beyond every distance
 };
@@ -46,6 +47,13 @@ struct Args {
   Bias bias;
 };
 
+// The arguments of a kernel whose first is an Args, read again where they are used: what is needed only after a loop holds no
+// scalar registers in it.
+__device__ __forceinline__ const Args &args_here() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args *)p;
+}
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Keys of image b; the position of its first query. Both are uniform (scalar loads: a vector load's wait would also wait
@@ -112,7 +120,8 @@ __device__ __forceinline__ float pair_sum(float v) {
 
 // ------------------------------------------------------------------ the bias by distance
 
-// The table of head `head` as a function of distance d = key - query, times log2(e). Beyond `reach` it is constant, so
+// The table of head `head` as a function of distance d = key - query, divided by the scale, so that it is added to the
+// products of queries and keys. Beyond `reach` it is constant, so
 // d in [-reach - 8, reach + 8] is all of it: runs of 8 distances starting anywhere are entries of it once their start is
 // clamped to [-reach - 8, reach + 1]. Lanes read runs of 4 distances that start anywhere, in one 16-byte read each: copy c
 // (of 4) begins c entries later, so that a run starting at i is aligned in copy i % 4. The copies are `bias_pitch` floats
@@ -129,12 +138,12 @@ __device__ __forceinline__ int bucket_of(const Bias &t, int d) {
   return r;
 }
 
-__device__ __forceinline__ float bias_at(const Bias &t, int head, int d) {
+__device__ __forceinline__ float bias_at(const Bias &t, int head, int d, float mul) {
   const int64_t i = bucket_of(t, d) * t.row + head;
   const float v = t.dtype == SELAS_F32   ? load_f<SELAS_F32>(t.table, i)
                   : t.dtype == SELAS_F16 ? load_f<SELAS_F16>(t.table, i)
                                          : load_f<SELAS_BF16>(t.table, i);
-  return v * kLog2e;
+  return v * mul;
 }
 
 // The four copies of a head's table, by a thread per distance, into global memory: workgroups then only copy them to LDS.
@@ -142,7 +151,7 @@ __device__ __forceinline__ float bias_at(const Bias &t, int head, int d) {
 __device__ __forceinline__ void write_bias(float *out, const Bias &t, int head, int i, bool reversed) {
   const int pitch = bias_pitch(t.reach), d = i - t.reach - 8;
   if (i >= 2 * t.reach + 17) return;
-  const float v = bias_at(t, head, reversed ? -d : d);
+  const float v = bias_at(t, head, reversed ? -d : d, t.inv_scale);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     if (i >= c) out[c * pitch + i - c] = v;

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(Args a, int parts, float *
   if constexpr (BIAS) {
     for (int i = threadIdx.x; i < a.group * span; i += 64 * NW) {
       const int g = i / span;
-      table[i] = bias_at(a.bias, hk * a.group + g, i - g * span - reach);
+      table[i] = bias_at(a.bias, hk * a.group + g, i - g * span - reach, kLog2e);
     }
     __syncthreads();
   }
@@ -369,17 +369,14 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
   float m_run = kLowest, l_run = 0.0f;
   constexpr float kRoom = headroom<BF>();
 
-  // kMode 0: all 64 keys are seen by all of the wave's queries and the bias is one value (`bc`); 1: all are seen, the bias
-  // by distance; 2: whatever is seen, the bias by distance.
-  auto compute = [&](int stage, float bc, auto mode) __attribute__((always_inline)) {
-    constexpr int kMode = decltype(mode)::value;
-    constexpr bool kNear = BIAS && kMode > 0;
+  // One tile. near: the bias differs among its scores (otherwise it is `bc`, times log2(e), for all); part: some are not seen.
+  auto compute = [&](int stage, float bc, bool near, bool part) __attribute__((always_inline)) {
     uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
     const int pos = x.start + x.row0 + c;
     f32x16 sc[2] = {f32x16{}, f32x16{}};
 #pragma unroll
     for (int i = 0; i < 2 * (D / 16); ++i) sc[i / (D / 16)] = mfma<BF>(rows.read(ks, i / (D / 16), i % (D / 16)), q.f[i % (D / 16)], sc[i / (D / 16)]);
-    if constexpr (kNear) {
+    if (BIAS && near) {
       const float *table = reinterpret_cast<const float *>(tables);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -388,10 +385,10 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
           float bv[8];
           bias_run(table, pitch, reach, kt * kRows + 32 * kb + 16 * t2 + 8 * h - pos, bv);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sc[kb][8 * t2 + e] = __builtin_fmaf(sc[kb][8 * t2 + e], a.c2, bv[e]);
+          for (int e = 0; e < 8; ++e) sc[kb][8 * t2 + e] += bv[e];
         }
     }
-    if constexpr (kMode == 2) {
+    if (part) {
       const uint64_t seen = (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h);
       const uint32_t w[2] = {static_cast<uint32_t>(seen), static_cast<uint32_t>(seen >> 32)};
 #pragma unroll
@@ -405,8 +402,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kb][r]);
-    mx = pair_max(mx);
-    if constexpr (!kNear) mx = __builtin_fmaf(mx, a.c2, bc);
+    mx = __builtin_fmaf(pair_max(mx), a.c2, bc);
     const bool raise = mx - kRoom > m_run + 8.0f;
     if (__builtin_amdgcn_ballot_w64(raise)) {
       const float to = mx - kRoom, alpha = raise ? __builtin_amdgcn_exp2f(m_run - to) : 1.0f;
@@ -415,7 +411,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
       l_run *= alpha;
       m_run = raise ? to : m_run;
     }
-    const float sub = kNear ? m_run : m_run - bc;
+    const float sub = m_run - bc;
     float ls = 0.0f;
     uint4 pb[2][2];
 #pragma unroll
@@ -426,7 +422,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           auto prob = [&](float s) {
-            return materialize(__builtin_amdgcn_exp2f(kNear ? s - sub : __builtin_fmaf(s, a.c2, -sub)));
+            return materialize(__builtin_amdgcn_exp2f(__builtin_fmaf(s, a.c2, -sub)));
           };
           const float p0 = prob(sc[kb][8 * t2 + 2 * e]), p1 = prob(sc[kb][8 * t2 + 2 * e + 1]);
           ls += p0 + p1;
@@ -450,21 +446,15 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
     const int key0 = kt * kRows, first = x.start + x.row0;
     if (bits && !(a.causal && key0 > first + 31)) {
       const bool all = bits == ~0ull && !(a.causal && key0 + kRows - 1 > first);
-      bool one = !BIAS;  // the bias is one value
+      bool near = BIAS;
       float bc = 0.0f;
       if constexpr (BIAS) {
         const float *table = reinterpret_cast<const float *>(tables);
-        if (key0 + kRows - 1 - first <= -reach) {
-          one = true;
-          bc = table[0];
-        } else if (key0 - first - 31 >= (a.bias.ahead ? reach : 0)) {
-          one = true;
-          bc = table[2 * reach + 16];
-        }
+        const bool behind = key0 + kRows - 1 - first <= -reach, ahead = key0 - first - 31 >= (a.bias.ahead ? reach : 0);
+        near = !behind && !ahead;
+        if (!near) bc = table[behind ? 0 : 2 * reach + 16] * a.c2;
       }
-      if (!all) compute(stage, 0.0f, std::integral_constant<int, 2>{});
-      else if (one) compute(stage, bc, std::integral_constant<int, 0>{});
-      else if constexpr (BIAS) compute(stage, 0.0f, std::integral_constant<int, 1>{});
+      compute(stage, bc, near, !all);
     }
     bits = bits_next;
     wait_vmcnt<0>();
@@ -480,6 +470,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
   }
 
   // The result: divided by the sums, or as it is where the keys are in parts.
+  const Args &e = args_here();
       const float l_all = pair_sum(l_run);
       const int row = x.row0 + c;
       if (cut.parts > 1) {
@@ -491,12 +482,12 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
         *reinterpret_cast<float2 *>(w + 32 * D + 2 * lane) = make_float2(m_run, l_all);
       } else {
         const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
-        if (a.lse && h == 0 && row < a.Lq)
-          a.lse[(static_cast<int64_t>(x.b) * a.H + x.head) * a.Lq + row] = (m_run + __builtin_log2f(l_all)) * kLn2;
-        const int rows = min(a.Lq - x.row0, 32);
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(a.out + x.b * a.out_sb + x.row0 * a.out_sl + x.head * a.dh,
-                                                   rows > 0 ? 2 * ((rows - 1) * static_cast<uint32_t>(a.out_sl) + a.dh) : 0);
-        const uint32_t at = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(2 * a.out_sl);
+        if (e.lse && h == 0 && row < e.Lq)
+          e.lse[(static_cast<int64_t>(x.b) * e.H + x.head) * e.Lq + row] = (m_run + __builtin_log2f(l_all)) * kLn2;
+        const int rows = min(e.Lq - x.row0, 32);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(e.out + x.b * e.out_sb + x.row0 * e.out_sl + x.head * e.dh,
+                                                   rows > 0 ? 2 * ((rows - 1) * static_cast<uint32_t>(e.out_sl) + e.dh) : 0);
+        const uint32_t at = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(2 * e.out_sl);
         // Lanes c and c + 32 hold the halves of 8 channels: they exchange halves, and each stores 8 channels of row c.
         // What does not exist is out of the buffer's range.
   #pragma unroll
@@ -505,15 +496,15 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
   #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const f32x16 &z = o[i >> 2];
-            const int e = 4 * (i & 3) + 2 * u;
-            const auto p = __builtin_amdgcn_permlane32_swap(pack<BF>(materialize(z[e] * inv), materialize(z[e + 1] * inv)),
-                                                            pack<BF>(materialize(z[e + 4] * inv), materialize(z[e + 5] * inv)), false, false);
+            const int y = 4 * (i & 3) + 2 * u;
+            const auto p = __builtin_amdgcn_permlane32_swap(pack<BF>(materialize(z[y] * inv), materialize(z[y + 1] * inv)),
+                                                            pack<BF>(materialize(z[y + 4] * inv), materialize(z[y + 5] * inv)), false, false);
             w[0][u] = p[0];
             w[1][u] = p[1];
           }
           typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
           const int ch = 8 * (i + h);
-          __builtin_amdgcn_raw_buffer_store_b128(u32x4{w[0][0], w[0][1], w[1][0], w[1][1]}, r, ch < a.dh ? at + 2 * ch : kPast, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(u32x4{w[0][0], w[0][1], w[1][0], w[1][1]}, r, ch < e.dh ? at + 2 * ch : kPast, 0, 0);
         }
       }
 }
@@ -695,8 +686,8 @@ int check_args(const char *what, const selas_text_attention_problem *p, int dtyp
     return set_error(SELAS_EINVAL, "%s: %lld heads do not share %lld key heads evenly", what, (long long)p->H, (long long)p->Hk);
   if (!valid_dtype(dtype)) return set_error(SELAS_EINVAL, "%s: bad dtype %d", what, dtype);
   if (p->reserved != 0) return set_error(SELAS_EINVAL, "%s: reserved must be 0", what);
-  if (!(p->scale >= 1e-30 && p->scale <= 1e30))
-    return set_error(SELAS_EINVAL, "%s: scale %g is outside 1e-30 .. 1e30", what, p->scale);
+  if (!(p->scale >= 1e-10 && p->scale <= 1e10))
+    return set_error(SELAS_EINVAL, "%s: scale %g is outside 1e-10 .. 1e10", what, p->scale);
   if (p->table && !valid_dtype(p->table_dtype)) return set_error(SELAS_EINVAL, "%s: bad table dtype %d", what, p->table_dtype);
   if (dtype == SELAS_F32 || p->Dh % 8 || p->Dh > 128)
     return set_error(SELAS_EUNSUPPORTED, "%s: takes bf16 or fp16 and head dims of whole 8 up to 128 (got %s, %lld)", what,
@@ -712,6 +703,7 @@ int check_args(const char *what, const selas_text_attention_problem *p, int dtyp
     a.bias.reach = a.bias.edge[a.bias.n - 1];
     a.bias.row = p->table_sl;
     a.bias.table = p->table;
+    a.bias.inv_scale = static_cast<float>(1.0 / p->scale);
     if (p->table_sl < 0) return set_error(SELAS_EINVAL, "%s: the table has a negative stride", what);
   }
   a.B = static_cast<int>(p->B);

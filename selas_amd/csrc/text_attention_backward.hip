@@ -196,10 +196,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
 #pragma unroll
   for (int db = 0; db < D / 32; ++db) dk[db] = dv[db] = f32x16{};
 
-  // kMode as in the forward pass: 0 one value of the bias and no mask, 1 by distance, 2 by distance and causal.
-  auto compute = [&](int stage, int qt, const float *table, float bc, auto mode) __attribute__((always_inline)) {
-    constexpr int kMode = decltype(mode)::value;
-    constexpr bool kNear = BIAS && kMode > 0;
+  // One tile; near and part as in the forward pass.
+  auto compute = [&](int stage, int qt, const float *table, float bc, bool near, bool part) __attribute__((always_inline)) {
     uint8_t *qs = stage ? smem1 : smem0, *gs = qs + T::kBytes;
     const float *stats = reinterpret_cast<const float *>(qs + 2 * T::kBytes);
     const int pos0 = start + qt * kRows;  // of the tile's first query
@@ -210,13 +208,24 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
       for (int x = 0; x < D / 16; ++x) s = mfma<BF>(rows.read(qs, qb, x), k.f[x], s);
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) dp = mfma<BF>(rows.read(gs, qb, x), v.f[x], dp);
+      if (BIAS && near) {
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+          float bv[8];
+          bias_run(table, pitch, reach, pos0 + 32 * qb + 16 * t2 + 8 * h - key, bv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[8 * t2 + e] += bv[e];
+        }
+      }
+      if (part) {
+        const uint32_t seen = static_cast<uint32_t>(~up_to(key - pos0 - 32 * qb - 8 * h - 1));  // queries at or after the key
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = (seen >> (16 * (r >> 3) + (r & 7))) & 1 ? s[r] : -__builtin_inff();
+      }
       uint4 pb[2], sb[2];
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
         const int at = 32 * qb + 16 * t2 + 8 * h;  // the first of this lane's 8 queries
-        float bv[8];
-        if constexpr (kNear) bias_run(table, pitch, reach, pos0 + at - key, bv);
-        const uint32_t seen = kMode == 2 ? static_cast<uint32_t>(~up_to(key - pos0 - at - 1)) : 0;  // queries at or after the key
         float p[8], ds[8];
 #pragma unroll
         for (int e4 = 0; e4 < 2; ++e4) {
@@ -225,10 +234,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             const int e = 4 * e4 + y, r = 8 * t2 + e;
-            float x = __builtin_fmaf(s[r], a.c2, nl[y] + prob_shift<BF>());
-            if constexpr (kNear) x += bv[e];
-            else if constexpr (BIAS) x += bc;
-            if constexpr (kMode == 2) x = (seen >> e) & 1 ? x : -__builtin_inff();
+            const float x = __builtin_fmaf(s[r], a.c2, BIAS || !BF ? nl[y] + bc : nl[y]);
             p[e] = materialize(__builtin_amdgcn_exp2f(x));
             ds[e] = materialize(p[e] * (dp[r] - dd[y]) * ds_mul);
           }
@@ -266,20 +272,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
     }
     const int pos0 = start + at * kRows;
     if (key0 < keys && !(a.causal && pos0 + kRows - 1 < key0)) {
-      bool one = !BIAS;
-      float bc = 0.0f;
+      bool near = BIAS;
+      float bc = prob_shift<BF>();
       if constexpr (BIAS) {
-        if (key0 + 31 - pos0 <= -reach) {
-          one = true;
-          bc = table[2 * reach + 16];
-        } else if (key0 - (pos0 + kRows - 1) >= (a.bias.ahead ? reach : 0)) {
-          one = true;
-          bc = table[0];
-        }
+        const bool behind = key0 + 31 - pos0 <= -reach, ahead = key0 - (pos0 + kRows - 1) >= (a.bias.ahead ? reach : 0);
+        near = !behind && !ahead;
+        if (!near) bc += table[behind ? 2 * reach + 16 : 0] * a.c2;
       }
-      if (a.causal && pos0 < key0 + 31) compute(stage, at, table, 0.0f, std::integral_constant<int, 2>{});
-      else if (one) compute(stage, at, table, bc, std::integral_constant<int, 0>{});
-      else if constexpr (BIAS) compute(stage, at, table, 0.0f, std::integral_constant<int, 1>{});
+      compute(stage, at, table, bc, near, a.causal && pos0 < key0 + 31);
     }
   };
   while (i < end) {
@@ -440,17 +440,15 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
   wait_vmcnt<0>();
   __syncthreads();
   if constexpr (BIAS) {
-    far_behind = table[0];
-    far_ahead = table[2 * reach + 16];
+    far_behind = table[0] * a.c2;
+    far_ahead = table[2 * reach + 16] * a.c2;
   }
 
-  // kMode 0: all keys seen, one value of the bias; 1: all seen, bias by distance; 2 and 3: whatever is seen, one value / by
-  // distance.
-  auto compute = [&](int stage, int kt, float bc, auto mode) __attribute__((always_inline)) {
-    constexpr int kMode = decltype(mode)::value;
-    constexpr bool kNear = BIAS && (kMode & 1), kPart = kMode >= 2;
+  // One tile; near and part as in the forward pass, near at compile time for the sums along the diagonals.
+  auto compute = [&](int stage, int kt, float bc, bool part, auto mode) __attribute__((always_inline)) {
+    constexpr bool kNear = decltype(mode)::value;
     uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
-    const uint64_t seen = kPart ? (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h) : 0;
+    const uint64_t seen = part ? (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h) : 0;
     const float base = nl + bc;
     float add = 0.0f;
     Diagonals diagonals;
@@ -462,20 +460,27 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
       for (int x = 0; x < D / 16; ++x) s = mfma<BF>(rows.read(ks, kb, x), q.f[x], s);
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) dp = mfma<BF>(rows.read(vs, kb, x), dO.f[x], dp);
+      if constexpr (kNear) {
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+          float bv[8];
+          bias_run(table, pitch, reach, kt * kRows + 32 * kb + 16 * t2 + 8 * h - pos, bv);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[8 * t2 + e] += bv[e];
+        }
+      }
+      if (part) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = (word >> (16 * (r >> 3) + (r & 7))) & 1 ? s[r] : -__builtin_inff();
+      }
       uint4 sb[2];
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
-        const int d = kt * kRows + 32 * kb + 16 * t2 + 8 * h - pos;  // distance of this lane's first key
-        float bv[8];
-        if constexpr (kNear) bias_run(table, pitch, reach, d, bv);
         float ds[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int r = 8 * t2 + e;
-          float x = __builtin_fmaf(s[r], a.c2, base);
-          if constexpr (kNear) x += bv[e];
-          if constexpr (kPart) x = (word >> (16 * t2 + e)) & 1 ? x : -__builtin_inff();
-          ds[e] = materialize(__builtin_amdgcn_exp2f(x) * (dp[r] - dd));
+          ds[e] = materialize(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, base)) * (dp[r] - dd));
           if constexpr (BIAS && !kNear) add += ds[e];
         }
         if constexpr (kNear) diagonals.add(2 * kb + t2, ds, lane);
@@ -501,15 +506,9 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
       const bool all = bits == ~0ull && !(a.causal && key0 + kRows - 1 > first);
       const bool behind = BIAS && key0 + kRows - 1 - first <= -reach;
       const bool ahead = BIAS && !behind && key0 - first - 31 >= (a.bias.ahead ? reach : 0);
-      const float bc = behind ? far_behind : far_ahead;
       float add = 0.0f;
-      if (!BIAS || behind || ahead) {
-        if (all) add = compute(stage, kt, bc, std::integral_constant<int, 0>{});
-        else add = compute(stage, kt, bc, std::integral_constant<int, 2>{});
-      } else if constexpr (BIAS) {
-        if (all) compute(stage, kt, 0.0f, std::integral_constant<int, 1>{});
-        else compute(stage, kt, 0.0f, std::integral_constant<int, 3>{});
-      }
+      if (!BIAS || behind || ahead) add = compute(stage, kt, behind ? far_behind : far_ahead, !all, std::false_type{});
+      else if constexpr (BIAS) compute(stage, kt, 0.0f, !all, std::true_type{});
       sum_behind += behind ? add : 0.0f;
       sum_ahead += behind ? 0.0f : add;
     }
