@@ -142,7 +142,7 @@ __device__ __forceinline__ float ds_shift(const Args &a, const Grads &w, int b, 
 // registers. A key's column depends on nothing of the other keys, so masked keys need no select: their results are zeroed at
 // the end.
 template <bool BF, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, Grads w, Cut cut) {
+__global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cut) {
   using T = Tile<D>;
   constexpr int KJ = T::kLoads / NW, kStats = 2 * kRows * 4;
   __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes + kStats], smem1[2 * T::kBytes + kStats];
@@ -222,7 +222,6 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = (seen >> (16 * (r >> 3) + (r & 7))) & 1 ? s[r] : -__builtin_inff();
       }
-      uint4 pb[2], sb[2];
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
         const int at = 32 * qb + 16 * t2 + 8 * h;  // the first of this lane's 8 queries
@@ -239,16 +238,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
             ds[e] = materialize(p[e] * (dp[r] - dd[y]) * ds_mul);
           }
         }
-        pb[t2] = make_uint4(pack<BF>(p[0], p[1]), pack<BF>(p[2], p[3]), pack<BF>(p[4], p[5]), pack<BF>(p[6], p[7]));
-        sb[t2] = make_uint4(pack<BF>(ds[0], ds[1]), pack<BF>(ds[2], ds[3]), pack<BF>(ds[4], ds[5]), pack<BF>(ds[6], ds[7]));
-      }
-#pragma unroll
-      for (int t2 = 0; t2 < 2; ++t2)
+        const uint4 pb = make_uint4(pack<BF>(p[0], p[1]), pack<BF>(p[2], p[3]), pack<BF>(p[4], p[5]), pack<BF>(p[6], p[7]));
+        const uint4 sb = make_uint4(pack<BF>(ds[0], ds[1]), pack<BF>(ds[2], ds[3]), pack<BF>(ds[4], ds[5]), pack<BF>(ds[6], ds[7]));
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) {
-          dv[db] = mfma<BF>(cols.read(gs, db, qb, t2), pb[t2], dv[db]);
-          dk[db] = mfma<BF>(cols.read(qs, db, qb, t2), sb[t2], dk[db]);
+          dv[db] = mfma<BF>(cols.read(gs, db, qb, t2), pb, dv[db]);
+          dk[db] = mfma<BF>(cols.read(qs, db, qb, t2), sb, dk[db]);
         }
+      }
     }
   };
 
@@ -289,20 +286,21 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
     ++i;
   }
 
-  if (key >= a.Lk) return;
-  const float k_mul = a.c2 * kLn2 * (BF ? 1.0f : __builtin_exp2f(-shift)), v_mul = BF ? 1.0f : __builtin_exp2f(-kProbShift);
-  const int64_t at = (static_cast<int64_t>(bhk) * a.Lk + key) * a.dh, all = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.dh;
+  const Args &e = args_here();
+  if (key >= e.Lk) return;
+  const float k_mul = e.c2 * kLn2 * (BF ? 1.0f : __builtin_exp2f(-shift)), v_mul = BF ? 1.0f : __builtin_exp2f(-kProbShift);
+  const int64_t at = (static_cast<int64_t>(bhk) * e.Lk + key) * e.dh, all = static_cast<int64_t>(e.B) * e.Hk * e.Lk * e.dh;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const int ch = 32 * db + 8 * y + 4 * h;
-      if (32 * db + 8 * y >= a.dh) continue;
+      if (32 * db + 8 * y >= e.dh) continue;
       float x[4], z[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = materialize(valid ? dk[db][4 * y + e] * k_mul : 0.0f);
-        z[e] = materialize(valid ? dv[db][4 * y + e] * v_mul : 0.0f);
+      for (int i = 0; i < 4; ++i) {
+        x[i] = materialize(valid ? dk[db][4 * y + i] * k_mul : 0.0f);
+        z[i] = materialize(valid ? dv[db][4 * y + i] * v_mul : 0.0f);
       }
       if (cut.parts > 1) {
         float *p = cut.partial + 2 * part * all + at + ch;
@@ -329,45 +327,40 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 2 : 1) void key_kernel(Args a, G
 constexpr int kSpill = 112;
 __host__ __device__ inline int hist_floats(int reach) { return 2 * reach + 2 * kSpill + 1; }
 
-// Sums along the diagonals of a wave's 64 keys x 32 queries. v[e] of lane q belongs to distance o + e - q. With
+// Sums along the diagonals of a wave's 32 keys x 32 queries. v[e] of lane q belongs to distance o + e - q. With
 // t_e[p] = v[e][p] + t_{e+1}[p + 1], the lanes' indices modulo 16, t_0[p] holds distance o - p and, from the lanes below e
 // that wrapped, o + 16 - p; the latter are summed apart and belong to the next 16 keys' first part.
 struct Diagonals {
-  float u[5] = {};  // u[m] of lane q: distance d0 + 16 m of that lane
+  float u[3] = {};  // u[m] of lane q: distance d0 + 16 m of that lane
   __device__ __forceinline__ static float next_lane(float v) {  // row_ror:15
     return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x12F, 0xF, 0xF, false));
   }
-  __device__ __forceinline__ void add(int m, const float (&v)[8], int lane) {
+  __device__ __forceinline__ void add(int m, const f32x16 &v, int lane) {  // the m-th 8 of v
     const int p = lane & 15;
-    float all = v[7], low = p < 7 ? v[7] : 0.0f;
+    float all = v[8 * m + 7], low = p < 7 ? all : 0.0f;
 #pragma unroll
     for (int e = 6; e >= 0; --e) {
-      all = v[e] + next_lane(all);
+      all = v[8 * m + e] + next_lane(all);
       low = next_lane(low);
-      if (e) low += p < e ? v[e] : 0.0f;
+      if (e) low += p < e ? v[8 * m + e] : 0.0f;
     }
     u[m] += all - low;
     u[m + 1] += low;
   }
-  // u[m + 1] of the lanes 16 .. 31 meets u[m] of the lanes 0 .. 15: first the even ones, then the odd ones. LDS
-  // instructions of a wave are in order.
+  // u[m + 1] of the lanes 16 .. 31 meets u[m] of the lanes 0 .. 15: first the even ones, then the odd one. LDS instructions
+  // of a wave are in order.
   __device__ __forceinline__ void store(float *at) const {
-    float x[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) x[i] = at[32 * i];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) at[32 * i] = x[i] + u[2 * i];
+    const float x = at[0], y = at[32];
+    at[0] = x + u[0];
+    at[32] = y + u[2];
     asm volatile("" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] = at[32 * i + 16];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) at[32 * i + 16] = x[i] + u[2 * i + 1];
+    at[16] += u[1];
     asm volatile("" ::: "memory");
   }
 };
 
 template <bool BF, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut cut) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a, Grads w, Cut cut) {
   using T = Tile<D>;
   constexpr int KJ = T::kLoads / NW;
   __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
@@ -444,14 +437,12 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
     far_ahead = table[2 * reach + 16] * a.c2;
   }
 
-  // One tile; near and part as in the forward pass, near at compile time for the sums along the diagonals.
-  auto compute = [&](int stage, int kt, float bc, bool part, auto mode) __attribute__((always_inline)) {
-    constexpr bool kNear = decltype(mode)::value;
+  // One tile; near and part as in the forward pass. Returns the sum of dS where the bias is one value.
+  auto compute = [&](int stage, int kt, float bc, bool near, bool part) __attribute__((always_inline)) {
     uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
     const uint64_t seen = part ? (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h) : 0;
     const float base = nl + bc;
     float add = 0.0f;
-    Diagonals diagonals;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       const uint32_t word = static_cast<uint32_t>(kb ? seen >> 32 : seen);
@@ -460,7 +451,7 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
       for (int x = 0; x < D / 16; ++x) s = mfma<BF>(rows.read(ks, kb, x), q.f[x], s);
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) dp = mfma<BF>(rows.read(vs, kb, x), dO.f[x], dp);
-      if constexpr (kNear) {
+      if (BIAS && near) {
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
           float bv[8];
@@ -473,20 +464,24 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = (word >> (16 * (r >> 3) + (r & 7))) & 1 ? s[r] : -__builtin_inff();
       }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[r] = materialize(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, base)) * (dp[r] - dd));  // dS from here on
+      if (BIAS && near) {
+        Diagonals diagonals;
+        diagonals.add(0, s, lane);
+        diagonals.add(1, s, lane);
+        diagonals.store(mine + kt * kRows + 32 * kb + 8 * h - pos + reach + kSpill);
+      } else if (BIAS) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) add += s[r];
+      }
       uint4 sb[2];
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2) {
         float ds[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int r = 8 * t2 + e;
-          ds[e] = materialize(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, base)) * (dp[r] - dd));
-          if constexpr (BIAS && !kNear) add += ds[e];
-        }
-        if constexpr (kNear) diagonals.add(2 * kb + t2, ds, lane);
-        if constexpr (!BF)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ds[e] = materialize(ds[e] * ds_mul);
+        for (int e = 0; e < 8; ++e) ds[e] = BF ? s[8 * t2 + e] : materialize(s[8 * t2 + e] * ds_mul);
         sb[t2] = make_uint4(pack<BF>(ds[0], ds[1]), pack<BF>(ds[2], ds[3]), pack<BF>(ds[4], ds[5]), pack<BF>(ds[6], ds[7]));
       }
 #pragma unroll
@@ -494,7 +489,6 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) dq[db] = mfma<BF>(cols.read(ks, db, kb, t2), sb[t2], dq[db]);
     }
-    if constexpr (kNear) diagonals.store(mine + kt * kRows + 8 * h - pos + reach + kSpill);
     return add;
   };
   auto step = [&](int stage) __attribute__((always_inline)) {
@@ -506,9 +500,8 @@ __global__ __launch_bounds__(64 * NW, 2) void query_kernel(Args a, Grads w, Cut 
       const bool all = bits == ~0ull && !(a.causal && key0 + kRows - 1 > first);
       const bool behind = BIAS && key0 + kRows - 1 - first <= -reach;
       const bool ahead = BIAS && !behind && key0 - first - 31 >= (a.bias.ahead ? reach : 0);
-      float add = 0.0f;
-      if (!BIAS || behind || ahead) add = compute(stage, kt, behind ? far_behind : far_ahead, !all, std::false_type{});
-      else if constexpr (BIAS) compute(stage, kt, 0.0f, !all, std::true_type{});
+      const float bc = behind ? far_behind : ahead ? far_ahead : 0.0f;
+      const float add = compute(stage, kt, bc, !behind && !ahead, !all);
       sum_behind += behind ? add : 0.0f;
       sum_ahead += behind ? 0.0f : add;
     }
