@@ -2,10 +2,10 @@
 //   D_i = dO_i . out_i,  dP_ij = dO_i . v_j,  dS_ij = p_ij (dP_ij - D_i)
 //   dv_j = sum_i p_ij dO_i,  dk_j = scale sum_i dS_ij q_i,  dq_i = scale sum_j dS_ij k_j,  dtable[r, h] = sum of dS_ij over
 //   the pairs in bucket r; dk and dv sum over the query heads that share the key head.
-// p is formed again from q, k and the forward pass's lse. Three kernels: row_kernel leaves D and lse per row; key_kernel has
-// the keys as owners and streams queries past them (dk, dv); query_kernel has the queries as owners and streams keys (dq,
-// dtable). S and dP are formed in both: 7 products where one kernel would need 5 and floating-point atomics, whose order
-// would change the bits from call to call.
+// p is formed again from q, k and the forward pass's lse. Two kernels: query_kernel has the queries as owners and streams keys
+// past them (dq, dtable; it also leaves lse and D per row), then key_kernel has the keys as owners and streams queries (dk,
+// dv). S and dP are formed in both: 7 products where one kernel would need 5 and floating-point atomics, whose order would
+// change the bits from call to call.
 #include <algorithm>
 #include <type_traits>
 
@@ -41,76 +41,44 @@ struct Cut {
   float *partial;
 };
 
-// D and lse of 64 rows, 4 lanes to a row. fp16: the tiles' largest norms of dO, and (blocks past the queries') of v.
-template <bool BF>
-__global__ __launch_bounds__(256) void row_kernel(Args a, Grads w) {
-  const int lane = threadIdx.x & 63, r = threadIdx.x >> 2, part = threadIdx.x & 3;
-  int t = blockIdx.x;
+// fp16: the largest squared norm among 64 rows of dO, or (blocks past the queries') of 64 values; 4 lanes to a row.
+__global__ __launch_bounds__(256) void norm_kernel(Args a, Grads w) {
   __shared__ float red[4];
-  float norm = 0.0f;
-  float *norm_out;
-  auto add4 = [](float v) {
-    v += __shfl_xor(v, 1, 64);
-    return v + __shfl_xor(v, 2, 64);
-  };
-  if (t < a.B * a.H * w.qblocks) {
-    const int qt = t % w.qblocks, bh = t / w.qblocks, b = bh / a.H, head = bh - b * a.H;
-    const int row = qt * kRows + r;
-    norm_out = w.g_norm + t;
-    float dot = 0.0f;
-    if (row < a.Lq) {
-      const uint16_t *g = w.g.p + b * w.g.sb + head * w.g.sh + row * w.g.sl;
-      const uint16_t *o = a.out + b * a.out_sb + row * a.out_sl + head * a.dh;
-      for (int ch = 8 * part; ch < a.dh; ch += 32) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(g + ch);
-        const uint2 y0 = *reinterpret_cast<const uint2 *>(o + ch), y1 = *reinterpret_cast<const uint2 *>(o + ch + 4);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y0.x, y0.y, y1.x, y1.y};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float lo = lo_of<BF>(xs[e]), hi = hi_of<BF>(xs[e]);
-          dot = __builtin_fmaf(lo, lo_of<BF>(ys[e]), dot);
-          dot = __builtin_fmaf(hi, hi_of<BF>(ys[e]), dot);
-          norm = __builtin_fmaf(lo, lo, norm);
-          norm = __builtin_fmaf(hi, hi, norm);
-        }
-      }
-    }
-    dot = add4(dot);
-    norm = add4(norm);
-    if (part == 0) {
-      const int64_t at = static_cast<int64_t>(bh) * w.Lqp + row;
-      const float lse = row < a.Lq ? a.lse[static_cast<int64_t>(bh) * a.Lq + row] : -__builtin_inff();
-      const bool none = lse == -__builtin_inff();
-      w.neg_lse[at] = none ? lse : -lse * kLog2e;
-      w.dot[at] = none ? 0.0f : dot;
-    }
+  const int lane = threadIdx.x & 63, r = threadIdx.x >> 2, part = threadIdx.x & 3;
+  const int queries = a.B * a.H * w.qblocks;
+  int t = blockIdx.x;
+  const uint16_t *p = nullptr;
+  float *out;
+  if (t < queries) {
+    const int qt = t % w.qblocks, bh = t / w.qblocks, b = bh / a.H, row = qt * kRows + r;
+    out = w.g_norm + t;
+    if (row < a.Lq) p = w.g.p + b * w.g.sb + (bh - b * a.H) * w.g.sh + row * w.g.sl;
   } else {
-    t -= a.B * a.H * w.qblocks;
-    const int kt = t % w.kblocks, bh = t / w.kblocks, b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int row = kt * kRows + r;
-    norm_out = w.v_norm + t;
-    if (row < keys_of(a, b) && (!a.mask || a.mask[b * a.mask_sb + row])) {
-      const uint16_t *v = a.v.p + b * a.v.sb + hk * a.v.sh + row * a.v.sl;
-      for (int ch = 8 * part; ch < a.dh; ch += 32) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(v + ch);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+    t -= queries;
+    const int kt = t % w.kblocks, bh = t / w.kblocks, b = bh / a.Hk, row = kt * kRows + r;
+    out = w.v_norm + t;
+    if (row < keys_of(a, b) && (!a.mask || a.mask[b * a.mask_sb + row]))
+      p = a.v.p + b * a.v.sb + (bh - b * a.Hk) * a.v.sh + row * a.v.sl;
+  }
+  float norm = 0.0f;
+  if (p)
+    for (int ch = 8 * part; ch < a.dh; ch += 32) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(p + ch);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float lo = lo_of<BF>(xs[e]), hi = hi_of<BF>(xs[e]);
-          norm = __builtin_fmaf(lo, lo, norm);
-          norm = __builtin_fmaf(hi, hi, norm);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float lo = lo_of<false>(xs[e]), hi = hi_of<false>(xs[e]);
+        norm = __builtin_fmaf(lo, lo, norm);
+        norm = __builtin_fmaf(hi, hi, norm);
       }
     }
-    norm = add4(norm);
-  }
-  if constexpr (!BF) {
+  norm += __shfl_xor(norm, 1, 64);
+  norm += __shfl_xor(norm, 2, 64);
 #pragma unroll
-    for (int o = 4; o < 64; o <<= 1) norm = fmaxf(norm, __shfl_xor(norm, o, 64));
-    if (lane == 0) red[threadIdx.x >> 6] = norm;
-    __syncthreads();
-    if (threadIdx.x == 0) *norm_out = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  }
+  for (int o = 4; o < 64; o <<= 1) norm = fmaxf(norm, __shfl_xor(norm, o, 64));
+  if (lane == 0) red[threadIdx.x >> 6] = norm;
+  __syncthreads();
+  if (threadIdx.x == 0) *out = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
 // log2 of the factor that dS of image b and key head hk is stored with.
@@ -324,7 +292,12 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
 // left, a value per lane and 16 distances, is added to a histogram by distance in LDS, one for each half of each wave. It
 // covers every distance that such a tile can hold (kSpill past `reach` on either side). At the end the histograms are summed
 // by bucket, and by dtable_kernel over workgroups.
-constexpr int kSpill = 112;
+//
+// D is first the product of dO and out in the order of the matrix unit, as dP is: where a row sees one key, out is that key's
+// value and dS is exactly 0. But out was rounded, and where few keys carry a row, D's share of that is as large as the
+// roundings of dS and of the result. So rows that see up to 64 kRefine keys add what the sum of p (dP - D) over all their
+// keys says is missing, by a pass over those tiles ahead of the others.
+constexpr int kSpill = 112, kRefine = 4;
 __host__ __device__ inline int hist_floats(int reach) { return 2 * reach + 2 * kSpill + 1; }
 
 // Sums along the diagonals of a wave's 32 keys x 32 queries. v[e] of lane q belongs to distance o + e - q. With
@@ -388,9 +361,24 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   Held<D> q, dO;
   q.load(a.q.p + b * a.q.sb + head * a.q.sh + row0 * a.q.sl, a.q.sl, a.dh, a.Lq - row0, lane);
   dO.load(w.g.p + b * w.g.sb + head * w.g.sh + row0 * w.g.sl, w.g.sl, a.dh, a.Lq - row0, lane);
-  const bool here = row0 + c < a.Lq;
-  const int64_t stat = (static_cast<int64_t>(b) * a.H + head) * w.Lqp + row0 + c;
-  const float nl = here ? w.neg_lse[stat] : -__builtin_inff(), dd = here ? w.dot[stat] : 0.0f;
+  float nl = -__builtin_inff(), dd;
+  if (row0 + c < a.Lq) {
+    nl = a.lse[(static_cast<int64_t>(b) * a.H + head) * a.Lq + row0 + c];
+    nl = nl == -__builtin_inff() ? nl : -nl * kLog2e;
+  }
+  {
+    Held<D> out;
+    out.load(a.out + b * a.out_sb + row0 * a.out_sl + head * a.dh, a.out_sl, a.dh, a.Lq - row0, lane);
+    f32x16 x = f32x16{};
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) x = mfma<BF>(out.f[s], dO.f[s], x);
+    // Row c of column c: register 4 (c / 8) + c % 4 of the lanes of half (c / 4) % 2.
+    float d = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) d = r == 4 * (c >> 3) + (c & 3) ? x[r] : d;
+    dd = pair_sum(h == ((c >> 2) & 1) ? d : 0.0f);
+    if (nl == -__builtin_inff()) dd = 0.0f;
+  }
   const uint16_t *kp = a.k.p + b * a.k.sb + hk * a.k.sh, *vp = a.v.p + b * a.v.sb + hk * a.v.sh;
   const typename T::template Loader<KJ> kl(wave, lane, a.k.sl, a.dh), vl(wave, lane, a.v.sl, a.dh);
   const typename T::RowReader rows(lane);
@@ -425,48 +413,56 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   for (int db = 0; db < D / 32; ++db) dq[db] = f32x16{};
   uint64_t bits = 0;
   int byte = 0;
-  if (kt < end) {
-    bits = keybits.word(kt, keybits.load(kt));
-    issue(0, kt, bits);
-    byte = keybits.load(kt + 1);
-  }
-  wait_vmcnt<0>();
-  __syncthreads();
-  if constexpr (BIAS) {
-    far_behind = table[0] * a.c2;
-    far_ahead = table[2 * reach + 16] * a.c2;
-  }
-
-  // One tile; near and part as in the forward pass. Returns the sum of dS where the bias is one value.
-  auto compute = [&](int stage, int kt, float bc, bool near, bool part) __attribute__((always_inline)) {
-    uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
-    const uint64_t seen = part ? (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h) : 0;
-    const float base = nl + bc;
+  // What is known of a tile ahead of its scores: whether any are needed, whether some are not seen, where the bias is one value.
+  struct Kind {
+    bool any, part, behind, ahead;
+    float bc;
+  };
+  auto kind_of = [&](int kt) __attribute__((always_inline)) {
+    const int key0 = kt * kRows;
+    Kind x;
+    x.any = bits && !(a.causal && key0 > first + 31);
+    x.part = bits != ~0ull || (a.causal && key0 + kRows - 1 > first);
+    x.behind = BIAS && key0 + kRows - 1 - first <= -reach;
+    x.ahead = BIAS && !x.behind && key0 - first - 31 >= (a.bias.ahead ? reach : 0);
+    x.bc = x.behind ? far_behind : x.ahead ? far_ahead : 0.0f;
+    return x;
+  };
+  // dS of 32 keys.
+  auto scores = [&](const uint8_t *ks, int kt, int kb, const Kind &x) __attribute__((always_inline)) {
+    const uint8_t *vs = ks + T::kBytes;
+    f32x16 s = f32x16{}, dp = f32x16{};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) s = mfma<BF>(rows.read(ks, kb, i), q.f[i], s);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) dp = mfma<BF>(rows.read(vs, kb, i), dO.f[i], dp);
+    if (BIAS && !x.behind && !x.ahead) {
+#pragma unroll
+      for (int t2 = 0; t2 < 2; ++t2) {
+        float bv[8];
+        bias_run(table, pitch, reach, kt * kRows + 32 * kb + 16 * t2 + 8 * h - pos, bv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[8 * t2 + e] += bv[e];
+      }
+    }
+    if (x.part) {
+      const uint64_t seen = (a.causal ? bits & up_to(pos - kt * kRows) : bits) >> (8 * h);
+      const uint32_t word = static_cast<uint32_t>(kb ? seen >> 32 : seen);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = (word >> (16 * (r >> 3) + (r & 7))) & 1 ? s[r] : -__builtin_inff();
+    }
+    const float base = nl + x.bc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = materialize(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, base)) * (dp[r] - dd));
+    return s;
+  };
+  auto compute = [&](int stage, int kt, const Kind &x) __attribute__((always_inline)) {
+    uint8_t *ks = stage ? smem1 : smem0;
     float add = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const uint32_t word = static_cast<uint32_t>(kb ? seen >> 32 : seen);
-      f32x16 s = f32x16{}, dp = f32x16{};
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) s = mfma<BF>(rows.read(ks, kb, x), q.f[x], s);
-#pragma unroll
-      for (int x = 0; x < D / 16; ++x) dp = mfma<BF>(rows.read(vs, kb, x), dO.f[x], dp);
-      if (BIAS && near) {
-#pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2) {
-          float bv[8];
-          bias_run(table, pitch, reach, kt * kRows + 32 * kb + 16 * t2 + 8 * h - pos, bv);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s[8 * t2 + e] += bv[e];
-        }
-      }
-      if (part) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = (word >> (16 * (r >> 3) + (r & 7))) & 1 ? s[r] : -__builtin_inff();
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[r] = materialize(__builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c2, base)) * (dp[r] - dd));  // dS from here on
+      const f32x16 s = scores(ks, kt, kb, x);
+      const bool near = !x.behind && !x.ahead;
       if (BIAS && near) {
         Diagonals diagonals;
         diagonals.add(0, s, lane);
@@ -489,26 +485,51 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) dq[db] = mfma<BF>(cols.read(ks, db, kb, t2), sb[t2], dq[db]);
     }
-    return add;
+    sum_behind += x.behind ? add : 0.0f;
+    sum_ahead += x.behind ? 0.0f : add;
   };
   auto step = [&](int stage) __attribute__((always_inline)) {
     const uint64_t bits_next = keybits.word(kt + 1, byte);
     if (kt + 1 < end) issue(stage ^ 1, kt + 1, bits_next);
     byte = keybits.load(kt + 2);
-    const int key0 = kt * kRows;
-    if (bits && !(a.causal && key0 > first + 31)) {
-      const bool all = bits == ~0ull && !(a.causal && key0 + kRows - 1 > first);
-      const bool behind = BIAS && key0 + kRows - 1 - first <= -reach;
-      const bool ahead = BIAS && !behind && key0 - first - 31 >= (a.bias.ahead ? reach : 0);
-      const float bc = behind ? far_behind : ahead ? far_ahead : 0.0f;
-      const float add = compute(stage, kt, bc, !behind && !ahead, !all);
-      sum_behind += behind ? add : 0.0f;
-      sum_ahead += behind ? 0.0f : add;
-    }
+    const Kind x = kind_of(kt);
+    if (x.any) compute(stage, kt, x);
     bits = bits_next;
     wait_vmcnt<0>();
     __syncthreads();
   };
+  auto begin = [&](int kt) {
+    bits = keybits.word(kt, keybits.load(kt));
+    issue(0, kt, bits);
+    byte = keybits.load(kt + 1);
+    wait_vmcnt<0>();
+    __syncthreads();
+    if constexpr (BIAS) {
+      far_behind = table[0] * a.c2;
+      far_ahead = table[2 * reach + 16] * a.c2;
+    }
+  };
+  if (ntiles <= kRefine) {
+    float missing = 0.0f;
+    for (int i = 0; i < ntiles; ++i) {
+      begin(i);
+      const Kind x = kind_of(i);
+      if (x.any)
+        for (int kb = 0; kb < 2; ++kb) {
+          const f32x16 s = scores(smem0, i, kb, x);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) missing += s[r];
+        }
+      __syncthreads();
+    }
+    dd += pair_sum(missing);
+  }
+  if (part == 0 && h == 0 && row0 + c < w.Lqp) {  // for key_kernel
+    const int64_t at = (static_cast<int64_t>(b) * a.H + head) * w.Lqp + row0 + c;
+    w.neg_lse[at] = nl;
+    w.dot[at] = dd;
+  }
+  if (kt < end) begin(kt);
   while (kt < end) {
     step(0);
     if (++kt >= end) break;
@@ -517,6 +538,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   }
 
   if constexpr (BIAS) {
+    wait_vmcnt<0>();  // without keys nothing has waited for the table, whose load must not outlive the workgroup
+    __syncthreads();
     // The histograms added up, then each bucket by one wave.
     float *sums = hist + 2 * NW * span;
     sum_behind = wave_sum(sum_behind);
@@ -662,24 +685,21 @@ Plan plan_of(const Args &a, bool bf) {
 
 template <bool BF, int D, bool BIAS>
 void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
-  const int row_blocks = a.B * a.H * p.qblocks + (BF ? 0 : a.B * a.Hk * p.kblocks);
-  if (row_blocks) row_kernel<BF><<<dim3(row_blocks), dim3(256), 0, st>>>(a, w);
   const int reach = a.bias.reach;
+  auto sum = [&](const Cut &cut, int64_t rows, int arrays, uint16_t *y0, uint16_t *y1) {
+    if (cut.parts > 1)
+      sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(rows * a.dh, 1024)), arrays), dim3(256), 0, st>>>(cut.partial, cut.parts, rows * a.dh, arrays, y0, y1);
+  };
   if constexpr (BIAS) launch_bias(a.bias, a.H, 2, w.tables, st);
-  if (p.key.total) {
-    key_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.key.per_xcd), dim3(64 * kNW), BIAS ? 2 * bias_lds(reach) : 0, st>>>(a, w, p.key);
-    if (p.key.parts > 1) {
-      const int64_t n = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.dh;
-      sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(n, 1024)), 2), dim3(256), 0, st>>>(p.key.partial, p.key.parts, n, 2, w.dk, w.dv);
-    }
-  }
+  if (!BF && p.query.total + p.key.total) norm_kernel<<<dim3(a.B * a.H * p.qblocks + a.B * a.Hk * p.kblocks), dim3(256), 0, st>>>(a, w);
   if (p.query.total) {
     const size_t lds = BIAS ? bias_lds(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
     query_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.query.per_xcd), dim3(64 * kNW), lds, st>>>(a, w, p.query);
-    if (p.query.parts > 1) {
-      const int64_t n = static_cast<int64_t>(a.B) * a.H * a.Lq * a.dh;
-      sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(n, 1024))), dim3(256), 0, st>>>(p.query.partial, p.query.parts, n, 1, w.dq, nullptr);
-    }
+    sum(p.query, static_cast<int64_t>(a.B) * a.H * a.Lq, 1, w.dq, nullptr);
+  }
+  if (p.key.total) {
+    key_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.key.per_xcd), dim3(64 * kNW), BIAS ? 2 * bias_lds(reach) : 0, st>>>(a, w, p.key);
+    sum(p.key, static_cast<int64_t>(a.B) * a.Hk * a.Lk, 2, w.dk, w.dv);
   }
   if constexpr (BIAS)
     dtable_kernel<<<dim3(a.H), dim3(256), 0, st>>>(w.dtable_part, a.B, a.H, p.query.tiles * p.query.parts, p.buckets, w.dtable,
