@@ -276,6 +276,7 @@ struct Cut {
   int qblocks;  // of 32 queries, per head
   int tiles;    // items per head, or per group (pack)
   int parts, pack, total, per_xcd;
+  FastDiv by_tiles, by_group, by_parts, by_hk, by_qblocks;
   float *partial, *tables;  // tables: every head's bias by distance
 };
 constexpr int partial_floats(int D) { return 64 * (D / 2) + 2 * 64; }  // per wave: outputs in register order, maxima, sums
@@ -290,29 +291,25 @@ struct Item {
 
 __device__ __forceinline__ Item item_at(const Args &a, const Cut &cut, int t, int nw, int wave) {
   Item x;
-  const int tile0 = t % cut.tiles;
-  int rest = t / cut.tiles, g = 0;
-  if (!cut.pack) {
-    g = rest % a.group;
-    rest /= a.group;
-  }
-  const int part = rest % cut.parts;
-  rest /= cut.parts;
-  x.hk = rest % a.Hk;
-  x.b = rest / a.Hk;
+  auto split = [](int v, FastDiv by, int d, int &rest) {  // v % d, and rest = v / d
+    rest = static_cast<int>(div31(v, by));
+    return v - rest * d;
+  };
+  int rest, g = 0;
+  const int tile0 = split(t, cut.by_tiles, cut.tiles, rest);
+  if (!cut.pack) g = split(rest, cut.by_group, a.group, rest);
+  const int part = split(rest, cut.by_parts, cut.parts, rest);
+  x.hk = split(rest, cut.by_hk, a.Hk, x.b);
   const int tile = a.causal ? cut.tiles - 1 - tile0 : tile0;  // the longest first
   int block = tile * nw + wave;
-  if (cut.pack) {
-    g = block / cut.qblocks;
-    block -= g * cut.qblocks;
-  }
+  if (cut.pack) block = split(block, cut.by_qblocks, cut.qblocks, g);
   x.row0 = g < a.group ? min(32 * block, a.Lq) : a.Lq;
   x.head = x.hk * a.group + min(g, a.group - 1);
   x.keys = keys_of(a, x.b);
   x.start = start_of(a, x.b);
   int n = (x.keys + kRows - 1) / kRows;
   if (a.causal) n = min(n, max(x.start + min((tile + 1) * nw * 32, a.Lq) + kRows - 1, 0) / kRows);
-  const int per = (n + cut.parts - 1) / cut.parts;
+  const int per = static_cast<int>(div31(n + cut.parts - 1, cut.by_parts));
   x.kt = part * per;
   x.end = max(min(n, x.kt + per), x.kt + 1);  // without keys: one tile of which nothing is seen
   x.kp = a.k.p + x.b * a.k.sb + x.hk * a.k.sh;
@@ -776,6 +773,11 @@ Plan plan_of(const Args &a) {
   c.parts = static_cast<int>(std::max<int64_t>(1, std::min(resident / std::max<int64_t>(whole, 1), tiles / 4)));
   c.total = static_cast<int>(whole * c.parts);
   c.per_xcd = static_cast<int>(cdiv(c.total, 8));
+  c.by_tiles = fast_div(c.tiles);
+  c.by_group = fast_div(a.group);
+  c.by_parts = fast_div(c.parts);
+  c.by_hk = fast_div(a.Hk);
+  c.by_qblocks = fast_div(c.qblocks);
   auto take = [&](int64_t bytes) {
     const int64_t at = p.bytes;
     p.bytes += (bytes + 255) / 256 * 256;
