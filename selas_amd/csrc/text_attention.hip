@@ -468,42 +468,42 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
 
   // The result: divided by the sums, or as it is where the keys are in parts.
   const Args &e = args_here();
-      const float l_all = pair_sum(l_run);
-      const int row = x.row0 + c;
-      if (cut.parts > 1) {
-        float *w = cut.partial + (static_cast<int64_t>(t) * NW + wave) * partial_floats(D);
-  #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<float4 *>(w + (i * 64 + lane) * 4) =
-              make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
-        *reinterpret_cast<float2 *>(w + 32 * D + 2 * lane) = make_float2(m_run, l_all);
-      } else {
-        const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
-        if (e.lse && h == 0 && row < e.Lq)
-          e.lse[(static_cast<int64_t>(x.b) * e.H + x.head) * e.Lq + row] = (m_run + __builtin_log2f(l_all)) * kLn2;
-        const int rows = min(e.Lq - x.row0, 32);
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(e.out + x.b * e.out_sb + x.row0 * e.out_sl + x.head * e.dh,
-                                                   rows > 0 ? 2 * ((rows - 1) * static_cast<uint32_t>(e.out_sl) + e.dh) : 0);
-        const uint32_t at = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(2 * e.out_sl);
-        // Lanes c and c + 32 hold the halves of 8 channels: they exchange halves, and each stores 8 channels of row c.
-        // What does not exist is out of the buffer's range.
-  #pragma unroll
-        for (int i = 0; i < D / 8; i += 2) {
-          uint32_t w[2][2];
-  #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const f32x16 &z = o[i >> 2];
-            const int y = 4 * (i & 3) + 2 * u;
-            const auto p = __builtin_amdgcn_permlane32_swap(pack<BF>(materialize(z[y] * inv), materialize(z[y + 1] * inv)),
-                                                            pack<BF>(materialize(z[y + 4] * inv), materialize(z[y + 5] * inv)), false, false);
-            w[0][u] = p[0];
-            w[1][u] = p[1];
-          }
-          typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-          const int ch = 8 * (i + h);
-          __builtin_amdgcn_raw_buffer_store_b128(u32x4{w[0][0], w[0][1], w[1][0], w[1][1]}, r, ch < e.dh ? at + 2 * ch : kPast, 0, 0);
-        }
+  const float l_all = pair_sum(l_run);
+  const int row = x.row0 + c;
+  if (cut.parts > 1) {
+    float *w = cut.partial + (static_cast<int64_t>(t) * NW + wave) * partial_floats(D);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+      *reinterpret_cast<float4 *>(w + (i * 64 + lane) * 4) =
+          make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
+    *reinterpret_cast<float2 *>(w + 32 * D + 2 * lane) = make_float2(m_run, l_all);
+  } else {
+    const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
+    if (e.lse && h == 0 && row < e.Lq)
+      e.lse[(static_cast<int64_t>(x.b) * e.H + x.head) * e.Lq + row] = (m_run + __builtin_log2f(l_all)) * kLn2;
+    const int rows = min(e.Lq - x.row0, 32);
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(e.out + x.b * e.out_sb + x.row0 * e.out_sl + x.head * e.dh,
+                                               rows > 0 ? 2 * ((rows - 1) * static_cast<uint32_t>(e.out_sl) + e.dh) : 0);
+    const uint32_t at = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(2 * e.out_sl);
+    // Lanes c and c + 32 hold the halves of 8 channels: they exchange halves, and each stores 8 channels of row c.
+    // What does not exist is out of the buffer's range.
+#pragma unroll
+    for (int i = 0; i < D / 8; i += 2) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const f32x16 &z = o[i >> 2];
+        const int y = 4 * (i & 3) + 2 * u;
+        const auto p = __builtin_amdgcn_permlane32_swap(pack<BF>(materialize(z[y] * inv), materialize(z[y + 1] * inv)),
+                                                        pack<BF>(materialize(z[y + 4] * inv), materialize(z[y + 5] * inv)), false, false);
+        w[0][u] = p[0];
+        w[1][u] = p[1];
       }
+      typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+      const int ch = 8 * (i + h);
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{w[0][0], w[0][1], w[1][0], w[1][1]}, r, ch < e.dh ? at + 2 * ch : kPast, 0, 0);
+    }
+  }
 }
 
 // The parts of fwd_kernel, joined: a workgroup per 32 queries and 32 channels, whose four waves take parts in turn, in the lane
