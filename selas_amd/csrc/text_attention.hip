@@ -323,12 +323,14 @@ __device__ __forceinline__ Item item_at(const Args &a, const Cut &cut, int t, in
 // bits 2 and 3 of the row exchanged, so that register r of a lane holds key 16 (r / 8) + 8 h + r % 8 of it, as the second
 // product's operand wants them).
 template <bool BF, int D, int NW, bool BIAS>
-__global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_kernel(Args a, Cut cut) {
+__global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, Cut cut) {
   using T = Tile<D>;
   constexpr int KJ = T::kLoads / NW;
   static_assert(KJ * NW == T::kLoads, "loads per wave");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
-  extern __shared__ __attribute__((aligned(1024))) uint8_t tables[];  // the head's bias by distance
+  constexpr bool kTwo = D == 64;  // two stages of the values as well
+  __shared__ __attribute__((aligned(16))) uint8_t keys0[T::kBytes], keys1[T::kBytes], values0[T::kBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t values1[kTwo ? T::kBytes : 16];
+  extern __shared__ __attribute__((aligned(16))) uint8_t tables[];  // the head's bias by distance
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const int t = item_of(cut.per_xcd);
   if (t >= cut.total) return;
@@ -339,25 +341,27 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
   const typename T::ColReader cols(lane);
   const int reach = a.bias.reach, pitch = bias_pitch(reach);
 
-  auto issue = [&](int stage, int kt, uint64_t bits) __attribute__((always_inline)) {
-    uint8_t *base = stage ? smem1 : smem0;
-    const int64_t key0 = static_cast<int64_t>(kt) * kRows;
+  auto issue_keys = [&](int stage, int kt, uint64_t bits) __attribute__((always_inline)) {
+    uint8_t *to = stage ? keys1 : keys0;
+    const uint16_t *p = x.kp + static_cast<int64_t>(kt) * kRows * a.k.sl;
     const int left = x.keys - kt * kRows;
-    const uint16_t *kp = x.kp + key0 * a.k.sl, *vp = x.vp + key0 * a.v.sl;
-    if (a.mask) {
-      kl.template issue<true>(base, kp, a.k.sl, a.dh, left, bits);
-      vl.template issue<true>(base + T::kBytes, vp, a.v.sl, a.dh, left, bits);
-    } else {
-      kl.template issue<false>(base, kp, a.k.sl, a.dh, left, bits);
-      vl.template issue<false>(base + T::kBytes, vp, a.v.sl, a.dh, left, bits);
-    }
+    if (a.mask) kl.template issue<true>(to, p, a.k.sl, a.dh, left, bits);
+    else kl.template issue<false>(to, p, a.k.sl, a.dh, left, bits);
+  };
+  auto issue_values = [&](int stage, int kt, uint64_t bits) __attribute__((always_inline)) {
+    uint8_t *to = kTwo && stage ? values1 : values0;
+    const uint16_t *p = x.vp + static_cast<int64_t>(kt) * kRows * a.v.sl;
+    const int left = x.keys - kt * kRows;
+    if (a.mask) vl.template issue<true>(to, p, a.v.sl, a.dh, left, bits);
+    else vl.template issue<false>(to, p, a.v.sl, a.dh, left, bits);
   };
   int kt = x.kt;
   uint64_t bits = keybits.word(kt, keybits.load(kt));
   int byte = keybits.load(kt + 1);  // mask bytes a tile ahead of the loads that they are for
   Held<D> q;
   if constexpr (BIAS) load_bytes(tables, cut.tables + static_cast<int64_t>(x.head) * 4 * pitch, bias_bytes(reach), wave, NW, lane);
-  issue(0, kt, bits);
+  issue_keys(0, kt, bits);
+  if (kTwo) issue_values(0, kt, bits);
   q.load(a.q.p + x.b * a.q.sb + x.head * a.q.sh + x.row0 * a.q.sl, a.q.sl, a.dh, a.Lq - x.row0, lane);
 
   f32x16 o[D / 32];
@@ -366,9 +370,11 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
   float m_run = kLowest, l_run = 0.0f;
   constexpr float kRoom = headroom<BF>();
 
-  // One tile. near: the bias differs among its scores (otherwise it is `bc`, times log2(e), for all); part: some are not seen.
-  auto compute = [&](int stage, float bc, bool near, bool part) __attribute__((always_inline)) {
-    uint8_t *ks = stage ? smem1 : smem0, *vs = ks + T::kBytes;
+  // The probabilities of a tile. near: the bias differs among its scores (otherwise it is `bc`, times log2(e), for all); part:
+  // some are not seen.
+  uint4 pb[2][2];
+  auto scores = [&](int stage, float bc, bool near, bool part) __attribute__((always_inline)) {
+    const uint8_t *ks = stage ? keys1 : keys0;
     const int pos = x.start + x.row0 + c;
     f32x16 sc[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -410,7 +416,6 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
     }
     const float sub = m_run - bc;
     float ls = 0.0f;
-    uint4 pb[2][2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -428,20 +433,26 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
         pb[kb][t2] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     l_run += ls;
+  };
+  auto products = [&](int stage) __attribute__((always_inline)) {
+    uint8_t *vs = kTwo && stage ? values1 : values0;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
       o[i / 4] = mfma<BF>(cols.read(vs, i / 4, (i / 2) % 2, i % 2), pb[(i / 2) % 2][i % 2], o[i / 4]);
   };
 
   auto step = [&](int stage) __attribute__((always_inline)) {
+    const bool more = kt + 1 < x.end;
     uint64_t bits_next = 0;
-    if (kt + 1 < x.end) {
+    if (more) {
       bits_next = keybits.word(kt + 1, byte);
-      issue(stage ^ 1, kt + 1, bits_next);
+      issue_keys(stage ^ 1, kt + 1, bits_next);
+      if (kTwo) issue_values(stage ^ 1, kt + 1, bits_next);
       byte = keybits.load(kt + 2);
     }
     const int key0 = kt * kRows, first = x.start + x.row0;
-    if (bits && !(a.causal && key0 > first + 31)) {
+    const bool any = bits && !(a.causal && key0 > first + 31);
+    if (any) {
       const bool all = bits == ~0ull && !(a.causal && key0 + kRows - 1 > first);
       bool near = BIAS;
       float bc = 0.0f;
@@ -451,14 +462,29 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? (D == 64 ? 3 : 2) : 1) void fwd_
         near = !behind && !ahead;
         if (!near) bc = table[behind ? 0 : 2 * reach + 16] * a.c2;
       }
-      compute(stage, bc, near, !all);
+      scores(stage, bc, near, !all);
     }
+    if (!kTwo) {
+      // This tile's values have landed: only the next keys, loaded after them, may be on their way.
+      if (more) wait_vmcnt<KJ>();
+      else wait_vmcnt<0>();
+      __syncthreads();
+    }
+    if (any) products(stage);
     bits = bits_next;
     wait_vmcnt<0>();
-    __syncthreads();  // the next tile has landed for every wave, and no wave reads this stage any more
+    __syncthreads();  // the next tile has landed for every wave, and no wave reads this one any more
+    if (!kTwo && more) {
+      issue_values(0, kt + 1, bits);
+      asm volatile("" ::: "memory");  // counted by the wait above: no load moves across
+    }
   };
   wait_vmcnt<0>();
   __syncthreads();
+  if (!kTwo) {
+    issue_values(0, kt, bits);
+    asm volatile("" ::: "memory");
+  }
   while (true) {
     step(0);
     if (++kt >= x.end) break;
@@ -767,7 +793,7 @@ Plan plan_of(const Args &a) {
   p.nw = blocks <= 1 ? 1 : blocks <= 2 ? 2 : 4;
   c.tiles = static_cast<int>(cdiv(blocks, p.nw));
   // Workgroups that are resident at once: two to a CU, of one or two waves with narrow heads four.
-  const int64_t resident = cu * (p.D == 128 ? 2 : p.nw < 4 ? 4 : 3);
+  const int64_t resident = cu * (p.nw < 4 ? 4 : 3);
   const int64_t whole = items * (c.pack ? 1 : a.group) * c.tiles, tiles = cdiv(a.Lk, kRows);
   // Parts where items are too few to fill the CUs, of four tiles at least.
   c.parts = static_cast<int>(std::max<int64_t>(1, std::min(resident / std::max<int64_t>(whole, 1), tiles / 4)));
