@@ -359,10 +359,16 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
   uint64_t bits = keybits.word(kt, keybits.load(kt));
   int byte = keybits.load(kt + 1);  // mask bytes a tile ahead of the loads that they are for
   Held<D> q;
-  if constexpr (BIAS) load_bytes(tables, cut.tables + static_cast<int64_t>(x.head) * 4 * pitch, bias_bytes(reach), wave, NW, lane);
   issue_keys(0, kt, bits);
   if (kTwo) issue_values(0, kt, bits);
   q.load(a.q.p + x.b * a.q.sb + x.head * a.q.sh + x.row0 * a.q.sl, a.q.sl, a.dh, a.Lq - x.row0, lane);
+  if constexpr (BIAS) {
+    if (cut.tables)
+      load_bytes(tables, cut.tables + static_cast<int64_t>(x.head) * 4 * pitch, bias_bytes(reach), wave, NW, lane);
+    else
+      for (int i = threadIdx.x; i < 2 * reach + 17; i += 64 * NW)
+        write_bias(reinterpret_cast<float *>(tables), a.bias, x.head, i, false);
+  }
 
   f32x16 o[D / 32];
 #pragma unroll
@@ -768,6 +774,7 @@ struct Plan {
   int D, nw;
   Cut cut{};
   int few_parts;
+  bool shared_tables;
   int64_t partial = 0, tables = 0, bytes = 0;  // offsets into the workspace, its size
 };
 
@@ -792,11 +799,12 @@ Plan plan_of(const Args &a) {
   const int64_t blocks = c.pack ? static_cast<int64_t>(a.group) * c.qblocks : c.qblocks;
   p.nw = blocks <= 1 ? 1 : blocks <= 2 ? 2 : 4;
   c.tiles = static_cast<int>(cdiv(blocks, p.nw));
-  // Workgroups that are resident at once: two to a CU, of one or two waves with narrow heads four.
-  const int64_t resident = cu * (p.nw < 4 ? 4 : 3);
   const int64_t whole = items * (c.pack ? 1 : a.group) * c.tiles, tiles = cdiv(a.Lk, kRows);
-  // Parts where items are too few to fill the CUs, of four tiles at least.
-  c.parts = static_cast<int>(std::max<int64_t>(1, std::min(resident / std::max<int64_t>(whole, 1), tiles / 4)));
+  // Parts where items are too few for two to a CU, of eight tiles at least: a part's output is written and read again, and the
+  // merge is a launch of its own. us, parts of four tiles / eight: 64 heads of 512 with a bias 25.8 / 20.0, 4 heads of 256 rows
+  // over 20,280 keys 36.9 / 34.6. Parts for one to a CU instead: 32.0 there, but 24 heads of 1024 rows over 2048 keys 46.8 ->
+  // 51.8.
+  c.parts = static_cast<int>(std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(whole, 1), tiles / 8)));
   c.total = static_cast<int>(whole * c.parts);
   c.per_xcd = static_cast<int>(cdiv(c.total, 8));
   c.by_tiles = fast_div(c.tiles);
@@ -810,7 +818,9 @@ Plan plan_of(const Args &a) {
     return at;
   };
   if (c.parts > 1) p.partial = take(static_cast<int64_t>(c.total) * p.nw * partial_floats(p.D) * 4);
-  if (a.bias.table) p.tables = take(static_cast<int64_t>(a.H) * bias_bytes(a.bias.reach));
+  // The tables by distance are built by a launch of their own, unless every workgroup starts at once: then each builds its own.
+  p.shared_tables = a.bias.table && c.total > 2 * cu;
+  if (p.shared_tables) p.tables = take(static_cast<int64_t>(a.H) * bias_bytes(a.bias.reach));
   return p;
 }
 
@@ -826,8 +836,8 @@ template <bool BF, int D, int NW, bool BIAS>
 void launch_tiles(const Args &a, const Plan &p, float *ws, hipStream_t st) {
   Cut cut = p.cut;
   cut.partial = ws + p.partial / 4;
-  cut.tables = ws + p.tables / 4;
-  if constexpr (BIAS) launch_bias(a.bias, a.H, 1, cut.tables, st);
+  cut.tables = p.shared_tables ? ws + p.tables / 4 : nullptr;
+  if (BIAS && p.shared_tables) launch_bias(a.bias, a.H, 1, cut.tables, st);
   fwd_kernel<BF, D, NW, BIAS><<<dim3(8 * cut.per_xcd), dim3(64 * NW), BIAS ? bias_lds(a.bias.reach) : 0, st>>>(a, cut);
   if (cut.parts > 1)
     merge_kernel<BF, D><<<dim3(a.B * a.H * cut.qblocks * (D / 32)), dim3(256), 0, st>>>(a, cut, NW);
