@@ -26,7 +26,7 @@ namespace {
 template <int D, int R>
 struct Few {
   static constexpr int kLanes = D / 8, kSlots = 64 / kLanes;
-  static constexpr int kU = R <= 2 ? 8 : 4;        // keys of a slot per unit
+  static constexpr int kU = R <= 2 ? 8 : 2;  // keys of a slot per unit
   static constexpr int kUnit = kU * kSlots;        // keys per wave and step (at most 64)
   static constexpr int kFloats = R * (D + 2);      // a part's result: R x D outputs, maxima, sums
 };
@@ -44,20 +44,25 @@ __device__ __forceinline__ float key_sum(float v) {
   return v;
 }
 
+// Eight products, two an instruction, summed in fp32.
 template <bool BF>
 __device__ __forceinline__ float dot8(uint4 a, uint4 b) {
-  float s = 0.0f;
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
   const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+  float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    s = __builtin_fmaf(lo_of<BF>(x[i]), lo_of<BF>(y[i]), s);
-    s = __builtin_fmaf(hi_of<BF>(x[i]), hi_of<BF>(y[i]), s);
+    if constexpr (BF)
+      s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x[i]), __builtin_bit_cast(bf16x2, y[i]), s, false);
+    else
+      s = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x[i]), __builtin_bit_cast(f16x2, y[i]), s, false);
   }
   return s;
 }
 
 template <bool BF, int D, int R, int NW, bool BIAS>
-__global__ __launch_bounds__(64 * NW) void few_kernel(Args a, int parts, float *__restrict__ partial) {
+__global__ __launch_bounds__(64 * NW, R == 4 ? 4 : 2) void few_kernel(Args a, int parts, float *__restrict__ partial) {
   using F = Few<D, R>;
   constexpr int kSlots = F::kSlots, kU = F::kU, kUnit = F::kUnit;
   extern __shared__ __attribute__((aligned(16))) float table[];  // [group][2 reach + 1], by distance
@@ -91,13 +96,8 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(Args a, int parts, float *
 
   const uint16_t *kp = a.k.p + b * a.k.sb + hk * a.k.sh, *vp = a.v.p + b * a.v.sb + hk * a.v.sh;
   const uint8_t *mask = a.mask ? a.mask + b * a.mask_sb : nullptr;
-  uint32_t koff[kU], voff[kU];
-#pragma unroll
-  for (int u = 0; u < kU; ++u) {
-    const uint32_t r = u * kSlots + slot;
-    koff[u] = given ? r * static_cast<uint32_t>(2 * a.k.sl) + 2 * ch : kPast;
-    voff[u] = given ? r * static_cast<uint32_t>(2 * a.v.sl) + 2 * ch : kPast;
-  }
+  const uint32_t koff = given ? slot * static_cast<uint32_t>(2 * a.k.sl) + 2 * ch : kPast;
+  const uint32_t voff = given ? slot * static_cast<uint32_t>(2 * a.v.sl) + 2 * ch : kPast;
   auto bytes_of = [&](int64_t sl, int n) {
     n = min(n, kUnit);
     return n > 0 ? 2 * ((n - 1) * static_cast<uint32_t>(sl) + a.dh) : 0u;
@@ -107,13 +107,14 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(Args a, int parts, float *
     const int64_t key0 = static_cast<int64_t>(unit) * kUnit;
     const __amdgpu_buffer_rsrc_t r = make_rsrc(kp + key0 * a.k.sl, bytes_of(a.k.sl, keys - static_cast<int>(key0)));
 #pragma unroll
-    for (int u = 0; u < kU; ++u) kf[u] = load_b128(r, koff[u], 0);
+    for (int u = 0; u < kU; ++u) kf[u] = load_b128(r, koff, u * kSlots * static_cast<uint32_t>(2 * a.k.sl));
   };
   auto load_v = [&](int unit, uint64_t bits) {  // masked values read as zeros: what they hold must not reach a product
     const int64_t key0 = static_cast<int64_t>(unit) * kUnit;
     const __amdgpu_buffer_rsrc_t r = make_rsrc(vp + key0 * a.v.sl, bytes_of(a.v.sl, keys - static_cast<int>(key0)));
 #pragma unroll
-    for (int u = 0; u < kU; ++u) vf[u] = load_b128(r, (bits >> (u * kSlots + slot)) & 1 ? voff[u] : kPast, 0);
+    for (int u = 0; u < kU; ++u)
+      vf[u] = load_b128(r, (bits >> (u * kSlots + slot)) & 1 ? voff : kPast, u * kSlots * static_cast<uint32_t>(2 * a.v.sl));
   };
   auto load_byte = [&](int unit) {
     const int64_t key = static_cast<int64_t>(unit) * kUnit + lane;
@@ -786,7 +787,7 @@ Plan plan_of(const Args &a) {
   if (rows <= 8) {
     p.few = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
     p.nw = 8;
-    const int unit = (p.few <= 2 ? 8 : 4) * (512 / p.D);
+    const int unit = (p.few <= 2 ? 8 : 2) * (512 / p.D);
     const int64_t units = cdiv(a.Lk, unit);
     // Parts for two workgroups a CU, of four units a wave at least.
     p.few_parts = static_cast<int>(std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(items, 1), units / (4 * p.nw))));
