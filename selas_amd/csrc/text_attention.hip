@@ -276,7 +276,8 @@ __global__ __launch_bounds__(128) void few_merge_kernel(Args a, int parts, int D
 struct Cut {
   int qblocks;  // of 32 queries, per head
   int tiles;    // items per head, or per group (pack)
-  int parts, pack, total, per_xcd;
+  int parts, pack;
+  Deal deal;
   FastDiv by_tiles, by_group, by_parts, by_hk, by_qblocks;
   float *partial, *tables;  // tables: every head's bias by distance
 };
@@ -292,10 +293,6 @@ struct Item {
 
 __device__ __forceinline__ Item item_at(const Args &a, const Cut &cut, int t, int nw, int wave) {
   Item x;
-  auto split = [](int v, FastDiv by, int d, int &rest) {  // v % d, and rest = v / d
-    rest = static_cast<int>(div31(v, by));
-    return v - rest * d;
-  };
   int rest, g = 0;
   const int tile0 = split(t, cut.by_tiles, cut.tiles, rest);
   if (!cut.pack) g = split(rest, cut.by_group, a.group, rest);
@@ -333,8 +330,8 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
   __shared__ __attribute__((aligned(16))) uint8_t values1[kTwo ? T::kBytes : 16];
   extern __shared__ __attribute__((aligned(16))) uint8_t tables[];  // the head's bias by distance
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
-  const int t = item_of(cut.per_xcd);
-  if (t >= cut.total) return;
+  const int t = item_of(cut.deal);
+  if (t >= cut.deal.total) return;
   const Item x = item_at(a, cut, t, NW, wave);
   const KeyBits keybits(a, x.b, x.keys, lane);
   const typename T::template Loader<KJ> kl(wave, lane, a.k.sl, a.dh), vl(wave, lane, a.v.sl, a.dh);
@@ -806,8 +803,7 @@ Plan plan_of(const Args &a) {
   // over 20,280 keys 36.9 / 34.6. Parts for one to a CU instead: 32.0 there, but 24 heads of 1024 rows over 2048 keys 46.8 ->
   // 51.8.
   c.parts = static_cast<int>(std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(whole, 1), tiles / 8)));
-  c.total = static_cast<int>(whole * c.parts);
-  c.per_xcd = static_cast<int>(cdiv(c.total, 8));
+  c.deal = deal(whole * c.parts, static_cast<int64_t>(c.pack ? 1 : a.group) * c.tiles, a.lengths || a.mask);
   c.by_tiles = fast_div(c.tiles);
   c.by_group = fast_div(a.group);
   c.by_parts = fast_div(c.parts);
@@ -818,9 +814,9 @@ Plan plan_of(const Args &a) {
     p.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  if (c.parts > 1) p.partial = take(static_cast<int64_t>(c.total) * p.nw * partial_floats(p.D) * 4);
+  if (c.parts > 1) p.partial = take(static_cast<int64_t>(c.deal.total) * p.nw * partial_floats(p.D) * 4);
   // The tables by distance are built by a launch of their own, unless every workgroup starts at once: then each builds its own.
-  p.shared_tables = a.bias.table && c.total > 2 * cu;
+  p.shared_tables = a.bias.table && c.deal.total > 2 * cu;
   if (p.shared_tables) p.tables = take(static_cast<int64_t>(a.H) * bias_bytes(a.bias.reach));
   return p;
 }
@@ -839,7 +835,7 @@ void launch_tiles(const Args &a, const Plan &p, float *ws, hipStream_t st) {
   cut.partial = ws + p.partial / 4;
   cut.tables = p.shared_tables ? ws + p.tables / 4 : nullptr;
   if (BIAS && p.shared_tables) launch_bias(a.bias, a.H, 1, cut.tables, st);
-  fwd_kernel<BF, D, NW, BIAS><<<dim3(8 * cut.per_xcd), dim3(64 * NW), BIAS ? bias_lds(a.bias.reach) : 0, st>>>(a, cut);
+  fwd_kernel<BF, D, NW, BIAS><<<dim3(cut.deal.blocks), dim3(64 * NW), BIAS ? bias_lds(a.bias.reach) : 0, st>>>(a, cut);
   if (cut.parts > 1)
     merge_kernel<BF, D><<<dim3(a.B * a.H * cut.qblocks * (D / 32)), dim3(256), 0, st>>>(a, cut, NW);
 }

@@ -37,7 +37,9 @@ struct Grads {
 
 // A kernel's work items: `parts` ranges of the streamed axis; sums of a part go to `partial` (fp32) where parts > 1.
 struct Cut {
-  int tiles, parts, total, per_xcd;
+  int tiles, parts;
+  Deal deal;
+  FastDiv by_tiles, by_parts, by_group, by_hk;
   float *partial;
 };
 
@@ -115,10 +117,11 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
   constexpr int KJ = T::kLoads / NW, kStats = 2 * kRows * 4;
   __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes + kStats], smem1[2 * T::kBytes + kStats];
   extern __shared__ __attribute__((aligned(1024))) uint8_t tables[];  // two heads' bias by distance
-  const int t = item_of(cut.per_xcd);
-  if (t >= cut.total) return;
-  const int tile = t % cut.tiles, part = t / cut.tiles % cut.parts, bhk = t / cut.tiles / cut.parts;
-  const int b = bhk / a.Hk, hk = bhk - b * a.Hk;
+  const int t = item_of(cut.deal);
+  if (t >= cut.deal.total) return;
+  int rest, bhk, b;
+  const int tile = split(t, cut.by_tiles, cut.tiles, rest), part = split(rest, cut.by_parts, cut.parts, bhk);
+  const int hk = split(bhk, cut.by_hk, a.Hk, b);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const int keys = keys_of(a, b), start = start_of(a, b);
   const int wg_key = tile * NW * 32, key0 = wg_key + wave * 32, key = key0 + c;
@@ -338,16 +341,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   constexpr int KJ = T::kLoads / NW;
   __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
   extern __shared__ __attribute__((aligned(1024))) uint8_t dynamic[];
-  const int t = item_of(cut.per_xcd);
-  if (t >= cut.total) return;
-  int rest = t;
-  const int qt0 = rest % cut.tiles;
-  rest /= cut.tiles;
-  const int g = rest % a.group;
-  rest /= a.group;
-  const int part = rest % cut.parts;
-  rest /= cut.parts;
-  const int hk = rest % a.Hk, b = rest / a.Hk, head = hk * a.group + g;
+  const int t = item_of(cut.deal);
+  if (t >= cut.deal.total) return;
+  int rest, b;
+  const int qt0 = split(t, cut.by_tiles, cut.tiles, rest), g = split(rest, cut.by_group, a.group, rest);
+  const int part = split(rest, cut.by_parts, cut.parts, rest), hk = split(rest, cut.by_hk, a.Hk, b), head = hk * a.group + g;
   const int qt = a.causal ? cut.tiles - 1 - qt0 : qt0;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const int keys = keys_of(a, b), start = start_of(a, b);
@@ -656,14 +654,16 @@ Plan plan_of(const Args &a, bool bf) {
   p.kblocks = static_cast<int>(cdiv(a.Lk, kRows));
   p.buckets = a.bias.ahead ? 2 * a.bias.n : a.bias.n;
   const int64_t cu = cu_count();
-  auto cut = [&](int64_t heads, int tiles, int64_t streamed) {
+  auto cut = [&](int64_t heads, int tiles, int64_t streamed, int64_t inner) {
     const int64_t whole = heads * tiles;
     // Workgroups for two to a CU, of four streamed tiles at least.
     const int64_t parts = std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(whole, 1), streamed / 4));
-    return Cut{tiles, static_cast<int>(parts), static_cast<int>(whole * parts), static_cast<int>(cdiv(whole * parts, 8)), nullptr};
+    return Cut{tiles, static_cast<int>(parts), deal(whole * parts, inner, a.lengths || a.mask), fast_div(std::max(tiles, 1)),
+               fast_div(static_cast<uint32_t>(parts)), fast_div(std::max(a.group, 1)), fast_div(std::max(a.Hk, 1)), nullptr};
   };
-  p.key = cut(static_cast<int64_t>(a.B) * a.Hk, static_cast<int>(cdiv(a.Lk, 32 * kNW)), static_cast<int64_t>(a.group) * p.qblocks);
-  p.query = cut(static_cast<int64_t>(a.B) * a.H, static_cast<int>(cdiv(a.Lq, 32 * kNW)), p.kblocks);
+  const int ktiles = static_cast<int>(cdiv(a.Lk, 32 * kNW)), qtiles = static_cast<int>(cdiv(a.Lq, 32 * kNW));
+  p.key = cut(static_cast<int64_t>(a.B) * a.Hk, ktiles, static_cast<int64_t>(a.group) * p.qblocks, ktiles);
+  p.query = cut(static_cast<int64_t>(a.B) * a.H, qtiles, p.kblocks, static_cast<int64_t>(a.group) * qtiles);
   auto take = [&](int64_t floats) {
     const int64_t at = p.bytes;
     p.bytes += (floats * 4 + 255) / 256 * 256;
@@ -691,14 +691,14 @@ void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
       sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(rows * a.dh, 1024)), arrays), dim3(256), 0, st>>>(cut.partial, cut.parts, rows * a.dh, arrays, y0, y1);
   };
   if constexpr (BIAS) launch_bias(a.bias, a.H, 2, w.tables, st);
-  if (!BF && p.query.total + p.key.total) norm_kernel<<<dim3(a.B * a.H * p.qblocks + a.B * a.Hk * p.kblocks), dim3(256), 0, st>>>(a, w);
-  if (p.query.total) {
+  if (!BF && p.query.deal.total + p.key.deal.total) norm_kernel<<<dim3(a.B * a.H * p.qblocks + a.B * a.Hk * p.kblocks), dim3(256), 0, st>>>(a, w);
+  if (p.query.deal.total) {
     const size_t lds = BIAS ? bias_lds(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
-    query_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.query.per_xcd), dim3(64 * kNW), lds, st>>>(a, w, p.query);
+    query_kernel<BF, D, kNW, BIAS><<<dim3(p.query.deal.blocks), dim3(64 * kNW), lds, st>>>(a, w, p.query);
     sum(p.query, static_cast<int64_t>(a.B) * a.H * a.Lq, 1, w.dq, nullptr);
   }
-  if (p.key.total) {
-    key_kernel<BF, D, kNW, BIAS><<<dim3(8 * p.key.per_xcd), dim3(64 * kNW), BIAS ? 2 * bias_lds(reach) : 0, st>>>(a, w, p.key);
+  if (p.key.deal.total) {
+    key_kernel<BF, D, kNW, BIAS><<<dim3(p.key.deal.blocks), dim3(64 * kNW), BIAS ? 2 * bias_lds(reach) : 0, st>>>(a, w, p.key);
     sum(p.key, static_cast<int64_t>(a.B) * a.Hk * a.Lk, 2, w.dk, w.dv);
   }
   if constexpr (BIAS)
