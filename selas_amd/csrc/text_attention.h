@@ -154,23 +154,18 @@ __device__ __forceinline__ float bias_at(const Bias &t, int head, int d, float m
   return v * mul;
 }
 
-// The four copies of a head's table, by a thread per distance, into global memory: workgroups then only copy them to LDS.
-// reversed: by query - key.
-__device__ __forceinline__ void write_bias(float *out, const Bias &t, int head, int i, bool reversed) {
-  const int pitch = bias_pitch(t.reach), d = i - t.reach - 8;
-  if (i >= 2 * t.reach + 17) return;
-  const float v = bias_at(t, head, reversed ? -d : d, t.inv_scale);
+// The four copies of a head's table, into LDS, by all threads of the workgroup; reversed: by query - key. Building them once
+// per call, by a launch of its own, took 5 us and gained nothing at any batch.
+__device__ __forceinline__ void build_bias(float *lds, const Bias &t, int head, int threads, bool reversed) {
+  const int pitch = bias_pitch(t.reach);
+  for (int i = threadIdx.x; i < 2 * t.reach + 17; i += threads) {
+    const int d = i - t.reach - 8;
+    const float v = bias_at(t, head, reversed ? -d : d, t.inv_scale);
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (i >= c) out[c * pitch + i - c] = v;
+    for (int c = 0; c < 4; ++c)
+      if (i >= c) lds[c * pitch + i - c] = v;
+  }
 }
-
-// `bytes` (whole 16) from global memory to LDS, 1 KiB an instruction, dealt to the waves; LDS is written to the next KiB.
-__device__ __forceinline__ void load_bytes(uint8_t *lds, const void *p, int bytes, int wave, int waves, int lane) {
-  const __amdgpu_buffer_rsrc_t r = make_rsrc(p, bytes);
-  for (int i = wave; i * 1024 < bytes; i += waves) load_lds16(r, lds + i * 1024, i * 1024 + 16 * lane, 0);
-}
-__host__ __device__ inline int bias_lds(int reach) { return (bias_bytes(reach) + 1023) / 1024 * 1024; }
 
 // Eight entries from distance d on.
 __device__ __forceinline__ void bias_run(const float *lds, int pitch, int reach, int d, float (&v)[8]) {
@@ -309,17 +304,6 @@ struct KeyBits {
 
 // The low n + 1 bits (none below 0, all from 63 on): the keys at or before position n of a tile.
 __device__ __forceinline__ uint64_t up_to(int n) { return n < 0 ? 0ull : n >= 63 ? ~0ull : (2ull << n) - 1; }
-
-namespace {
-// Every head's table by distance, [orders][H][4 bias_pitch]; blockIdx = (distances / 256, head, order).
-__global__ __launch_bounds__(256) void bias_kernel(Bias t, float *out) {
-  const int64_t at = static_cast<int64_t>(blockIdx.z * gridDim.y + blockIdx.y) * 4 * bias_pitch(t.reach);
-  write_bias(out + at, t, blockIdx.y, blockIdx.x * 256 + threadIdx.x, blockIdx.z);
-}
-inline void launch_bias(const Bias &t, int H, int orders, float *out, hipStream_t st) {
-  bias_kernel<<<dim3((2 * t.reach + 17 + 255) / 256, H, orders), dim3(256), 0, st>>>(t, out);
-}
-}  // namespace
 
 // ------------------------------------------------------------------ host side
 

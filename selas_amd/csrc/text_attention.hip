@@ -279,7 +279,7 @@ struct Cut {
   int parts, pack;
   Deal deal;
   FastDiv by_tiles, by_group, by_parts, by_hk, by_qblocks;
-  float *partial, *tables;  // tables: every head's bias by distance
+  float *partial;
 };
 constexpr int partial_floats(int D) { return 64 * (D / 2) + 2 * 64; }  // per wave: outputs in register order, maxima, sums
 
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
   constexpr bool kTwo = D == 64;  // two stages of the values as well
   __shared__ __attribute__((aligned(16))) uint8_t keys0[T::kBytes], keys1[T::kBytes], values0[T::kBytes];
   __shared__ __attribute__((aligned(16))) uint8_t values1[kTwo ? T::kBytes : 16];
-  extern __shared__ __attribute__((aligned(16))) uint8_t tables[];  // the head's bias by distance
+  extern __shared__ __attribute__((aligned(16))) float table[];  // the head's bias by distance
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5, c = lane & 31;
   const int t = item_of(cut.deal);
   if (t >= cut.deal.total) return;
@@ -360,13 +360,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
   issue_keys(0, kt, bits);
   if (kTwo) issue_values(0, kt, bits);
   q.load(a.q.p + x.b * a.q.sb + x.head * a.q.sh + x.row0 * a.q.sl, a.q.sl, a.dh, a.Lq - x.row0, lane);
-  if constexpr (BIAS) {
-    if (cut.tables)
-      load_bytes(tables, cut.tables + static_cast<int64_t>(x.head) * 4 * pitch, bias_bytes(reach), wave, NW, lane);
-    else
-      for (int i = threadIdx.x; i < 2 * reach + 17; i += 64 * NW)
-        write_bias(reinterpret_cast<float *>(tables), a.bias, x.head, i, false);
-  }
+  if constexpr (BIAS) build_bias(table, a.bias, x.head, 64 * NW, false);
 
   f32x16 o[D / 32];
 #pragma unroll
@@ -384,7 +378,6 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
 #pragma unroll
     for (int i = 0; i < 2 * (D / 16); ++i) sc[i / (D / 16)] = mfma<BF>(rows.read(ks, i / (D / 16), i % (D / 16)), q.f[i % (D / 16)], sc[i / (D / 16)]);
     if (BIAS && near) {
-      const float *table = reinterpret_cast<const float *>(tables);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -461,8 +454,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
       bool near = BIAS;
       float bc = 0.0f;
       if constexpr (BIAS) {
-        const float *table = reinterpret_cast<const float *>(tables);
-        const bool behind = key0 + kRows - 1 - first <= -reach, ahead = key0 - first - 31 >= (a.bias.ahead ? reach : 0);
+          const bool behind = key0 + kRows - 1 - first <= -reach, ahead = key0 - first - 31 >= (a.bias.ahead ? reach : 0);
         near = !behind && !ahead;
         if (!near) bc = table[behind ? 0 : 2 * reach + 16] * a.c2;
       }
@@ -772,8 +764,7 @@ struct Plan {
   int D, nw;
   Cut cut{};
   int few_parts;
-  bool shared_tables;
-  int64_t partial = 0, tables = 0, bytes = 0;  // offsets into the workspace, its size
+  int64_t bytes = 0;  // workspace
 };
 
 Plan plan_of(const Args &a) {
@@ -809,15 +800,7 @@ Plan plan_of(const Args &a) {
   c.by_parts = fast_div(c.parts);
   c.by_hk = fast_div(a.Hk);
   c.by_qblocks = fast_div(c.qblocks);
-  auto take = [&](int64_t bytes) {
-    const int64_t at = p.bytes;
-    p.bytes += (bytes + 255) / 256 * 256;
-    return at;
-  };
-  if (c.parts > 1) p.partial = take(static_cast<int64_t>(c.deal.total) * p.nw * partial_floats(p.D) * 4);
-  // The tables by distance are built by a launch of their own, unless every workgroup starts at once: then each builds its own.
-  p.shared_tables = a.bias.table && c.deal.total > 2 * cu;
-  if (p.shared_tables) p.tables = take(static_cast<int64_t>(a.H) * bias_bytes(a.bias.reach));
+  if (c.parts > 1) p.bytes = static_cast<int64_t>(c.deal.total) * p.nw * partial_floats(p.D) * 4;
   return p;
 }
 
@@ -832,10 +815,8 @@ void launch_few(const Args &a, const Plan &p, float *ws, hipStream_t st) {
 template <bool BF, int D, int NW, bool BIAS>
 void launch_tiles(const Args &a, const Plan &p, float *ws, hipStream_t st) {
   Cut cut = p.cut;
-  cut.partial = ws + p.partial / 4;
-  cut.tables = p.shared_tables ? ws + p.tables / 4 : nullptr;
-  if (BIAS && p.shared_tables) launch_bias(a.bias, a.H, 1, cut.tables, st);
-  fwd_kernel<BF, D, NW, BIAS><<<dim3(cut.deal.blocks), dim3(64 * NW), BIAS ? bias_lds(a.bias.reach) : 0, st>>>(a, cut);
+  cut.partial = ws;
+  fwd_kernel<BF, D, NW, BIAS><<<dim3(cut.deal.blocks), dim3(64 * NW), BIAS ? bias_bytes(a.bias.reach) : 0, st>>>(a, cut);
   if (cut.parts > 1)
     merge_kernel<BF, D><<<dim3(a.B * a.H * cut.qblocks * (D / 32)), dim3(256), 0, st>>>(a, cut, NW);
 }

@@ -30,7 +30,6 @@ struct Grads {
   float *neg_lse, *dot;    // [B, H, Lqp]: -lse log2(e) (-inf for rows that see nothing and rows past Lq), D (0 there)
   int Lqp, qblocks, kblocks;  // rows padded to whole tiles; tiles of queries, of keys
   float *g_norm, *v_norm;  // fp16: largest squared norms of the rows of dO and v, per tile
-  float *tables;           // bias by distance, [2 (by key - query, by query - key)][H][4 bias_pitch]
   float *dtable_part;      // [B, H, qtiles * parts, buckets]
   void *dtable;
 };
@@ -115,8 +114,8 @@ template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cut) {
   using T = Tile<D>;
   constexpr int KJ = T::kLoads / NW, kStats = 2 * kRows * 4;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes + kStats], smem1[2 * T::kBytes + kStats];
-  extern __shared__ __attribute__((aligned(1024))) uint8_t tables[];  // two heads' bias by distance
+  __shared__ __attribute__((aligned(16))) uint8_t smem0[2 * T::kBytes + kStats], smem1[2 * T::kBytes + kStats];
+  extern __shared__ __attribute__((aligned(16))) float tables[];  // two heads' bias by distance
   const int t = item_of(cut.deal);
   if (t >= cut.deal.total) return;
   int rest, bhk, b;
@@ -156,9 +155,10 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
     }
   };
   const int reach = a.bias.reach, pitch = bias_pitch(reach);
-  auto load_table = [&](int g) {  // the heads of the group take the two buffers in turn
-    load_bytes(tables + (g & 1) * bias_lds(reach), w.tables + static_cast<int64_t>(a.H + hk * a.group + g) * 4 * pitch,
-               bias_bytes(reach), wave, NW, lane);
+  auto table_of = [&](int g) { return tables + (g & 1) * 4 * pitch; };  // the heads of the group take the two in turn
+  auto next_table = [&](int g) __attribute__((always_inline)) {
+    const Args &a = args_here();
+    build_bias(table_of(g), a.bias, hk * a.group + g, 64 * NW, true);
   };
   const float shift = ds_shift<BF>(a, w, b, hk, lane);
   const float ds_mul = BF ? 1.0f : __builtin_exp2f(shift - kProbShift);
@@ -221,21 +221,21 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
   };
 
   if (i < end) {
-    if constexpr (BIAS) load_table(g);
+    if constexpr (BIAS) next_table(g);
     issue(0, g, qt);
   }
   auto step = [&](int stage) __attribute__((always_inline)) {
     wait_vmcnt<0>();
     __syncthreads();  // this tile has landed for every wave, and no wave reads the other stage any more
     const int at = qt;
-    const float *table = reinterpret_cast<const float *>(tables + (g & 1) * bias_lds(reach));
+    const float *table = table_of(g);
     if (++qt == w.qblocks) {
       qt = qt0;
       ++g;
     }
     if (i + 1 < end) {
       if constexpr (BIAS)
-        if (qt == qt0) load_table(g);
+        if (qt == qt0) next_table(g);
       issue(stage ^ 1, g, qt);
     }
     const int pos0 = start + at * kRows;
@@ -339,8 +339,8 @@ template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a, Grads w, Cut cut) {
   using T = Tile<D>;
   constexpr int KJ = T::kLoads / NW;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
-  extern __shared__ __attribute__((aligned(1024))) uint8_t dynamic[];
+  __shared__ __attribute__((aligned(16))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
+  extern __shared__ __attribute__((aligned(16))) float table[];
   const int t = item_of(cut.deal);
   if (t >= cut.deal.total) return;
   int rest, b;
@@ -396,12 +396,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   };
 
   const int reach = a.bias.reach, pitch = bias_pitch(reach), span = hist_floats(reach);
-  const float *table = reinterpret_cast<const float *>(dynamic);
-  float *hist = reinterpret_cast<float *>(dynamic + bias_lds(reach));  // [2 NW][span]; after that [NW][2] sums
+  float *hist = table + 4 * pitch;  // [2 NW][span]; after that [NW][2] sums
   float *mine = hist + (2 * wave + h) * span;
   float sum_behind = 0.0f, sum_ahead = 0.0f, far_behind = 0.0f, far_ahead = 0.0f;
   if constexpr (BIAS) {
-    load_bytes(dynamic, w.tables + static_cast<int64_t>(head) * 4 * pitch, bias_bytes(reach), wave, NW, lane);
+    build_bias(table, a.bias, head, 64 * NW, false);
     for (int i = threadIdx.x; i < 2 * NW * span; i += 64 * NW) hist[i] = 0.0f;
   }
   const float shift = ds_shift<BF>(a, w, b, hk, lane), ds_mul = BF ? 1.0f : __builtin_exp2f(shift);
@@ -536,7 +535,6 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   }
 
   if constexpr (BIAS) {
-    wait_vmcnt<0>();  // without keys nothing has waited for the table, whose load must not outlive the workgroup
     __syncthreads();
     // The histograms added up, then each bucket by one wave.
     float *sums = hist + 2 * NW * span;
@@ -643,7 +641,7 @@ __global__ __launch_bounds__(256) void dtable_kernel(const float *__restrict__ p
 struct Plan {
   int D, qblocks, kblocks, buckets;
   Cut key, query;
-  int64_t neg_lse, dot, g_norm, v_norm, tables, dtable, key_partial, query_partial, bytes;  // offsets into the workspace
+  int64_t neg_lse, dot, g_norm, v_norm, dtable, key_partial, query_partial, bytes;  // offsets into the workspace
 };
 constexpr int kNW = 4;
 
@@ -676,7 +674,6 @@ Plan plan_of(const Args &a, bool bf) {
     p.g_norm = take(static_cast<int64_t>(a.B) * a.H * p.qblocks);
     p.v_norm = take(static_cast<int64_t>(a.B) * a.Hk * p.kblocks);
   }
-  if (a.bias.table) p.tables = take(2ll * a.H * 4 * bias_pitch(a.bias.reach));
   if (a.bias.table) p.dtable = take(static_cast<int64_t>(a.B) * a.H * p.query.tiles * p.query.parts * p.buckets);
   if (p.key.parts > 1) p.key_partial = take(2ll * p.key.parts * a.B * a.Hk * a.Lk * a.dh);
   if (p.query.parts > 1) p.query_partial = take(static_cast<int64_t>(p.query.parts) * a.B * a.H * a.Lq * a.dh);
@@ -690,15 +687,14 @@ void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
     if (cut.parts > 1)
       sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(rows * a.dh, 1024)), arrays), dim3(256), 0, st>>>(cut.partial, cut.parts, rows * a.dh, arrays, y0, y1);
   };
-  if constexpr (BIAS) launch_bias(a.bias, a.H, 2, w.tables, st);
   if (!BF && p.query.deal.total + p.key.deal.total) norm_kernel<<<dim3(a.B * a.H * p.qblocks + a.B * a.Hk * p.kblocks), dim3(256), 0, st>>>(a, w);
   if (p.query.deal.total) {
-    const size_t lds = BIAS ? bias_lds(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
+    const size_t lds = BIAS ? bias_bytes(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
     query_kernel<BF, D, kNW, BIAS><<<dim3(p.query.deal.blocks), dim3(64 * kNW), lds, st>>>(a, w, p.query);
     sum(p.query, static_cast<int64_t>(a.B) * a.H * a.Lq, 1, w.dq, nullptr);
   }
   if (p.key.deal.total) {
-    key_kernel<BF, D, kNW, BIAS><<<dim3(p.key.deal.blocks), dim3(64 * kNW), BIAS ? 2 * bias_lds(reach) : 0, st>>>(a, w, p.key);
+    key_kernel<BF, D, kNW, BIAS><<<dim3(p.key.deal.blocks), dim3(64 * kNW), BIAS ? 2 * bias_bytes(reach) : 0, st>>>(a, w, p.key);
     sum(p.key, static_cast<int64_t>(a.B) * a.Hk * a.Lk, 2, w.dk, w.dv);
   }
   if constexpr (BIAS)
@@ -757,7 +753,6 @@ extern "C" int selas_text_attention_backward(const selas_text_attention_problem 
   w.kblocks = p.kblocks;
   w.g_norm = at(p.g_norm);
   w.v_norm = at(p.v_norm);
-  w.tables = at(p.tables);
   w.dtable_part = at(p.dtable);
   w.dtable = dtable;
   p.key.partial = at(p.key_partial);
