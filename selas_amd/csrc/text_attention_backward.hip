@@ -110,6 +110,12 @@ __device__ __forceinline__ float ds_shift(const Args &a, const Grads &w, int b, 
 // key, in runs of 8; then dV^T += dO^T P and dK^T += Q^T dS with the same tiles read transposed and P, dS straight from the
 // registers. A key's column depends on nothing of the other keys, so masked keys need no select: their results are zeroed at
 // the end.
+//
+// Bounded by LDS reads (an MFMA reads 1 KiB) and by waiting: dk and dv of 32 keys take D registers a lane and k and v D / 2
+// more, which leaves three workgroups a CU at D = 64 and two at D = 128 (MFMA 30 % busy at 4 x 64 heads of 512 tokens, 57 us;
+// 24 heads of 128, 4096 queries over 512 keys 63 to 68 us, 800 TFLOP/s). With each 16 rows' products right behind their
+// packing one pair of packed operands is live instead of two (178 -> 164 registers); a lone workgroup a CU at D = 128 took
+// 100 us there.
 template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cut) {
   using T = Tile<D>;
@@ -290,16 +296,22 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
 // held. S^T = K Q^T and dP^T = V dO^T leave a lane's registers with keys of one query, in runs of 8; dQ^T += K^T dS^T reads
 // the same K tile transposed.
 //
+// Bounded as key_kernel: 3 products of 7, 128 to 143 registers at D = 64 (61 us at 4 x 64 heads of 512 with a bias), 201 at
+// D = 128 (66 to 72 us at 4096 queries over 512 keys).
+//
 // dtable: tiles that hold only one value of the bias add dS up in a register. In the others dS is summed along the diagonals
 // (one distance each): a lane's run of 8 keys moves a lane per key through the 16 lanes of its row (Diagonals), and what is
 // left, a value per lane and 16 distances, is added to a histogram by distance in LDS, one for each half of each wave. It
 // covers every distance that such a tile can hold (kSpill past `reach` on either side). At the end the histograms are summed
-// by bucket, and by dtable_kernel over workgroups.
+// by bucket, and by dtable_kernel over workgroups. LDS float additions of every element instead took 120 cycles an
+// instruction: all gradients of 16 x 64 heads of 512 with a bias 1160 us, this way 567 at the time.
 //
 // D is first the product of dO and out in the order of the matrix unit, as dP is: where a row sees one key, out is that key's
 // value and dS is exactly 0. But out was rounded, and where few keys carry a row, D's share of that is as large as the
 // roundings of dS and of the result. So rows that see up to 64 kRefine keys add what the sum of p (dP - D) over all their
-// keys says is missing, by a pass over those tiles ahead of the others.
+// keys says is missing, by a pass over those tiles ahead of the others (77 keys: 14.4 -> 20.9 us; errors of dq against 64 bits
+// 1.65 -> 1.4 times those of one rounding). Where weight is spread over more keys out is small beside the values, and so is
+// that share: from 257 seen keys on it is left in, also where a few of them carry the row.
 constexpr int kSpill = 112, kRefine = 4;
 __host__ __device__ inline int hist_floats(int reach) { return 2 * reach + 2 * kSpill + 1; }
 
