@@ -30,8 +30,8 @@ _SIZES = ctypes.c_int64
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """t [B, heads, L, Dh] as the kernels read it: unit channel stride, rows of whole 16 bytes at aligned addresses."""
-    s = t.stride()
-    if s[3] != 1 or (s[0] | s[1] | s[2]) & 7 or s[2] > 1 << 23 or t.data_ptr() & 15:
+    sb, sh, sl, sc = t.stride()
+    if sc != 1 or (sb | sh | sl) & 7 or sl > 1 << 23 or t.data_ptr() & 15:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -65,7 +65,9 @@ class _Call:
             raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
         if k.dtype != q.dtype or v.dtype != q.dtype:
             raise ValueError(f"{what}: q {q.dtype}, k {k.dtype} and v {v.dtype} must have one type")
-        self.dev = _lib.require_gpu(q, k, v, table, lengths, mask)
+        dev = self.dev = q.device
+        if not q.is_cuda or k.device != dev or v.device != dev or table is not None or lengths is not None or mask is not None:
+            _lib.require_gpu(q, k, v, table, lengths, mask)
         dtype = _lib.DTYPE_CODES.get(q.dtype)
         if dtype is None or dtype == _lib.F32:
             raise _lib.Unsupported(f"{what}: takes bf16 or fp16, got {q.dtype}")
@@ -94,21 +96,23 @@ class _Call:
             if table.dim() != 2 or table.shape[1] != h:
                 raise ValueError(f"{what}: the table must be [buckets, {h}], got {tuple(table.shape)}")
             table_type, buckets = _lib.dtype_code(table.dtype), table.shape[0]
-            if (h > 1 and table.stride(1) != 1) or not buckets:
+            if not buckets:
+                raise ValueError(f"{what}: the table has no buckets")
+            if h > 1 and table.stride(1) != 1:
                 table = table.contiguous()
             self.table, table_row = table, table.stride(0)
-        self.scale = dh ** -0.5 if scale is None else float(scale)
-        ptr = _lib.ptr
-        qs, ks, vs = self.q.stride(), self.k.stride(), self.v.stride()
-        self._head = (self.q.data_ptr(), qs[0], qs[1], qs[2], self.k.data_ptr(), ks[0], ks[1], ks[2], self.v.data_ptr(),
-                      vs[0], vs[1], vs[2])
-        self._tail = (ptr(self.lengths), ptr(mask), 0 if mask is None or mask.shape[0] == 1 else mask.stride(0),
-                      ptr(self.start), start0, ptr(self.table), table_row, b, h, hk, lq, lk, dh, buckets,
-                      int(max_distance), self.scale, table_type, bool(bidirectional), bool(causal), 0)
+        q, k, v, (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _) = (self.q, self.k, self.v, self.q.stride(), self.k.stride(),
+                                                                     self.v.stride())
+        self._head = (q.data_ptr(), q0, q1, q2, k.data_ptr(), k0, k1, k2, v.data_ptr(), v0, v1, v2)
+        self._tail = (0 if lengths is None else self.lengths.data_ptr(), 0 if mask is None else mask.data_ptr(),
+                      0 if mask is None or mask.shape[0] == 1 else mask.stride(0),
+                      0 if self.start is None else self.start.data_ptr(), start0, 0 if table is None else table.data_ptr(),
+                      table_row, b, h, hk, lq, lk, dh, buckets, int(max_distance),
+                      dh ** -0.5 if scale is None else float(scale), table_type, bool(bidirectional), bool(causal), 0)
 
     def problem(self, out, lse) -> bytes:
-        return _PROBLEM.pack(*self._head, out.data_ptr(), out.stride(0), out.stride(1), 0 if lse is None else lse.data_ptr(),
-                             *[0 if x is None else x for x in self._tail])
+        o0, o1, _ = out.stride()
+        return _PROBLEM.pack(*self._head, out.data_ptr(), o0, o1, 0 if lse is None else lse.data_ptr(), *self._tail)
 
     def reads(self):
         return [t for t in (self.q, self.k, self.v, self.lengths, self.mask, self.start, self.table) if t is not None]

@@ -93,6 +93,9 @@ def test_refusals_beside_a_gpu():
             cross_attention(q, k, v, **kw)
     with pytest.raises(ValueError, match="table must be"):
         text_attention(q, k, v, table_of(32, 3))
+    for buckets, match in ((0, "no buckets"), (2, "two buckets"), (31, "halve")):
+        with pytest.raises(ValueError, match=match):
+            text_attention(q, k, v, table_of(buckets, 4))
     with pytest.raises(ValueError, match="q_start"):
         text_attention(q, k, v, q_start=1 << 30)
     with pytest.raises(ValueError, match="q_start"):
