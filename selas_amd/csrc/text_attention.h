@@ -265,6 +265,10 @@ struct Tile {
   };
 };
 
+// The kernels are built for 64, 96 and 128 channels; 96 are laid out as 128, whose last quarter no instruction reads.
+template <int D>
+using TileOf = Tile<D == 64 ? 64 : 128>;
+
 // A wave's 32 rows as the B operand, in registers for the whole loop: lane (c, h) holds channels 16 s + 8 h .. + 8 of row c.
 // Rows that do not exist and channels from dh on are zeros.
 template <int D>
@@ -308,6 +312,7 @@ __device__ __forceinline__ uint64_t up_to(int n) { return n < 0 ? 0ull : n >= 63
 // ------------------------------------------------------------------ host side
 
 int cu_count();
+inline int width_of(int dh) { return dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 // Fills and checks the arguments; `pointers`: of a call, not only of a question about sizes.
 int check_args(const char *what, const selas_text_attention_problem *p, int dtype, bool pointers, Args &a);
 // Which work item a block takes: the XCDs, which blocks reach in turn, take chunks of consecutive items in turn. One chunk

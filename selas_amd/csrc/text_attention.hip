@@ -324,7 +324,7 @@ __device__ __forceinline__ Item item_at(const Args &a, const Cut &cut, int t, in
 // product's operand wants them).
 template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, Cut cut) {
-  using T = Tile<D>;
+  using T = TileOf<D>;
   constexpr int KJ = T::kLoads / NW;
   static_assert(KJ * NW == T::kLoads, "loads per wave");
   constexpr bool kTwo = D == 64;  // two stages of the values as well
@@ -771,12 +771,13 @@ struct Plan {
 
 Plan plan_of(const Args &a) {
   Plan p{};
-  p.D = a.dh <= 64 ? 64 : 128;
+  p.D = width_of(a.dh);
   const int64_t cu = cu_count();
   const int64_t rows = static_cast<int64_t>(a.group) * a.Lq, items = static_cast<int64_t>(a.B) * a.Hk;
   if (rows <= 8) {
     p.few = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
     p.nw = 8;
+    p.D = a.dh <= 64 ? 64 : 128;
     const int unit = (p.few <= 2 ? 8 : 2) * (512 / p.D);
     const int64_t units = cdiv(a.Lk, unit);
     // Parts for two workgroups a CU, of four units a wave at least.
@@ -825,11 +826,13 @@ void launch_tiles(const Args &a, const Plan &p, float *ws, hipStream_t st) {
 
 template <bool BF, int D, bool BIAS>
 void launch(const Args &a, const Plan &p, float *ws, hipStream_t st) {
-  switch (p.few) {
-    case 1: return launch_few<BF, D, 1, BIAS>(a, p, ws, st);
-    case 2: return launch_few<BF, D, 2, BIAS>(a, p, ws, st);
-    case 4: return launch_few<BF, D, 4, BIAS>(a, p, ws, st);
-    case 8: return launch_few<BF, D, 8, BIAS>(a, p, ws, st);
+  if constexpr (D != 96) {
+    switch (p.few) {
+      case 1: return launch_few<BF, D, 1, BIAS>(a, p, ws, st);
+      case 2: return launch_few<BF, D, 2, BIAS>(a, p, ws, st);
+      case 4: return launch_few<BF, D, 4, BIAS>(a, p, ws, st);
+      case 8: return launch_few<BF, D, 8, BIAS>(a, p, ws, st);
+    }
   }
   switch (p.nw) {
     case 1: return launch_tiles<BF, D, 1, BIAS>(a, p, ws, st);
@@ -882,8 +885,9 @@ extern "C" int selas_text_attention(const selas_text_attention_problem *problem,
     else launch<kBf, kD, false>(a, p, ws, st);
   };
   using I64 = std::integral_constant<int, 64>;
+  using I96 = std::integral_constant<int, 96>;
   using I128 = std::integral_constant<int, 128>;
-  if (dtype == SELAS_BF16) p.D == 64 ? go(std::true_type{}, I64{}) : go(std::true_type{}, I128{});
-  else p.D == 64 ? go(std::false_type{}, I64{}) : go(std::false_type{}, I128{});
+  if (dtype == SELAS_BF16) p.D == 64 ? go(std::true_type{}, I64{}) : p.D == 96 ? go(std::true_type{}, I96{}) : go(std::true_type{}, I128{});
+  else p.D == 64 ? go(std::false_type{}, I64{}) : p.D == 96 ? go(std::false_type{}, I96{}) : go(std::false_type{}, I128{});
   return check_launch("text_attention");
 }

@@ -118,7 +118,7 @@ __device__ __forceinline__ float ds_shift(const Args &a, const Grads &w, int b, 
 // 100 us there.
 template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cut) {
-  using T = Tile<D>;
+  using T = TileOf<D>;
   constexpr int KJ = T::kLoads / NW, kStats = 2 * kRows * 4;
   __shared__ __attribute__((aligned(16))) uint8_t smem0[2 * T::kBytes + kStats], smem1[2 * T::kBytes + kStats];
   extern __shared__ __attribute__((aligned(16))) float tables[];  // two heads' bias by distance
@@ -349,7 +349,7 @@ struct Diagonals {
 
 template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a, Grads w, Cut cut) {
-  using T = Tile<D>;
+  using T = TileOf<D>;
   constexpr int KJ = T::kLoads / NW;
   __shared__ __attribute__((aligned(16))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
   extern __shared__ __attribute__((aligned(16))) float table[];
@@ -659,7 +659,7 @@ constexpr int kNW = 4;
 
 Plan plan_of(const Args &a, bool bf) {
   Plan p{};
-  p.D = a.dh <= 64 ? 64 : 128;
+  p.D = width_of(a.dh);
   p.qblocks = static_cast<int>(cdiv(a.Lq, kRows));
   p.kblocks = static_cast<int>(cdiv(a.Lk, kRows));
   p.buckets = a.bias.ahead ? 2 * a.bias.n : a.bias.n;
@@ -777,8 +777,9 @@ extern "C" int selas_text_attention_backward(const selas_text_attention_problem 
     else launch<kBf, kD, false>(a, w, p, st);
   };
   using I64 = std::integral_constant<int, 64>;
+  using I96 = std::integral_constant<int, 96>;
   using I128 = std::integral_constant<int, 128>;
-  if (bf) p.D == 64 ? go(std::true_type{}, I64{}) : go(std::true_type{}, I128{});
-  else p.D == 64 ? go(std::false_type{}, I64{}) : go(std::false_type{}, I128{});
+  if (bf) p.D == 64 ? go(std::true_type{}, I64{}) : p.D == 96 ? go(std::true_type{}, I96{}) : go(std::true_type{}, I128{});
+  else p.D == 64 ? go(std::false_type{}, I64{}) : p.D == 96 ? go(std::false_type{}, I96{}) : go(std::false_type{}, I128{});
   return check_launch(what);
 }

@@ -145,3 +145,11 @@ def test_later_tokens_over_a_cache_equal_the_whole_texts_rows(lq):
     assert torch.equal(out, text_attention(last, k, v, table, q_start=start.long(), lengths=lengths.long(), **kw))
     same = text_attention(last, k, v, table, q_start=300, **kw)
     assert torch.equal(same, text_attention(last, k, v, table, q_start=torch.full((b,), 300).cuda(), **kw))
+
+
+@pytest.mark.parametrize("dh", [8, 32, 48, 56, 80, 88, 96, 104, 120])
+@pytest.mark.parametrize("lq", [3, 70, 200])
+def test_head_dims(dh, lq):
+    q, k, v = inputs(2, 4, 2, lq, 210, dh, seed=dh + lq)
+    check(cross_attention, q, k, v)
+    check(text_attention, q, k, v, table_of(32, 4), causal=True, q_start=5)

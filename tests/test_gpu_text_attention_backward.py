@@ -167,3 +167,11 @@ def test_gradients_lose_no_more_than_two_roundings(l, dtype, half):
     got = text_attention_backward(grad, q, k, v, out, lse, table, **kw)
     for y, (ref, _) in zip(got, Reference(q, k, v, table, **kw).backward(grad)):
         assert (y.cpu().double() - ref).norm() <= 1.1 * 0.6 * half * ref.norm()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dh", [8, 32, 48, 56, 80, 88, 96, 104, 120])
+def test_head_dims(dh, dtype):
+    q, k, v = inputs(2, 4, 2, 150, 210, dh, seed=dh, dtype=dtype)
+    check(q, k, v)
+    check(q, k, v, table_of(32, 4), causal=True, q_start=5)
