@@ -565,7 +565,7 @@ typedef struct selas_text_attention_problem {
 /*
  * s_ij = scale * q_i . k_j + table[bucket(j - (start + i)), h];  out_i = sum_j softmax_j(s_ij) v_j over the keys
  * that query i sees; lse_i = log(sum_j exp(s_ij)). A query that sees no key gets zeros and an lse of -inf. What
- * masked keys and values hold (NaN, infinities) does not reach a result. dtype (bf16 or fp16, otherwise SELAS_EUNSUPPORTED)
+ * keys and values that no query sees hold (NaN, infinities) does not reach a result. dtype (bf16 or fp16, otherwise SELAS_EUNSUPPORTED)
  * is that of q, k, v and out; scores, maxima and sums are fp32, the probabilities are rounded to dtype for the second product.
  * Takes Dh a multiple of 8 up to 128, addresses of 16 bytes and strides of 8 elements (out: 8 bytes and 4 elements), row
  * strides up to 2^23 elements; otherwise SELAS_EUNSUPPORTED. scale is in 1e-10 .. 1e10. out and lse overlap nothing.

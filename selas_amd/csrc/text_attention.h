@@ -63,12 +63,15 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ int scalar_load(const int32_t *p, int i) {
   return reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(p))[uniform(i)];
 }
-__device__ __forceinline__ int keys_of(const Args &a, int b) {
-  return a.lengths ? min(max(scalar_load(a.lengths, b), 0), a.Lk) : a.Lk;
-}
 __device__ __forceinline__ int start_of(const Args &a, int b) {
   const int s = a.start ? scalar_load(a.start, b) : a.start0;
   return min(max(s, -(1 << 29)), 1 << 29);
+}
+// With a causal mask the keys past the last query's position are none: what they hold must not reach a product either.
+__device__ __forceinline__ int keys_of(const Args &a, int b) {
+  int n = a.lengths ? min(scalar_load(a.lengths, b), a.Lk) : a.Lk;
+  if (a.causal) n = min(n, start_of(a, b) + a.Lq);
+  return max(n, 0);
 }
 
 __device__ __forceinline__ int split(int v, FastDiv by, int d, int &rest) {  // v % d, and rest = v / d

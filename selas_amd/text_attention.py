@@ -180,7 +180,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, length
 
     H is a multiple of Hk: query head h reads key head h // (H // Hk). Any strides (views of linears' outputs); what the
     kernels cannot read in 16-byte chunks is copied first. ``lengths`` [B] (int32, int64): image b has its first lengths[b]
-    keys. ``mask`` [B, Lk] or [1, Lk] (bool): True where the key is seen. What keys that are not seen hold does not
+    keys. ``mask`` [B, Lk] or [1, Lk] (bool): True where the key is seen. What keys that no query sees hold does not
     matter, NaN included; a query that sees none gets zeros and an lse of -inf. ``scale``: 1 / sqrt(Dh) unless given.
     ``out``: optional destination with unit column stride and rows of whole 8 bytes, overlapping nothing the call reads.
 
@@ -201,7 +201,8 @@ def text_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: tor
     the query, and bucket 0 for those after it) distance a has bucket a below n // 2, and above it
     n // 2 + floor((n - n // 2) log(a / (n // 2)) / log(max_distance / (n // 2))), at most n - 1; keys after the query
     have the second half. Distances are compared in exact arithmetic. 2 to 128 buckets a direction, max_distance up to 512.
-    ``causal``: a query sees the keys up to its own position. For one more token over a cache give q [B, H, 1, Dh],
+    ``causal``: a query sees the keys up to its own position (a NaN in the value of a key that later queries see reaches
+    the earlier ones too, as in a product with weights of 0). For one more token over a cache give q [B, H, 1, Dh],
     ``lengths`` and ``q_start = lengths - 1`` (int32: no conversion)."""
     return _forward("text_attention", q, k, v, table, max_distance, bidirectional, causal, q_start, lengths, mask, scale, out,
                     return_lse)

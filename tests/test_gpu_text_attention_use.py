@@ -218,3 +218,19 @@ def test_an_encoders_layer_and_what_reads_its_states(dtype):
     for y, want in zip(got, first.backward(dout)):
         within(y, *want)
     assert not got[1][1, :, 31:].any() and not got[2][1, :, 31:].any()
+
+
+@pytest.mark.parametrize("lq,group", [(1, 1), (2, 4), (40, 2), (150, 1)])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_a_cache_whose_later_keys_were_never_written(lq, group, dh):
+    # No lengths: the causal mask alone says where the text ends, for each at a place of its own.
+    b, hk, lk = 3, 2, 400
+    q, k, v = inputs(b, hk * group, hk, lq, lk, dh, seed=lq)
+    start = torch.tensor([0, 63, 217], dtype=torch.int32).cuda()
+    table = table_of(32, hk * group)
+    kw = dict(causal=True, q_start=start, bidirectional=False)
+    want = step(q, k, v, table, **kw)
+    later = (torch.arange(lk, device="cuda") >= start[:, None] + lq)[:, None, :, None]
+    got = step(q, k.masked_fill(later, float("nan")), v.masked_fill(later, float("inf")), table, **kw)
+    assert same(got, want) and not any(x.isnan().any() for x in got)
+    assert not got[3].masked_select(later).any() and not got[4].masked_select(later).any()
