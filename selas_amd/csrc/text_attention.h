@@ -105,6 +105,10 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 }
 
 template <bool BF>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack<BF>(v[0], v[1]), pack<BF>(v[2], v[3]), pack<BF>(v[4], v[5]), pack<BF>(v[6], v[7]));
+}
+template <bool BF>
 __device__ __forceinline__ float lo_of(uint32_t w) {
   return BF ? __uint_as_float(w << 16) : f16_bits_to_f32(static_cast<uint16_t>(w));
 }

@@ -378,7 +378,9 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
     const int pos = x.start + x.row0 + c;
     f32x16 sc[2] = {f32x16{}, f32x16{}};
 #pragma unroll
-    for (int i = 0; i < 2 * (D / 16); ++i) sc[i / (D / 16)] = mfma<BF>(rows.read(ks, i / (D / 16), i % (D / 16)), q.f[i % (D / 16)], sc[i / (D / 16)]);
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) sc[kb] = mfma<BF>(rows.read(ks, kb, i), q.f[i], sc[kb]);
     if (BIAS && near) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -518,8 +520,9 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
       for (int u = 0; u < 2; ++u) {
         const f32x16 &z = o[i >> 2];
         const int y = 4 * (i & 3) + 2 * u;
-        const auto p = __builtin_amdgcn_permlane32_swap(pack<BF>(materialize(z[y] * inv), materialize(z[y + 1] * inv)),
-                                                        pack<BF>(materialize(z[y + 4] * inv), materialize(z[y + 5] * inv)), false, false);
+        const uint32_t lo = pack<BF>(materialize(z[y] * inv), materialize(z[y + 1] * inv));
+        const uint32_t hi = pack<BF>(materialize(z[y + 4] * inv), materialize(z[y + 5] * inv));
+        const auto p = __builtin_amdgcn_permlane32_swap(lo, hi, false, false);
         w[0][u] = p[0];
         w[1][u] = p[1];
       }
@@ -887,7 +890,8 @@ extern "C" int selas_text_attention(const selas_text_attention_problem *problem,
   using I64 = std::integral_constant<int, 64>;
   using I96 = std::integral_constant<int, 96>;
   using I128 = std::integral_constant<int, 128>;
-  if (dtype == SELAS_BF16) p.D == 64 ? go(std::true_type{}, I64{}) : p.D == 96 ? go(std::true_type{}, I96{}) : go(std::true_type{}, I128{});
-  else p.D == 64 ? go(std::false_type{}, I64{}) : p.D == 96 ? go(std::false_type{}, I96{}) : go(std::false_type{}, I128{});
+  auto width = [&](auto bf) { p.D == 64 ? go(bf, I64{}) : p.D == 96 ? go(bf, I96{}) : go(bf, I128{}); };
+  if (dtype == SELAS_BF16) width(std::true_type{});
+  else width(std::false_type{});
   return check_launch("text_attention");
 }

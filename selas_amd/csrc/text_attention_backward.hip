@@ -215,8 +215,7 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
             ds[e] = materialize(p[e] * (dp[r] - dd[y]) * ds_mul);
           }
         }
-        const uint4 pb = make_uint4(pack<BF>(p[0], p[1]), pack<BF>(p[2], p[3]), pack<BF>(p[4], p[5]), pack<BF>(p[6], p[7]));
-        const uint4 sb = make_uint4(pack<BF>(ds[0], ds[1]), pack<BF>(ds[2], ds[3]), pack<BF>(ds[4], ds[5]), pack<BF>(ds[6], ds[7]));
+        const uint4 pb = pack8<BF>(p), sb = pack8<BF>(ds);
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) {
           dv[db] = mfma<BF>(cols.read(gs, db, qb, t2), pb, dv[db]);
@@ -487,7 +486,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
         float ds[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) ds[e] = BF ? s[8 * t2 + e] : materialize(s[8 * t2 + e] * ds_mul);
-        sb[t2] = make_uint4(pack<BF>(ds[0], ds[1]), pack<BF>(ds[2], ds[3]), pack<BF>(ds[4], ds[5]), pack<BF>(ds[6], ds[7]));
+        sb[t2] = pack8<BF>(ds);
       }
 #pragma unroll
       for (int t2 = 0; t2 < 2; ++t2)
@@ -565,7 +564,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
     }
     __syncthreads();
     const int n = a.bias.n, buckets = a.bias.ahead ? 2 * n : n;
-    float *out = w.dtable_part + ((static_cast<int64_t>(b) * a.H + head) * cut.tiles * cut.parts + qt * cut.parts + part) * buckets;
+    const int64_t bh = static_cast<int64_t>(b) * a.H + head;
+    float *out = w.dtable_part + ((bh * cut.tiles + qt) * cut.parts + part) * buckets;
     for (int r = wave; r < buckets; r += NW) {
       const bool up = r >= n;  // keys after the query
       const int bt = up ? r - n : r;
@@ -696,10 +696,13 @@ template <bool BF, int D, bool BIAS>
 void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
   const int reach = a.bias.reach;
   auto sum = [&](const Cut &cut, int64_t rows, int arrays, uint16_t *y0, uint16_t *y1) {
+    const int64_t n = rows * a.dh;
     if (cut.parts > 1)
-      sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(rows * a.dh, 1024)), arrays), dim3(256), 0, st>>>(cut.partial, cut.parts, rows * a.dh, arrays, y0, y1);
+      sum_kernel<BF><<<dim3(static_cast<uint32_t>(cdiv(n, 1024)), arrays), dim3(256), 0, st>>>(cut.partial, cut.parts, n, arrays,
+                                                                                               y0, y1);
   };
-  if (!BF && p.query.deal.total + p.key.deal.total) norm_kernel<<<dim3(a.B * a.H * p.qblocks + a.B * a.Hk * p.kblocks), dim3(256), 0, st>>>(a, w);
+  const int norms = a.B * a.H * p.qblocks + a.B * a.Hk * p.kblocks;
+  if (!BF && norms) norm_kernel<<<dim3(norms), dim3(256), 0, st>>>(a, w);
   if (p.query.deal.total) {
     const size_t lds = BIAS ? bias_bytes(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
     query_kernel<BF, D, kNW, BIAS><<<dim3(p.query.deal.blocks), dim3(64 * kNW), lds, st>>>(a, w, p.query);
@@ -779,7 +782,8 @@ extern "C" int selas_text_attention_backward(const selas_text_attention_problem 
   using I64 = std::integral_constant<int, 64>;
   using I96 = std::integral_constant<int, 96>;
   using I128 = std::integral_constant<int, 128>;
-  if (bf) p.D == 64 ? go(std::true_type{}, I64{}) : p.D == 96 ? go(std::true_type{}, I96{}) : go(std::true_type{}, I128{});
-  else p.D == 64 ? go(std::false_type{}, I64{}) : p.D == 96 ? go(std::false_type{}, I96{}) : go(std::false_type{}, I128{});
+  auto width = [&](auto t) { p.D == 64 ? go(t, I64{}) : p.D == 96 ? go(t, I96{}) : go(t, I128{}); };
+  if (bf) width(std::true_type{});
+  else width(std::false_type{});
   return check_launch(what);
 }

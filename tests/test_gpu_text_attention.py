@@ -153,3 +153,11 @@ def test_head_dims(dh, lq):
     q, k, v = inputs(2, 4, 2, lq, 210, dh, seed=dh + lq)
     check(cross_attention, q, k, v)
     check(text_attention, q, k, v, table_of(32, 4), causal=True, q_start=5)
+
+
+@pytest.mark.parametrize("lq,h,hk", [(1, 8, 1), (150, 4, 2)])
+def test_the_widest_tables(lq, h, hk):
+    # As much LDS as a call can take: 128 channels and the largest distances.
+    q, k, v = inputs(1, h, hk, lq, 1300, 128, seed=lq)
+    check(text_attention, q, k, v, table_of(256, h), max_distance=512, q_start=600)
+    check(text_attention, q, k, v, table_of(128, h), max_distance=512, bidirectional=False, causal=True, q_start=1100)

@@ -175,3 +175,11 @@ def test_head_dims(dh, dtype):
     q, k, v = inputs(2, 4, 2, 150, 210, dh, seed=dh, dtype=dtype)
     check(q, k, v)
     check(q, k, v, table_of(32, 4), causal=True, q_start=5)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_the_widest_tables(dtype):
+    # As much LDS as a call can take: 128 channels and the largest distances.
+    q, k, v = inputs(1, 4, 2, 150, 1300, 128, seed=1, dtype=dtype)
+    check(q, k, v, table_of(256, 4), max_distance=512, q_start=600)
+    check(q, k, v, table_of(128, 4), max_distance=512, bidirectional=False, causal=True, q_start=1100)
