@@ -626,6 +626,12 @@ __global__ __launch_bounds__(256) void sum_kernel(const float *__restrict__ part
       make_uint2(pack<BF>(materialize(s.x), materialize(s.y)), pack<BF>(materialize(s.z), materialize(s.w)));
 }
 
+// dk and dv of n values each where there are no queries; 4 values a thread. blockIdx.y: dv.
+__global__ __launch_bounds__(256) void zero_kernel(int64_t n, uint16_t *dk, uint16_t *dv) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i < n) *reinterpret_cast<uint2 *>((blockIdx.y ? dv : dk) + i) = make_uint2(0, 0);
+}
+
 // dtable[r, head] = the sum over images and workgroups, in a fixed order. One workgroup per head.
 __global__ __launch_bounds__(256) void dtable_kernel(const float *__restrict__ part, int B, int H, int each, int buckets,
                                                      void *dtable, int dtype) {
@@ -692,6 +698,18 @@ Plan plan_of(const Args &a, bool bf) {
   return p;
 }
 
+void sum_table(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
+  dtable_kernel<<<dim3(a.H), dim3(256), 0, st>>>(w.dtable_part, a.B, a.H, p.query.tiles * p.query.parts, p.buckets, w.dtable,
+                                                 a.bias.dtype);
+}
+
+// Without queries every gradient is zero. q, k and v are not looked at (their pointers were not checked).
+void launch_zeros(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
+  const int64_t n = static_cast<int64_t>(a.B) * a.Hk * a.Lk * a.dh;
+  if (n) zero_kernel<<<dim3(static_cast<uint32_t>(cdiv(n, 1024)), 2), dim3(256), 0, st>>>(n, w.dk, w.dv);
+  if (a.bias.table) sum_table(a, w, p, st);
+}
+
 template <bool BF, int D, bool BIAS>
 void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
   const int reach = a.bias.reach;
@@ -712,9 +730,7 @@ void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
     key_kernel<BF, D, kNW, BIAS><<<dim3(p.key.deal.blocks), dim3(64 * kNW), BIAS ? 2 * bias_bytes(reach) : 0, st>>>(a, w, p.key);
     sum(p.key, static_cast<int64_t>(a.B) * a.Hk * a.Lk, 2, w.dk, w.dv);
   }
-  if constexpr (BIAS)
-    dtable_kernel<<<dim3(a.H), dim3(256), 0, st>>>(w.dtable_part, a.B, a.H, p.query.tiles * p.query.parts, p.buckets, w.dtable,
-                                                   a.bias.dtype);
+  if constexpr (BIAS) sum_table(a, w, p, st);
 }
 
 }  // namespace
@@ -773,6 +789,10 @@ extern "C" int selas_text_attention_backward(const selas_text_attention_problem 
   p.key.partial = at(p.key_partial);
   p.query.partial = at(p.query_partial);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (!a.B || !a.Lq) {
+    launch_zeros(a, w, p, st);
+    return check_launch(what);
+  }
   auto go = [&](auto t, auto d) {
     constexpr bool kBf = decltype(t)::value;
     constexpr int kD = decltype(d)::value;
