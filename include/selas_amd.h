@@ -533,8 +533,8 @@ int selas_raw_linear_tile(const selas_raw_linear_problem *problems, int64_t coun
 /* ------------------------------------------------------------ attention of the text side */
 
 /* One call of selas_text_attention (host memory): q [B, H, Lq, Dh], k and v [B, Hk, Lk, Dh] with unit channel stride and
- * any batch, head and row strides (*_sb, *_sh, *_sl, elements), H a multiple of Hk; query head h reads key head
- * h / (H / Hk). out is [B, Lq, H*Dh] (o_sb, o_sl); lse [B, H, Lq] fp32, contiguous, or NULL.
+ * any batch, head and row strides (*_sb, *_sh, *_sl, elements; that of an axis of one element is not looked at, but not
+ * negative), H a multiple of Hk; query head h reads key head h / (H / Hk). out is [B, Lq, H*Dh] (o_sb, o_sl); lse [B, H, Lq] fp32, contiguous, or NULL.
  * Key j of image b exists where j < lengths[b] (NULL: all Lk; values outside 0 .. Lk count as the nearer end) and
  * mask[b * mask_sb + j] != 0 (NULL: all). start[b], or start0 where start is NULL, is the position of the image's first
  * query among the keys' positions 0 .. Lk - 1: with causal != 0 query i sees the keys j <= start + i.

@@ -319,6 +319,9 @@ __device__ __forceinline__ uint64_t up_to(int n) { return n < 0 ? 0ull : n >= 63
 // ------------------------------------------------------------------ host side
 
 int cu_count();
+// A stride as the kernels take it. That of an axis of one element says nothing and may be anything: one row's becomes a
+// head's width, so that the rows after it are past the buffers' ranges as they are elsewhere.
+inline int64_t stride_of(int64_t n, int64_t given, int64_t alone) { return n > 1 ? given : alone; }
 inline int width_of(int dh) { return dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 // Fills and checks the arguments; `pointers`: of a call, not only of a question about sizes.
 int check_args(const char *what, const selas_text_attention_problem *p, int dtype, bool pointers, Args &a);

@@ -512,7 +512,7 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
                                                rows > 0 ? 2 * ((rows - 1) * static_cast<uint32_t>(e.out_sl) + e.dh) : 0);
     const uint32_t at = static_cast<uint32_t>(lane & 31) * static_cast<uint32_t>(2 * e.out_sl);
     // Lanes c and c + 32 hold the halves of 8 channels: they exchange halves, and each stores 8 channels of row c.
-    // What does not exist is out of the buffer's range.
+    // What does not exist is steered out of the buffer's range.
 #pragma unroll
     for (int i = 0; i < D / 8; i += 2) {
       uint32_t w[2][2];
@@ -528,7 +528,8 @@ __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, C
       }
       typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
       const int ch = 8 * (i + h);
-      __builtin_amdgcn_raw_buffer_store_b128(u32x4{w[0][0], w[0][1], w[1][0], w[1][1]}, r, ch < e.dh ? at + 2 * ch : kPast, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4{w[0][0], w[0][1], w[1][0], w[1][1]}, r,
+                                             ch < e.dh && row < e.Lq ? at + 2 * ch : kPast, 0, 0);
     }
   }
 }
@@ -689,9 +690,13 @@ int fill_buckets(const char *what, int64_t buckets, int64_t max_distance, int bi
   return SELAS_OK;
 }
 
-int check_side(const char *what, const char *name, const void *p, int64_t sb, int64_t sh, int64_t sl, Side &side) {
+int check_side(const char *what, const char *name, const void *p, int64_t sb, int64_t sh, int64_t sl, const Args &a, int heads,
+               int rows, Side &side) {
   if (!p) return set_error(SELAS_EINVAL, "%s: null pointer (%s)", what, name);
   if (sb < 0 || sh < 0 || sl < 0) return set_error(SELAS_EINVAL, "%s: %s has a negative stride", what, name);
+  sb = stride_of(a.B, sb, 0);
+  sh = stride_of(heads, sh, 0);
+  sl = stride_of(rows, sl, a.dh);
   if (!aligned(p, 16) || sb % 8 || sh % 8 || sl % 8)
     return set_error(SELAS_EUNSUPPORTED, "%s: %s must be 16-byte aligned with strides of whole 16 bytes", what, name);
   if (sl > (1 << 23)) return set_error(SELAS_EUNSUPPORTED, "%s: %s has a row stride above 2^23 elements", what, name);
@@ -746,19 +751,19 @@ int check_args(const char *what, const selas_text_attention_problem *p, int dtyp
   a.start = p->start;
   a.start0 = static_cast<int>(std::min<int64_t>(std::max<int64_t>(p->start0, -(1 << 29)), 1 << 29));
   if (!pointers || p->B == 0 || p->H == 0 || p->Lq == 0) return SELAS_OK;
-  if (int e = check_side(what, "q", p->q, p->q_sb, p->q_sh, p->q_sl, a.q)) return e;
+  if (int e = check_side(what, "q", p->q, p->q_sb, p->q_sh, p->q_sl, a, a.H, a.Lq, a.q)) return e;
   if (p->Lk) {  // without keys there may be no memory
-    if (int e = check_side(what, "k", p->k, p->k_sb, p->k_sh, p->k_sl, a.k)) return e;
-    if (int e = check_side(what, "v", p->v, p->v_sb, p->v_sh, p->v_sl, a.v)) return e;
+    if (int e = check_side(what, "k", p->k, p->k_sb, p->k_sh, p->k_sl, a, a.Hk, a.Lk, a.k)) return e;
+    if (int e = check_side(what, "v", p->v, p->v_sb, p->v_sh, p->v_sl, a, a.Hk, a.Lk, a.v)) return e;
   }
   if (!p->out) return set_error(SELAS_EINVAL, "%s: null pointer (out)", what);
   if (p->o_sb < 0 || p->o_sl < 0 || p->mask_sb < 0) return set_error(SELAS_EINVAL, "%s: negative stride", what);
-  if (!aligned(p->out, 8) || p->o_sb % 4 || p->o_sl % 4)
-    return set_error(SELAS_EUNSUPPORTED, "%s: out must be 8-byte aligned with strides of whole 8 bytes", what);
-  if (p->o_sl > (1 << 23)) return set_error(SELAS_EUNSUPPORTED, "%s: out has a row stride above 2^23 elements", what);
   a.out = static_cast<uint16_t *>(p->out);
-  a.out_sb = p->o_sb;
-  a.out_sl = p->o_sl;
+  a.out_sb = stride_of(a.B, p->o_sb, 0);
+  a.out_sl = stride_of(a.Lq, p->o_sl, a.dh);
+  if (!aligned(p->out, 8) || a.out_sb % 4 || a.out_sl % 4)
+    return set_error(SELAS_EUNSUPPORTED, "%s: out must be 8-byte aligned with strides of whole 8 bytes", what);
+  if (a.out_sl > (1 << 23)) return set_error(SELAS_EUNSUPPORTED, "%s: out has a row stride above 2^23 elements", what);
   return SELAS_OK;
 }
 

@@ -126,7 +126,8 @@ def _forward(what, q, k, v, table, max_distance, bidirectional, causal, q_start,
         out = torch.empty(b, lq, h * dh, dtype=q.dtype, device=call.dev)
     else:
         if (out.shape != (b, lq, h * dh) or out.dtype != q.dtype or out.device != call.dev
-                or (h * dh > 1 and out.stride(2) != 1) or (out.stride(0) | out.stride(1)) & 3 or out.data_ptr() & 7):
+                or (h * dh > 1 and out.stride(2) != 1) or (b > 1 and out.stride(0) & 3) or (lq > 1 and out.stride(1) & 3)
+                or out.data_ptr() & 7):
             raise ValueError(f"{what}: out must be [{b}, {lq}, {h * dh}] {q.dtype} on {call.dev} with unit column stride and "
                              f"rows of whole 8 bytes, got {tuple(out.shape)} {out.dtype} strides {out.stride()}")
         if not distinct(out):
