@@ -762,7 +762,6 @@ extern "C" int selas_text_attention_backward(const selas_text_attention_problem 
   if (a.B && a.Lq) {
     if (!grad || !a.lse || !dq) return set_error(SELAS_EINVAL, "%s: null pointer (grad, lse or dq)", what);
     if (g_sb < 0 || g_sl < 0) return set_error(SELAS_EINVAL, "%s: grad has a negative stride", what);
-    g_sb = stride_of(a.B, g_sb, 0);
     g_sl = stride_of(a.Lq, g_sl, a.dh);
     if (!aligned(grad, 16) || g_sb % 8 || g_sl % 8 || g_sl > (1 << 23))
       return set_error(SELAS_EUNSUPPORTED, "%s: grad must be 16-byte aligned with strides of whole 16 bytes, rows up to 2^23 elements", what);
