@@ -40,6 +40,8 @@ struct Cut {
   Deal deal;
   FastDiv by_tiles, by_parts, by_group, by_hk;
   float *partial;
+  float2 *missing;  // query_kernel with parts: [parts][B, H, Lqp], the sums of dS and of |dS|
+  int again;        // its second launch
 };
 
 // fp16: the largest squared norm among 64 rows of dO, or (blocks past the queries') of 64 values; 4 lanes to a row.
@@ -295,7 +297,7 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
 // held. S^T = K Q^T and dP^T = V dO^T leave a lane's registers with keys of one query, in runs of 8; dQ^T += K^T dS^T reads
 // the same K tile transposed.
 //
-// Bounded as key_kernel: 3 products of 7, 128 to 143 registers at D = 64 (61 us at 4 x 64 heads of 512 with a bias), 201 at
+// Bounded as key_kernel: 3 products of 7, 153 to 168 registers at D = 64 (61 us at 4 x 64 heads of 512 with a bias), 223 at
 // D = 128 (66 to 72 us at 4096 queries over 512 keys).
 //
 // dtable: tiles that hold only one value of the bias add dS up in a register. In the others dS is summed along the diagonals
@@ -306,12 +308,23 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
 // instruction: all gradients of 16 x 64 heads of 512 with a bias 1160 us, this way 567 at the time.
 //
 // D is first the product of dO and out in the order of the matrix unit, as dP is: where a row sees one key, out is that key's
-// value and dS is exactly 0. But out was rounded, and where few keys carry a row, D's share of that is as large as the
-// roundings of dS and of the result. So rows that see up to 64 kRefine keys add what the sum of p (dP - D) over all their
-// keys says is missing, by a pass over those tiles ahead of the others (77 keys: 14.4 -> 20.9 us; errors of dq against 64 bits
-// 1.65 -> 1.4 times those of one rounding). Where weight is spread over more keys out is small beside the values, and so is
-// that share: from 257 seen keys on it is left in, also where a few of them carry the row.
+// value and dS is exactly 0. But out was rounded, and where a few keys carry a row, or all values are alike, dP - D is small
+// beside dP and D, and D's share of that rounding is many times those of dS and of the result. The sum of dS over a row's keys
+// is 0 but for that share, so it says what D lacks. Workgroups of up to kRefine tiles of keys take that sum in a pass over them
+// ahead of the others (77 keys: 14.4 -> 20.9 us). Longer ones take it, and the sum of |dS|, as they go; where in any of their
+// rows it is above off_limit of the latter, three quarters of half a step of dS, they add it to D and begin again. Where
+// the keys are in parts, a second launch does both, of which most workgroups end at once.
+// Errors of dq against 64 bits in the 2-norm, in halves of a step, out's rounding left in / this way (0.6 is two roundings):
+// 600 causal keys with 0.97 of the weight on a row's own 6.9 / 0.59; 3 seen keys of 300 0.93 / 0.60; 600 keys and scores of
+// deviation 3 0.92 / 0.61; scores of deviation 1 0.61 / 0.61. It costs 2 % (the two sums; 24 heads of 128, 4096 queries over 512
+// keys, all of forward and backward 174 -> 177 us), 4 % where a few rows of most heads are that far off (4 x 64 heads of 512
+// with a random bias: 151 -> 157; at half instead of three quarters 160, with nothing gained), 8 % in parts (64 queries over
+// 20,280 keys: 101 -> 109). Two launches in every case instead: 180 and 195 for the first two.
 constexpr int kSpill = 112, kRefine = 4;
+template <bool BF>
+__device__ constexpr float off_limit() {
+  return BF ? 0x1.8p-9f : 0x1.8p-12f;
+}
 __host__ __device__ inline int hist_floats(int reach) { return 2 * reach + 2 * kSpill + 1; }
 
 // Sums along the diagonals of a wave's 32 keys x 32 queries. v[e] of lane q belongs to distance o + e - q. With
@@ -351,6 +364,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   using T = TileOf<D>;
   constexpr int KJ = T::kLoads / NW;
   __shared__ __attribute__((aligned(16))) uint8_t smem0[2 * T::kBytes], smem1[2 * T::kBytes];
+  __shared__ int off[NW];
   extern __shared__ __attribute__((aligned(16))) float table[];
   const int t = item_of(cut.deal);
   if (t >= cut.deal.total) return;
@@ -366,6 +380,30 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   const int per = (ntiles + cut.parts - 1) / cut.parts;
   int kt = part * per;
   const int end = min(ntiles, kt + per);
+
+  // Whether D of any of the workgroup's rows is off by more than it may, where dS sums to `sum` and |dS| to `size`.
+  auto any_off = [&](float sum, float size) __attribute__((always_inline)) {
+    const uint64_t found = __builtin_amdgcn_ballot_w64(fabsf(sum) > off_limit<BF>() * size);
+    if (lane == 0) off[wave] = found != 0;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) any |= off[i];
+    return any != 0;
+  };
+  const int64_t stat = (static_cast<int64_t>(b) * a.H + head) * w.Lqp + row0 + c;
+  float missing = 0.0f, size = 0.0f;  // of this lane's keys: the sums of dS and of |dS|, which is infinite once D is right
+  if (cut.again) {
+    if (row0 + c < w.Lqp)
+      for (int i = h; i < cut.parts; i += 2) {
+        const float2 x = cut.missing[i * (static_cast<int64_t>(a.B) * a.H * w.Lqp) + stat];
+        missing += x.x;
+        size += x.y;
+      }
+    missing = pair_sum(missing);
+    if (!any_off(missing, pair_sum(size))) return;
+    size = __builtin_inff();
+  }
 
   Held<D> q, dO;
   q.load(a.q.p + b * a.q.sb + head * a.q.sh + row0 * a.q.sl, a.q.sl, a.dh, a.Lq - row0, lane);
@@ -387,6 +425,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
     for (int r = 0; r < 16; ++r) d = r == 4 * (c >> 3) + (c & 3) ? x[r] : d;
     dd = pair_sum(h == ((c >> 2) & 1) ? d : 0.0f);
     if (nl == -__builtin_inff()) dd = 0.0f;
+    dd += missing;  // 0 but in the second launch
   }
   const uint16_t *kp = a.k.p + b * a.k.sb + hk * a.k.sh, *vp = a.v.p + b * a.v.sb + hk * a.v.sh;
   const typename T::template Loader<KJ> kl(wave, lane, a.k.sl, a.dh), vl(wave, lane, a.v.sl, a.dh);
@@ -410,9 +449,12 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
   float *hist = table + 4 * pitch;  // [2 NW][span]; after that [NW][2] sums
   float *mine = hist + (2 * wave + h) * span;
   float sum_behind = 0.0f, sum_ahead = 0.0f, far_behind = 0.0f, far_ahead = 0.0f;
+  auto clear_hist = [&]() __attribute__((always_inline)) {
+    for (int i = threadIdx.x; i < 2 * NW * span; i += 64 * NW) hist[i] = 0.0f;
+  };
   if constexpr (BIAS) {
     build_bias(table, a.bias, head, 64 * NW, false);
-    for (int i = threadIdx.x; i < 2 * NW * span; i += 64 * NW) hist[i] = 0.0f;
+    clear_hist();
   }
   const float shift = ds_shift<BF>(a, w, b, hk, lane), ds_mul = BF ? 1.0f : __builtin_exp2f(shift);
 
@@ -476,9 +518,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
         diagonals.add(0, s, lane);
         diagonals.add(1, s, lane);
         diagonals.store(mine + kt * kRows + 32 * kb + 8 * h - pos + reach + kSpill);
-      } else if (BIAS) {
+      }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) add += s[r];
+      for (int r = 0; r < 16; ++r) {
+        add += s[r];
+        size += fabsf(s[r]);
       }
       uint4 sb[2];
 #pragma unroll
@@ -493,8 +537,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) dq[db] = mfma<BF>(cols.read(ks, db, kb, t2), sb[t2], dq[db]);
     }
-    sum_behind += x.behind ? add : 0.0f;
-    sum_ahead += x.behind ? 0.0f : add;
+    missing += add;
+    if constexpr (BIAS) {
+      sum_behind += x.behind ? add : 0.0f;
+      sum_ahead += x.ahead ? add : 0.0f;
+    }
   };
   auto step = [&](int stage) __attribute__((always_inline)) {
     const uint64_t bits_next = keybits.word(kt + 1, byte);
@@ -518,7 +565,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
     }
   };
   if (ntiles <= kRefine) {
-    float missing = 0.0f;
+    float lacks = 0.0f;
     for (int i = 0; i < ntiles; ++i) {
       begin(i);
       const Kind x = kind_of(i);
@@ -526,23 +573,42 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
         for (int kb = 0; kb < 2; ++kb) {
           const f32x16 s = scores(smem0, i, kb, x);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) missing += s[r];
+          for (int r = 0; r < 16; ++r) lacks += s[r];
         }
       __syncthreads();
     }
-    dd += pair_sum(missing);
+    dd += pair_sum(lacks);
+    size = __builtin_inff();
   }
-  if (part == 0 && h == 0 && row0 + c < w.Lqp) {  // for key_kernel
-    const int64_t at = (static_cast<int64_t>(b) * a.H + head) * w.Lqp + row0 + c;
-    w.neg_lse[at] = nl;
-    w.dot[at] = dd;
+  while (true) {
+    if (kt < end) begin(kt);
+    while (kt < end) {
+      step(0);
+      if (++kt >= end) break;
+      step(1);
+      ++kt;
+    }
+    missing = pair_sum(missing);
+    size = pair_sum(size);
+    if (cut.parts > 1) break;
+    if (!any_off(missing, size)) break;  // no wave is at the tiles or the histograms any more
+    dd += missing;
+    size = __builtin_inff();
+    kt = 0;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) dq[db] = f32x16{};
+    if constexpr (BIAS) {
+      sum_behind = sum_ahead = 0.0f;
+      clear_hist();
+    }
   }
-  if (kt < end) begin(kt);
-  while (kt < end) {
-    step(0);
-    if (++kt >= end) break;
-    step(1);
-    ++kt;
+  if (h == 0 && row0 + c < w.Lqp) {
+    if (cut.parts > 1 && !cut.again)
+      cut.missing[part * (static_cast<int64_t>(a.B) * a.H * w.Lqp) + stat] = make_float2(missing, size);
+    if (part == 0) {  // for key_kernel
+      w.neg_lse[stat] = nl;
+      w.dot[stat] = dd;
+    }
   }
 
   if constexpr (BIAS) {
@@ -659,7 +725,7 @@ __global__ __launch_bounds__(256) void dtable_kernel(const float *__restrict__ p
 struct Plan {
   int D, qblocks, kblocks, buckets;
   Cut key, query;
-  int64_t neg_lse, dot, g_norm, v_norm, dtable, key_partial, query_partial, bytes;  // offsets into the workspace
+  int64_t neg_lse, dot, g_norm, v_norm, dtable, key_partial, query_partial, missing, bytes;  // offsets into the workspace
 };
 constexpr int kNW = 4;
 
@@ -675,7 +741,7 @@ Plan plan_of(const Args &a, bool bf) {
     // Workgroups for two to a CU, of four streamed tiles at least.
     const int64_t parts = std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(whole, 1), streamed / 4));
     return Cut{tiles, static_cast<int>(parts), deal(whole * parts, inner, a.lengths || a.mask), fast_div(std::max(tiles, 1)),
-               fast_div(static_cast<uint32_t>(parts)), fast_div(std::max(a.group, 1)), fast_div(std::max(a.Hk, 1)), nullptr};
+               fast_div(static_cast<uint32_t>(parts)), fast_div(std::max(a.group, 1)), fast_div(std::max(a.Hk, 1)), nullptr, nullptr, 0};
   };
   const int ktiles = static_cast<int>(cdiv(a.Lk, 32 * kNW)), qtiles = static_cast<int>(cdiv(a.Lq, 32 * kNW));
   p.key = cut(static_cast<int64_t>(a.B) * a.Hk, ktiles, static_cast<int64_t>(a.group) * p.qblocks, ktiles);
@@ -694,7 +760,10 @@ Plan plan_of(const Args &a, bool bf) {
   }
   if (a.bias.table) p.dtable = take(static_cast<int64_t>(a.B) * a.H * p.query.tiles * p.query.parts * p.buckets);
   if (p.key.parts > 1) p.key_partial = take(2ll * p.key.parts * a.B * a.Hk * a.Lk * a.dh);
-  if (p.query.parts > 1) p.query_partial = take(static_cast<int64_t>(p.query.parts) * a.B * a.H * a.Lq * a.dh);
+  if (p.query.parts > 1) {
+    p.query_partial = take(static_cast<int64_t>(p.query.parts) * a.B * a.H * a.Lq * a.dh);
+    p.missing = take(2 * p.query.parts * stats);
+  }
   return p;
 }
 
@@ -723,7 +792,10 @@ void launch(const Args &a, const Grads &w, const Plan &p, hipStream_t st) {
   if (!BF && norms) norm_kernel<<<dim3(norms), dim3(256), 0, st>>>(a, w);
   if (p.query.deal.total) {
     const size_t lds = BIAS ? bias_bytes(reach) + 4 * (2 * kNW * hist_floats(reach) + 2 * kNW) : 0;
-    query_kernel<BF, D, kNW, BIAS><<<dim3(p.query.deal.blocks), dim3(64 * kNW), lds, st>>>(a, w, p.query);
+    Cut cut = p.query;
+    query_kernel<BF, D, kNW, BIAS><<<dim3(cut.deal.blocks), dim3(64 * kNW), lds, st>>>(a, w, cut);
+    cut.again = 1;
+    if (cut.parts > 1) query_kernel<BF, D, kNW, BIAS><<<dim3(cut.deal.blocks), dim3(64 * kNW), lds, st>>>(a, w, cut);
     sum(p.query, static_cast<int64_t>(a.B) * a.H * a.Lq, 1, w.dq, nullptr);
   }
   if (p.key.deal.total) {
@@ -789,6 +861,7 @@ extern "C" int selas_text_attention_backward(const selas_text_attention_problem 
   w.dtable = dtable;
   p.key.partial = at(p.key_partial);
   p.query.partial = at(p.query_partial);
+  p.query.missing = reinterpret_cast<float2 *>(at(p.missing));
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (!a.B || !a.Lq) {
     launch_zeros(a, w, p, st);

@@ -8,7 +8,10 @@ import torch
 
 from selas_amd.text_attention import (cross_attention, cross_attention_backward, text_attention, text_attention_backward)
 
+from .conftest import seeded
 from .test_gpu_text_attention import BF, F32, FP, inputs, table_of
+from .test_gpu_text_attention_backward import grad_of
+from .text_attention_reference import Reference
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +83,104 @@ def test_gradients_of_one_query_and_one_key_at_any_stride(dtype):
             out, lse = cross_attention(*x, return_lse=True)
             got = (out, lse, *cross_attention_backward(folded(grad, stride), *x, folded(out, stride), lse))
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def roundings(q, k, v, *args, **kw):
+    """Holds the gradients to what rounding dS and each result once costs these very inputs, in the 2-norm against 64 bits.
+
+    Beyond that D may be off where it does not pay to mend it, by three quarters of half a step of what |dS| sums to in the row
+    (`left`, spread evenly below it and over rows: 1 / sqrt(3) of it in the mean square): dS of key j is then off by p times
+    that. A tenth is left for chance. p is rounded for dv, and the table's gradient is not made of rounded dS."""
+    grad = grad_of(q)
+    out, lse = text_attention(q, k, v, *args, return_lse=True, **kw)
+
+    def run():
+        return text_attention_backward(grad, q, k, v, out, lse, *args, **kw)
+
+    got = run()
+    assert all(torch.equal(x, y) for x, y in zip(got, run()) if x is not None)
+    ref = Reference(q, k, v, *args, **kw)
+    want, half, hk = ref.backward(grad), torch.finfo(q.dtype).eps / 2, k.shape[1]
+
+    def rounded(x, like):
+        return x.to(like.dtype).double()
+
+    def shared(x):
+        return x.unflatten(1, (hk, -1)).sum(2)
+
+    g = grad.cpu().double().view(*out.shape[:2], q.shape[1], -1).transpose(1, 2)
+    dp = g @ ref.v.mT
+    ds = ref.p * (dp - (g * ref.o).sum(-1, keepdim=True))
+    left = 0.75 / 3 ** 0.5 * half * ds.abs().sum(-1, keepdim=True)
+    twice = [rounded(ref.scale * rounded(ds, q) @ ref.k, q), rounded(shared(ref.scale * rounded(ds, q).mT @ ref.q), q),
+             rounded(shared(rounded(ref.p, q).mT @ g), q)]
+    share = [ref.scale * left * (ref.p @ ref.k), shared((ref.scale * left * ref.p).mT.square() @ ref.q.square()).sqrt(), 0.0]
+    if want[3] is not None:
+        hot = torch.nn.functional.one_hot(ref.bucket, want[3][0].shape[0]).double()  # [b, lq, lk, buckets]
+        twice.append(rounded(want[3][0], got[3]))
+        share.append(torch.einsum("bhij,bijr->bhir", left * ref.p, hot).square().sum((0, 2)).sqrt().t())
+    for name, y, (x, _), two, rest in zip(("dq", "dk", "dv", "dtable"), got, want, twice, share):
+        error, least = (y.cpu().double() - x).norm(), (two - x).norm()
+        rest = rest.norm() if torch.is_tensor(rest) else 0.0
+        unit = half * x.norm()
+        print(f"{name}: off by {error / unit:.3f}, rounded {least / unit:.3f}, of D {rest / unit:.3f}", flush=True)
+        assert error <= 1.1 * (least ** 2 + rest ** 2) ** 0.5, name
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("l", [256, 257, 300, 600])
+@pytest.mark.parametrize("raised", [6.0, 10.0])
+@pytest.mark.parametrize("both,causal", [(False, True), (True, False)])
+def test_weight_on_few_of_many_keys(l, raised, both, causal, dtype):
+    # The learned bias draws the weight to the nearest keys; with 10, 0.9 and more of it to a row's own.
+    q, k, v = inputs(2, 4, 2, l, l, 64, seed=l, dtype=dtype)
+    table = table_of(32, 4, dtype=dtype)
+    table[0] = raised
+    roundings(q, k, v, table, causal=causal, bidirectional=both)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dh", [40, 72, 128])
+@pytest.mark.parametrize("h,lq,lk", [(8, 300, 600), (1, 40, 3000), (2, 2049, 700)])  # the second with its keys split
+def test_scores_far_apart_and_values_of_one_mean(h, lq, lk, dh, dtype):
+    q, k, v = inputs(1, h, h, lq, lk, dh, seed=dh, dtype=dtype)
+    roundings(q * 3, k, v)
+    mean = torch.randn(dh, generator=seeded(9)).to(dtype).cuda()
+    for size in (1, 5):
+        roundings(q, k, v + size * mean)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("h,l", [(8, 300), (1, 3000)])
+def test_few_seen_keys_of_many(h, l, dtype):
+    # Rows see 3 keys, which are all over the tiles.
+    q, k, v = inputs(2, h, h, 130, l, 64, seed=l, dtype=dtype)
+    mask = torch.zeros(2, l, dtype=torch.bool)
+    mask[:, [0, l // 2, l - 1]] = True
+    roundings(q, k, v, mask=mask.cuda())
+
+
+@pytest.mark.parametrize("lq,lk", [(40, 3000), (300, 700)])  # keys split, and not
+def test_a_captured_backward_pass_follows_its_inputs(lq, lk):
+    # Values of one mean, whose rows begin again, and values of none, whose rows do not, replayed in turn.
+    q, k, v = inputs(1, 2, 1, lq, lk, 64, seed=lq)
+    plain, grad, mean = v.clone(), grad_of(q), torch.randn(64, generator=seeded(9)).to(BF).cuda()
+
+    def work():
+        out, lse = cross_attention(q, k, v, return_lse=True)
+        return out, lse, *cross_attention_backward(grad, q, k, v, out, lse)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for turn in range(5):
+        v.copy_(plain + 5 * mean if turn % 2 else plain)
+        want = work()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
