@@ -568,7 +568,8 @@ typedef struct selas_text_attention_problem {
  * keys and values that no query sees hold (NaN, infinities) does not reach a result. dtype (bf16 or fp16, otherwise SELAS_EUNSUPPORTED)
  * is that of q, k, v and out; scores, maxima and sums are fp32, the probabilities are rounded to dtype for the second product.
  * Takes Dh a multiple of 8 up to 128, addresses of 16 bytes and strides of 8 elements (out: 8 bytes and 4 elements), row
- * strides up to 2^23 elements; otherwise SELAS_EUNSUPPORTED. scale is in 1e-10 .. 1e10. out and lse overlap nothing.
+ * strides up to 2^23 elements, and what its launches hold (each under 2^32 threads: 2^23 images times key heads of few
+ * queries, 2^24 tiles of 128 queries); otherwise SELAS_EUNSUPPORTED. scale is in 1e-10 .. 1e10. out and lse overlap nothing.
  * workspace: at least selas_text_attention_workspace_bytes, 16-byte aligned, not used by anything else until the call has
  * run; NULL and 0 where that size is 0. Kernels and the split of the keys depend on the sizes, on which of lengths, mask and
  * table are given and on the CU count only, so equal calls give equal bits.

@@ -325,6 +325,15 @@ inline int64_t stride_of(int64_t n, int64_t given, int64_t alone) { return n > 1
 inline int width_of(int dh) { return dh <= 64 ? 64 : dh <= 96 ? 96 : 128; }
 // Fills and checks the arguments; `pointers`: of a call, not only of a question about sizes.
 int check_args(const char *what, const selas_text_attention_problem *p, int dtype, bool pointers, Args &a);
+// The largest launch of a call, in threads of one dimension: a grid holds fewer than 2^32.
+struct Threads {
+  int64_t most = 0;
+  void add(int64_t blocks, int64_t threads) { most = std::max(most, blocks * threads); }
+  int check(const char *what) const {
+    if (most < (1ll << 32)) return SELAS_OK;
+    return set_error(SELAS_EUNSUPPORTED, "%s: a launch of 2^32 threads or more (%lld)", what, (long long)most);
+  }
+};
 // Which work item a block takes: the XCDs, which blocks reach in turn, take chunks of consecutive items in turn. One chunk
 // each, so that most items that read the same rows meet one L2; where images differ in length (`ragged`) the `inner` items
 // of one (image, key head, part), which read the same, are a chunk, so that every XCD has short and long images: 16 x 64

@@ -775,6 +775,7 @@ struct Plan {
   Cut cut{};
   int few_parts;
   int64_t bytes = 0;  // workspace
+  Threads threads;
 };
 
 Plan plan_of(const Args &a) {
@@ -791,6 +792,8 @@ Plan plan_of(const Args &a) {
     // Parts for two workgroups a CU, of four units a wave at least.
     p.few_parts = static_cast<int>(std::max<int64_t>(1, std::min(2 * cu / std::max<int64_t>(items, 1), units / (4 * p.nw))));
     if (p.few_parts > 1) p.bytes = items * p.few_parts * p.few * (p.D + 2) * 4;
+    p.threads.add(items * p.few_parts, 512);
+    if (p.few_parts > 1) p.threads.add(items * rows, 128);
     return p;
   }
   Cut &c = p.cut;
@@ -812,6 +815,8 @@ Plan plan_of(const Args &a) {
   c.by_hk = fast_div(a.Hk);
   c.by_qblocks = fast_div(c.qblocks);
   if (c.parts > 1) p.bytes = static_cast<int64_t>(c.deal.total) * p.nw * partial_floats(p.D) * 4;
+  p.threads.add(c.deal.blocks, 64 * p.nw);
+  if (c.parts > 1) p.threads.add(static_cast<int64_t>(a.B) * a.H * c.qblocks * (p.D / 32), 256);
   return p;
 }
 
@@ -872,7 +877,10 @@ extern "C" int selas_text_attention_workspace_bytes(const selas_text_attention_p
   *bytes = 0;
   Args a;
   if (int e = check_args("text_attention_workspace_bytes", problem, dtype, false, a)) return e;
-  if (a.B && a.H && a.Lq) *bytes = plan_of(a).bytes;
+  if (!a.B || !a.H || !a.Lq) return ok();
+  const Plan p = plan_of(a);
+  if (int e = p.threads.check("text_attention_workspace_bytes")) return e;
+  *bytes = p.bytes;
   return ok();
 }
 
@@ -882,6 +890,7 @@ extern "C" int selas_text_attention(const selas_text_attention_problem *problem,
   if (int e = check_args("text_attention", problem, dtype, true, a)) return e;
   if (!a.B || !a.H || !a.Lq) return ok();
   const Plan p = plan_of(a);
+  if (int e = p.threads.check("text_attention")) return e;
   if (p.bytes && (workspace_bytes < p.bytes || !workspace || !aligned(workspace, 16)))
     return set_error(SELAS_EINVAL, "text_attention: needs a 16-byte aligned workspace of %lld bytes", (long long)p.bytes);
   const hipStream_t st = static_cast<hipStream_t>(stream);

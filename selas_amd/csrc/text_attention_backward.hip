@@ -726,6 +726,7 @@ struct Plan {
   int D, qblocks, kblocks, buckets;
   Cut key, query;
   int64_t neg_lse, dot, g_norm, v_norm, dtable, key_partial, query_partial, missing, bytes;  // offsets into the workspace
+  Threads threads;
 };
 constexpr int kNW = 4;
 
@@ -764,6 +765,13 @@ Plan plan_of(const Args &a, bool bf) {
     p.query_partial = take(static_cast<int64_t>(p.query.parts) * a.B * a.H * a.Lq * a.dh);
     p.missing = take(2 * p.query.parts * stats);
   }
+  const int64_t heads = static_cast<int64_t>(a.B) * a.H, key_heads = static_cast<int64_t>(a.B) * a.Hk;
+  if (!bf) p.threads.add(heads * p.qblocks + key_heads * p.kblocks, 256);
+  p.threads.add(p.query.deal.blocks, 64 * kNW);
+  p.threads.add(p.key.deal.blocks, 64 * kNW);
+  if (p.query.parts > 1) p.threads.add(cdiv(heads * a.Lq * a.dh, 1024), 256);
+  if (p.key.parts > 1 || !a.Lq) p.threads.add(cdiv(key_heads * a.Lk * a.dh, 1024), 256);
+  if (a.bias.table) p.threads.add(a.H, 256);
   return p;
 }
 
@@ -818,7 +826,10 @@ extern "C" int selas_text_attention_backward_workspace_bytes(const selas_text_at
   *bytes = 0;
   Args a;
   if (int e = check_args("text_attention_backward_workspace_bytes", problem, dtype, false, a)) return e;
-  if (a.H) *bytes = plan_of(a, dtype == SELAS_BF16).bytes;
+  if (!a.H) return ok();
+  const Plan p = plan_of(a, dtype == SELAS_BF16);
+  if (int e = p.threads.check("text_attention_backward_workspace_bytes")) return e;
+  *bytes = p.bytes;
   return ok();
 }
 
@@ -843,6 +854,7 @@ extern "C" int selas_text_attention_backward(const selas_text_attention_problem 
   if (!aligned(dq, 8) || !aligned(dk, 8) || !aligned(dv, 8))
     return set_error(SELAS_EUNSUPPORTED, "%s: dq, dk and dv must be 8-byte aligned", what);
   Plan p = plan_of(a, bf);
+  if (int e = p.threads.check(what)) return e;
   if (p.bytes && (workspace_bytes < p.bytes || !workspace || !aligned(workspace, 16)))
     return set_error(SELAS_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)p.bytes);
   auto at = [&](int64_t offset) { return reinterpret_cast<float *>(static_cast<char *>(workspace) + offset); };
