@@ -539,7 +539,7 @@ int selas_raw_linear_tile(const selas_raw_linear_problem *problems, int64_t coun
  * mask[b * mask_sb + j] != 0 (NULL: all). start[b], or start0 where start is NULL, is the position of the image's first
  * query among the keys' positions 0 .. Lk - 1: with causal != 0 query i sees the keys j <= start + i.
  * table [buckets, H] (row stride table_sl, type table_dtype) is the learned bias, or NULL. Its buckets are those of
- * selas_relative_buckets. */
+ * selas_relative_buckets. Finite entries beyond +-2^17 count as +-2^17, one of -inf hides its keys. */
 typedef struct selas_text_attention_problem {
   const void *q;
   int64_t q_sb, q_sh, q_sl;

@@ -15,6 +15,7 @@ constexpr int kRows = 64;              // rows (keys or queries) per LDS tile
 constexpr int kMaxSide = 128;          // buckets per direction
 constexpr int kMaxDistance = 512;      // tables and histograms by distance have to fit LDS beside the tiles
 constexpr float kLowest = -3.402823466e38f;
+constexpr float kEntry = 131072.0f;  // the largest entry of a bias table that counts as it is
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kPast = 0x80000000u;  // a byte offset past every buffer range here (ranges stay below 2^31): loads read 0
 
@@ -158,7 +159,10 @@ __device__ __forceinline__ float bias_at(const Bias &t, int head, int d, float m
   const float v = t.dtype == SELAS_F32   ? load_f<SELAS_F32>(t.table, i)
                   : t.dtype == SELAS_F16 ? load_f<SELAS_F16>(t.table, i)
                                          : load_f<SELAS_BF16>(t.table, i);
-  return v * mul;
+  // Finite entries count as +-2^17 beyond it. The lowest numbers of fp32 and bf16, divided by the scale, would be -inf and hide
+  // the key; from 1e9 on the difference of a score and its rounded maximum would overflow as an exponent; and products of
+  // queries and keys would be lost beside the entry (at 2^17 scores keep 2^-7).
+  return (fabsf(v) < __builtin_inff() ? fminf(fmaxf(v, -kEntry), kEntry) : v) * mul;
 }
 
 // The four copies of a head's table, into LDS, by all threads of the workgroup; reversed: by query - key. Building them once

@@ -11,7 +11,7 @@ from selas_amd.text_attention import (cross_attention, cross_attention_backward,
 from .conftest import seeded
 from .test_gpu_text_attention import BF, F32, FP, inputs, table_of
 from .test_gpu_text_attention_backward import grad_of
-from .text_attention_reference import Reference
+from .text_attention_reference import Reference, within
 
 pytestmark = pytest.mark.gpu
 
@@ -184,3 +184,61 @@ def test_a_captured_backward_pass_follows_its_inputs(lq, lk):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def checked(q, k, v, table, ref_table, ref_kw=None, **kw):
+    """Forward and gradients of a call with `table` against the definition with `ref_table`."""
+    grad = grad_of(q)
+    out, lse = text_attention(q, k, v, table, return_lse=True, **kw)
+    ref = Reference(q, k, v, ref_table, **kw, **(ref_kw or {}))
+    within(out, ref.out, ref.out_bound)
+    within(lse, ref.lse, ref.lse_bound)
+    for name, y, want in zip(("dq", "dk", "dv", "dtable"), text_attention_backward(grad, q, k, v, out, lse, table, **kw),
+                             ref.backward(grad)):
+        print(name, flush=True)
+        within(y, *want)
+    return out, lse
+
+
+LIMIT = 2.0 ** 17
+
+
+@pytest.mark.parametrize("dtype,ttype,low", [(BF, F32, -torch.finfo(F32).max), (BF, BF, -torch.finfo(BF).max), (FP, F32, -1e9),
+                                             (FP, FP, -torch.finfo(FP).max), (FP, F32, -torch.finfo(F32).max), (BF, F32, -1e30)])
+@pytest.mark.parametrize("lq,scale", [(1, None), (2, 1.0), (40, None), (130, 1e-3)])
+def test_lowest_entries_of_the_table(lq, scale, dtype, ttype, low):
+    # Keys after the query have the lowest entry: no weight beside any other key, and weights by their products among
+    # themselves, where the first row sees no other. Entries count as 2^17 beyond that.
+    q, k, v = inputs(2, 8, 4, lq, 150, 64, seed=lq, dtype=dtype)
+    table = table_of(32, 8, dtype=ttype)
+    table[16:] = low
+    mask = torch.ones(2, 150, dtype=torch.bool)
+    mask[0, 0] = False
+    checked(q, k, v, table, table.clamp(-LIMIT, LIMIT), mask=mask.cuda(), scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("lq", [1, 40, 130])
+def test_largest_entries_of_the_table(lq, dtype):
+    q, k, v = inputs(2, 8, 4, lq, 150, 64, seed=lq, dtype=dtype)
+    table = table_of(32, 8, dtype=F32)
+    table[0] = torch.finfo(F32).max
+    out, _ = checked(q, k, v, table, table.clamp(-LIMIT, LIMIT))
+    # Each row's own key alone. Its weight is 2^r, r what the maximum of the scores was rounded by; that is rounded to the type
+    # for the product and not for the sum, and the result again: two halves of a step, the second of a value larger by the first.
+    own, half = v[:, :, :lq].repeat_interleave(2, 1).double().cpu(), torch.finfo(dtype).eps / 2
+    within(out.view(2, lq, 8, 64).transpose(1, 2), own, own.abs() * (2 * half + 2 * half ** 2))
+
+
+@pytest.mark.parametrize("dtype,ttype", [(BF, F32), (BF, BF), (FP, FP)])
+@pytest.mark.parametrize("lq", [1, 40, 130])
+def test_entries_of_minus_infinity_hide_their_keys(lq, dtype, ttype):
+    q, k, v = inputs(2, 8, 4, lq, 150, 64, seed=lq, dtype=dtype)
+    table = table_of(32, 8, dtype=ttype)
+    table[16:] = 0.0
+    hiding = table.clone()
+    hiding[16:] = -torch.inf
+    mask = torch.ones(2, 150, dtype=torch.bool)
+    mask[0, 0] = False
+    out, lse = checked(q, k, v, hiding, table, ref_kw=dict(causal=True), mask=mask.cuda())
+    assert not out[0, 0].any() and bool((lse[0, :, 0] == -torch.inf).all())  # a row that sees no key
