@@ -583,9 +583,10 @@ int selas_text_attention_workspace_bytes(const selas_text_attention_problem *pro
  * The gradients of that call for grad, the gradient of out ([B, Lq, H*Dh], g_sb, g_sl): problem is the forward call's, with
  * the out and lse that it wrote (out may be a copy at other strides). dq [B, H, Lq, Dh], dk and dv [B, Hk, Lk, Dh] are
  * contiguous, in dtype; dtable [buckets, H] contiguous, in table_dtype (unused where table is NULL). Keys that are not seen
- * have gradients of 0, and so have queries that see none. grad's address and strides are as q's, dq, dk and dv 8-byte
- * aligned. dk and dv are summed over the query heads that share a key head, dtable over everything, in fp32 and in one
- * order: no atomics. workspace as in selas_text_attention, of selas_text_attention_backward_workspace_bytes. */
+ * have gradients of 0, and so have queries that see none; what those hold, or their rows of grad, reaches nothing. grad's
+ * address and strides are as q's (the batch stride always), dq, dk and dv 8-byte aligned. dk and dv are summed over the query
+ * heads that share a key head, dtable over everything, in fp32 and in one order: no atomics. workspace as in
+ * selas_text_attention, of selas_text_attention_backward_workspace_bytes. */
 int selas_text_attention_backward(const selas_text_attention_problem *problem, const void *grad, int64_t g_sb, int64_t g_sl,
                                   void *dq, void *dk, void *dv, void *dtable, int dtype, void *workspace,
                                   int64_t workspace_bytes, void *stream);

@@ -44,7 +44,8 @@ struct Cut {
   int again;        // its second launch
 };
 
-// fp16: the largest squared norm among 64 rows of dO, or (blocks past the queries') of 64 values; 4 lanes to a row.
+// fp16: the largest squared norm among 64 rows of dO, or (blocks past the queries') of 64 values; 4 lanes to a row. What
+// queries that see no key or masked values hold is left out.
 __global__ __launch_bounds__(256) void norm_kernel(Args a, Grads w) {
   __shared__ float red[4];
   const int lane = threadIdx.x & 63, r = threadIdx.x >> 2, part = threadIdx.x & 3;
@@ -55,7 +56,8 @@ __global__ __launch_bounds__(256) void norm_kernel(Args a, Grads w) {
   if (t < queries) {
     const int qt = t % w.qblocks, bh = t / w.qblocks, b = bh / a.H, row = qt * kRows + r;
     out = w.g_norm + t;
-    if (row < a.Lq) p = w.g.p + b * w.g.sb + (bh - b * a.H) * w.g.sh + row * w.g.sl;
+    if (row < a.Lq && a.lse[static_cast<int64_t>(bh) * a.Lq + row] != -__builtin_inff())
+      p = w.g.p + b * w.g.sb + (bh - b * a.H) * w.g.sh + row * w.g.sl;
   } else {
     t -= queries;
     const int kt = t % w.kblocks, bh = t / w.kblocks, b = bh / a.Hk, row = kt * kRows + r;
@@ -111,7 +113,8 @@ __device__ __forceinline__ float ds_shift(const Args &a, const Grads &w, int b, 
 // queries: S = Q K^T and dP = dO V^T with the query rows read row-wise, so that a lane's registers hold 16 queries of one
 // key, in runs of 8; then dV^T += dO^T P and dK^T += Q^T dS with the same tiles read transposed and P, dS straight from the
 // registers. A key's column depends on nothing of the other keys, so masked keys need no select: their results are zeroed at
-// the end.
+// the end. A query that sees no key has p = 0, but what it and its dO hold, NaN included, meets that in a product: where an
+// image may have such a query and others (a causal mask with masked keys or a negative start) its rows are cleared in LDS.
 //
 // Bounded by LDS reads (an MFMA reads 1 KiB) and by waiting: dk and dv of 32 keys take D registers a lane and k and v D / 2
 // more, which leaves three workgroups a CU at D = 64 and two at D = 128 (MFMA 30 % busy at 4 x 64 heads of 512 tokens, 57 us;
@@ -231,10 +234,29 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
     if constexpr (BIAS) next_table(g);
     issue(0, g, qt);
   }
+  const bool blind = a.causal && (a.mask || start < 0);  // some queries may see no key
   auto step = [&](int stage) __attribute__((always_inline)) {
     wait_vmcnt<0>();
     __syncthreads();  // this tile has landed for every wave, and no wave reads the other stage any more
     const int at = qt;
+    if (blind) {
+      static_assert(NW == 4, "four threads a row");
+      uint8_t *base = stage ? smem1 : smem0;
+      const float nl = reinterpret_cast<const float *>(base + 2 * T::kBytes)[lane];
+      const uint64_t rows = __builtin_amdgcn_ballot_w64(nl == -__builtin_inff()) & up_to(a.Lq - 1 - at * kRows);
+      if (rows) {
+        int thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));  // addresses of this rare branch hold no registers in the loop
+        const int r = thread >> 2;
+        if ((rows >> r) & 1)
+          for (int i = thread & 3; i < T::kChunks; i += 4) {
+            uint8_t *to = base + T::at(r) + r % T::kGroupRows * T::kRow + 16 * i;
+            *reinterpret_cast<uint4 *>(to) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(to + T::kBytes) = make_uint4(0, 0, 0, 0);
+          }
+        __syncthreads();
+      }
+    }
     const float *table = table_of(g);
     if (++qt == w.qblocks) {
       qt = qt0;
@@ -424,8 +446,12 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void query_kernel(Args a,
 #pragma unroll
     for (int r = 0; r < 16; ++r) d = r == 4 * (c >> 3) + (c & 3) ? x[r] : d;
     dd = pair_sum(h == ((c >> 2) & 1) ? d : 0.0f);
-    if (nl == -__builtin_inff()) dd = 0.0f;
     dd += missing;  // 0 but in the second launch
+    if (nl == -__builtin_inff()) {  // a row that sees no key: what its dO holds must not meet p = 0
+      dd = 0.0f;
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s) dO.f[s] = make_uint4(0, 0, 0, 0);
+    }
   }
   const uint16_t *kp = a.k.p + b * a.k.sb + hk * a.k.sh, *vp = a.v.p + b * a.v.sb + hk * a.v.sh;
   const typename T::template Loader<KJ> kl(wave, lane, a.k.sl, a.dh), vl(wave, lane, a.v.sl, a.dh);

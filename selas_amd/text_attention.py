@@ -220,7 +220,7 @@ def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tenso
 
     Each is the gradient of the tensor as given: dk and dv are summed over the query heads that share a key head; a
     broadcast input (an expanded batch) still has its own sum to take. Keys that are not seen and queries that see none
-    have zeros. Sums are fp32 in one order: equal calls give equal bits."""
+    have zeros, and what they and their rows of ``grad`` hold does not matter. Sums are fp32 in one order: equal calls give equal bits."""
     return _backward("cross_attention_backward", grad, q, k, v, out, lse, None, 0, True, False, 0, lengths, mask, scale)[:3]
 
 

@@ -242,3 +242,29 @@ def test_entries_of_minus_infinity_hide_their_keys(lq, dtype, ttype):
     mask[0, 0] = False
     out, lse = checked(q, k, v, hiding, table, ref_kw=dict(causal=True), mask=mask.cuda())
     assert not out[0, 0].any() and bool((lse[0, :, 0] == -torch.inf).all())  # a row that sees no key
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("dh,bias", [(64, True), (72, False), (128, True)])
+@pytest.mark.parametrize("l", [1, 70, 300, 2000])
+def test_what_queries_that_see_no_key_hold_does_not_matter(l, dh, bias, dtype):
+    # Texts padded at their front under a causal mask: the padding is hidden as keys, by the mask or by negative positions,
+    # and its queries see nothing.
+    q, k, v = inputs(3, 4, 2, l, l, dh, seed=l, dtype=dtype)
+    table, grad = table_of(32, 4) if bias else None, grad_of(q)
+    pads = torch.tensor([0, l // 3, l]).cuda()
+    dead = torch.arange(l, device="cuda") < pads[:, None]
+    shifted = -pads.to(torch.int32)
+    for kw in (dict(mask=~dead), dict(q_start=shifted), dict(mask=~dead, q_start=shifted // 2)):
+        at = dead if "mask" in kw else torch.arange(l, device="cuda") < pads[:, None]
+        out, lse = text_attention(q, k, v, table, causal=True, return_lse=True, **kw)
+        assert not out[at].any() and bool((lse.transpose(1, 2)[at] == -torch.inf).all())
+        want = text_attention_backward(grad, q, k, v, out, lse, table, causal=True, **kw)
+        assert not want[0].transpose(1, 2)[at].any()
+        q2, grad2 = q.masked_fill(at[:, None, :, None], float("nan")), grad.masked_fill(at[:, :, None], float("nan"))
+        grad3 = grad.masked_fill(at[:, :, None], float("inf"))
+        out, lse = text_attention(q2, k, v, table, causal=True, return_lse=True, **kw)
+        assert not out[at].any()
+        for g in (grad2, grad3):
+            got = text_attention_backward(g, q2, k, v, out, lse, table, causal=True, **kw)
+            assert all(torch.equal(x, y) for x, y in zip(got, want) if x is not None)
