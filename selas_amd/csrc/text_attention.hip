@@ -23,8 +23,10 @@ namespace {
 // enough (MFMAs would fill 1 to 8 of their 32 columns). A lane holds 8 channels; D / 8 lanes make a key, 64 / (D / 8) key
 // slots a wave; each slot keeps a softmax of its own over the keys it meets, joined once at the end. k and v go from memory
 // to registers, the next unit's loads ahead of this one's arithmetic: units of 8 keys a slot hold 16 KiB a wave in flight.
-// Units of 4, at four waves a SIMD instead of three, were ahead only from 4 rows on (32,768 keys: 90 -> 74 us; 16 texts of one
-// row over up to 2048 keys: 38 against 44). 64 x 32 heads of 64, one row over 2048 keys: 217 us, 4.9 TB/s; 16 x 32: 57.
+// From 3 rows on the registers of a softmax per row and key leave room for units of 2: us with 2 / 4 / 8, 64 x 8 key heads of 64
+// and 4 rows over 2048 keys 56 / 90 / 220, 16 x 8 key heads of 128 and 4 rows 36 / 55 / 148, 16 x 4 of 64 and 8 rows over up to
+// 2048 keys 23 / 28 / 69; where 4 key heads alone leave a workgroup or two to a CU 4 are ahead (32,768 keys, 4 rows: 81 / 59 /
+// 95). 64 x 32 heads of 64, one row over 2048 keys: 215 us, 5.0 TB/s; 16 x 32: 57.
 template <int D, int R>
 struct Few {
   static constexpr int kLanes = D / 8, kSlots = 64 / kLanes;
@@ -321,7 +323,7 @@ __device__ __forceinline__ Item item_at(const Args &a, const Cut &cut, int t, in
 // waves share. Per tile: S^T = K Q^T (K row-wise from LDS, Q held), the softmax on the scores in registers, O^T += V^T P^T
 // (V transposed by the LDS reads, the probabilities straight from the score registers: the K rows of a block are read with
 // bits 2 and 3 of the row exchanged, so that register r of a lane holds key 16 (r / 8) + 8 h + r % 8 of it, as the second
-// product's operand wants them).
+// product's operand wants them). Three workgroups a CU; with 128 channels and a bias 4 registers spill for that.
 template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, NW >= 4 ? 3 : 1) void fwd_kernel(Args a, Cut cut) {
   using T = TileOf<D>;

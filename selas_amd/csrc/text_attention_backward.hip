@@ -117,10 +117,10 @@ __device__ __forceinline__ float ds_shift(const Args &a, const Grads &w, int b, 
 // image may have such a query and others (a causal mask with masked keys or a negative start) its rows are cleared in LDS.
 //
 // Bounded by LDS reads (an MFMA reads 1 KiB) and by waiting: dk and dv of 32 keys take D registers a lane and k and v D / 2
-// more, which leaves three workgroups a CU at D = 64 and two at D = 128 (MFMA 30 % busy at 4 x 64 heads of 512 tokens, 57 us;
-// 24 heads of 128, 4096 queries over 512 keys 63 to 68 us, 800 TFLOP/s). With each 16 rows' products right behind their
-// packing one pair of packed operands is live instead of two (178 -> 164 registers); a lone workgroup a CU at D = 128 took
-// 100 us there.
+// more, which leaves three workgroups a CU at D = 64 and two at D = 128, where 4 to 8 registers spill but for bf16 without a
+// bias (MFMA 30 % busy at 4 x 64 heads of 512 tokens, 58 us; 24 heads of 128, 4096 queries over 512 keys 66 us, 780 TFLOP/s).
+// With each 16 rows' products right behind their packing one pair of packed operands is live instead of two (178 -> 164
+// registers); a lone workgroup a CU at D = 128 took 100 us there.
 template <bool BF, int D, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cut) {
   using T = TileOf<D>;
@@ -319,8 +319,8 @@ __global__ __launch_bounds__(64 * NW, 2) void key_kernel(Args a, Grads w, Cut cu
 // held. S^T = K Q^T and dP^T = V dO^T leave a lane's registers with keys of one query, in runs of 8; dQ^T += K^T dS^T reads
 // the same K tile transposed.
 //
-// Bounded as key_kernel: 3 products of 7, 153 to 168 registers at D = 64 (61 us at 4 x 64 heads of 512 with a bias), 223 at
-// D = 128 (66 to 72 us at 4096 queries over 512 keys).
+// Bounded as key_kernel: 3 products of 7, 153 to 168 registers at D = 64 (75 us at 4 x 64 heads of 512 with a bias), 223 at
+// D = 128 (72 us at 4096 queries over 512 keys).
 //
 // dtable: tiles that hold only one value of the bias add dS up in a register. In the others dS is summed along the diagonals
 // (one distance each): a lane's run of 8 keys moves a lane per key through the 16 lanes of its row (Diagonals), and what is
