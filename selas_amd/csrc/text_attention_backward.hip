@@ -351,7 +351,8 @@ __host__ __device__ inline int hist_floats(int reach) { return 2 * reach + 2 * k
 
 // Sums along the diagonals of a wave's 32 keys x 32 queries. v[e] of lane q belongs to distance o + e - q. With
 // t_e[p] = v[e][p] + t_{e+1}[p + 1], the lanes' indices modulo 16, t_0[p] holds distance o - p and, from the lanes below e
-// that wrapped, o + 16 - p; the latter are summed apart and belong to the next 16 keys' first part.
+// that wrapped, o + 16 - p. Each is summed apart (subtracting the latter from the sum of both would leave its rounding in the
+// other's bucket); the latter belong to the next 16 keys' first part.
 struct Diagonals {
   float u[3] = {};  // u[m] of lane q: distance d0 + 16 m of that lane
   __device__ __forceinline__ static float next_lane(float v) {  // row_ror:15
@@ -359,14 +360,18 @@ struct Diagonals {
   }
   __device__ __forceinline__ void add(int m, const f32x16 &v, int lane) {  // the m-th 8 of v
     const int p = lane & 15;
-    float all = v[8 * m + 7], low = p < 7 ? all : 0.0f;
+    float high = 0.0f, low = 0.0f;
 #pragma unroll
-    for (int e = 6; e >= 0; --e) {
-      all = v[8 * m + e] + next_lane(all);
-      low = next_lane(low);
-      if (e) low += p < e ? v[8 * m + e] : 0.0f;
+    for (int e = 7; e >= 0; --e) {
+      const float x = v[8 * m + e];
+      if (e < 7) {
+        high = next_lane(high);
+        low = next_lane(low);
+      }
+      high += p >= e ? x : 0.0f;
+      if (e) low += p < e ? x : 0.0f;
     }
-    u[m] += all - low;
+    u[m] += high;
     u[m + 1] += low;
   }
   // u[m + 1] of the lanes 16 .. 31 meets u[m] of the lanes 0 .. 15: first the even ones, then the odd one. LDS instructions

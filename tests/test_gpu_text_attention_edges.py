@@ -268,3 +268,18 @@ def test_what_queries_that_see_no_key_hold_does_not_matter(l, dh, bias, dtype):
         for g in (grad2, grad3):
             got = text_attention_backward(g, q2, k, v, out, lse, table, causal=True, **kw)
             assert all(torch.equal(x, y) for x, y in zip(got, want) if x is not None)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("both,distance", [(True, 200), (False, 33), (False, 128)])
+@pytest.mark.parametrize("lq,lk,start", [(129, 128, -43), (31, 200, 170), (333, 128, 99), (300, 300, 0)])
+def test_a_buckets_gradient_holds_no_rounding_of_anothers(lq, lk, start, both, distance, dtype):
+    # The entries are far apart: some buckets' sums are 1e-8 of their neighbours', element by element within their own bounds
+    # (but for weights below fp32's normal numbers).
+    q, k, v = inputs(2, 48, 3, lq, lk, 64, seed=lq, dtype=dtype)
+    table, kw = table_of(32, 48, dtype=F32, std=4.0), dict(bidirectional=both, max_distance=distance, causal=not both, q_start=start)
+    out, lse = text_attention(q, k, v, table, return_lse=True, **kw)
+    grad = grad_of(q)
+    dtable = text_attention_backward(grad, q, k, v, out, lse, table, **kw)[3]
+    want, bound = Reference(q, k, v, table, **kw).backward(grad)[3]
+    within(dtable, want, bound + 2.0 ** -100)
