@@ -534,12 +534,13 @@ int selas_raw_linear_tile(const selas_raw_linear_problem *problems, int64_t coun
 
 /* One call of selas_text_attention (host memory): q [B, H, Lq, Dh], k and v [B, Hk, Lk, Dh] with unit channel stride and
  * any batch, head and row strides (*_sb, *_sh, *_sl, elements; that of an axis of one element is not looked at, but not
- * negative), H a multiple of Hk; query head h reads key head h / (H / Hk). out is [B, Lq, H*Dh] (o_sb, o_sl); lse [B, H, Lq] fp32, contiguous, or NULL.
+ * negative), H a multiple of Hk; query head h reads key head h / (H / Hk). out is [B, Lq, H*Dh] (o_sb, o_sl); lse
+ * [B, H, Lq] fp32, contiguous, or NULL.
  * Key j of image b exists where j < lengths[b] (NULL: all Lk; values outside 0 .. Lk count as the nearer end) and
  * mask[b * mask_sb + j] != 0 (NULL: all). start[b], or start0 where start is NULL, is the position of the image's first
  * query among the keys' positions 0 .. Lk - 1: with causal != 0 query i sees the keys j <= start + i.
  * table [buckets, H] (row stride table_sl, type table_dtype) is the learned bias, or NULL. Its buckets are those of
- * selas_relative_buckets. Finite entries beyond +-2^17 count as +-2^17, one of -inf hides its keys. */
+ * selas_relative_buckets. Finite entries beyond +-2^17 count as +-2^17, one of -inf leaves its keys no weight. */
 typedef struct selas_text_attention_problem {
   const void *q;
   int64_t q_sb, q_sh, q_sl;

@@ -185,9 +185,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, length
     matter, NaN included; a query that sees none gets zeros and an lse of -inf. ``scale``: 1 / sqrt(Dh) unless given.
     ``out``: optional destination with unit column stride and rows of whole 8 bytes, overlapping nothing the call reads.
 
-    bf16 or fp16, Dh of whole 8 up to 128, otherwise ``Unsupported``. Scores, maxima and sums are fp32 (scores are to stay
-    below 10^7 in magnitude, where fp32 no longer tells neighbouring whole numbers apart), the probabilities
-    are rounded to the type for the product with v. No graph is recorded: tensors that require grad are refused outside
+    bf16 or fp16, Dh of whole 8 up to 128, otherwise ``Unsupported``. Scores, maxima and sums are fp32
+    (scores are to stay below 10^7 in magnitude, where fp32 holds little more than whole numbers), the probabilities are
+    rounded to the type for the product with v. No graph is recorded: tensors that require grad are refused outside
     torch.no_grad(), and ``cross_attention_backward`` gives the gradients."""
     return _forward("cross_attention", q, k, v, None, 0, True, False, 0, lengths, mask, scale, out, return_lse)
 
@@ -203,8 +203,8 @@ def text_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: tor
     the query, and bucket 0 for those after it) distance a has bucket a below n // 2, and above it
     n // 2 + floor((n - n // 2) log(a / (n // 2)) / log(max_distance / (n // 2))), at most n - 1; keys after the query
     have the second half. Distances are compared in exact arithmetic. 2 to 128 buckets a direction, max_distance up to 512.
-    An entry of -inf hides its keys; finite ones beyond +-2^17 count as +-2^17, which leaves such a key no weight beside others,
-    and weights by their products to keys that all have it.
+    An entry of -inf leaves its keys no weight; finite ones beyond +-2^17 count as +-2^17, which leaves a key no weight
+    beside others, and weights by their products to keys that all have it.
     ``causal``: a query sees the keys up to its own position (a NaN in the value of a key that later queries see reaches
     the earlier ones too, as in a product with weights of 0). For one more token over a cache give q [B, H, 1, Dh],
     ``lengths`` and ``q_start = lengths - 1`` (int32: no conversion)."""
@@ -220,7 +220,8 @@ def cross_attention_backward(grad: torch.Tensor, q: torch.Tensor, k: torch.Tenso
 
     Each is the gradient of the tensor as given: dk and dv are summed over the query heads that share a key head; a
     broadcast input (an expanded batch) still has its own sum to take. Keys that are not seen and queries that see none
-    have zeros, and what they and their rows of ``grad`` hold does not matter. Sums are fp32 in one order: equal calls give equal bits."""
+    (by ``lengths``, ``mask`` or a causal mask) have zeros, and what they and their rows of ``grad`` hold does not matter.
+    Sums are fp32 in one order: equal calls give equal bits."""
     return _backward("cross_attention_backward", grad, q, k, v, out, lse, None, 0, True, False, 0, lengths, mask, scale)[:3]
 
 
